@@ -5,7 +5,8 @@ Usage: python build.py [--force]
 Every object is compiled with ``-gencode arch=compute_100a,code=sm_100a`` and
 ``--fmad=false`` (no FMA contraction anywhere on the parity path, as in the
 reference's CUDA build) and linked into one shared library whose only exported
-symbols are the ``eps_b200_*`` entry points declared in include/eps_b200.h.
+symbols are the ``eps_b200_*`` entry points declared in include/eps_b200.h and
+include/eps_b200_dense.h.
 """
 from __future__ import annotations
 
@@ -22,7 +23,8 @@ BUILD = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "libeps_b200.so")
 
 SOURCES = ["store.cu", "lookup.cu", "sort.cu", "push.cu", "route.cu", "noalloc.cu", "runtime.cu",
-           "comm.cu", "client.cu", "sync.cu", "runtime_api.cu"]
+           "comm.cu", "client.cu", "sync.cu", "runtime_api.cu",
+           "block_norm.cu", "route_experts.cu", "int8_product.cu", "adamw.cu"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-std=c++17", "-lineinfo", "--fmad=false", "-Xcompiler", "-fPIC",
          "-Xcompiler", "-fvisibility=hidden", "-I", CSRC, "-I", INCLUDE]
@@ -45,7 +47,7 @@ def _stale(target: str, deps: list[str]) -> bool:
 def build(force: bool = False, verbose: bool = False) -> str:
     os.makedirs(BUILD, exist_ok=True)
     headers = [os.path.join(CSRC, h) for h in os.listdir(CSRC) if h.endswith((".h", ".cuh"))]
-    headers.append(os.path.join(INCLUDE, "eps_b200.h"))
+    headers += [os.path.join(INCLUDE, h) for h in ("eps_b200.h", "eps_b200_dense.h")]
     objs = []
     procs = []
     for src in SOURCES:

@@ -1,0 +1,614 @@
+"""The dense block beside the embedding store: Python binding of include/eps_b200_dense.h.
+
+    h, z = dense.block_norm(x, y, gate, post_weight=..., pre_weight=..., scale=0.5)
+    routing = dense.route(logits, top_k=8, score="sigmoid", bias=balance)
+    experts = dense.QuantizedExperts.from_weights(weight)          # [experts, channels, inner]
+    out = experts.product(z, offsets=routing.offsets, rows=routing.order, rows_divisor=8)
+    dense.AdamW(parameters, gradients, state_bits=8).step()
+
+Every tensor is a torch CUDA tensor; work goes to torch's current stream of the
+tensors' device and is asynchronous, results and workspaces come from torch's
+allocator, and nothing is kept between calls but what the two classes hold.  Calls
+can be captured in a CUDA graph.  There is no CPU fallback; a refused call raises
+``EpsError`` with ``code`` INVALID_ARGUMENT before anything is launched.
+
+Leading axes of a tensor count as rows; the last axis must be contiguous, rows may
+have any stride.  Element types are float32, bfloat16 and float16.
+"""
+from __future__ import annotations
+
+import ctypes as C
+import threading
+from typing import NamedTuple, Sequence
+
+import torch
+
+from . import EpsError, INVALID_ARGUMENT, Status, load_library
+
+__all__ = ["block_norm", "block_norm_backward", "BlockNormGradients", "route", "route_backward",
+           "Routing", "quantize_rows", "QuantizedExperts", "AdamW", "ENTRY_POINTS"]
+
+ENTRY_POINTS = ("eps_b200_block_norm", "eps_b200_block_norm_workspace",
+                "eps_b200_block_norm_backward", "eps_b200_route_experts_workspace",
+                "eps_b200_route_experts", "eps_b200_route_experts_backward",
+                "eps_b200_int8_stride", "eps_b200_int8_quantize",
+                "eps_b200_int8_product_workspace", "eps_b200_int8_product", "eps_b200_int8_linear",
+                "eps_b200_adamw_plan_bytes", "eps_b200_adamw_plan", "eps_b200_adamw")
+
+_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_KINDS = {"rms": 0, "layer": 1}
+_ACTIVATIONS = {"none": 0, "sigmoid": 1, "silu": 2, "tanh": 3}
+_SCORES = {"softmax": 0, "sigmoid": 1}
+ADAMW_BLOCK = 256           # elements of a tensor that share a scale (EPS_B200_ADAMW_BLOCK)
+
+
+# ------------------------------------------------------------------ C structs
+class BlockNorm(C.Structure):
+    _fields_ = [("device", C.c_int32), ("kind", C.c_int32), ("gate_kind", C.c_int32),
+                ("activation", C.c_int32), ("post_norm", C.c_int32), ("pre_norm", C.c_int32),
+                ("type", C.c_int32), ("residual_type", C.c_int32), ("parameter_type", C.c_int32),
+                ("columns", C.c_uint32), ("rows", C.c_uint64), ("epsilon", C.c_float),
+                ("scale", C.c_float), ("y", C.c_void_p), ("gate", C.c_void_p),
+                ("y_stride", C.c_int64), ("gate_stride", C.c_int64), ("post_weight", C.c_void_p),
+                ("post_bias", C.c_void_p), ("channel_scale", C.c_void_p),
+                ("pre_weight", C.c_void_p), ("pre_bias", C.c_void_p)]
+
+
+class BlockNormGradientArgs(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("dh", "dz", "h")] + \
+               [(n, C.c_int64) for n in ("dh_stride", "dz_stride", "h_stride")] + \
+               [(n, C.c_void_p) for n in ("dx", "dy", "dgate")] + \
+               [(n, C.c_int64) for n in ("dx_stride", "dy_stride", "dgate_stride")] + \
+               [(n, C.c_void_p) for n in ("dpost_weight", "dpost_bias", "dchannel_scale",
+                                          "dpre_weight", "dpre_bias", "workspace")] + \
+               [("workspace_bytes", C.c_uint64)]
+
+
+class RouteExperts(C.Structure):
+    _fields_ = [("device", C.c_int32), ("type", C.c_int32), ("score", C.c_int32),
+                ("renormalise", C.c_int32), ("experts", C.c_uint32), ("top_k", C.c_uint32),
+                ("groups", C.c_uint32), ("top_groups", C.c_uint32), ("tokens", C.c_uint64),
+                ("scale", C.c_float), ("reserved", C.c_int32), ("logits", C.c_void_p),
+                ("logits_stride", C.c_int64)]
+
+
+class Int8Product(C.Structure):
+    _fields_ = [("device", C.c_int32), ("type", C.c_int32), ("experts", C.c_uint32),
+                ("channels", C.c_uint32), ("inner", C.c_uint32), ("rows_divisor", C.c_uint32),
+                ("rows", C.c_uint64), ("weight", C.c_void_p), ("weight_scale", C.c_void_p),
+                ("bias", C.c_void_p), ("offsets", C.c_void_p), ("out", C.c_void_p),
+                ("workspace", C.c_void_p), ("workspace_bytes", C.c_uint64)]
+
+
+class AdamWTensor(C.Structure):
+    _fields_ = [("parameter", C.c_void_p), ("gradient", C.c_void_p), ("elements", C.c_uint64),
+                ("state_begin", C.c_uint64)]
+
+
+class AdamWArgs(C.Structure):
+    _fields_ = [("device", C.c_int32), ("parameter_type", C.c_int32), ("gradient_type", C.c_int32),
+                ("state_bits", C.c_int32), ("master", C.c_void_p), ("first", C.c_void_p),
+                ("second", C.c_void_p), ("first_scale", C.c_void_p), ("second_scale", C.c_void_p),
+                ("gradient_scale", C.c_void_p), ("skip", C.c_void_p), ("learning_rate", C.c_double),
+                ("beta1", C.c_double), ("beta2", C.c_double), ("epsilon", C.c_double),
+                ("weight_decay", C.c_double), ("step", C.c_uint64), ("seed", C.c_uint64)]
+
+
+def _bind():
+    lib, P, vp, i64, u64, u32, i32 = (load_library(), C.POINTER, C.c_void_p, C.c_int64, C.c_uint64,
+                                      C.c_uint32, C.c_int32)
+    st = P(Status)
+    lib.eps_b200_block_norm.argtypes = [P(BlockNorm), vp, i64, vp, i64, vp, i64, vp, st]
+    lib.eps_b200_block_norm_workspace.argtypes = [u64, u32]
+    lib.eps_b200_block_norm_backward.argtypes = [P(BlockNorm), P(BlockNormGradientArgs), vp, st]
+    lib.eps_b200_route_experts_workspace.argtypes = [u64, u32, u32]
+    lib.eps_b200_route_experts.argtypes = [P(RouteExperts), vp, vp, vp, vp, vp, vp, vp, u64, vp, st]
+    lib.eps_b200_route_experts_backward.argtypes = [P(RouteExperts), vp, vp, vp, i64, vp, st]
+    lib.eps_b200_int8_stride.argtypes = [u32]
+    lib.eps_b200_int8_quantize.argtypes = [i32, i32, vp, i64, u64, u32, vp, u32, u64, vp, vp, vp, st]
+    lib.eps_b200_int8_product_workspace.argtypes = [u64, u32, u32, u32]
+    lib.eps_b200_int8_product.argtypes = [P(Int8Product), vp, vp, vp, st]
+    lib.eps_b200_int8_linear.argtypes = [P(Int8Product), vp, i64, u64, vp, vp, st]
+    lib.eps_b200_adamw_plan_bytes.argtypes = [P(AdamWTensor), u64]
+    lib.eps_b200_adamw_plan.argtypes = [P(AdamWTensor), u64, vp, u64, P(u64), st]
+    lib.eps_b200_adamw.argtypes = [P(AdamWArgs), vp, u64, u64, vp, st]
+    for name in ENTRY_POINTS:
+        sized = name.endswith(("_workspace", "_bytes", "_stride"))
+        getattr(lib, name).restype = u64 if sized else C.c_int
+    return lib
+
+
+_lib = _bind()
+_local = threading.local()
+
+
+def _status():
+    st = getattr(_local, "status", None)
+    if st is None:
+        st = _local.status = Status()
+        _local.ref = C.byref(st)
+    return st, _local.ref
+
+
+def _call(fn, *args):
+    st, ref = _status()
+    rc = fn(*args, ref)
+    if rc:
+        raise EpsError(rc, st.message.decode(errors="replace"))
+
+
+def _refuse(message):
+    raise EpsError(INVALID_ARGUMENT, message)
+
+
+def _choice(table, value, what):
+    try:
+        return table[value]
+    except (KeyError, TypeError):
+        _refuse(f"{what} is one of {', '.join(map(str, table))}: got {value!r}")
+
+
+def _stream(device):
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+def _tensor(t, what, like=None):
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        _refuse(f"{what} must be a CUDA tensor")
+    if like is not None and t.device != like.device:
+        _refuse(f"{what} is on {t.device}, not on {like.device}")
+    return t
+
+
+def _matrix(t, what, like=None, columns=None, rows=None):
+    """(t as rows by columns, its row stride); its last axis contiguous."""
+    _tensor(t, what, like)
+    if t.dtype not in _TYPES:
+        _refuse(f"{what} must be float32, bfloat16 or float16")
+    if t.dim() < 1:
+        _refuse(f"{what} must have a last axis")
+    if t.dim() != 2:
+        try:
+            t = t.view(-1, t.shape[-1]) if t.numel() else t.reshape(0, t.shape[-1])
+        except RuntimeError:
+            _refuse(f"{what}: its leading axes cannot be seen as one")
+    if columns is not None and t.shape[1] != columns:
+        _refuse(f"{what} has {t.shape[1]} columns, not {columns}")
+    if rows is not None and t.shape[0] != rows:
+        _refuse(f"{what} has {t.shape[0]} rows, not {rows}")
+    if t.shape[1] > 1 and t.stride(1) != 1:
+        _refuse(f"the last axis of {what} must be contiguous")
+    return t, t.stride(0)
+
+
+def _vector(t, what, like, n, dtype):
+    """The address of a contiguous vector of n elements, or None."""
+    if t is None:
+        return None
+    _tensor(t, what, like)
+    if t.dtype != dtype or t.numel() != n or not t.is_contiguous():
+        _refuse(f"{what} must be a contiguous {dtype} vector of {n}")
+    return t.data_ptr()
+
+
+# ------------------------------------------------------------ norms and gate
+class BlockNormGradients(NamedTuple):
+    """Gradients of block_norm's inputs; None for what was not given."""
+    x: torch.Tensor
+    y: torch.Tensor | None
+    gate: torch.Tensor | None
+    post_weight: torch.Tensor | None
+    post_bias: torch.Tensor | None
+    channel_scale: torch.Tensor | None
+    pre_weight: torch.Tensor | None
+    pre_bias: torch.Tensor | None
+
+
+def _block_norm_args(residual, y, gate, post_weight, post_bias, pre_weight, pre_bias, channel_scale,
+                     scale, kind, activation, epsilon, post_norm, pre_norm, dtype):
+    """(C struct, y, gate) for a residual given as rows by columns."""
+    rows, columns = residual.shape
+    parameters = [p for p in (post_weight, post_bias, channel_scale, pre_weight, pre_bias) if p is not None]
+    ptype = parameters[0].dtype if parameters else torch.float32
+    if ptype != torch.float32 and ptype != dtype:
+        _refuse("weights, biases and channel_scale have the block's type or float32, all the same")
+    y_stride = gate_stride = gate_kind = 0
+    if y is not None:
+        y, y_stride = _matrix(y, "y", residual, columns, rows)
+    if gate is not None:
+        if y is None:
+            _refuse("a gate needs a block output y")
+        _tensor(gate, "gate", residual)
+        if gate.dtype != dtype:
+            _refuse("the gate has the type of y")
+        # one value a row: [rows] or [..., 1]; a matrix of one column is an element gate where D is 1
+        if gate.numel() == rows and columns > 1:
+            gate_kind = 1
+            if not gate.is_contiguous():
+                _refuse("a gate of one value a row must be contiguous")
+        else:
+            gate_kind = 2
+            gate, gate_stride = _matrix(gate, "gate", residual, columns, rows)
+    vectors = [_vector(p, what, residual, columns, ptype) for p, what in (
+        (post_weight, "post_weight"), (post_bias, "post_bias"), (channel_scale, "channel_scale"),
+        (pre_weight, "pre_weight"), (pre_bias, "pre_bias"))]
+    args = BlockNorm(residual.device.index, _choice(_KINDS, kind, "kind"), gate_kind,
+                     _choice(_ACTIVATIONS, activation, "activation"), bool(post_norm), bool(pre_norm),
+                     _TYPES[dtype], _TYPES[residual.dtype], _TYPES[ptype], columns, rows, epsilon, scale,
+                     None if y is None else y.data_ptr(), None if gate is None else gate.data_ptr(),
+                     y_stride, gate_stride, *vectors)
+    return args, y, gate
+
+
+def block_norm(x, y=None, gate=None, *, post_weight=None, post_bias=None, pre_weight=None,
+               pre_bias=None, channel_scale=None, scale: float = 1.0, kind: str = "rms",
+               activation: str = "sigmoid", epsilon: float = 1e-6, post_norm: bool = True,
+               pre_norm: bool = True):
+    """The joint between two blocks of a residual network, in one pass.
+
+        h = x + scale * channel_scale * activation(gate) * post_norm(y)
+        z = pre_norm(h)
+
+    x is the residual, y the output of the block before ([..., D]; None: h is x
+    itself), gate its gate ([..., D] or one value a row), z the input of the block
+    after.  x has the type of y, or is float32; z has the type of y.  kind "rms" or
+    "layer"; activation "none", "sigmoid", "silu" or "tanh".  Weights, biases and
+    channel_scale are vectors of D, all float32 or all of y's type.  D is at most
+    8192.  Returns (h, z), z None without pre_norm."""
+    residual, x_stride = _matrix(x, "x")
+    dtype = residual.dtype if y is None else _tensor(y, "y", residual).dtype
+    args, y2, g2 = _block_norm_args(residual, y, gate, post_weight, post_bias, pre_weight, pre_bias,
+                                    channel_scale, scale, kind, activation, epsilon, post_norm, pre_norm,
+                                    dtype)
+    columns = residual.shape[1]
+    h = x if y is None else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    z = torch.empty(x.shape, dtype=dtype, device=x.device) if pre_norm else None
+    _call(_lib.eps_b200_block_norm, C.byref(args), residual.data_ptr(), x_stride,
+          None if y is None else h.data_ptr(), columns, None if z is None else z.data_ptr(), columns,
+          _stream(residual.device))
+    return h, z
+
+
+def block_norm_backward(dh, dz, h, y=None, gate=None, *, post_weight=None, post_bias=None,
+                        pre_weight=None, pre_bias=None, channel_scale=None, scale: float = 1.0,
+                        kind: str = "rms", activation: str = "sigmoid", epsilon: float = 1e-6,
+                        post_norm: bool = True, pre_norm: bool = True) -> BlockNormGradients:
+    """Gradients of block_norm from those of its outputs, dh and dz (either may be
+    None: no gradient comes that way).  h is the forward's output, the other
+    arguments are the forward's inputs; x itself is not needed.  The statistics are
+    computed again from h and y.  Gradients of x, y and gate have their types,
+    gradients of weights, biases and channel_scale are float32.  Sums over rows are
+    taken in a fixed order."""
+    residual, h_stride = _matrix(h, "h")
+    rows, columns = residual.shape
+    dtype = residual.dtype if y is None else _tensor(y, "y", residual).dtype
+    args, y2, g2 = _block_norm_args(residual, y, gate, post_weight, post_bias, pre_weight, pre_bias,
+                                    channel_scale, scale, kind, activation, epsilon, post_norm, pre_norm,
+                                    dtype)
+    if dz is not None and not pre_norm:
+        _refuse("dz needs pre_norm")
+    dh2, dh_stride = (None, 0) if dh is None else _matrix(dh, "dh", residual, columns, rows)
+    dz2, dz_stride = (None, 0) if dz is None else _matrix(dz, "dz", residual, columns, rows)
+    if dh2 is not None and dh2.dtype != residual.dtype:
+        _refuse("dh has the type of h")
+    if dz2 is not None and dz2.dtype != dtype:
+        _refuse("dz has the type of y")
+    device = residual.device
+    dx = torch.empty(h.shape, dtype=h.dtype, device=device)
+    dy = None if y is None else torch.empty(y.shape, dtype=dtype, device=device)
+    dgate = None if gate is None else torch.empty(gate.shape, dtype=dtype, device=device)
+    post, pre = y is not None and post_norm, pre_norm
+    wanted = [post_weight is not None and post, post_bias is not None and post,
+              channel_scale is not None and y is not None, pre_weight is not None and pre,
+              pre_bias is not None and pre]
+    sums = torch.empty((sum(wanted), columns), dtype=torch.float32, device=device)
+    rest = iter(sums)
+    vectors = [next(rest) if w else None for w in wanted]
+    space = _lib.eps_b200_block_norm_workspace(rows, columns) if any(wanted) else 0
+    workspace = torch.empty(space, dtype=torch.uint8, device=device)
+    ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
+    grads = BlockNormGradientArgs(ptr(dh2), ptr(dz2), residual.data_ptr(), dh_stride, dz_stride, h_stride,
+                                  dx.data_ptr(), ptr(dy), ptr(dgate), columns, columns, columns,
+                                  *[ptr(v) for v in vectors], workspace.data_ptr(), space)
+    _call(_lib.eps_b200_block_norm_backward, C.byref(args), C.byref(grads), _stream(device))
+    return BlockNormGradients(dx, dy, dgate, *vectors)
+
+
+# ------------------------------------------------------------------- routing
+class Routing(NamedTuple):
+    """experts [tokens, top_k] int32, best first; weights [tokens, top_k] float32.
+    Entry token * top_k + slot lies at position[token, slot] of `order`, the entries
+    sorted by expert; expert e owns order[offsets[e]:offsets[e + 1]].  order, position
+    and offsets are None if not asked for."""
+    experts: torch.Tensor
+    weights: torch.Tensor
+    order: torch.Tensor | None
+    position: torch.Tensor | None
+    offsets: torch.Tensor | None
+
+
+def _route_args(logits, stride, top_k, score, renormalise, scale, groups, top_groups):
+    return RouteExperts(logits.device.index, _TYPES[logits.dtype], _choice(_SCORES, score, "score"),
+                        bool(renormalise), logits.shape[1], top_k, groups, top_groups, logits.shape[0],
+                        scale, 0, logits.data_ptr(), stride)
+
+
+def route(logits, top_k: int, *, score: str = "softmax", bias=None, groups: int = 1,
+          top_groups: int | None = None, renormalise: bool = True, scale: float = 1.0,
+          sort: bool = True) -> Routing:
+    """Routes tokens to their top_k experts.
+
+    logits [tokens, experts].  Scores are softmax or sigmoid of the logits; `bias`
+    (float32 [experts]) is added for the ranking alone.  With groups, only experts of
+    the top_groups best of `groups` equal runs are eligible, a group counting the sum
+    of its two best keys.  Weights are the chosen scores, divided by their sum if
+    `renormalise`, times `scale`.  Equal keys go to the lower index; a masked logit
+    is -inf.  At most 1024 experts and top_k 32.  With `sort`, the entries sorted
+    by expert come too."""
+    logits, stride = _matrix(logits, "logits")
+    if min(top_k, groups, groups if top_groups is None else top_groups) <= 0:
+        _refuse("top_k, groups and top_groups are positive")
+    tokens, experts = logits.shape
+    args = _route_args(logits, stride, top_k, score, renormalise, scale, groups,
+                       groups if top_groups is None else top_groups)
+    device = logits.device
+    b = _vector(bias, "bias", logits, experts, torch.float32)
+    chosen = torch.empty((tokens, top_k), dtype=torch.int32, device=device)
+    weights = torch.empty((tokens, top_k), dtype=torch.float32, device=device)
+    if not sort:
+        _call(_lib.eps_b200_route_experts, C.byref(args), b, chosen.data_ptr(), weights.data_ptr(), None, None, None,
+              None, 0, _stream(device))
+        return Routing(chosen, weights, None, None, None)
+    order = torch.empty(tokens * top_k, dtype=torch.int32, device=device)
+    position = torch.empty((tokens, top_k), dtype=torch.int32, device=device)
+    offsets = torch.empty(experts + 1, dtype=torch.int32, device=device)
+    space = _lib.eps_b200_route_experts_workspace(tokens, experts, top_k)
+    workspace = torch.empty(space, dtype=torch.uint8, device=device)
+    # an empty tensor has no address, yet it is asked for
+    _call(_lib.eps_b200_route_experts, C.byref(args), b, chosen.data_ptr(), weights.data_ptr(),
+          order.data_ptr() or offsets.data_ptr(), position.data_ptr() or offsets.data_ptr(), offsets.data_ptr(),
+          workspace.data_ptr(), space, _stream(device))
+    return Routing(chosen, weights, order, position, offsets)
+
+
+def route_backward(logits, experts, dweights, *, score: str = "softmax", renormalise: bool = True,
+                   scale: float = 1.0):
+    """The logits' gradient from that of route's weights, for the experts it chose;
+    the choice itself, the bias and the groups take none."""
+    flat, stride = _matrix(logits, "logits")
+    _tensor(experts, "experts", flat)
+    _tensor(dweights, "dweights", flat)
+    if experts.dim() < 1 or experts.shape[-1] == 0 or experts.dtype != torch.int32 or not experts.is_contiguous():
+        _refuse("experts must be a contiguous int32 tensor, as route gives it")
+    top_k = experts.shape[-1]
+    if experts.numel() != flat.shape[0] * top_k:
+        _refuse("experts and logits have different numbers of tokens")
+    if dweights.dtype != torch.float32 or dweights.numel() != experts.numel() or not dweights.is_contiguous():
+        _refuse("dweights must be contiguous float32, in the shape of experts")
+    args = _route_args(flat, stride, top_k, score, renormalise, scale, 1, 1)
+    out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    _call(_lib.eps_b200_route_experts_backward, C.byref(args), experts.data_ptr(), dweights.data_ptr(), out.data_ptr(),
+          flat.shape[1], _stream(flat.device))
+    return out
+
+
+# ------------------------------------------------------------- 8-bit products
+def _row_index(rows, rows_divisor, like):
+    if rows is None:
+        return None
+    _tensor(rows, "rows", like)
+    if rows.dtype != torch.int32 or rows.dim() != 1 or not rows.is_contiguous():
+        _refuse("rows must be a contiguous int32 vector")
+    if rows_divisor <= 0:
+        _refuse("rows_divisor is positive")
+    return rows.data_ptr()
+
+
+def quantize_rows(x, rows=None, rows_divisor: int = 1):
+    """x [..., inner] in 8-bit integers with one scale a row: (q, scale) with q
+    [n, stride] int8, zeros behind `inner`, and scale [n] float32.  Row r is
+    x[rows[r] // rows_divisor], or x[r] without `rows`."""
+    x, stride = _matrix(x, "x")
+    index = _row_index(rows, rows_divisor, x)
+    n, inner = x.shape[0] if rows is None else rows.shape[0], x.shape[1]
+    padded = _lib.eps_b200_int8_stride(inner)
+    q = torch.empty((n, padded), dtype=torch.int8, device=x.device)
+    scale = torch.empty(n, dtype=torch.float32, device=x.device)
+    _call(_lib.eps_b200_int8_quantize, x.device.index, _TYPES[x.dtype], x.data_ptr(), stride, x.shape[0], inner,
+          index, rows_divisor, n, q.data_ptr(), scale.data_ptr(), _stream(x.device))
+    return q, scale
+
+
+class QuantizedExperts:
+    """The weights of one linear layer, or of one for each of several experts, held
+    in 8-bit integers with a scale for each output channel; laid out once."""
+
+    def __init__(self, weight, scale, bias=None):
+        """weight int8 [experts, channels, inner] (or [channels, inner]), scale and
+        bias float32 [experts, channels]."""
+        _tensor(weight, "weight")
+        if weight.dtype != torch.int8 or weight.dim() not in (2, 3) or 0 in weight.shape:
+            _refuse("weight must be int8 [experts, channels, inner] or [channels, inner]")
+        weight = weight if weight.dim() == 3 else weight[None]
+        self.experts, self.channels, self.inner = weight.shape
+        self.device = weight.device
+        n = self.experts * self.channels
+        for t, what in ((scale, "scale"), (bias, "bias")):
+            _vector(t, what, weight, n, torch.float32)
+        if scale is None:
+            _refuse("the weights need their scales")
+        self.stride = _lib.eps_b200_int8_stride(self.inner)
+        self.weight = torch.zeros((self.experts, self.channels, self.stride), dtype=torch.int8, device=self.device)
+        self.weight[..., : self.inner] = weight
+        self.scale = scale.reshape(self.experts, self.channels)
+        self.bias = None if bias is None else bias.reshape(self.experts, self.channels)
+
+    @classmethod
+    def from_weights(cls, weight, bias=None):
+        """Quantizes weight [experts, channels, inner] (or [channels, inner])."""
+        _tensor(weight, "weight")
+        if weight.dim() not in (2, 3) or 0 in weight.shape:
+            _refuse("weight must be [experts, channels, inner] or [channels, inner]")
+        q, scale = quantize_rows(weight)
+        q = q[:, : weight.shape[-1]].reshape(weight.shape)
+        return cls(q, scale, None if bias is None else bias.float().contiguous())
+
+    def product(self, x, offsets=None, rows=None, rows_divisor: int = 1):
+        """Rows of x [..., inner], each quantized with its own scale, times the
+        weights of their expert: [n, channels] in x's type.
+
+        offsets int32 [experts + 1]: expert e takes rows offsets[e]:offsets[e + 1]
+        (may be left out with one expert).  rows int32 [n]: row r of the product is
+        made from x[rows[r] // rows_divisor] -- a Routing's `order` with rows_divisor
+        = top_k; without it from x[r].  Rows in no expert's run are left unwritten."""
+        flat, stride = _matrix(x, "x", columns=self.inner)
+        if flat.device != self.device:
+            _refuse(f"x is on {flat.device}, not on {self.device}")
+        index = _row_index(rows, rows_divisor, flat)
+        n = flat.shape[0] if rows is None else rows.shape[0]
+        if offsets is not None:
+            _tensor(offsets, "offsets", flat)
+            if offsets.dtype != torch.int32 or offsets.numel() != self.experts + 1 or not offsets.is_contiguous():
+                _refuse("offsets must be a contiguous int32 vector of experts + 1")
+        elif self.experts != 1:
+            _refuse("several experts need offsets")
+        shape = (*x.shape[:-1], self.channels) if rows is None else (n, self.channels)
+        out = torch.empty(shape, dtype=flat.dtype, device=self.device)
+        space = _lib.eps_b200_int8_product_workspace(n, self.experts, self.channels, self.inner)
+        workspace = torch.empty(space, dtype=torch.uint8, device=self.device)
+        args = Int8Product(self.device.index, _TYPES[flat.dtype], self.experts, self.channels, self.inner,
+                           rows_divisor, n, self.weight.data_ptr(), self.scale.data_ptr(),
+                           None if self.bias is None else self.bias.data_ptr(),
+                           None if offsets is None else offsets.data_ptr(), out.data_ptr(), workspace.data_ptr(), space)
+        _call(_lib.eps_b200_int8_linear, C.byref(args), flat.data_ptr(), stride, flat.shape[0], index,
+              _stream(self.device))
+        return out
+
+
+# --------------------------------------------------------------------- AdamW
+class AdamW:
+    """AdamW over many tensors, one launch a step.
+
+        m = beta1 m + (1 - beta1) g,  v = beta2 v + (1 - beta2) g^2
+        p -= learning_rate * (m_hat / (sqrt(v_hat) + epsilon) + weight_decay * p)
+
+    The dense counterpart of the store's LazyAdam: every element moves at every
+    step.  `gradients` are the buffers that step() reads; step(gradients) takes
+    others.  state_bits 32 holds the moments in float32; 8 holds m and sqrt(v) as
+    float8_e4m3fn with a scale for each 256 elements, m rounded to the nearest and
+    sqrt(v) at random (a function of `seed`, the step and the element) so that small
+    changes are right on average.  master=True keeps a float32 copy of 16-bit
+    parameters, which is the one updated.
+
+    The moments lie one tensor after the other in `first` and `second` (and `master`),
+    tensor i from element starts[i] on; `first_scale` and `second_scale` hold the
+    scales of 8-bit moments."""
+
+    def __init__(self, parameters: Sequence[torch.Tensor], gradients: Sequence[torch.Tensor] | None = None, *,
+                 learning_rate: float = 1e-3, beta1: float = 0.9, beta2: float = 0.999,
+                 epsilon: float = 1e-8, weight_decay: float = 0.01, state_bits: int = 32,
+                 master: bool = False, seed: int = 0):
+        self.parameters = list(parameters)
+        if not self.parameters:
+            _refuse("no parameters")
+        head = _tensor(self.parameters[0], "a parameter")
+        if head.dtype not in _TYPES:
+            _refuse("parameters are float32, bfloat16 or float16")
+        for p in self.parameters:
+            _tensor(p, "a parameter", head)
+            if p.dtype != head.dtype or not p.is_contiguous():
+                _refuse("parameters are contiguous and of one type")
+        if state_bits not in (8, 32):
+            _refuse("moments have 32 or 8 bits")
+        if master and head.dtype == torch.float32:
+            _refuse("float32 parameters take no master copy")
+        self.device, self.state_bits, self.steps = head.device, state_bits, 0
+        self.starts, total = [], 0
+        for p in self.parameters:
+            self.starts.append(total)
+            total += -(-p.numel() // ADAMW_BLOCK) * ADAMW_BLOCK
+        state = dict(dtype=torch.float32 if state_bits == 32 else torch.float8_e4m3fn, device=self.device)
+        self.first, self.second = torch.zeros(total, **state), torch.zeros(total, **state)
+        self.first_scale = self.second_scale = self.master = None
+        if state_bits == 8:
+            self.first_scale = torch.zeros(total // ADAMW_BLOCK, device=self.device)
+            self.second_scale = torch.zeros(total // ADAMW_BLOCK, device=self.device)
+        if master:
+            self.master = torch.zeros(total, device=self.device)
+            for p, a in zip(self.parameters, self.starts):
+                self.master[a:a + p.numel()] = p.detach().reshape(-1)
+        ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
+        self._args = AdamWArgs(self.device.index, _TYPES[head.dtype], 0, state_bits, ptr(self.master),
+                               ptr(self.first), ptr(self.second), ptr(self.first_scale), ptr(self.second_scale),
+                               None, None, learning_rate, beta1, beta2, epsilon, weight_decay, 0, seed)
+        self._bound = None
+        if gradients is not None:
+            self.bind(gradients)
+
+    @property
+    def learning_rate(self) -> float:
+        return self._args.learning_rate
+
+    @learning_rate.setter
+    def learning_rate(self, value: float):
+        self._args.learning_rate = value
+
+    def bind(self, gradients: Sequence[torch.Tensor]):
+        """Makes these the buffers that step() reads: their addresses go to the GPU
+        now, their values are read at each step."""
+        gradients = list(gradients)
+        if len(gradients) != len(self.parameters):
+            _refuse("a gradient for each parameter")
+        dtype = gradients[0].dtype if isinstance(gradients[0], torch.Tensor) else None
+        if dtype not in (self.parameters[0].dtype, torch.float32):
+            _refuse("gradients have the parameters' type or float32")
+        tensors = (AdamWTensor * len(gradients))()
+        for i, (p, g, a) in enumerate(zip(self.parameters, gradients, self.starts)):
+            _tensor(g, "a gradient", p)
+            if g.dtype != dtype or g.shape != p.shape or not g.is_contiguous():
+                _refuse("gradients are contiguous, of one type and of the parameters' shapes")
+            tensors[i] = AdamWTensor(p.data_ptr(), g.data_ptr(), p.numel(), a)
+        size = _lib.eps_b200_adamw_plan_bytes(tensors, len(gradients))
+        host = torch.empty(size, dtype=torch.uint8)
+        blocks = C.c_uint64(0)
+        _call(_lib.eps_b200_adamw_plan, tensors, len(gradients), host.data_ptr(), size, C.byref(blocks))
+        plan = host.to(self.device)
+        self._bound = (gradients, plan, blocks.value, _TYPES[dtype])
+
+    def step(self, gradients: Sequence[torch.Tensor] | None = None, *, gradient_scale=None, skip=None):
+        """One step.  gradient_scale: a float32 scalar on the GPU that multiplies
+        every gradient (a clip factor, one over a loss scale).  skip: an int32 scalar
+        on the GPU; where it is not 0 the step changes no parameter and no moment
+        (it still counts as a step)."""
+        if gradients is not None:
+            self.bind(gradients)
+        if self._bound is None:
+            _refuse("no gradients: give them to AdamW, bind or step")
+        _, plan, blocks, gtype = self._bound
+        a = self._args
+        a.gradient_type = gtype
+        a.gradient_scale = _vector(gradient_scale, "gradient_scale", self.first, 1, torch.float32)
+        a.skip = _vector(skip, "skip", self.first, 1, torch.int32)
+        a.step = self.steps + 1
+        _call(_lib.eps_b200_adamw, C.byref(a), plan.data_ptr(), len(self.parameters), blocks, _stream(self.device))
+        self.steps += 1
+
+    def state(self) -> dict:
+        """What load_state takes, by reference."""
+        held = {k: getattr(self, k) for k in ("first", "second", "first_scale", "second_scale", "master")}
+        return {"steps": self.steps, **{k: v for k, v in held.items() if v is not None}}
+
+    def load_state(self, steps: int, **tensors):
+        """Copies moments (and scales, master parameters) of the same layout in, and
+        sets the number of steps taken."""
+        mine = self.state()
+        mine.pop("steps")
+        if steps < 0 or set(tensors) != set(mine):
+            _refuse(f"a state has steps and {', '.join(mine)}")
+        for k, t in tensors.items():
+            if not isinstance(t, torch.Tensor) or t.shape != mine[k].shape or t.dtype != mine[k].dtype:
+                _refuse(f"{k} must be {mine[k].dtype} of {tuple(mine[k].shape)}")
+        for k, t in tensors.items():
+            mine[k].copy_(t)
+        self.steps = steps
+        return self
