@@ -78,7 +78,8 @@ __device__ __forceinline__ void parameter(const void* p, int narrow, unsigned c,
 
 // Mean and reciprocal deviation of a row held as v[NIT][V] by its lanes.  Two
 // passes over the registers for a layer norm: the squares of what is left after
-// the mean cannot cancel.
+// the mean cannot cancel.  A lane divides its own sums by the columns, so that they
+// cannot overflow across lanes where the mean square itself does not.
 template <int V, int NIT>
 __device__ __forceinline__ void statistics(const Norm& n, const float (&v)[NIT][V], unsigned lane, bool live,
                                            float* shared, unsigned& turn, float* mean, float* r) {
@@ -89,8 +90,9 @@ __device__ __forceinline__ void statistics(const Norm& n, const float (&v)[NIT][
     for (int i = 0; i < NIT; ++i)
 #pragma unroll
       for (int j = 0; j < V; ++j) s[0] += v[i][j];     // lanes past the row hold 0
+    s[0] *= n.inverse_columns;
     row_sum<1>(s, n.width, shared, turn);
-    *mean = s[0] * n.inverse_columns;
+    *mean = s[0];
   }
   float s[1] = {0.f};
 #pragma unroll
@@ -102,8 +104,9 @@ __device__ __forceinline__ void statistics(const Norm& n, const float (&v)[NIT][
         s[0] = fmaf(d, d, s[0]);
       }
     }
+  s[0] *= n.inverse_columns;
   row_sum<1>(s, n.width, shared, turn);
-  *r = __frsqrt_rn(fmaf(s[0], n.inverse_columns, n.epsilon));
+  *r = __frsqrt_rn(s[0] + n.epsilon);
 }
 
 template <class TX, class TY, int V, int NIT>
@@ -431,8 +434,9 @@ Norm checked(const EpsB200BlockNorm* a) {
   need(a->rows < (1ull << 40), "too many rows");
   need(a->epsilon > 0.f && a->epsilon < 1e30f, "epsilon must be positive");
   need(a->scale == a->scale, "the scale is not a number");
-  need((a->gate_kind != EPS_B200_GATE_NONE) == (a->gate != nullptr), "gate and gate_kind disagree");
-  need(!a->gate || a->y, "a gate needs a block output");
+  // tensors without rows may have no address
+  need(!a->rows || (a->gate_kind != EPS_B200_GATE_NONE) == (a->gate != nullptr), "gate and gate_kind disagree");
+  need(!a->rows || !a->gate || a->y, "a gate needs a block output");
   Norm n{};
   n.columns = a->columns;
   n.rows = a->rows;
@@ -509,11 +513,12 @@ int eps_b200_block_norm_backward(const EpsB200BlockNorm* a, const EpsB200BlockNo
     Norm n = checked(a);
     need(d, "null gradients");
     need(!d->dz || n.pre_norm, "a gradient of the norm that is not there");
+    const bool y = n.y || !n.rows;
     need(!n.rows || !d->dz || d->h, "the norm's gradient needs h");
-    need((!d->dy && !d->dgate) || n.y, "gradients of a block output that is not there");
+    need((!d->dy && !d->dgate) || y, "gradients of a block output that is not there");
     need(!d->dgate || n.gate != EPS_B200_GATE_NONE, "gradient of a gate that is not there");
-    need((!d->dpost_weight && !d->dpost_bias) || (n.y && n.post_norm), "gradients of a norm that is not there");
-    need(!d->dchannel_scale || n.y, "gradient of a channel scale without a block output");
+    need((!d->dpost_weight && !d->dpost_bias) || (y && n.post_norm), "gradients of a norm that is not there");
+    need(!d->dchannel_scale || y, "gradient of a channel scale without a block output");
     need((!d->dpre_weight && !d->dpre_bias) || n.pre_norm, "gradients of a norm that is not there");
     n.dh = d->dh; n.dhs = d->dh_stride;
     n.dz = d->dz; n.dzs = d->dz_stride;

@@ -2,7 +2,7 @@
 // and channel, rows grouped by expert (eps_b200_int8_quantize, eps_b200_int8_product,
 // eps_b200_int8_linear).
 //
-// Mathematics: q[r, k] = round-half-even(x[r, k] * (127 / amax_r)), scale_r = amax_r / 127;
+// Mathematics: q[r, k] = round-half-even(x[r, k] * (127 * (1 / amax_r))), scale_r = amax_r / 127;
 //   out[r, n] = (sum_k q[r, k] w[e, n, k]) * (scale_r * weight_scale[e, n]) + bias[e, n]
 // with the sum exact in 32-bit integers (inner <= 131072: 127 * 127 * 131072 < 2^31).
 #include <cmath>
@@ -54,7 +54,7 @@ __global__ void __launch_bounds__(256) quantize_rows(const Quantize a) {
   for (int w = 0; w < 8; ++w) top = max(top, tops[w]);
   const float amax = __uint_as_float(top);
   const bool finite = known && top < 0x7F800000u;
-  const float by = finite && amax >= 0x1p-120f ? __fdiv_rn(127.f, amax) : 0.f;
+  const float by = finite && amax >= 0x1p-120f ? __fmul_rn(127.f, __fdiv_rn(1.f, amax)) : 0.f;
   if (threadIdx.x == 0) a.scale[r] = !finite ? NAN : by == 0.f ? 0.f : __fdiv_rn(amax, 127.f);
   int8_t* const q = a.q + r * a.padded;
   auto round = [by](float v) { return by == 0.f ? 0 : __float2int_rn(__fmul_rn(v, by)); };

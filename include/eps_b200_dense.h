@@ -134,10 +134,10 @@ EPS_B200_EXPORT int eps_b200_route_experts_backward(const EpsB200RouteExperts* a
                                                     void* stream, EpsB200Status* status);
 
 /* ---- Matrix products in 8-bit integers, a scale for each token and channel.
- * quantize: q[r, k] = round-half-even(x[row(r), k] * (127 / amax)), scale[r] =
- * amax / 127 with amax = max_k |x[row(r), k]|; row(r) = rows[r] / rows_divisor, or
- * r without `rows`.  q has a row stride of eps_b200_int8_stride(inner) bytes, zeros
- * behind `inner`.  Where 127 / amax would overflow (amax < 2^-120) the row's q and
+ * quantize: q[r, k] = round-half-even(x[row(r), k] * (127 * (1 / amax))) and
+ * scale[r] = amax / 127, every operation rounded to float, with amax =
+ * max_k |x[row(r), k]|; row(r) = rows[r] / rows_divisor, or r without `rows`.  q has a row stride of eps_b200_int8_stride(inner) bytes, zeros
+ * behind `inner`.  Where 1 / amax could overflow (amax < 2^-120) the row's q and
  * scale are 0; a row holding NaN or infinity has a NaN scale; an entry of `rows`
  * outside x counts as such a row. */
 EPS_B200_EXPORT uint64_t eps_b200_int8_stride(uint32_t inner);
