@@ -5,6 +5,8 @@
 // Mathematics: q[r, k] = round-half-even(x[r, k] * (127 * (1 / amax_r))), scale_r = amax_r / 127;
 //   out[r, n] = (sum_k q[r, k] w[e, n, k]) * (scale_r * weight_scale[e, n]) + bias[e, n]
 // with the sum exact in 32-bit integers (inner <= 131072: 127 * 127 * 131072 < 2^31).
+#include <cuda.h>
+
 #include <cmath>
 #include <type_traits>
 
@@ -143,6 +145,235 @@ __global__ void __launch_bounds__(256) product_rows(const Product a, unsigned ch
   }
 }
 
+// ------------------------------------------------ the tensor cores' product
+//
+// A tile is 128 channels x BN rows of one expert: D[channel, row] = W q^T, so the
+// channels lie on the lanes of tensor memory and a store of a warp covers 32
+// neighbouring channels of one output row.  Both operands are K-major int8, 128
+// bytes of inner size a stage, brought by TMA with the 128-byte swizzle that the
+// matrix instruction reads; out-of-range rows and bytes arrive as zeros, and rows of
+// the next expert or channel group, which a ragged tile also covers, are not stored.
+//
+// One block an SM walks the tiles: warp 0 fills the stages, warp 1 issues
+// tcgen05.mma (kind::i8, 32-bit sums in tensor memory), warps 4..7 scale, round and
+// store the tile before while the next is being summed (two halves of tensor memory).
+constexpr int kMmaThreads = 256;
+constexpr unsigned kStageK = 128;          // bytes of inner size a stage
+constexpr unsigned kTileM = 128;           // channels of a tile
+
+template <int BN>
+struct MmaShape {
+  static constexpr unsigned stage_bytes = (kTileM + BN) * kStageK;
+  static constexpr unsigned stages = 196608 / stage_bytes < 8 ? 196608 / stage_bytes : 8;
+  static constexpr unsigned shared = stages * stage_bytes + 1024;      // and room to align
+  static constexpr unsigned columns = 2 * BN;                          // of tensor memory
+};
+
+__device__ __forceinline__ unsigned shared_address(const void* p) { return (unsigned)__cvta_generic_to_shared(p); }
+
+__device__ __forceinline__ void barrier_init(uint64_t* b, unsigned count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(shared_address(b)), "r"(count) : "memory");
+}
+
+__device__ __forceinline__ void barrier_arrive(uint64_t* b) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(shared_address(b)) : "memory");
+}
+
+__device__ __forceinline__ void barrier_expect(uint64_t* b, unsigned bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(shared_address(b)), "r"(bytes) : "memory");
+}
+
+__device__ __forceinline__ uint64_t nanoseconds() {
+  uint64_t t;
+  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+  return t;
+}
+
+// Waits for the phase of this parity to end; false after two seconds, which no
+// working kernel comes near.  The caller then leaves its loop, and the tile's rows
+// become NaN instead of the GPU hanging.
+__device__ __forceinline__ bool barrier_wait(uint64_t* b, unsigned parity) {
+  const unsigned address = shared_address(b);
+  uint64_t start = 0;
+  for (unsigned tries = 1;; ++tries) {
+    unsigned done;
+    asm volatile(
+        "{\n .reg .pred p;\n"
+        " mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+        " selp.u32 %0, 1, 0, p;\n}\n"
+        : "=r"(done) : "r"(address), "r"(parity) : "memory");
+    if (done) return true;
+    if (tries % 256 == 0) {
+      const uint64_t now = nanoseconds();
+      if (!start) start = now;
+      else if (now - start > 2000000000ull) return false;
+    }
+  }
+}
+
+__device__ __forceinline__ void tma_load(void* to, const CUtensorMap* map, uint64_t* barrier, int x, int y) {
+  asm volatile("cp.async.bulk.tensor.2d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+               ::"r"(shared_address(to)), "l"(map), "r"(shared_address(barrier)), "r"(x), "r"(y) : "memory");
+}
+
+// Shared-memory descriptor of a K-major operand in the 128-byte swizzle: rows of 128
+// bytes, groups of eight rows 1024 bytes apart.
+__device__ __forceinline__ uint64_t operand(const void* p) {
+  return (uint64_t)(shared_address(p) >> 4 & 0x3FFF) | 1ull << 16 | (uint64_t)(1024 >> 4) << 32 | 1ull << 46 | 2ull << 61;
+}
+
+template <int BN>
+__device__ __forceinline__ void mma_i8(unsigned d, uint64_t a, uint64_t b, bool accumulate) {
+  // 32-bit signed sums, signed 8-bit operands, both K-major, N = BN, M = 128
+  constexpr unsigned shape = 2u << 4 | 1u << 7 | 1u << 10 | (unsigned)(BN / 8) << 17 | (kTileM / 16) << 24;
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n}\n"
+      ::"r"(d), "l"(a), "l"(b), "r"(shape), "r"((unsigned)accumulate) : "memory");
+}
+
+__device__ __forceinline__ void mma_commit(uint64_t* barrier) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(shared_address(barrier)) : "memory");
+}
+
+// 32 lanes x 32 columns of tensor memory: lane l of the warp gets its 32 columns.
+__device__ __forceinline__ void tensor_load(unsigned address, int (&v)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+        "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]),
+        "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]),
+        "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+      : "r"(address));
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+
+template <class T, int BN>
+__global__ void __launch_bounds__(kMmaThreads, 1)
+    product_tiles(const Product a, const __grid_constant__ CUtensorMap weights, const __grid_constant__ CUtensorMap rows,
+                  unsigned channel_tiles) {
+  using Shape = MmaShape<BN>;
+  extern __shared__ unsigned char raw[];
+  __shared__ uint64_t full[Shape::stages], empty[Shape::stages], summed[2], drained[2];
+  __shared__ unsigned tensor_base;
+  unsigned char* const stages = raw + (1024 - shared_address(raw) % 1024) % 1024;
+  const unsigned warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  if (threadIdx.x == 0) {
+    for (unsigned s = 0; s < Shape::stages; ++s) {
+      barrier_init(full + s, 1);
+      barrier_init(empty + s, 1);
+    }
+    for (int s = 0; s < 2; ++s) {
+      barrier_init(summed + s, 1);
+      barrier_init(drained + s, 4);
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&weights) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&rows) : "memory");
+  }
+  if (warp == 2) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(shared_address(&tensor_base)),
+                 "r"(Shape::columns) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const unsigned base = tensor_base;
+  const unsigned steps = (a.padded + kStageK - 1) / kStageK;
+
+  if (warp == 0) {
+    unsigned stage = 0, phase = 0, filled = 0;
+    bool ok = true;
+    for (unsigned t = blockIdx.x; ok; t += gridDim.x) {
+      const Tile tile = locate(a, BN, t / channel_tiles);
+      if (!tile.rows) break;
+      if (lane == 0) {
+        const int y = (int)(tile.expert * a.channels + t % channel_tiles * kTileM);
+        for (unsigned k = 0; k < steps; ++k) {
+          if (!(ok = barrier_wait(empty + stage, phase ^ 1))) break;
+          unsigned char* const p = stages + stage * Shape::stage_bytes;
+          barrier_expect(full + stage, Shape::stage_bytes);
+          tma_load(p, &weights, full + stage, (int)(k * kStageK), y);
+          tma_load(p + kTileM * kStageK, &rows, full + stage, (int)(k * kStageK), (int)tile.row);
+          if (++filled > Shape::stages) filled = Shape::stages;
+          if (++stage == Shape::stages) { stage = 0; phase ^= 1; }
+        }
+      }
+      ok = __shfl_sync(~0u, ok, 0);
+    }
+    // no block ends with copies into its shared memory in flight
+    if (lane == 0 && !ok)
+      for (unsigned n = 0; n < filled; ++n) {
+        stage = stage ? stage - 1 : Shape::stages - 1;
+        if (stage == Shape::stages - 1) phase ^= 1;
+        barrier_wait(full + stage, phase);
+      }
+  } else if (warp == 1) {
+    unsigned stage = 0, phase = 0, half = 0, turn = 0;
+    bool ok = true;
+    for (unsigned t = blockIdx.x; ok; t += gridDim.x) {
+      if (!locate(a, BN, t / channel_tiles).rows) break;
+      if (lane == 0) {
+        ok = barrier_wait(drained + half, turn ^ 1);
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        for (unsigned k = 0; ok && k < steps; ++k) {
+          if (!(ok = barrier_wait(full + stage, phase))) break;
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          const unsigned char* const p = stages + stage * Shape::stage_bytes;
+          const uint64_t w = operand(p), q = operand(p + kTileM * kStageK);
+#pragma unroll
+          for (unsigned i = 0; i < kStageK / 32; ++i) mma_i8<BN>(base + half * BN, w + 2 * i, q + 2 * i, k || i);
+          mma_commit(empty + stage);
+          if (++stage == Shape::stages) { stage = 0; phase ^= 1; }
+        }
+        if (ok) mma_commit(summed + half);
+      }
+      ok = __shfl_sync(~0u, ok, 0);
+      half ^= 1;
+      turn ^= half == 0;
+    }
+  } else if (warp >= 4) {
+    unsigned half = 0, turn = 0;
+    bool ok = true;
+    for (unsigned t = blockIdx.x; ok; t += gridDim.x) {
+      const Tile tile = locate(a, BN, t / channel_tiles);
+      if (!tile.rows) break;
+      const unsigned n = t % channel_tiles * kTileM + (warp - 4) * 32 + lane;
+      const uint64_t c = (uint64_t)tile.expert * a.channels + n;
+      const bool in = n < a.channels;
+      const float ws = in ? a.weight_scale[c] : 0.f, b = in && a.bias ? a.bias[c] : 0.f;
+      ok = __all_sync(~0u, barrier_wait(summed + half, turn));
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      T* const out = static_cast<T*>(a.out) + (uint64_t)tile.row * a.channels + n;
+#pragma unroll 1
+      for (unsigned r0 = 0; r0 < tile.rows; r0 += 32) {
+        int v[32];
+        tensor_load(base + half * BN + r0 + ((warp - 4) * 32 << 16), v);
+        const float mine = r0 + lane < tile.rows ? a.scale[tile.row + r0 + lane] : 0.f;
+#pragma unroll
+        for (unsigned j = 0; j < 32; ++j) {
+          const float s = __shfl_sync(~0u, mine, j);
+          const float value = ok ? fmaf((float)v[j], s * ws, b) : NAN;
+          if (in && r0 + j < tile.rows) out[(uint64_t)(r0 + j) * a.channels] = from_float<T>(value);
+        }
+      }
+      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) barrier_arrive(drained + half);
+      half ^= 1;
+      turn ^= half == 0;
+    }
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  if (warp == 2)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(base), "r"(Shape::columns) : "memory");
+}
+
 template <class F>
 void by_type(int type, F f) {
   if (type == EPS_B200_F32) f(float{});
@@ -156,13 +387,72 @@ void quantize(int type, const Quantize& a, cudaStream_t stream) {
   check(cudaGetLastError(), "int8_quantize");
 }
 
-void product(int type, const Product& a, cudaStream_t stream) {
-  const unsigned channel_blocks = (unsigned)ceil_div(a.channels, 8);
-  const uint64_t tiles = ceil_div(a.rows, 8) + (a.offsets ? a.experts - 1 : 0);
-  need(tiles * channel_blocks < (1ull << 31), "too many rows");
+using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                            const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                            CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+// The driver's encoder, asked for once.
+Encode encoder() {
+  static const Encode found = [] {
+    void* fn = nullptr;
+    cudaDriverEntryPointQueryResult q{};
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q) != cudaSuccess ||
+        q != cudaDriverEntryPointSuccess)
+      fn = nullptr;
+    return reinterpret_cast<Encode>(fn);
+  }();
+  if (!found) throw Fail(EPS_B200_UNAVAILABLE, "the driver offers no cuTensorMapEncodeTiled");
+  return found;
+}
+
+// A matrix of `rows` rows of `padded` bytes in boxes of box_rows x 128 bytes.
+CUtensorMap tensor_map(const void* p, uint64_t rows, unsigned padded, unsigned box_rows) {
+  CUtensorMap m;
+  const cuuint64_t dims[2] = {padded, rows}, strides[1] = {padded};
+  const cuuint32_t box[2] = {kStageK, box_rows}, step[2] = {1, 1};
+  const CUresult r = encoder()(&m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(p), dims, strides, box, step,
+                               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) throw Fail(EPS_B200_RUN_FAILED, "cuTensorMapEncodeTiled failed");
+  return m;
+}
+
+// Upper bound of the tiles of `tile_rows` rows that the groups make.
+uint64_t tile_bound(const Product& a, unsigned tile_rows) {
+  const uint64_t extra = a.offsets ? (a.experts < a.rows ? a.experts : a.rows) - 1 : 0;
+  return ceil_div(a.rows, tile_rows) + extra;
+}
+
+template <int BN>
+void tiles(int type, const Product& a, unsigned sms, cudaStream_t stream) {
+  using Shape = MmaShape<BN>;
+  const CUtensorMap w = tensor_map(a.weight, (uint64_t)a.experts * a.channels, a.padded, kTileM);
+  const CUtensorMap q = tensor_map(a.q, a.rows, a.padded, BN);
+  const unsigned channel_tiles = (unsigned)ceil_div(a.channels, kTileM);
+  const uint64_t most = tile_bound(a, BN) * channel_tiles;
+  need(most < (1ull << 31), "too many rows");
   by_type(type, [&](auto t) {
-    product_rows<decltype(t), 8><<<(unsigned)(tiles * channel_blocks), 256, 0, stream>>>(a, channel_blocks);
+    auto* kernel = product_tiles<decltype(t), BN>;
+    check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Shape::shared), "cudaFuncSetAttribute");
+    kernel<<<(unsigned)(most < sms ? most : sms), kMmaThreads, Shape::shared, stream>>>(a, w, q, channel_tiles);
   });
+  check(cudaGetLastError(), "int8_product");
+}
+
+void product(int type, const Product& a, unsigned sms, cudaStream_t stream) {
+  const uint64_t each = ceil_div(a.rows, a.experts);      // rows of an expert, on average
+  if (a.rows > 8 && each > 2) {
+    need((uint64_t)a.experts * a.channels < (1ull << 31), "too many channels");
+    if (each > 128) tiles<256>(type, a, sms, stream);
+    else if (each > 64) tiles<128>(type, a, sms, stream);
+    else if (each > 32) tiles<64>(type, a, sms, stream);
+    else tiles<32>(type, a, sms, stream);
+    return;
+  }
+  const unsigned channel_blocks = (unsigned)ceil_div(a.channels, 8);
+  const uint64_t most = tile_bound(a, 8) * channel_blocks;
+  need(most < (1ull << 31), "too many rows");
+  by_type(type, [&](auto t) { product_rows<decltype(t), 8><<<(unsigned)most, 256, 0, stream>>>(a, channel_blocks); });
   check(cudaGetLastError(), "int8_product");
 }
 
@@ -236,7 +526,7 @@ int eps_b200_int8_product(const EpsB200Int8Product* a, const int8_t* q, const fl
     p.q = q;
     p.scale = scale;
     OnDevice on(a->device);
-    product(a->type, p, static_cast<cudaStream_t>(stream));
+    product(a->type, p, sm_count(a->device), static_cast<cudaStream_t>(stream));
   });
 }
 
@@ -255,7 +545,7 @@ int eps_b200_int8_linear(const EpsB200Int8Product* a, const void* x, int64_t x_s
     OnDevice on(a->device);
     const auto st = static_cast<cudaStream_t>(stream);
     quantize(a->type, z, st);
-    product(a->type, p, st);
+    product(a->type, p, sm_count(a->device), st);
   });
 }
 
