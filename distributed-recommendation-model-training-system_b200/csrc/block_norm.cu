@@ -38,25 +38,62 @@ struct Norm {
   int64_t out_hs, out_zs, dxs, dys, dgs;
   float* partial;                  // [blocks][5][columns]
   int want;                        // bit i: column sum i is wanted
+  const void* somewhere;           // 16-byte aligned device memory, for copies of nothing
 };
 
 // The column sums of the backward pass, in this order in `partial`.
 enum { kPostWeight, kPostBias, kChannel, kPreWeight, kPreBias, kSums };
 
-__device__ __forceinline__ float sigmoid(float v) { return __fdividef(1.f, 1.f + __expf(-v)); }
+// 1 / (1 + 2^(-g log2 e)): two instructions of the special-function unit, each good
+// to two units of the last place; subnormal powers count as 0, which 1 + hides.
+template <int V>
+__device__ __forceinline__ void sigmoid(const float (&g)[V], float (&s)[V]) {
+  vmul<V>(s, g, -1.4426950408889634f);
+#pragma unroll
+  for (int j = 0; j < V; ++j) asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(s[j]));
+  vadd<V>(s, s, 1.f);
+#pragma unroll
+  for (int j = 0; j < V; ++j) asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(s[j]));
+}
 
-// act(g) and its derivative.
-__device__ __forceinline__ float activate(float g, int activation, float* slope) {
-  if (activation == EPS_B200_ACT_NONE) { *slope = 1.f; return g; }
-  if (activation == EPS_B200_ACT_TANH) {
-    const float t = tanhf(g);
-    *slope = fmaf(-t, t, 1.f);
-    return t;
+// act(g) and, where SLOPE, its derivative for V values; the choice is made once for
+// all of them.
+template <int V, bool SLOPE>
+__device__ __forceinline__ void activate(const float (&g)[V], int activation, float (&a)[V], float (&slope)[V]) {
+  if (activation == EPS_B200_ACT_SIGMOID) {
+    sigmoid<V>(g, a);
+    if (SLOPE) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) slope[j] = fmaf(-a[j], a[j], a[j]);
+    }
+  } else if (activation == EPS_B200_ACT_SILU) {
+    float s[V];
+    sigmoid<V>(g, s);
+    vmul<V>(a, g, s);
+    if (SLOPE) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) slope[j] = fmaf(a[j], 1.f - s[j], s[j]);
+    }
+  } else if (activation == EPS_B200_ACT_TANH) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      a[j] = tanhf(g[j]);
+      slope[j] = fmaf(-a[j], a[j], 1.f);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      a[j] = g[j];
+      slope[j] = 1.f;
+    }
   }
-  const float s = sigmoid(g);
-  if (activation == EPS_B200_ACT_SIGMOID) { *slope = s * (1.f - s); return s; }
-  *slope = s * fmaf(g, 1.f - s, 1.f);
-  return g * s;
+}
+
+__device__ __forceinline__ float activate_one(float g, int activation, float* slope) {
+  float v[1] = {g}, a[1], s[1];
+  activate<1, true>(v, activation, a, s);
+  *slope = s[0];
+  return a[0];
 }
 
 // A parameter vector's V elements from column c on, `missing` where there is none.
@@ -66,270 +103,502 @@ __device__ __forceinline__ void parameter(const void* p, int narrow, unsigned c,
 #pragma unroll
     for (int i = 0; i < V; ++i) r[i] = missing;
   } else if (narrow) {
-    const Pack<T, V> k = load_pack<T, V>(static_cast<const T*>(p) + c);
-#pragma unroll
-    for (int i = 0; i < V; ++i) r[i] = to_float(k.v[i]);
+    widen(load_pack<T, V>(static_cast<const T*>(p) + c), r);
   } else {
-    const Pack<float, V> k = load_pack<float, V>(static_cast<const float*>(p) + c);
-#pragma unroll
-    for (int i = 0; i < V; ++i) r[i] = k.v[i];
+    widen(load_pack<float, V>(static_cast<const float*>(p) + c), r);
   }
 }
 
-// Mean and reciprocal deviation of a row held as v[NIT][V] by its lanes.  Two
-// passes over the registers for a layer norm: the squares of what is left after
-// the mean cannot cancel.  A lane divides its own sums by the columns, so that they
-// cannot overflow across lanes where the mean square itself does not.
-template <int V, int NIT>
-__device__ __forceinline__ void statistics(const Norm& n, const float (&v)[NIT][V], unsigned lane, bool live,
-                                           float* shared, unsigned& turn, float* mean, float* r) {
-  *mean = 0.f;
-  if (n.layer) {
-    float s[1] = {0.f};
-#pragma unroll
-    for (int i = 0; i < NIT; ++i)
-#pragma unroll
-      for (int j = 0; j < V; ++j) s[0] += v[i][j];     // lanes past the row hold 0
-    s[0] *= n.inverse_columns;
-    row_sum<1>(s, n.width, shared, turn);
-    *mean = s[0];
-  }
-  float s[1] = {0.f};
-#pragma unroll
-  for (int i = 0; i < NIT; ++i)
-    if (live && (i * n.width + lane) * V < n.columns) {
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const float d = v[i][j] - *mean;
-        s[0] = fmaf(d, d, s[0]);
-      }
+// The parameter vectors as a lane uses them.  Where a lane has few columns, a block
+// lays its lanes' values out in shared memory once, in float and with what is missing
+// filled in: rows then read them without a branch and without a bank conflict.
+enum { kPostW, kPostB, kScaleC, kPreW, kPreB, kVectors };
+
+template <class T, int V, int NIT, bool STAGED>
+struct Parameters {
+  const Norm& n;
+  float* staged;           // [kVectors][NIT][V / 4][blockDim.x][4], or [kVectors][NIT][blockDim.x] for V == 1
+  unsigned lane;
+
+  __device__ __forceinline__ float* at(int k, int i) const { return staged + (unsigned)((k * NIT + i) * V) * blockDim.x + threadIdx.x * (V < 4 ? V : 4); }
+  __device__ __forceinline__ void read(int k, int i, float (&r)[V]) const {
+    const unsigned c = (i * n.width + lane) * V;
+    switch (k) {
+      case kPostW: parameter<T, V>(n.post_w, n.narrow, c, 1.f, r); break;
+      case kPostB: parameter<T, V>(n.post_b, n.narrow, c, 0.f, r); break;
+      case kScaleC: parameter<T, V>(n.channel, n.narrow, c, 1.f, r); vmul<V>(r, r, n.scale); break;
+      case kPreW: parameter<T, V>(n.pre_w, n.narrow, c, 1.f, r); break;
+      default: parameter<T, V>(n.pre_b, n.narrow, c, 0.f, r);
     }
-  s[0] *= n.inverse_columns;
-  row_sum<1>(s, n.width, shared, turn);
-  *r = __frsqrt_rn(s[0] + n.epsilon);
-}
-
-template <class TX, class TY, int V, int NIT>
-__global__ void __launch_bounds__(V == 8 ? 512 : 1024) block_norm_forward(const Norm n) {
-  __shared__ float shared[kRowSumShared];
-  unsigned turn = 0;
-  const unsigned lane = threadIdx.x % n.width;
-  const uint64_t row = (uint64_t)blockIdx.x * (blockDim.x / n.width) + threadIdx.x / n.width;
-  const bool live = row < n.rows;
-  const TY* const y = static_cast<const TY*>(n.y);
-  Pack<TY, V> gate[NIT];
-  Pack<TX, V> x[NIT];
-  float v[NIT][V];
-#pragma unroll
-  for (int i = 0; i < NIT; ++i) {
-    const unsigned c = (i * n.width + lane) * V;
-    const bool in = live && c < n.columns;
-    Pack<TY, V> k{};
-    if (in && y) k = load_once<TY, V>(y + row * n.ys + c);
-    if (in && y && n.gate == EPS_B200_GATE_ELEMENT) gate[i] = load_once<TY, V>(static_cast<const TY*>(n.g) + row * n.gs + c);
-    if (in) x[i] = load_once<TX, V>(static_cast<const TX*>(n.x) + row * n.xs + c);
-#pragma unroll
-    for (int j = 0; j < V; ++j) v[i][j] = to_float(k.v[j]);
   }
-  float mean = 0.f, r = 1.f, row_gate = 1.f, slope;
-  if (y && n.post_norm) statistics<V, NIT>(n, v, lane, live, shared, turn, &mean, &r);
-  if (y && live && n.gate == EPS_B200_GATE_ROW)
-    row_gate = activate(to_float(static_cast<const TY*>(n.g)[row]), n.activation, &slope);
+  __device__ __forceinline__ void stage() const {
+    if constexpr (STAGED) {
 #pragma unroll
-  for (int i = 0; i < NIT; ++i) {
-    const unsigned c = (i * n.width + lane) * V;
-    if (!live || c >= n.columns) continue;
-    if (!y) {
+      for (int k = 0; k < kVectors; ++k)
 #pragma unroll
-      for (int j = 0; j < V; ++j) v[i][j] = to_float(x[i].v[j]);
+        for (int i = 0; i < NIT; ++i) {
+          float r[V] = {};          // 0 behind the last column: what a lane holds there adds nothing
+          if ((i * n.width + lane) * V < n.columns) read(k, i, r);
+#pragma unroll
+          for (int j = 0; j < V; j += 4) {
+            if constexpr (V >= 4) *reinterpret_cast<float4*>(at(k, i) + j * blockDim.x) = make_float4(r[j], r[j + 1], r[j + 2], r[j + 3]);
+            else *at(k, i) = r[0];
+          }
+        }
+      // each thread reads back its own values only: no barrier
+    }
+  }
+  __device__ __forceinline__ void get(int k, int i, float (&r)[V]) const {
+    if constexpr (STAGED) {
+#pragma unroll
+      for (int j = 0; j < V; j += 4) {
+        if constexpr (V >= 4) {
+          const float4 x = *reinterpret_cast<const float4*>(at(k, i) + j * blockDim.x);
+          r[j] = x.x; r[j + 1] = x.y; r[j + 2] = x.z; r[j + 3] = x.w;
+        } else {
+          r[0] = *at(k, i);
+        }
+      }
     } else {
-      float w[V], b[V], s[V];
-      if (n.post_norm) {
-        parameter<TY, V>(n.post_w, n.narrow, c, 1.f, w);
-        parameter<TY, V>(n.post_b, n.narrow, c, 0.f, b);
-      }
-      parameter<TY, V>(n.channel, n.narrow, c, 1.f, s);
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        float u = n.post_norm ? fmaf((v[i][j] - mean) * r, w[j], b[j]) : v[i][j];
-        if (n.gate == EPS_B200_GATE_ROW) u *= row_gate;
-        else if (n.gate == EPS_B200_GATE_ELEMENT) u *= activate(to_float(gate[i].v[j]), n.activation, &slope);
-        v[i][j] = fmaf(n.scale * s[j], u, to_float(x[i].v[j]));
-      }
-    }
-    if (n.out_h) {
-      Pack<TX, V> o;
-#pragma unroll
-      for (int j = 0; j < V; ++j) o.v[j] = from_float<TX>(v[i][j]);
-      store_pack<TX, V>(static_cast<TX*>(n.out_h) + row * n.out_hs + c, o);
+      for (int j = 0; j < V; ++j) r[j] = 0.f;
+      if ((i * n.width + lane) * V < n.columns) read(k, i, r);
     }
   }
-  if (!n.pre_norm) return;
-  statistics<V, NIT>(n, v, lane, live, shared, turn, &mean, &r);
+};
+
+template <int V>
+__device__ __forceinline__ float total(const float (&v)[V]) {
+  if constexpr (V == 8) {
+    float a[4] = {v[0], v[1], v[2], v[3]}, b[4] = {v[4], v[5], v[6], v[7]};
+    vadd<4>(a, a, b);
+    float c[2] = {a[0], a[1]}, d[2] = {a[2], a[3]};
+    vadd<2>(c, c, d);
+    return c[0] + c[1];
+  } else {
+    float s = v[0];
 #pragma unroll
-  for (int i = 0; i < NIT; ++i) {
-    const unsigned c = (i * n.width + lane) * V;
-    if (!live || c >= n.columns) continue;
-    float w[V], b[V];
-    parameter<TY, V>(n.pre_w, n.narrow, c, 1.f, w);
-    parameter<TY, V>(n.pre_b, n.narrow, c, 0.f, b);
-    Pack<TY, V> o;
-#pragma unroll
-    for (int j = 0; j < V; ++j) o.v[j] = from_float<TY>(fmaf((v[i][j] - mean) * r, w[j], b[j]));
-    store_pack<TY, V>(static_cast<TY*>(n.out_z) + row * n.out_zs + c, o);
+    for (int j = 1; j < V; ++j) s += v[j];
+    return s;
   }
 }
 
-// One block walks rows blockIdx, blockIdx + grid, ... and keeps the column sums of
-// its lanes in shared memory (each lane its own columns: no conflict, no atomic);
-// they leave it once, and block_norm_columns adds them up in block order.
+// Means and reciprocal deviations of K rows held by the same lanes.  Two passes over
+// the registers for a layer norm: the squares of what is left after the mean cannot
+// cancel.  A lane divides its own sums by the columns, so that they cannot overflow
+// across lanes where the mean square itself does not.
+template <int V, int NIT, int K>
+__device__ __forceinline__ void statistics(const Norm& n, const float (*const (&v)[K])[V], unsigned lane, float* shared,
+                                           unsigned& turn, float (&mean)[K], float (&r)[K]) {
+  float s[K];
+#pragma unroll
+  for (int k = 0; k < K; ++k) mean[k] = 0.f;
+  if (n.layer) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      s[k] = 0.f;
+#pragma unroll
+      for (int i = 0; i < NIT; ++i) s[k] += total<V>(v[k][i]);     // lanes past the row hold 0
+      s[k] *= n.inverse_columns;
+    }
+    row_sum<K>(s, n.width, shared, turn);
+#pragma unroll
+    for (int k = 0; k < K; ++k) mean[k] = s[k];
+  }
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    s[k] = 0.f;
+#pragma unroll
+    for (int i = 0; i < NIT; ++i) {
+      float d[V];
+      vadd<V>(d, v[k][i], -mean[k]);
+      vmul<V>(d, d, d);
+      s[k] = fmaf(total<V>(d), (i * n.width + lane) * V < n.columns ? n.inverse_columns : 0.f, s[k]);
+    }
+  }
+  row_sum<K>(s, n.width, shared, turn);
+#pragma unroll
+  for (int k = 0; k < K; ++k) r[k] = __frsqrt_rn(s[k] + n.epsilon);
+}
+
+template <int V, int NIT>
+__device__ __forceinline__ void one_row(const Norm& n, const float (&v)[NIT][V], unsigned lane, float* shared, unsigned& turn,
+                                        float* mean, float* r) {
+  const float(*const rows[1])[V] = {v};
+  float m[1], d[1];
+  statistics<V, NIT, 1>(n, rows, lane, shared, turn, m, d);
+  *mean = m[0];
+  *r = d[0];
+}
+
+// (v - mean) * r: the difference first, since v r and mean r may both be large.
+template <int V>
+__device__ __forceinline__ void centre(float (&v)[V], float mean, float r) {
+  vadd<V>(v, v, -mean);
+  vmul<V>(v, v, r);
+}
+
+// The rows of R tensors on their way into shared memory.  Blocks walk the rows, and
+// a lane asks for its own values two rows ahead, past registers and L1: the
+// reductions and barriers of a row then pass while its successors are under way.  A
+// lane reads back only what it asked for itself, so no barrier is involved; lanes
+// behind the row's end, rows behind the last one and missing tensors read zeros.
+// Without 16-byte alignment, or with more than eight elements a lane, values are
+// loaded as they are needed.
+constexpr unsigned kAhead = 2, kSlots = kAhead + 1;
+
+__device__ __forceinline__ void copy16(unsigned to, const void* from, bool there) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(there ? 16 : 0) : "memory");
+}
+
+template <class T, int V, int NIT, bool RING>
+struct Source {
+  const T* p;              // the tensor at the lane's first column, or NULL
+  int64_t stride;
+  unsigned to;             // RING: the lane's place in slot 0, a shared address; 16-byte planes blockDim.x apart
+  static constexpr unsigned kPlanes = V * sizeof(T) / 16;
+
+  __device__ __forceinline__ void ask(const Norm& n, unsigned slot, unsigned slot_bytes, uint64_t row, bool in) const {
+    static_assert(!RING || NIT == 1, "one pack a lane");
+    const bool there = in && p;
+    const char* const from = reinterpret_cast<const char*>(there ? p + row * stride : static_cast<const T*>(n.somewhere));
+#pragma unroll
+    for (unsigned k = 0; k < kPlanes; ++k) copy16(to + slot * slot_bytes + k * blockDim.x * 16, from + (there ? k * 16 : 0), there);
+  }
+  __device__ __forceinline__ void get(const Norm& n, unsigned slot, unsigned slot_bytes, uint64_t row, bool live, unsigned lane,
+                                      float (&r)[NIT][V]) const {
+    if constexpr (RING) {
+      Pack<T, V> x;
+#pragma unroll
+      for (unsigned k = 0; k < kPlanes; ++k) {
+        uint4& q = reinterpret_cast<uint4*>(&x)[k];
+        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(q.x), "=r"(q.y), "=r"(q.z), "=r"(q.w) : "r"(to + slot * slot_bytes + k * blockDim.x * 16) : "memory");
+      }
+      widen(x, r[0]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < NIT; ++i) {
+        Pack<T, V> x{};
+        if (live && p && (i * n.width + lane) * V < n.columns) x = load_once<T, V>(p + row * stride + i * n.width * V);
+        widen(x, r[i]);
+      }
+    }
+  }
+};
+
+template <class T, int V, int NIT>
+__device__ __forceinline__ void put(const Norm& n, void* p, int64_t stride, uint64_t row, int i, unsigned lane, bool live, const float (&v)[V]) {
+  const unsigned c = (i * n.width + lane) * V;
+  if (live && c < n.columns) store_pack<T, V>(static_cast<T*>(p) + row * stride + c, narrow<T, V>(v));
+}
+
 template <class TX, class TY, int V, int NIT>
-__global__ void __launch_bounds__(V == 8 ? 512 : 1024) block_norm_gradient(const Norm n) {
-  extern __shared__ float sums[];          // [wanted][NIT][V][blockDim.x]
+struct ForwardSources {
+  static constexpr bool kRing = V == 8 && NIT == 1;
+  Source<TX, V, NIT, kRing> x;
+  Source<TY, V, NIT, kRing> y, gate;
+  static constexpr unsigned kSlot = V * (sizeof(TX) + 2 * sizeof(TY));     // bytes of a lane
+};
+template <class TX, class TY, int V, int NIT>
+struct BackwardSources {
+  static constexpr bool kRing = V == 8 && NIT == 1;
+  Source<TX, V, NIT, kRing> dh, h;
+  Source<TY, V, NIT, kRing> dz, y, gate;
+  static constexpr unsigned kSlot = V * (2 * sizeof(TX) + 3 * sizeof(TY));
+};
+
+template <class T>
+__device__ __forceinline__ const T* column(const void* p, unsigned c) {
+  return p ? static_cast<const T*>(p) + c : nullptr;
+}
+
+template <class TX, class TY, int V, int NIT, int GATE>
+__global__ void __launch_bounds__(V == 8 ? 512 : 1024) block_norm_forward(const Norm n) {
+  using Sources = ForwardSources<TX, TY, V, NIT>;
+  constexpr bool kRing = Sources::kRing, kStaged = V * NIT <= 8;
+  extern __shared__ __align__(16) float room[];      // the staged parameters, then the ring
   __shared__ float shared[kRowSumShared];
   unsigned turn = 0;
   const unsigned lane = threadIdx.x % n.width, groups = blockDim.x / n.width;
-  const TY* const y = static_cast<const TY*>(n.y);
-  const unsigned cell = NIT * V * blockDim.x;
-  int slot[kSums];
-  int wanted = 0;
-#pragma unroll
-  for (int k = 0; k < kSums; ++k) slot[k] = n.want >> k & 1 ? wanted++ : -1;
-  for (unsigned i = threadIdx.x; i < wanted * cell; i += blockDim.x) sums[i] = 0.f;
-  __syncthreads();
-  auto add = [&](int k, int i, int j, float value) {
-    if (slot[k] >= 0) sums[slot[k] * cell + (i * V + j) * blockDim.x + threadIdx.x] += value;
+  const uint64_t stride = (uint64_t)gridDim.x * groups;
+  uint64_t row = (uint64_t)blockIdx.x * groups + threadIdx.x / n.width;
+  const uint64_t passes = (n.rows - (uint64_t)blockIdx.x * groups + stride - 1) / stride;   // blocks do not outnumber groups of rows
+  const bool in = lane * V < n.columns;
+  const unsigned ring = shared_at(room + (kStaged ? kVectors * NIT * V * blockDim.x : 0)) + threadIdx.x * 16;
+  const unsigned slot_bytes = Sources::kSlot * blockDim.x;
+  const Sources s{{column<TX>(n.x, lane * V), n.xs, ring},
+                  {column<TY>(n.y, lane * V), n.ys, ring + V * (unsigned)sizeof(TX) * blockDim.x},
+                  {column<TY>(GATE == EPS_B200_GATE_ELEMENT ? n.g : nullptr, lane * V), n.gs,
+                   ring + V * (unsigned)(sizeof(TX) + sizeof(TY)) * blockDim.x}};
+  auto ask = [&](unsigned slot, uint64_t r) {
+    if constexpr (kRing) {
+      const bool there = in && r < n.rows;
+      s.x.ask(n, slot, slot_bytes, r, there);
+      s.y.ask(n, slot, slot_bytes, r, there);
+      if (GATE == EPS_B200_GATE_ELEMENT) s.gate.ask(n, slot, slot_bytes, r, there);
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    }
   };
-
-  for (uint64_t base = (uint64_t)blockIdx.x * groups; base < n.rows; base += (uint64_t)gridDim.x * groups) {
-    const uint64_t row = base + threadIdx.x / n.width;
+#pragma unroll
+  for (unsigned k = 0; k < kAhead; ++k) ask(k, row + k * stride);
+  const Parameters<TY, V, NIT, kStaged> p{n, room, lane};
+  p.stage();
+  unsigned slot = 0;
+  for (uint64_t pass = 0; pass < passes; ++pass, row += stride) {
     const bool live = row < n.rows;
-    Pack<TY, V> gate[NIT];
-    float d[NIT][V], q[NIT][V], h[NIT][V], v[NIT][V];     // dh, dz, h, y
+    float v[NIT][V], x[NIT][V], g[NIT][V];
+    if constexpr (kRing) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(kAhead - 1) : "memory");
+      ask(slot == 0 ? kSlots - 1 : slot - 1, row + kAhead * stride);
+    }
+    s.y.get(n, slot, slot_bytes, row, live, lane, v);
+    float mean = 0.f, r = 1.f, row_gate = 1.f, unused;
+    if (n.y && n.post_norm) one_row<V, NIT>(n, v, lane, shared, turn, &mean, &r);
+    s.x.get(n, slot, slot_bytes, row, live, lane, x);
+    if (GATE == EPS_B200_GATE_ELEMENT) s.gate.get(n, slot, slot_bytes, row, live, lane, g);
+    slot = slot == kSlots - 1 ? 0 : slot + 1;
+    if (GATE == EPS_B200_GATE_ROW && live) row_gate = activate_one(to_float(static_cast<const TY*>(n.g)[row]), n.activation, &unused);
 #pragma unroll
     for (int i = 0; i < NIT; ++i) {
-      const unsigned c = (i * n.width + lane) * V;
-      const bool in = live && c < n.columns;
-      Pack<TX, V> kd{}, kh{};
-      Pack<TY, V> kq{}, ky{};
-      if (in && n.dh) kd = load_once<TX, V>(static_cast<const TX*>(n.dh) + row * n.dhs + c);
-      if (in && n.dz) kq = load_once<TY, V>(static_cast<const TY*>(n.dz) + row * n.dzs + c);
-      if (in && n.dz) kh = load_once<TX, V>(static_cast<const TX*>(n.h) + row * n.hs + c);
-      if (in && y) ky = load_once<TY, V>(y + row * n.ys + c);
-      gate[i] = Pack<TY, V>{};
-      if (in && y && n.gate == EPS_B200_GATE_ELEMENT) gate[i] = load_once<TY, V>(static_cast<const TY*>(n.g) + row * n.gs + c);
+      if (!n.y) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[i][j] = x[i][j];
+      } else {
+        float w[V], b[V];
+        if (n.post_norm) {
+          p.get(kPostW, i, w);
+          p.get(kPostB, i, b);
+          centre<V>(v[i], mean, r);
+          vfma<V>(v[i], v[i], w, b);
+        }
+        if (GATE == EPS_B200_GATE_ELEMENT) {
+          float a[V], slope[V];
+          activate<V, false>(g[i], n.activation, a, slope);
+          vmul<V>(v[i], v[i], a);
+        }
+        p.get(kScaleC, i, w);
+        if (GATE == EPS_B200_GATE_ROW) vmul<V>(w, w, row_gate);
+        vfma<V>(v[i], w, v[i], x[i]);
+      }
+      if (n.out_h) put<TX, V, NIT>(n, n.out_h, n.out_hs, row, i, lane, live, v[i]);
+    }
+    if (!n.pre_norm) continue;
+    one_row<V, NIT>(n, v, lane, shared, turn, &mean, &r);
+#pragma unroll
+    for (int i = 0; i < NIT; ++i) {
+      float w[V], b[V];
+      p.get(kPreW, i, w);
+      p.get(kPreB, i, b);
+      centre<V>(v[i], mean, r);
+      vfma<V>(v[i], v[i], w, b);
+      put<TY, V, NIT>(n, n.out_z, n.out_zs, row, i, lane, live, v[i]);
+    }
+  }
+}
+
+// The column sums of a lane stay in registers where a lane has few columns, else in
+// shared memory (each lane its own columns: no conflict, no atomic).  They leave a
+// block once; block_norm_columns adds the blocks up in order.
+template <class TX, class TY, int V, int NIT, int GATE>
+__global__ void __launch_bounds__(V == 8 ? 512 : 1024) block_norm_gradient(const Norm n) {
+  using Sources = BackwardSources<TX, TY, V, NIT>;
+  constexpr int N = V * NIT;
+  constexpr bool kRing = Sources::kRing, kHeld = kRing;
+  extern __shared__ __align__(16) float room[];     // [wanted][N][blockDim.x] sums; before them staged parameters and the ring
+  __shared__ float shared[kRowSumShared];
+  unsigned turn = 0;
+  const unsigned lane = threadIdx.x % n.width, groups = blockDim.x / n.width;
+  const unsigned cell = N * blockDim.x;
+  int slot_of[kSums];
+  int wanted = 0;
+#pragma unroll
+  for (int k = 0; k < kSums; ++k) slot_of[k] = n.want >> k & 1 ? wanted++ : -1;
+  float held[kHeld ? kSums : 1][V];
+  if constexpr (kHeld) {
+#pragma unroll
+    for (int k = 0; k < kSums; ++k)
+#pragma unroll
+      for (int j = 0; j < V; ++j) held[k][j] = 0.f;
+  } else {
+    for (unsigned i = threadIdx.x; i < wanted * cell; i += blockDim.x) room[i] = 0.f;
+    __syncthreads();
+  }
+  // column sums k of the lane's pack i grow by a * b, or by a
+  auto add = [&](int k, int i, const auto& a, const auto& b) {
+    if constexpr (kHeld) {
+      if constexpr (std::is_same_v<std::decay_t<decltype(b)>, float>) vadd<V>(held[k], held[k], a);
+      else vfma<V>(held[k], a, b, held[k]);
+    } else if (slot_of[k] >= 0) {
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        d[i][j] = to_float(kd.v[j]);
-        q[i][j] = to_float(kq.v[j]);
-        h[i][j] = to_float(kh.v[j]);
-        v[i][j] = to_float(ky.v[j]);
+        float* const s = room + slot_of[k] * cell + (i * V + j) * blockDim.x + threadIdx.x;
+        *s = fmaf(part<V>(a, j), part<V>(b, j), *s);
       }
     }
+  };
+
+  const uint64_t stride = (uint64_t)gridDim.x * groups;
+  uint64_t row = (uint64_t)blockIdx.x * groups + threadIdx.x / n.width;
+  const uint64_t passes = (n.rows - (uint64_t)blockIdx.x * groups + stride - 1) / stride;
+  const bool in = lane * V < n.columns;
+  const unsigned ring = shared_at(room + (kRing ? kVectors * N * blockDim.x : 0)) + threadIdx.x * 16;
+  const unsigned slot_bytes = Sources::kSlot * blockDim.x, bx = V * (unsigned)sizeof(TX) * blockDim.x, by = V * (unsigned)sizeof(TY) * blockDim.x;
+  const Sources s{{column<TX>(n.dh, lane * V), n.dhs, ring},
+                  {column<TX>(n.dz ? n.h : nullptr, lane * V), n.hs, ring + bx},
+                  {column<TY>(n.dz, lane * V), n.dzs, ring + 2 * bx},
+                  {column<TY>(n.y, lane * V), n.ys, ring + 2 * bx + by},
+                  {column<TY>(GATE == EPS_B200_GATE_ELEMENT ? n.g : nullptr, lane * V), n.gs, ring + 2 * bx + 2 * by}};
+  auto ask = [&](unsigned slot, uint64_t r) {
+    if constexpr (kRing) {
+      const bool there = in && r < n.rows;
+      s.dh.ask(n, slot, slot_bytes, r, there);
+      s.h.ask(n, slot, slot_bytes, r, there);
+      s.dz.ask(n, slot, slot_bytes, r, there);
+      s.y.ask(n, slot, slot_bytes, r, there);
+      if (GATE == EPS_B200_GATE_ELEMENT) s.gate.ask(n, slot, slot_bytes, r, there);
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    }
+  };
+#pragma unroll
+  for (unsigned k = 0; k < kAhead; ++k) ask(k, row + k * stride);
+  const Parameters<TY, V, NIT, kRing> p{n, room, lane};
+  p.stage();
+  unsigned slot = 0;
+  for (uint64_t pass = 0; pass < passes; ++pass, row += stride) {
+    const bool live = row < n.rows;
+    float d[NIT][V], q[NIT][V], h[NIT][V], y[NIT][V];
+    if constexpr (kRing) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(kAhead - 1) : "memory");
+      ask(slot == 0 ? kSlots - 1 : slot - 1, row + kAhead * stride);
+    }
+    s.h.get(n, slot, slot_bytes, row, live, lane, h);
+    s.y.get(n, slot, slot_bytes, row, live, lane, y);
+    float means[2], rs[2];
+    const float(*const both[2])[V] = {h, y};
+    statistics<V, NIT, 2>(n, both, lane, shared, turn, means, rs);
+    s.dh.get(n, slot, slot_bytes, row, live, lane, d);
     // through the norm after
     if (n.dz) {
-      float mean, r;
-      statistics<V, NIT>(n, h, lane, live, shared, turn, &mean, &r);
-      float s[2] = {0.f, 0.f};
+      const float r = rs[0];
+      float sum[2] = {0.f, 0.f};
+      s.dz.get(n, slot, slot_bytes, row, live, lane, q);
 #pragma unroll
       for (int i = 0; i < NIT; ++i) {
-        const unsigned c = (i * n.width + lane) * V;
-        if (!live || c >= n.columns) continue;
         float w[V];
-        parameter<TY, V>(n.pre_w, n.narrow, c, 1.f, w);
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-          h[i][j] = (h[i][j] - mean) * r;
-          add(kPreWeight, i, j, q[i][j] * h[i][j]);
-          add(kPreBias, i, j, q[i][j]);
-          q[i][j] *= w[j];
-          s[0] += q[i][j];
-          s[1] = fmaf(q[i][j], h[i][j], s[1]);
-        }
+        p.get(kPreW, i, w);
+        centre<V>(h[i], means[0], r);
+        add(kPreWeight, i, q[i], h[i]);
+        add(kPreBias, i, q[i], 1.f);
+        vmul<V>(q[i], q[i], w);
+        sum[0] += total<V>(q[i]);
+        vmul<V>(w, q[i], h[i]);
+        sum[1] += total<V>(w);
       }
-      row_sum<2>(s, n.width, shared, turn);
-      const float mq = n.layer ? s[0] * n.inverse_columns : 0.f, mh = s[1] * n.inverse_columns;
+      row_sum<2>(sum, n.width, shared, turn);
+      const float mq = n.layer ? sum[0] * n.inverse_columns : 0.f, mh = sum[1] * n.inverse_columns;
 #pragma unroll
-      for (int i = 0; i < NIT; ++i)
-#pragma unroll
-        for (int j = 0; j < V; ++j) d[i][j] = fmaf(r, q[i][j] - mq - h[i][j] * mh, d[i][j]);
+      for (int i = 0; i < NIT; ++i) {
+        vfma<V>(h[i], h[i], -mh, q[i]);
+        vadd<V>(h[i], h[i], -mq);
+        vfma<V>(d[i], h[i], r, d[i]);
+      }
     }
     if (n.dx) {
 #pragma unroll
-      for (int i = 0; i < NIT; ++i) {
-        const unsigned c = (i * n.width + lane) * V;
-        if (!live || c >= n.columns) continue;
-        Pack<TX, V> o;
-#pragma unroll
-        for (int j = 0; j < V; ++j) o.v[j] = from_float<TX>(d[i][j]);
-        store_pack<TX, V>(static_cast<TX*>(n.dx) + row * n.dxs + c, o);
-      }
+      for (int i = 0; i < NIT; ++i) put<TX, V, NIT>(n, n.dx, n.dxs, row, i, lane, live, d[i]);
     }
-    if (!y) continue;
+    const unsigned here = slot;
+    slot = slot == kSlots - 1 ? 0 : slot + 1;
+    if (!n.y) continue;
     // through the scale, the gate and the norm before
-    float mean = 0.f, r = 1.f, ra = 1.f, rslope = 0.f;
-    if (n.post_norm) statistics<V, NIT>(n, v, lane, live, shared, turn, &mean, &r);
-    if (live && n.gate == EPS_B200_GATE_ROW) ra = activate(to_float(static_cast<const TY*>(n.g)[row]), n.activation, &rslope);
-    float s[3] = {0.f, 0.f, 0.f};
+    const float r = rs[1];
+    float ra = 1.f, rslope = 0.f;
+    if (GATE == EPS_B200_GATE_ROW && live) ra = activate_one(to_float(static_cast<const TY*>(n.g)[row]), n.activation, &rslope);
+    float g[NIT][V];
+    if (GATE == EPS_B200_GATE_ELEMENT) s.gate.get(n, here, slot_bytes, row, live, lane, g);
+    float sum[3] = {0.f, 0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < NIT; ++i) {
-      const unsigned c = (i * n.width + lane) * V;
-      if (!live || c >= n.columns) continue;
-      float w[V], b[V], ch[V];
-      parameter<TY, V>(n.post_w, n.narrow, c, 1.f, w);
-      parameter<TY, V>(n.post_b, n.narrow, c, 0.f, b);
-      parameter<TY, V>(n.channel, n.narrow, c, 1.f, ch);
-      Pack<TY, V> og;
+      float w[V], nv[V], a[V], slope[V], t[V];
+      // y becomes its normed value, nv what the gate sees
+      if (n.post_norm) {
+        p.get(kPostW, i, w);
+        p.get(kPostB, i, t);
+        centre<V>(y[i], means[1], r);
+        vfma<V>(nv, y[i], w, t);
+      } else {
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        float a = ra, slope = rslope;
-        if (n.gate == EPS_B200_GATE_ELEMENT) a = activate(to_float(gate[i].v[j]), n.activation, &slope);
-        if (n.post_norm) v[i][j] = (v[i][j] - mean) * r;
-        const float nv = n.post_norm ? fmaf(v[i][j], w[j], b[j]) : v[i][j];
-        const float e = n.scale * d[i][j];
-        add(kChannel, i, j, e * a * nv);
-        const float ec = e * ch[j];
-        const float dgate = ec * nv * slope;
-        og.v[j] = from_float<TY>(dgate);
-        s[2] += dgate;
-        const float dn = ec * a;
-        if (n.post_norm) {
-          add(kPostWeight, i, j, dn * v[i][j]);
-          add(kPostBias, i, j, dn);
-        }
-        q[i][j] = n.post_norm ? dn * w[j] : dn;
-        s[0] += q[i][j];
-        s[1] = fmaf(q[i][j], v[i][j], s[1]);
+        for (int j = 0; j < V; ++j) { nv[j] = y[i][j]; w[j] = 1.f; }
       }
-      if (n.dg && n.gate == EPS_B200_GATE_ELEMENT) store_pack<TY, V>(static_cast<TY*>(n.dg) + row * n.dgs + c, og);
+      if (GATE == EPS_B200_GATE_ELEMENT) {
+        activate<V, true>(g[i], n.activation, a, slope);
+        vmul<V>(a, a, d[i]);
+      } else {
+        vmul<V>(a, d[i], ra);
+      }
+      add(kChannel, i, a, nv);          // without n.scale, which the block's sums take at the end
+      p.get(kScaleC, i, t);
+      if (GATE != EPS_B200_GATE_NONE) {
+        vmul<V>(nv, nv, d[i]);
+        vmul<V>(nv, nv, t);
+        if (GATE == EPS_B200_GATE_ELEMENT) {
+          vmul<V>(nv, nv, slope);
+          if (n.dg) put<TY, V, NIT>(n, n.dg, n.dgs, row, i, lane, live, nv);
+        } else {
+          sum[2] += total<V>(nv);
+        }
+      }
+      vmul<V>(q[i], a, t);
+      if (n.post_norm) {
+        add(kPostWeight, i, q[i], y[i]);
+        add(kPostBias, i, q[i], 1.f);
+        vmul<V>(q[i], q[i], w);
+        sum[0] += total<V>(q[i]);
+        vmul<V>(t, q[i], y[i]);
+        sum[1] += total<V>(t);
+      }
     }
-    if (n.post_norm || n.gate == EPS_B200_GATE_ROW) row_sum<3>(s, n.width, shared, turn);
-    if (live && lane == 0 && n.dg && n.gate == EPS_B200_GATE_ROW) static_cast<TY*>(n.dg)[row] = from_float<TY>(s[2]);
-    const float mp = n.layer ? s[0] * n.inverse_columns : 0.f, my = s[1] * n.inverse_columns;
+    if (GATE == EPS_B200_GATE_ROW) {
+      row_sum<3>(sum, n.width, shared, turn);
+      if (live && lane == 0 && n.dg) static_cast<TY*>(n.dg)[row] = from_float<TY>(sum[2] * rslope);
+    } else if (n.post_norm) {
+      row_sum<2>(reinterpret_cast<float(&)[2]>(sum), n.width, shared, turn);
+    }
+    const float mp = n.layer ? sum[0] * n.inverse_columns : 0.f, my = sum[1] * n.inverse_columns;
     if (n.dy) {
 #pragma unroll
       for (int i = 0; i < NIT; ++i) {
-        const unsigned c = (i * n.width + lane) * V;
-        if (!live || c >= n.columns) continue;
-        Pack<TY, V> o;
-#pragma unroll
-        for (int j = 0; j < V; ++j)
-          o.v[j] = from_float<TY>(n.post_norm ? r * (q[i][j] - mp - v[i][j] * my) : q[i][j]);
-        store_pack<TY, V>(static_cast<TY*>(n.dy) + row * n.dys + c, o);
+        if (n.post_norm) {
+          vfma<V>(q[i], y[i], -my, q[i]);
+          vadd<V>(q[i], q[i], -mp);
+          vmul<V>(q[i], q[i], r);
+        }
+        put<TY, V, NIT>(n, n.dy, n.dys, row, i, lane, live, q[i]);
       }
     }
   }
+  if constexpr (kRing) asm volatile("cp.async.wait_all;" ::: "memory");
   if (!wanted) return;
+  if constexpr (kHeld) {
+    __syncthreads();        // the staged parameters and the ring lie there
+#pragma unroll
+    for (int k = 0; k < kSums; ++k)
+      if (slot_of[k] >= 0) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) room[slot_of[k] * cell + j * blockDim.x + threadIdx.x] = held[k][j];
+      }
+  }
   __syncthreads();
   // the block's groups of lanes in order, then out
   for (unsigned c = threadIdx.x; c < n.columns; c += blockDim.x) {
     const unsigned at = c / V, i = at / n.width, l = at % n.width, j = c % V;
 #pragma unroll
     for (int k = 0; k < kSums; ++k) {
-      if (slot[k] < 0) continue;
-      float s = 0.f;
-      for (unsigned g = 0; g < groups; ++g) s += sums[slot[k] * cell + (i * V + j) * blockDim.x + g * n.width + l];
-      n.partial[((uint64_t)blockIdx.x * kSums + k) * n.columns + c] = s;
+      if (slot_of[k] < 0) continue;
+      float t = 0.f;
+      for (unsigned g = 0; g < groups; ++g) t += room[slot_of[k] * cell + (i * V + j) * blockDim.x + g * n.width + l];
+      n.partial[((uint64_t)blockIdx.x * kSums + k) * n.columns + c] = k == kChannel ? t * n.scale : t;
     }
   }
 }
@@ -341,21 +610,23 @@ struct Columns {
 };
 
 // out[k][c] = the sum over blocks of partial[block][k][c]: 32 columns a block of
-// threads, eight runs of blocks, joined in order.
-__global__ void __launch_bounds__(256) block_norm_columns(const Columns p) {
-  __shared__ float part[8][32];
-  const unsigned c = blockIdx.x * 32 + threadIdx.x % 32, run = threadIdx.x / 32, k = blockIdx.y;
+// threads, 32 runs of blocks, joined in order.
+constexpr unsigned kRuns = 32;
+__global__ void __launch_bounds__(32 * kRuns) block_norm_columns(const Columns p) {
+  __shared__ float part[kRuns][33];
+  const unsigned l = threadIdx.x % 32, c = blockIdx.x * 32 + l, run = threadIdx.x / 32, k = blockIdx.y;
   if (!p.out[k]) return;
   float s = 0.f;
-  if (c < p.columns)
-    for (unsigned b = run; b < p.blocks; b += 8) s += p.partial[((uint64_t)b * kSums + k) * p.columns + c];
-  part[run][threadIdx.x % 32] = s;
-  __syncthreads();
-  if (run == 0 && c < p.columns) {
-#pragma unroll
-    for (int i = 1; i < 8; ++i) s += part[i][threadIdx.x];
-    p.out[k][c] = s;
+  if (c < p.columns) {
+#pragma unroll 8
+    for (unsigned b = run; b < p.blocks; b += kRuns) s += p.partial[((uint64_t)b * kSums + k) * p.columns + c];
   }
+  part[run][l] = s;
+  __syncthreads();
+  s = part[l][run];                      // lane: run, warp: column
+#pragma unroll
+  for (int o = 16; o; o /= 2) s += __shfl_xor_sync(~0u, s, o);
+  if (l == 0 && blockIdx.x * 32 + run < p.columns) p.out[k][blockIdx.x * 32 + run] = s;
 }
 
 // How a row is spread: V elements a lane, `nit` times, over `width` lanes.
@@ -365,48 +636,69 @@ Spread spread_of(unsigned columns, bool wide) {
   Spread s{};
   s.v = wide ? 8 : 1;
   const unsigned packs = (unsigned)ceil_div(columns, s.v);
-  if (packs <= 32) {
-    s.nit = 1;
+  s.nit = wide ? (packs <= 512 ? 1 : 2) : (packs <= 32 ? 1 : packs <= 1024 ? 4 : 8);
+  const unsigned lanes = (unsigned)ceil_div(packs, s.nit);
+  if (lanes <= 32) {
     s.width = 1;
-    while (s.width < packs) s.width *= 2;
+    while (s.width < lanes) s.width *= 2;
     s.threads = 128;
   } else {
-    s.nit = wide ? (packs <= 512 ? 1 : 2) : (packs <= 1024 ? 1 : 8);
-    s.width = s.threads = (unsigned)round_up(ceil_div(packs, s.nit), 32);
+    s.width = s.threads = (unsigned)round_up(lanes, 32);
   }
   return s;
 }
 
-unsigned gradient_blocks(uint64_t rows, const Spread& s, unsigned sms) {
-  const uint64_t all = ceil_div(rows, s.threads / s.width);
-  const uint64_t resident = (uint64_t)sms * (s.threads <= 128 ? 8 : s.threads <= 256 ? 4 : s.threads <= 512 ? 2 : 1);
-  return (unsigned)(all < resident ? all : resident);
-}
-constexpr unsigned kMostBlocks = 8 * 160;   // of gradient_blocks, for up to 160 SMs
+constexpr unsigned kMostBlocks = 8 * 160;   // of the gradient: 8 an SM, 160 SMs
 
-template <class TX, class TY, int V, int NIT>
-void forward(const Norm& n, const Spread& s, cudaStream_t stream) {
-  const uint64_t blocks = ceil_div(n.rows, s.threads / s.width);
-  need(blocks < (1ull << 31), "too many rows");
-  block_norm_forward<TX, TY, V, NIT><<<(unsigned)blocks, s.threads, 0, stream>>>(n);
+// Blocks that fit the GPU at once, or fewer where the rows need fewer.
+template <class K>
+unsigned resident(K kernel, const Spread& s, size_t shared, uint64_t rows, unsigned sms, unsigned most) {
+  int each = 0;
+  check(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&each, kernel, (int)s.threads, shared), "occupancy");
+  need(each > 0, "no room for a block");
+  uint64_t n = (uint64_t)sms * (unsigned)each;
+  if (n > most) n = most;
+  const uint64_t all = ceil_div(rows, s.threads / s.width);
+  return (unsigned)(all < n ? all : n);
+}
+
+template <class TX, class TY, int V, int NIT, int GATE>
+void forward(const Norm& n, const Spread& s, unsigned sms, cudaStream_t stream) {
+  auto* kernel = block_norm_forward<TX, TY, V, NIT, GATE>;
+  using Sources = ForwardSources<TX, TY, V, NIT>;
+  const unsigned shared = ((V * NIT <= 8 ? kVectors * NIT * V * 4 : 0) + (Sources::kRing ? kSlots * Sources::kSlot : 0)) * s.threads;
+  check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 224 * 1024), "cudaFuncSetAttribute");
+  kernel<<<resident(kernel, s, shared, n.rows, sms, ~0u), s.threads, shared, stream>>>(n);
   check(cudaGetLastError(), "block_norm");
 }
 
-template <class TX, class TY, int V, int NIT>
-void backward(const Norm& n, const Spread& s, unsigned blocks, cudaStream_t stream) {
-  const unsigned shared = __builtin_popcount((unsigned)n.want) * NIT * V * s.threads * 4;
-  check(cudaFuncSetAttribute(block_norm_gradient<TX, TY, V, NIT>, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024),
-        "cudaFuncSetAttribute");
-  block_norm_gradient<TX, TY, V, NIT><<<blocks, s.threads, shared, stream>>>(n);
+// The number of blocks, which is the number of partial sums.
+template <class TX, class TY, int V, int NIT, int GATE>
+unsigned backward(const Norm& n, const Spread& s, unsigned sms, uint64_t room, cudaStream_t stream) {
+  auto* kernel = block_norm_gradient<TX, TY, V, NIT, GATE>;
+  using Sources = BackwardSources<TX, TY, V, NIT>;
+  const unsigned vectors = Sources::kRing ? kVectors : (unsigned)__builtin_popcount((unsigned)n.want);
+  const unsigned shared = (vectors * NIT * V * 4 + (Sources::kRing ? kSlots * Sources::kSlot : 0)) * s.threads;
+  check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 224 * 1024), "cudaFuncSetAttribute");
+  const unsigned blocks = resident(kernel, s, shared, n.rows, sms, kMostBlocks);
+  need(!n.want || room >= (uint64_t)blocks * kSums * n.columns * 4, "block norm workspace too small");
+  kernel<<<blocks, s.threads, shared, stream>>>(n);
   check(cudaGetLastError(), "block_norm_backward");
+  return blocks;
 }
 
-template <class TX, class TY, class F>
+template <int N> using Int = std::integral_constant<int, N>;
+
+template <class F>
+void by_gate(int gate, F f) {
+  gate == EPS_B200_GATE_NONE ? f(Int<EPS_B200_GATE_NONE>{}) : gate == EPS_B200_GATE_ROW ? f(Int<EPS_B200_GATE_ROW>{})
+                                                                                        : f(Int<EPS_B200_GATE_ELEMENT>{});
+}
+
+template <class F>
 void by_spread(const Spread& s, F f) {
-  if (s.v == 8) s.nit == 1 ? f(std::integral_constant<int, 8>{}, std::integral_constant<int, 1>{})
-                           : f(std::integral_constant<int, 8>{}, std::integral_constant<int, 2>{});
-  else s.nit == 1 ? f(std::integral_constant<int, 1>{}, std::integral_constant<int, 1>{})
-                  : f(std::integral_constant<int, 1>{}, std::integral_constant<int, 8>{});
+  if (s.v == 8) s.nit == 1 ? f(Int<8>{}, Int<1>{}) : f(Int<8>{}, Int<2>{});
+  else s.nit == 1 ? f(Int<1>{}, Int<1>{}) : s.nit == 4 ? f(Int<1>{}, Int<4>{}) : f(Int<1>{}, Int<8>{});
 }
 
 template <class F>
@@ -483,7 +775,7 @@ int eps_b200_block_norm(const EpsB200BlockNorm* a, const void* x, int64_t x_stri
     need(!n.rows || h || !n.y, "null output of the residual");
     need(!n.rows || z || !n.pre_norm, "null output of the norm");
     if (!n.rows) return;
-    n.x = x; n.xs = x_stride;
+    n.x = n.somewhere = x; n.xs = x_stride;
     n.out_h = h; n.out_hs = h_stride;
     n.out_z = z; n.out_zs = z_stride;
     if (!n.out_h && !n.pre_norm) return;
@@ -494,8 +786,11 @@ int eps_b200_block_norm(const EpsB200BlockNorm* a, const void* x, int64_t x_stri
     const Spread s = spread_of(n.columns, wide);
     n.width = s.width;
     by_type(a->residual_type, a->type, [&](auto tx, auto ty) {
-      by_spread<decltype(tx), decltype(ty)>(s, [&](auto v, auto nit) {
-        forward<decltype(tx), decltype(ty), decltype(v)::value, decltype(nit)::value>(n, s, static_cast<cudaStream_t>(stream));
+      by_spread(s, [&](auto v, auto nit) {
+        by_gate(n.gate, [&](auto gate) {
+          forward<decltype(tx), decltype(ty), decltype(v)::value, decltype(nit)::value, decltype(gate)::value>(
+              n, s, sm_count(a->device), static_cast<cudaStream_t>(stream));
+        });
       });
     });
   });
@@ -523,6 +818,7 @@ int eps_b200_block_norm_backward(const EpsB200BlockNorm* a, const EpsB200BlockNo
     n.dh = d->dh; n.dhs = d->dh_stride;
     n.dz = d->dz; n.dzs = d->dz_stride;
     n.h = d->h; n.hs = d->h_stride;
+    n.somewhere = n.dz ? n.dz : n.dh ? n.dh : n.y ? n.y : d->dx;
     n.dx = d->dx; n.dxs = d->dx_stride;
     n.dy = d->dy; n.dys = d->dy_stride;
     n.dg = d->dgate; n.dgs = d->dgate_stride;
@@ -542,14 +838,15 @@ int eps_b200_block_norm_backward(const EpsB200BlockNorm* a, const EpsB200BlockNo
     if (n.gate == EPS_B200_GATE_ELEMENT) wide = wide && rows_wide(n.g, n.gs, a->type) && rows_wide(n.dg, n.dgs, a->type);
     const Spread s = spread_of(n.columns, wide);
     n.width = s.width;
-    const unsigned blocks = gradient_blocks(n.rows, s, sm_count(a->device));
-    need(!n.want || (d->workspace && d->workspace_bytes >= (uint64_t)blocks * kSums * n.columns * 4),
-         "block norm workspace too small");
-    need(!n.want || aligned(d->workspace, 16), "the workspace must be 16-byte aligned");
+    need(!n.want || (d->workspace && aligned(d->workspace, 16)), "the workspace must be there and 16-byte aligned");
+    unsigned blocks = 0;
     n.partial = static_cast<float*>(d->workspace);
     by_type(a->residual_type, a->type, [&](auto tx, auto ty) {
-      by_spread<decltype(tx), decltype(ty)>(s, [&](auto v, auto nit) {
-        backward<decltype(tx), decltype(ty), decltype(v)::value, decltype(nit)::value>(n, s, blocks, st);
+      by_spread(s, [&](auto v, auto nit) {
+        by_gate(n.gate, [&](auto gate) {
+          blocks = backward<decltype(tx), decltype(ty), decltype(v)::value, decltype(nit)::value, decltype(gate)::value>(
+              n, s, sm_count(a->device), d->workspace_bytes, st);
+        });
       });
     });
     if (!n.want) return;
@@ -558,7 +855,7 @@ int eps_b200_block_norm_backward(const EpsB200BlockNorm* a, const EpsB200BlockNo
     for (int k = 0; k < kSums; ++k) c.out[k] = out[k];
     c.columns = n.columns;
     c.blocks = blocks;
-    block_norm_columns<<<dim3((unsigned)ceil_div(n.columns, 32), kSums), 256, 0, st>>>(c);
+    block_norm_columns<<<dim3((unsigned)ceil_div(n.columns, 32), kSums), 32 * kRuns, 0, st>>>(c);
     check(cudaGetLastError(), "block_norm_columns");
   });
 }

@@ -169,18 +169,16 @@ struct MmaShape {
   static constexpr unsigned columns = 2 * BN;                          // of tensor memory
 };
 
-__device__ __forceinline__ unsigned shared_address(const void* p) { return (unsigned)__cvta_generic_to_shared(p); }
-
 __device__ __forceinline__ void barrier_init(uint64_t* b, unsigned count) {
-  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(shared_address(b)), "r"(count) : "memory");
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(shared_at(b)), "r"(count) : "memory");
 }
 
 __device__ __forceinline__ void barrier_arrive(uint64_t* b) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(shared_address(b)) : "memory");
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(shared_at(b)) : "memory");
 }
 
 __device__ __forceinline__ void barrier_expect(uint64_t* b, unsigned bytes) {
-  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(shared_address(b)), "r"(bytes) : "memory");
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(shared_at(b)), "r"(bytes) : "memory");
 }
 
 __device__ __forceinline__ uint64_t nanoseconds() {
@@ -193,7 +191,7 @@ __device__ __forceinline__ uint64_t nanoseconds() {
 // working kernel comes near.  The caller then leaves its loop, and the tile's rows
 // become NaN instead of the GPU hanging.
 __device__ __forceinline__ bool barrier_wait(uint64_t* b, unsigned parity) {
-  const unsigned address = shared_address(b);
+  const unsigned address = shared_at(b);
   uint64_t start = 0;
   for (unsigned tries = 1;; ++tries) {
     unsigned done;
@@ -213,13 +211,13 @@ __device__ __forceinline__ bool barrier_wait(uint64_t* b, unsigned parity) {
 
 __device__ __forceinline__ void tma_load(void* to, const CUtensorMap* map, uint64_t* barrier, int x, int y) {
   asm volatile("cp.async.bulk.tensor.2d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
-               ::"r"(shared_address(to)), "l"(map), "r"(shared_address(barrier)), "r"(x), "r"(y) : "memory");
+               ::"r"(shared_at(to)), "l"(map), "r"(shared_at(barrier)), "r"(x), "r"(y) : "memory");
 }
 
 // Shared-memory descriptor of a K-major operand in the 128-byte swizzle: rows of 128
 // bytes, groups of eight rows 1024 bytes apart.
 __device__ __forceinline__ uint64_t operand(const void* p) {
-  return (uint64_t)(shared_address(p) >> 4 & 0x3FFF) | 1ull << 16 | (uint64_t)(1024 >> 4) << 32 | 1ull << 46 | 2ull << 61;
+  return (uint64_t)(shared_at(p) >> 4 & 0x3FFF) | 1ull << 16 | (uint64_t)(1024 >> 4) << 32 | 1ull << 46 | 2ull << 61;
 }
 
 template <int BN>
@@ -233,7 +231,7 @@ __device__ __forceinline__ void mma_i8(unsigned d, uint64_t a, uint64_t b, bool 
 }
 
 __device__ __forceinline__ void mma_commit(uint64_t* barrier) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(shared_address(barrier)) : "memory");
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(shared_at(barrier)) : "memory");
 }
 
 // 32 lanes x 32 columns of tensor memory: lane l of the warp gets its 32 columns.
@@ -258,7 +256,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
   extern __shared__ unsigned char raw[];
   __shared__ uint64_t full[Shape::stages], empty[Shape::stages], summed[2], drained[2];
   __shared__ unsigned tensor_base;
-  unsigned char* const stages = raw + (1024 - shared_address(raw) % 1024) % 1024;
+  unsigned char* const stages = raw + (1024 - shared_at(raw) % 1024) % 1024;
   const unsigned warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   if (threadIdx.x == 0) {
     for (unsigned s = 0; s < Shape::stages; ++s) {
@@ -274,7 +272,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
     asm volatile("prefetch.tensormap [%0];" ::"l"(&rows) : "memory");
   }
   if (warp == 2) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(shared_address(&tensor_base)),
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(shared_at(&tensor_base)),
                  "r"(Shape::columns) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
