@@ -12,10 +12,16 @@
 //   db_post = sum_rows dn, dchannel = sum_rows scale dh' a n
 //
 // Bound: bytes.  Forward reads x, y, gate and writes h, z; backward reads dh, dz,
-// h, y, gate and writes dx, dy, dgate: each value once, held in registers between
-// the passes over the row.  A row belongs to a group of lanes (a power of two up
-// to a warp, or a whole block), V consecutive elements a lane NIT times: V = 8
-// where all rows are 16-byte aligned, 1 otherwise.
+// h, y, gate and writes dx, dy, dgate: each value once.  What stands in the way is
+// the chain of each row (reduce, use, reduce again) and the instructions around it,
+// so: a row's values are copied into shared memory while its predecessors are worked
+// on; the statistics of the next row are reduced together with this row's sums, which
+// halves the barriers; and a kernel has no branch on what is given: missing weights
+// are staged as ones, missing tensors as zeros.
+//
+// A row belongs to a group of lanes (a power of two up to a warp, or a whole block),
+// V consecutive elements a lane NIT times.
+#include <cmath>
 #include <cstdint>
 #include <type_traits>
 
@@ -96,73 +102,71 @@ __device__ __forceinline__ float activate_one(float g, int activation, float* sl
   return a[0];
 }
 
-// A parameter vector's V elements from column c on, `missing` where there is none.
+// A lane's own record in shared memory: bytes rounded up to an odd number of 16-byte
+// words, so that eight neighbouring lanes reading word k of theirs meet all banks once.
+__host__ __device__ constexpr unsigned record(unsigned bytes) { return ((bytes + 15) / 16 | 1) * 16; }
+
+// A parameter vector's V elements from column c on: 1 or 0 (`missing`) where there is
+// none, 0 behind the last column.
 template <class T, int V>
-__device__ __forceinline__ void parameter(const void* p, int narrow, unsigned c, float missing, float (&r)[V]) {
-  if (!p) {
+__device__ __forceinline__ void parameter(const Norm& n, const void* p, unsigned c, float missing, float (&r)[V]) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) r[i] = missing;
-  } else if (narrow) {
-    widen(load_pack<T, V>(static_cast<const T*>(p) + c), r);
-  } else {
-    widen(load_pack<float, V>(static_cast<const float*>(p) + c), r);
-  }
+  for (int i = 0; i < V; ++i) r[i] = c < n.columns ? missing : 0.f;
+  if (!p || c >= n.columns) return;
+  if (n.narrow) widen(load_pack<T, V>(static_cast<const T*>(p) + c), r);
+  else widen(load_pack<float, V>(static_cast<const float*>(p) + c), r);
 }
 
-// The parameter vectors as a lane uses them.  Where a lane has few columns, a block
-// lays its lanes' values out in shared memory once, in float and with what is missing
-// filled in: rows then read them without a branch and without a bank conflict.
-enum { kPostW, kPostB, kScaleC, kPreW, kPreB, kVectors };
+// The four vectors that a row is worked on with, as a lane uses them.  Where a lane
+// has few columns it writes them down in its record once, in float: rows then read
+// them at fixed places.
+//   forward   0: c w_post   1: c b_post   2: w_pre    3: b_pre
+//   backward  0: w_post     1: b_post     2: w_pre    3: c
+constexpr int kVectors = 4;
 
-template <class T, int V, int NIT, bool STAGED>
+template <class T, int V, int NIT, bool STAGED, bool FORWARD>
 struct Parameters {
+  static constexpr unsigned kRecord = STAGED ? record(kVectors * NIT * V * 4) : 0;
   const Norm& n;
-  float* staged;           // [kVectors][NIT][V / 4][blockDim.x][4], or [kVectors][NIT][blockDim.x] for V == 1
   unsigned lane;
+  float* mine;             // STAGED: the lane's record, [kVectors][NIT][V]
 
-  __device__ __forceinline__ float* at(int k, int i) const { return staged + (unsigned)((k * NIT + i) * V) * blockDim.x + threadIdx.x * (V < 4 ? V : 4); }
-  __device__ __forceinline__ void read(int k, int i, float (&r)[V]) const {
-    const unsigned c = (i * n.width + lane) * V;
-    switch (k) {
-      case kPostW: parameter<T, V>(n.post_w, n.narrow, c, 1.f, r); break;
-      case kPostB: parameter<T, V>(n.post_b, n.narrow, c, 0.f, r); break;
-      case kScaleC: parameter<T, V>(n.channel, n.narrow, c, 1.f, r); vmul<V>(r, r, n.scale); break;
-      case kPreW: parameter<T, V>(n.pre_w, n.narrow, c, 1.f, r); break;
-      default: parameter<T, V>(n.pre_b, n.narrow, c, 0.f, r);
-    }
-  }
-  __device__ __forceinline__ void stage() const {
+  __device__ __forceinline__ Parameters(const Norm& norm, unsigned l, void* room)
+      : n(norm), lane(l), mine(reinterpret_cast<float*>(static_cast<char*>(room) + threadIdx.x * kRecord)) {
     if constexpr (STAGED) {
 #pragma unroll
       for (int k = 0; k < kVectors; ++k)
 #pragma unroll
         for (int i = 0; i < NIT; ++i) {
-          float r[V] = {};          // 0 behind the last column: what a lane holds there adds nothing
-          if ((i * n.width + lane) * V < n.columns) read(k, i, r);
+          float r[V];
+          read(k, i, r);
+          Pack<float, V> x;
 #pragma unroll
-          for (int j = 0; j < V; j += 4) {
-            if constexpr (V >= 4) *reinterpret_cast<float4*>(at(k, i) + j * blockDim.x) = make_float4(r[j], r[j + 1], r[j + 2], r[j + 3]);
-            else *at(k, i) = r[0];
-          }
+          for (int j = 0; j < V; ++j) x.v[j] = r[j];
+          *reinterpret_cast<Pack<float, V>*>(mine + (k * NIT + i) * V) = x;
         }
-      // each thread reads back its own values only: no barrier
     }
+  }
+  __device__ __forceinline__ void read(int k, int i, float (&r)[V]) const {
+    const unsigned c = (i * n.width + lane) * V;
+    if (k == 0) parameter<T, V>(n, n.post_w, c, 1.f, r);
+    if (k == 1) parameter<T, V>(n, n.post_b, c, 0.f, r);
+    if (k == 2) parameter<T, V>(n, n.pre_w, c, 1.f, r);
+    if (k == 3) FORWARD ? parameter<T, V>(n, n.pre_b, c, 0.f, r) : parameter<T, V>(n, n.channel, c, 1.f, r);
+    if (FORWARD && k < 2) {
+      float s[V];
+      parameter<T, V>(n, n.channel, c, 1.f, s);
+      vmul<V>(r, r, s);
+    }
+    if (FORWARD ? k < 2 : k == 3) vmul<V>(r, r, n.scale);
   }
   __device__ __forceinline__ void get(int k, int i, float (&r)[V]) const {
     if constexpr (STAGED) {
+      const Pack<float, V> x = *reinterpret_cast<const Pack<float, V>*>(mine + (k * NIT + i) * V);
 #pragma unroll
-      for (int j = 0; j < V; j += 4) {
-        if constexpr (V >= 4) {
-          const float4 x = *reinterpret_cast<const float4*>(at(k, i) + j * blockDim.x);
-          r[j] = x.x; r[j + 1] = x.y; r[j + 2] = x.z; r[j + 3] = x.w;
-        } else {
-          r[0] = *at(k, i);
-        }
-      }
+      for (int j = 0; j < V; ++j) r[j] = x.v[j];
     } else {
-#pragma unroll
-      for (int j = 0; j < V; ++j) r[j] = 0.f;
-      if ((i * n.width + lane) * V < n.columns) read(k, i, r);
+      read(k, i, r);
     }
   }
 };
@@ -183,54 +187,6 @@ __device__ __forceinline__ float total(const float (&v)[V]) {
   }
 }
 
-// Means and reciprocal deviations of K rows held by the same lanes.  Two passes over
-// the registers for a layer norm: the squares of what is left after the mean cannot
-// cancel.  A lane divides its own sums by the columns, so that they cannot overflow
-// across lanes where the mean square itself does not.
-template <int V, int NIT, int K>
-__device__ __forceinline__ void statistics(const Norm& n, const float (*const (&v)[K])[V], unsigned lane, float* shared,
-                                           unsigned& turn, float (&mean)[K], float (&r)[K]) {
-  float s[K];
-#pragma unroll
-  for (int k = 0; k < K; ++k) mean[k] = 0.f;
-  if (n.layer) {
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-      s[k] = 0.f;
-#pragma unroll
-      for (int i = 0; i < NIT; ++i) s[k] += total<V>(v[k][i]);     // lanes past the row hold 0
-      s[k] *= n.inverse_columns;
-    }
-    row_sum<K>(s, n.width, shared, turn);
-#pragma unroll
-    for (int k = 0; k < K; ++k) mean[k] = s[k];
-  }
-#pragma unroll
-  for (int k = 0; k < K; ++k) {
-    s[k] = 0.f;
-#pragma unroll
-    for (int i = 0; i < NIT; ++i) {
-      float d[V];
-      vadd<V>(d, v[k][i], -mean[k]);
-      vmul<V>(d, d, d);
-      s[k] = fmaf(total<V>(d), (i * n.width + lane) * V < n.columns ? n.inverse_columns : 0.f, s[k]);
-    }
-  }
-  row_sum<K>(s, n.width, shared, turn);
-#pragma unroll
-  for (int k = 0; k < K; ++k) r[k] = __frsqrt_rn(s[k] + n.epsilon);
-}
-
-template <int V, int NIT>
-__device__ __forceinline__ void one_row(const Norm& n, const float (&v)[NIT][V], unsigned lane, float* shared, unsigned& turn,
-                                        float* mean, float* r) {
-  const float(*const rows[1])[V] = {v};
-  float m[1], d[1];
-  statistics<V, NIT, 1>(n, rows, lane, shared, turn, m, d);
-  *mean = m[0];
-  *r = d[0];
-}
-
 // (v - mean) * r: the difference first, since v r and mean r may both be large.
 template <int V>
 __device__ __forceinline__ void centre(float (&v)[V], float mean, float r) {
@@ -238,182 +194,316 @@ __device__ __forceinline__ void centre(float (&v)[V], float mean, float r) {
   vmul<V>(v, v, r);
 }
 
-// The rows of R tensors on their way into shared memory.  Blocks walk the rows, and
-// a lane asks for its own values two rows ahead, past registers and L1: the
-// reductions and barriers of a row then pass while its successors are under way.  A
-// lane reads back only what it asked for itself, so no barrier is involved; lanes
-// behind the row's end, rows behind the last one and missing tensors read zeros.
-// Without 16-byte alignment, or with more than eight elements a lane, values are
-// loaded as they are needed.
+// A lane's part of a row's mean, or of its mean square about `mean`.  It divides by
+// the columns itself, so that sums cannot overflow across lanes where the mean does
+// not; what it holds behind the last column does not count.
+template <int V, int NIT, bool SQUARE>
+__device__ __forceinline__ float share(const Norm& n, unsigned lane, const float (&v)[NIT][V], float mean) {
+  float s = 0.f;
+#pragma unroll
+  for (int i = 0; i < NIT; ++i) {
+    const float inside = (i * n.width + lane) * V < n.columns ? n.inverse_columns : 0.f;
+    if constexpr (SQUARE) {
+      float d[V];
+      vadd<V>(d, v[i], -mean);
+      vmul<V>(d, d, d);
+      s = fmaf(total<V>(d), inside, s);
+    } else {
+      s = fmaf(total<V>(v[i]), inside, s);
+    }
+  }
+  return s;
+}
+
+// How rows reach the lanes.  Blocks walk the rows, and in the two ways with a ring a
+// row's values are under way two rows ahead, past registers and L1:
+//   kBulk    a block's row: one thread copies each tensor's row whole;
+//   kLanes   rows of a few lanes: a lane copies its own 16 bytes of each tensor and
+//            reads back only those, so that no barrier is involved;
+//   kDirect  without 16-byte alignment, or with several packs a lane: loaded as needed.
+// Lanes behind the row's end, rows behind the last one and missing tensors read zeros.
+enum Way { kDirect, kLanes, kBulk };
 constexpr unsigned kAhead = 2, kSlots = kAhead + 1;
+constexpr unsigned kLanesThreads = 128;      // of a block where rows have up to 32 lanes
+
+template <int V, int NIT, int P>
+constexpr Way kWay = V < 4 || NIT > 1 ? kDirect : P == 1 ? kLanes : kBulk;
 
 __device__ __forceinline__ void copy16(unsigned to, const void* from, bool there) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(there ? 16 : 0) : "memory");
 }
 
-template <class T, int V, int NIT, bool RING>
-struct Source {
-  const T* p;              // the tensor at the lane's first column, or NULL
-  int64_t stride;
-  unsigned to;             // RING: the lane's place in slot 0, a shared address; 16-byte planes blockDim.x apart
-  static constexpr unsigned kPlanes = V * sizeof(T) / 16;
-
-  __device__ __forceinline__ void ask(const Norm& n, unsigned slot, unsigned slot_bytes, uint64_t row, bool in) const {
-    static_assert(!RING || NIT == 1, "one pack a lane");
-    const bool there = in && p;
-    const char* const from = reinterpret_cast<const char*>(there ? p + row * stride : static_cast<const T*>(n.somewhere));
-#pragma unroll
-    for (unsigned k = 0; k < kPlanes; ++k) copy16(to + slot * slot_bytes + k * blockDim.x * 16, from + (there ? k * 16 : 0), there);
+// What both directions share: the block's rows, and the lane's.
+struct Walk {
+  unsigned lane, passes, mine;             // passes of the block, and how many of them have a row for this lane
+  uint64_t stride, row;
+  __device__ __forceinline__ explicit Walk(const Norm& n) {
+    lane = threadIdx.x % n.width;
+    const unsigned groups = blockDim.x / n.width;
+    stride = (uint64_t)gridDim.x * groups;
+    const uint64_t first = (uint64_t)blockIdx.x * groups;     // blocks do not outnumber groups of rows
+    row = first + threadIdx.x / n.width;
+    passes = (unsigned)((n.rows - first + stride - 1) / stride);
+    mine = row < n.rows ? (unsigned)((n.rows - row + stride - 1) / stride) : 0;
   }
-  __device__ __forceinline__ void get(const Norm& n, unsigned slot, unsigned slot_bytes, uint64_t row, bool live, unsigned lane,
-                                      float (&r)[NIT][V]) const {
-    if constexpr (RING) {
+};
+
+// One tensor of those rows.  In a slot of the ring a tensor takes V * sizeof(T) bytes
+// a thread: as its row lies (kBulk), or in planes of 16 bytes a lane (kLanes).
+template <class T, int V, int NIT, Way WAY>
+struct Source {
+  static constexpr unsigned kBytes = V * sizeof(T);
+  const char* p;           // kBulk: the next row; else the lane's place in it
+  int64_t step;            // bytes from one row of the walk to the next
+  bool there;              // the tensor is given (and the lane's first pack lies in its row)
+
+  __device__ __forceinline__ Source(const Norm& n, const Walk& w, const void* tensor, int64_t stride) {
+    there = tensor && (WAY == kBulk || w.lane * V < n.columns);
+    const int64_t from = (int64_t)w.row * stride + (WAY == kBulk ? 0 : w.lane * V);
+    p = there ? static_cast<const char*>(tensor) + from * (int64_t)sizeof(T) : static_cast<const char*>(n.somewhere);
+    step = there ? (int64_t)w.stride * stride * (int64_t)sizeof(T) : 0;
+  }
+  // to: the tensor's bytes in a slot, a shared address
+  __device__ __forceinline__ void ask(unsigned to, bool live) {
+#pragma unroll
+    for (unsigned k = 0; k < kBytes / 16; ++k) copy16(to + (k * kLanesThreads + threadIdx.x) * 16, p + k * 16, live && there);
+    p += step;
+  }
+  __device__ __forceinline__ void ask_row(unsigned to, unsigned row_bytes, uint64_t* barrier) {
+    if (there) bulk_copy(to, p, row_bytes, barrier);
+    p += step;
+  }
+  __device__ __forceinline__ void get(const Norm& n, unsigned from, bool live, unsigned lane, float (&r)[NIT][V]) {
+    if constexpr (WAY != kDirect) {
       Pack<T, V> x;
 #pragma unroll
-      for (unsigned k = 0; k < kPlanes; ++k) {
+      for (unsigned k = 0; k < kBytes / 16; ++k) {
         uint4& q = reinterpret_cast<uint4*>(&x)[k];
-        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
-                     : "=r"(q.x), "=r"(q.y), "=r"(q.z), "=r"(q.w) : "r"(to + slot * slot_bytes + k * blockDim.x * 16) : "memory");
+        const unsigned at = from + (WAY == kBulk ? threadIdx.x * kBytes + k * 16 : (k * kLanesThreads + threadIdx.x) * 16);
+        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(q.x), "=r"(q.y), "=r"(q.z), "=r"(q.w) : "r"(at) : "memory");
       }
       widen(x, r[0]);
     } else {
 #pragma unroll
       for (int i = 0; i < NIT; ++i) {
         Pack<T, V> x{};
-        if (live && p && (i * n.width + lane) * V < n.columns) x = load_once<T, V>(p + row * stride + i * n.width * V);
+        if (live && there && (i * n.width + lane) * V < n.columns) x = load_once<T, V>(reinterpret_cast<const T*>(p) + i * n.width * V);
         widen(x, r[i]);
       }
     }
   }
+  __device__ __forceinline__ void next() {
+    if constexpr (WAY == kDirect) p += step;
+  }
 };
 
+// One tensor that is written.
 template <class T, int V, int NIT>
-__device__ __forceinline__ void put(const Norm& n, void* p, int64_t stride, uint64_t row, int i, unsigned lane, bool live, const float (&v)[V]) {
-  const unsigned c = (i * n.width + lane) * V;
-  if (live && c < n.columns) store_pack<T, V>(static_cast<T*>(p) + row * stride + c, narrow<T, V>(v));
-}
-
-template <class TX, class TY, int V, int NIT>
-struct ForwardSources {
-  static constexpr bool kRing = V == 8 && NIT == 1;
-  Source<TX, V, NIT, kRing> x;
-  Source<TY, V, NIT, kRing> y, gate;
-  static constexpr unsigned kSlot = V * (sizeof(TX) + 2 * sizeof(TY));     // bytes of a lane
-};
-template <class TX, class TY, int V, int NIT>
-struct BackwardSources {
-  static constexpr bool kRing = V == 8 && NIT == 1;
-  Source<TX, V, NIT, kRing> dh, h;
-  Source<TY, V, NIT, kRing> dz, y, gate;
-  static constexpr unsigned kSlot = V * (2 * sizeof(TX) + 3 * sizeof(TY));
+struct Sink {
+  char* p;
+  int64_t step;
+  bool there;
+  __device__ __forceinline__ Sink(const Norm& n, const Walk& w, void* tensor, int64_t stride) {
+    there = tensor && w.lane * V < n.columns;
+    p = static_cast<char*>(tensor) + (there ? ((int64_t)w.row * stride + w.lane * V) * (int64_t)sizeof(T) : 0);
+    step = there ? (int64_t)w.stride * stride * (int64_t)sizeof(T) : 0;
+  }
+  __device__ __forceinline__ void put(const Norm& n, int i, unsigned lane, bool live, const float (&v)[V]) const {
+    if (live && there && (i == 0 || (i * n.width + lane) * V < n.columns))
+      store_pack<T, V>(reinterpret_cast<T*>(p) + i * n.width * V, narrow<T, V>(v));
+  }
+  __device__ __forceinline__ void next() { p += step; }
 };
 
-template <class T>
-__device__ __forceinline__ const T* column(const void* p, unsigned c) {
-  return p ? static_cast<const T*>(p) + c : nullptr;
+// The ring's shared memory before its first copy: zeros, which stay where nothing is
+// copied, and the slots' barriers.
+template <Way WAY>
+__device__ __forceinline__ void open_ring(char* ring, unsigned bytes, uint64_t (&arrived)[kSlots]) {
+  if constexpr (WAY == kBulk) {
+    for (unsigned i = threadIdx.x * 16; i < bytes; i += blockDim.x * 16) *reinterpret_cast<uint4*>(ring + i) = uint4{};
+    if (threadIdx.x < kSlots) barrier_init(arrived + threadIdx.x, 1);
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncthreads();
+  }
 }
 
-template <class TX, class TY, int V, int NIT, int GATE>
-__global__ void __launch_bounds__(V == 8 ? 512 : 1024) block_norm_forward(const Norm n) {
-  using Sources = ForwardSources<TX, TY, V, NIT>;
-  constexpr bool kRing = Sources::kRing, kStaged = V * NIT <= 8;
-  extern __shared__ __align__(16) float room[];      // the staged parameters, then the ring
+// A place in the ring: a slot, its bytes, and the parity of its barrier's phase.
+struct Place {
+  unsigned index = 0, bytes = 0, phase = 0;
+  __device__ __forceinline__ void next(unsigned slot_bytes) {
+    bytes += slot_bytes;
+    if (++index == kSlots) { index = bytes = 0; phase ^= 1; }
+  }
+};
+
+// Whether the row at `at` has arrived; what a lane reads then is its own row's.
+template <Way WAY>
+__device__ __forceinline__ bool arrive(uint64_t (&arrived)[kSlots], const Place& at, bool expected) {
+  if constexpr (WAY == kLanes) asm volatile("cp.async.wait_group %0;" ::"n"(kAhead - 1) : "memory");
+  if constexpr (WAY == kBulk) return !expected || barrier_wait(arrived + at.index, at.phase);
+  return true;
+}
+
+template <class TX, class TY, int V>
+__host__ __device__ constexpr unsigned forward_bytes() { return V * (sizeof(TX) + 2 * sizeof(TY)); }     // of a thread in a slot
+template <class TX, class TY, int V>
+__host__ __device__ constexpr unsigned backward_bytes() { return V * (2 * sizeof(TX) + 3 * sizeof(TY)); }
+
+template <class TX, class TY, int V, int NIT, int P, int GATE>
+__global__ void __launch_bounds__(512) block_norm_forward(const Norm n) {
+  constexpr Way kHow = kWay<V, NIT, P>;
+  constexpr bool kStaged = V * NIT <= 8;
+  using Given = Parameters<TY, V, NIT, kStaged, true>;
+  extern __shared__ __align__(16) char room[];       // the staged parameters, then the ring
   __shared__ float shared[kRowSumShared];
+  __shared__ uint64_t arrived[kSlots];
+  const unsigned slot_bytes = forward_bytes<TX, TY, V>() * blockDim.x;
+  clear_row_sums<P>(shared);
+  open_ring<kHow>(room + Given::kRecord * blockDim.x, kSlots * slot_bytes, arrived);
   unsigned turn = 0;
-  const unsigned lane = threadIdx.x % n.width, groups = blockDim.x / n.width;
-  const uint64_t stride = (uint64_t)gridDim.x * groups;
-  uint64_t row = (uint64_t)blockIdx.x * groups + threadIdx.x / n.width;
-  const uint64_t passes = (n.rows - (uint64_t)blockIdx.x * groups + stride - 1) / stride;   // blocks do not outnumber groups of rows
-  const bool in = lane * V < n.columns;
-  const unsigned ring = shared_at(room + (kStaged ? kVectors * NIT * V * blockDim.x : 0)) + threadIdx.x * 16;
-  const unsigned slot_bytes = Sources::kSlot * blockDim.x;
-  const Sources s{{column<TX>(n.x, lane * V), n.xs, ring},
-                  {column<TY>(n.y, lane * V), n.ys, ring + V * (unsigned)sizeof(TX) * blockDim.x},
-                  {column<TY>(GATE == EPS_B200_GATE_ELEMENT ? n.g : nullptr, lane * V), n.gs,
-                   ring + V * (unsigned)(sizeof(TX) + sizeof(TY)) * blockDim.x}};
-  auto ask = [&](unsigned slot, uint64_t r) {
-    if constexpr (kRing) {
-      const bool there = in && r < n.rows;
-      s.x.ask(n, slot, slot_bytes, r, there);
-      s.y.ask(n, slot, slot_bytes, r, there);
-      if (GATE == EPS_B200_GATE_ELEMENT) s.gate.ask(n, slot, slot_bytes, r, there);
+  const Walk w(n);
+  const unsigned lane = w.lane;
+  // the tensors' places in a slot
+  const unsigned at_x = shared_at(room) + Given::kRecord * blockDim.x, at_y = at_x + V * (unsigned)sizeof(TX) * blockDim.x,
+                 at_g = at_y + V * (unsigned)sizeof(TY) * blockDim.x;
+  Source<TX, V, NIT, kHow> x(n, w, n.x, n.xs);
+  Source<TY, V, NIT, kHow> y(n, w, n.y, n.ys), gate(n, w, GATE == EPS_B200_GATE_ELEMENT ? n.g : nullptr, n.gs);
+  Sink<TX, V, NIT> h(n, w, n.out_h, n.out_hs);
+  Sink<TY, V, NIT> z(n, w, n.out_z, n.out_zs);
+  unsigned asked = 0;
+  Place fill, here;
+  auto ask = [&] {
+    const bool live = asked++ < w.mine;
+    if constexpr (kHow == kBulk) {
+      if (threadIdx.x == 0 && live) {
+        const unsigned bx = n.columns * (unsigned)sizeof(TX), by = n.columns * (unsigned)sizeof(TY);
+        barrier_expect(arrived + fill.index, bx + (y.there ? by : 0) + (GATE == EPS_B200_GATE_ELEMENT ? by : 0));
+        x.ask_row(at_x + fill.bytes, bx, arrived + fill.index);
+        y.ask_row(at_y + fill.bytes, by, arrived + fill.index);
+        if (GATE == EPS_B200_GATE_ELEMENT) gate.ask_row(at_g + fill.bytes, by, arrived + fill.index);
+      }
+    } else if constexpr (kHow == kLanes) {
+      x.ask(at_x + fill.bytes, live);
+      y.ask(at_y + fill.bytes, live);
+      if (GATE == EPS_B200_GATE_ELEMENT) gate.ask(at_g + fill.bytes, live);
       asm volatile("cp.async.commit_group;" ::: "memory");
     }
+    fill.next(slot_bytes);
   };
-#pragma unroll
-  for (unsigned k = 0; k < kAhead; ++k) ask(k, row + k * stride);
-  const Parameters<TY, V, NIT, kStaged> p{n, room, lane};
-  p.stage();
-  unsigned slot = 0;
-  for (uint64_t pass = 0; pass < passes; ++pass, row += stride) {
-    const bool live = row < n.rows;
-    float v[NIT][V], x[NIT][V], g[NIT][V];
-    if constexpr (kRing) {
-      asm volatile("cp.async.wait_group %0;" ::"n"(kAhead - 1) : "memory");
-      ask(slot == 0 ? kSlots - 1 : slot - 1, row + kAhead * stride);
+  ask();
+  ask();
+  const Given p(n, lane, room);
+  const bool layer = n.layer, post = n.post_norm;
+  const TY* row_gates = static_cast<const TY*>(n.g) + w.row;
+
+  // the first row's y and its statistics
+  float v[NIT][V], mean = 0.f, r = 1.f;
+  bool good = arrive<kHow>(arrived, here, true);
+  y.get(n, at_y, 0 < w.mine, lane, v);
+  y.next();
+  {
+    float s[1];
+    if (layer) {
+      s[0] = share<V, NIT, false>(n, lane, v, 0.f);
+      row_sum<1, P>(s, n.width, shared, turn);
+      mean = s[0];
     }
-    s.y.get(n, slot, slot_bytes, row, live, lane, v);
-    float mean = 0.f, r = 1.f, row_gate = 1.f, unused;
-    if (n.y && n.post_norm) one_row<V, NIT>(n, v, lane, shared, turn, &mean, &r);
-    s.x.get(n, slot, slot_bytes, row, live, lane, x);
-    if (GATE == EPS_B200_GATE_ELEMENT) s.gate.get(n, slot, slot_bytes, row, live, lane, g);
-    slot = slot == kSlots - 1 ? 0 : slot + 1;
-    if (GATE == EPS_B200_GATE_ROW && live) row_gate = activate_one(to_float(static_cast<const TY*>(n.g)[row]), n.activation, &unused);
-#pragma unroll
-    for (int i = 0; i < NIT; ++i) {
-      if (!n.y) {
-#pragma unroll
-        for (int j = 0; j < V; ++j) v[i][j] = x[i][j];
-      } else {
-        float w[V], b[V];
-        if (n.post_norm) {
-          p.get(kPostW, i, w);
-          p.get(kPostB, i, b);
-          centre<V>(v[i], mean, r);
-          vfma<V>(v[i], v[i], w, b);
-        }
-        if (GATE == EPS_B200_GATE_ELEMENT) {
-          float a[V], slope[V];
-          activate<V, false>(g[i], n.activation, a, slope);
-          vmul<V>(v[i], v[i], a);
-        }
-        p.get(kScaleC, i, w);
-        if (GATE == EPS_B200_GATE_ROW) vmul<V>(w, w, row_gate);
-        vfma<V>(v[i], w, v[i], x[i]);
-      }
-      if (n.out_h) put<TX, V, NIT>(n, n.out_h, n.out_hs, row, i, lane, live, v[i]);
-    }
-    if (!n.pre_norm) continue;
-    one_row<V, NIT>(n, v, lane, shared, turn, &mean, &r);
-#pragma unroll
-    for (int i = 0; i < NIT; ++i) {
-      float w[V], b[V];
-      p.get(kPreW, i, w);
-      p.get(kPreB, i, b);
-      centre<V>(v[i], mean, r);
-      vfma<V>(v[i], v[i], w, b);
-      put<TY, V, NIT>(n, n.out_z, n.out_zs, row, i, lane, live, v[i]);
-    }
+    s[0] = share<V, NIT, true>(n, lane, v, mean);
+    row_sum<1, P>(s, n.width, shared, turn);
+    r = __frsqrt_rn(s[0] + n.epsilon);
   }
+  for (unsigned pass = 0; pass < w.passes; ++pass) {
+    const bool live = pass < w.mine;
+    if (!post) { mean = 0.f; r = 1.f; }
+    if (!good) r = NAN;
+    // the slot of the row before: every lane has passed a barrier since it read it
+    if constexpr (kHow != kDirect) ask();
+    float t[NIT][V];
+    x.get(n, at_x + here.bytes, live, lane, t);
+    x.next();
+    float open = 1.f, unused;
+    if (GATE == EPS_B200_GATE_ROW) {
+      if (live) open = activate_one(to_float(*row_gates), n.activation, &unused);
+      row_gates += w.stride;
+    }
+    float g[NIT][V];
+    if (GATE == EPS_B200_GATE_ELEMENT) {
+      gate.get(n, at_g + here.bytes, live, lane, g);
+      gate.next();
+    }
+#pragma unroll
+    for (int i = 0; i < NIT; ++i) {
+      float a[V], b[V];
+      p.get(0, i, a);
+      p.get(1, i, b);
+      centre<V>(v[i], mean, r);
+      vfma<V>(v[i], v[i], a, b);
+      if (GATE == EPS_B200_GATE_ELEMENT) {
+        activate<V, false>(g[i], n.activation, a, b);
+        vfma<V>(v[i], v[i], a, t[i]);
+      } else {
+        vfma<V>(v[i], v[i], open, t[i]);
+      }
+      h.put(n, i, lane, live, v[i]);
+    }
+    h.next();
+    // the next row's y; its statistics together with this row's h's
+    here.next(slot_bytes);
+    good = arrive<kHow>(arrived, here, pass + 1 < w.passes);
+    y.get(n, at_y + here.bytes, pass + 1 < w.mine, lane, t);
+    y.next();
+    float s[2], m = 0.f;
+    mean = 0.f;
+    if (layer) {
+      s[0] = share<V, NIT, false>(n, lane, v, 0.f);
+      s[1] = share<V, NIT, false>(n, lane, t, 0.f);
+      row_sum<2, P>(s, n.width, shared, turn);
+      m = s[0];
+      mean = s[1];
+    }
+    s[0] = share<V, NIT, true>(n, lane, v, m);
+    s[1] = share<V, NIT, true>(n, lane, t, mean);
+    row_sum<2, P>(s, n.width, shared, turn);
+    const float rh = __frsqrt_rn(s[0] + n.epsilon);
+    r = __frsqrt_rn(s[1] + n.epsilon);
+#pragma unroll
+    for (int i = 0; i < NIT; ++i) {
+      float a[V], b[V];
+      p.get(2, i, a);
+      p.get(3, i, b);
+      centre<V>(v[i], m, rh);
+      vfma<V>(v[i], v[i], a, b);
+      z.put(n, i, lane, live, v[i]);
+#pragma unroll
+      for (int j = 0; j < V; ++j) v[i][j] = t[i][j];
+    }
+    z.next();
+  }
+  if constexpr (kHow == kLanes) asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
 // The column sums of a lane stay in registers where a lane has few columns, else in
 // shared memory (each lane its own columns: no conflict, no atomic).  They leave a
 // block once; block_norm_columns adds the blocks up in order.
-template <class TX, class TY, int V, int NIT, int GATE>
-__global__ void __launch_bounds__(V == 8 ? 512 : 1024) block_norm_gradient(const Norm n) {
-  using Sources = BackwardSources<TX, TY, V, NIT>;
+template <class TX, class TY, int V, int NIT, int P, int GATE>
+__global__ void __launch_bounds__(512) block_norm_gradient(const Norm n) {
   constexpr int N = V * NIT;
-  constexpr bool kRing = Sources::kRing, kHeld = kRing;
-  extern __shared__ __align__(16) float room[];     // [wanted][N][blockDim.x] sums; before them staged parameters and the ring
+  constexpr Way kHow = kWay<V, NIT, P>;
+  constexpr bool kHeld = kHow != kDirect;
+  using Given = Parameters<TY, V, NIT, kHeld, false>;
+  extern __shared__ __align__(16) char room[];      // the staged parameters, then the ring; in the end the sums
+  float* const sums = reinterpret_cast<float*>(room);      // [wanted][N][blockDim.x]
   __shared__ float shared[kRowSumShared];
+  __shared__ uint64_t arrived[kSlots];
+  const unsigned slot_bytes = backward_bytes<TX, TY, V>() * blockDim.x;
+  clear_row_sums<P>(shared);
+  open_ring<kHow>(room + Given::kRecord * blockDim.x, kSlots * slot_bytes, arrived);
   unsigned turn = 0;
-  const unsigned lane = threadIdx.x % n.width, groups = blockDim.x / n.width;
+  const Walk w(n);
+  const unsigned lane = w.lane, groups = blockDim.x / n.width;
   const unsigned cell = N * blockDim.x;
-  int slot_of[kSums];
-  int wanted = 0;
-#pragma unroll
-  for (int k = 0; k < kSums; ++k) slot_of[k] = n.want >> k & 1 ? wanted++ : -1;
+  const unsigned wanted = __popc(n.want);
+  auto slot_of = [&](int k) { return __popc(n.want & ((1 << k) - 1)); };      // of a wanted sum
   float held[kHeld ? kSums : 1][V];
   if constexpr (kHeld) {
 #pragma unroll
@@ -421,7 +511,7 @@ __global__ void __launch_bounds__(V == 8 ? 512 : 1024) block_norm_gradient(const
 #pragma unroll
       for (int j = 0; j < V; ++j) held[k][j] = 0.f;
   } else {
-    for (unsigned i = threadIdx.x; i < wanted * cell; i += blockDim.x) room[i] = 0.f;
+    for (unsigned i = threadIdx.x; i < wanted * cell; i += blockDim.x) sums[i] = 0.f;
     __syncthreads();
   }
   // column sums k of the lane's pack i grow by a * b, or by a
@@ -429,164 +519,207 @@ __global__ void __launch_bounds__(V == 8 ? 512 : 1024) block_norm_gradient(const
     if constexpr (kHeld) {
       if constexpr (std::is_same_v<std::decay_t<decltype(b)>, float>) vadd<V>(held[k], held[k], a);
       else vfma<V>(held[k], a, b, held[k]);
-    } else if (slot_of[k] >= 0) {
+    } else if (n.want >> k & 1) {
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        float* const s = room + slot_of[k] * cell + (i * V + j) * blockDim.x + threadIdx.x;
+        float* const s = sums + slot_of(k) * cell + (i * V + j) * blockDim.x + threadIdx.x;
         *s = fmaf(part<V>(a, j), part<V>(b, j), *s);
       }
     }
   };
 
-  const uint64_t stride = (uint64_t)gridDim.x * groups;
-  uint64_t row = (uint64_t)blockIdx.x * groups + threadIdx.x / n.width;
-  const uint64_t passes = (n.rows - (uint64_t)blockIdx.x * groups + stride - 1) / stride;
-  const bool in = lane * V < n.columns;
-  const unsigned ring = shared_at(room + (kRing ? kVectors * N * blockDim.x : 0)) + threadIdx.x * 16;
-  const unsigned slot_bytes = Sources::kSlot * blockDim.x, bx = V * (unsigned)sizeof(TX) * blockDim.x, by = V * (unsigned)sizeof(TY) * blockDim.x;
-  const Sources s{{column<TX>(n.dh, lane * V), n.dhs, ring},
-                  {column<TX>(n.dz ? n.h : nullptr, lane * V), n.hs, ring + bx},
-                  {column<TY>(n.dz, lane * V), n.dzs, ring + 2 * bx},
-                  {column<TY>(n.y, lane * V), n.ys, ring + 2 * bx + by},
-                  {column<TY>(GATE == EPS_B200_GATE_ELEMENT ? n.g : nullptr, lane * V), n.gs, ring + 2 * bx + 2 * by}};
-  auto ask = [&](unsigned slot, uint64_t r) {
-    if constexpr (kRing) {
-      const bool there = in && r < n.rows;
-      s.dh.ask(n, slot, slot_bytes, r, there);
-      s.h.ask(n, slot, slot_bytes, r, there);
-      s.dz.ask(n, slot, slot_bytes, r, there);
-      s.y.ask(n, slot, slot_bytes, r, there);
-      if (GATE == EPS_B200_GATE_ELEMENT) s.gate.ask(n, slot, slot_bytes, r, there);
+  const unsigned bx = V * (unsigned)sizeof(TX) * blockDim.x, by = V * (unsigned)sizeof(TY) * blockDim.x;
+  const unsigned at_dh = shared_at(room) + Given::kRecord * blockDim.x, at_h = at_dh + bx, at_dz = at_h + bx, at_y = at_dz + by, at_g = at_y + by;
+  Source<TX, V, NIT, kHow> sdh(n, w, n.dh, n.dhs), sh(n, w, n.dz ? n.h : nullptr, n.hs);
+  Source<TY, V, NIT, kHow> sdz(n, w, n.dz, n.dzs), sy(n, w, n.y, n.ys), sg(n, w, GATE == EPS_B200_GATE_ELEMENT ? n.g : nullptr, n.gs);
+  Sink<TX, V, NIT> dx(n, w, n.dx, n.dxs);
+  Sink<TY, V, NIT> dy(n, w, n.dy, n.dys), dg(n, w, GATE == EPS_B200_GATE_ELEMENT ? n.dg : nullptr, n.dgs);
+  unsigned asked = 0;
+  Place fill, here;
+  auto ask = [&] {
+    const bool live = asked++ < w.mine;
+    if constexpr (kHow == kBulk) {
+      if (threadIdx.x == 0 && live) {
+        const unsigned rx = n.columns * (unsigned)sizeof(TX), ry = n.columns * (unsigned)sizeof(TY);
+        uint64_t* const b = arrived + fill.index;
+        barrier_expect(b, (sdh.there ? rx : 0) + (sdz.there ? rx + ry : 0) + (sy.there ? ry : 0) + (GATE == EPS_B200_GATE_ELEMENT ? ry : 0));
+        sdh.ask_row(at_dh + fill.bytes, rx, b);
+        sh.ask_row(at_h + fill.bytes, rx, b);
+        sdz.ask_row(at_dz + fill.bytes, ry, b);
+        sy.ask_row(at_y + fill.bytes, ry, b);
+        if (GATE == EPS_B200_GATE_ELEMENT) sg.ask_row(at_g + fill.bytes, ry, b);
+      }
+    } else if constexpr (kHow == kLanes) {
+      sdh.ask(at_dh + fill.bytes, live);
+      sh.ask(at_h + fill.bytes, live);
+      sdz.ask(at_dz + fill.bytes, live);
+      sy.ask(at_y + fill.bytes, live);
+      if (GATE == EPS_B200_GATE_ELEMENT) sg.ask(at_g + fill.bytes, live);
       asm volatile("cp.async.commit_group;" ::: "memory");
     }
+    fill.next(slot_bytes);
   };
-#pragma unroll
-  for (unsigned k = 0; k < kAhead; ++k) ask(k, row + k * stride);
-  const Parameters<TY, V, NIT, kRing> p{n, room, lane};
-  p.stage();
-  unsigned slot = 0;
-  for (uint64_t pass = 0; pass < passes; ++pass, row += stride) {
-    const bool live = row < n.rows;
-    float d[NIT][V], q[NIT][V], h[NIT][V], y[NIT][V];
-    if constexpr (kRing) {
-      asm volatile("cp.async.wait_group %0;" ::"n"(kAhead - 1) : "memory");
-      ask(slot == 0 ? kSlots - 1 : slot - 1, row + kAhead * stride);
+  ask();
+  ask();
+  const Given p(n, lane, room);
+  const bool layer = n.layer, post = n.post_norm;
+  const TY* row_gates = static_cast<const TY*>(n.g) + w.row;
+
+  // the first row's statistics, of h and of y
+  float mean[2] = {0.f, 0.f}, r[2];
+  float h[NIT][V], y[NIT][V];
+  bool good = arrive<kHow>(arrived, here, true);
+  sh.get(n, at_h, 0 < w.mine, lane, h);
+  sy.get(n, at_y, 0 < w.mine, lane, y);
+  {
+    float s[2];
+    if (layer) {
+      s[0] = share<V, NIT, false>(n, lane, h, 0.f);
+      s[1] = share<V, NIT, false>(n, lane, y, 0.f);
+      row_sum<2, P>(s, n.width, shared, turn);
+      mean[0] = s[0];
+      mean[1] = s[1];
     }
-    s.h.get(n, slot, slot_bytes, row, live, lane, h);
-    s.y.get(n, slot, slot_bytes, row, live, lane, y);
-    float means[2], rs[2];
-    const float(*const both[2])[V] = {h, y};
-    statistics<V, NIT, 2>(n, both, lane, shared, turn, means, rs);
-    s.dh.get(n, slot, slot_bytes, row, live, lane, d);
+    s[0] = share<V, NIT, true>(n, lane, h, mean[0]);
+    s[1] = share<V, NIT, true>(n, lane, y, mean[1]);
+    row_sum<2, P>(s, n.width, shared, turn);
+    r[0] = __frsqrt_rn(s[0] + n.epsilon);
+    r[1] = __frsqrt_rn(s[1] + n.epsilon);
+  }
+  for (unsigned pass = 0; pass < w.passes; ++pass) {
+    const bool live = pass < w.mine, more = pass + 1 < w.mine;
+    if (!post) { mean[1] = 0.f; r[1] = 1.f; }
+    if (!good) r[0] = r[1] = NAN;
+    // the slot of the row before: every lane has passed a barrier since it read it
+    if constexpr (kHow != kDirect) ask();
+    const unsigned now = here.bytes;
+    here.next(slot_bytes);
+    good = arrive<kHow>(arrived, here, pass + 1 < w.passes);
+    float d[NIT][V], q[NIT][V], s[4];
     // through the norm after
-    if (n.dz) {
-      const float r = rs[0];
-      float sum[2] = {0.f, 0.f};
-      s.dz.get(n, slot, slot_bytes, row, live, lane, q);
-#pragma unroll
-      for (int i = 0; i < NIT; ++i) {
-        float w[V];
-        p.get(kPreW, i, w);
-        centre<V>(h[i], means[0], r);
-        add(kPreWeight, i, q[i], h[i]);
-        add(kPreBias, i, q[i], 1.f);
-        vmul<V>(q[i], q[i], w);
-        sum[0] += total<V>(q[i]);
-        vmul<V>(w, q[i], h[i]);
-        sum[1] += total<V>(w);
-      }
-      row_sum<2>(sum, n.width, shared, turn);
-      const float mq = n.layer ? sum[0] * n.inverse_columns : 0.f, mh = sum[1] * n.inverse_columns;
-#pragma unroll
-      for (int i = 0; i < NIT; ++i) {
-        vfma<V>(h[i], h[i], -mh, q[i]);
-        vadd<V>(h[i], h[i], -mq);
-        vfma<V>(d[i], h[i], r, d[i]);
-      }
-    }
-    if (n.dx) {
-#pragma unroll
-      for (int i = 0; i < NIT; ++i) put<TX, V, NIT>(n, n.dx, n.dxs, row, i, lane, live, d[i]);
-    }
-    const unsigned here = slot;
-    slot = slot == kSlots - 1 ? 0 : slot + 1;
-    if (!n.y) continue;
-    // through the scale, the gate and the norm before
-    const float r = rs[1];
-    float ra = 1.f, rslope = 0.f;
-    if (GATE == EPS_B200_GATE_ROW && live) ra = activate_one(to_float(static_cast<const TY*>(n.g)[row]), n.activation, &rslope);
-    float g[NIT][V];
-    if (GATE == EPS_B200_GATE_ELEMENT) s.gate.get(n, here, slot_bytes, row, live, lane, g);
-    float sum[3] = {0.f, 0.f, 0.f};
+    sdz.get(n, at_dz + now, live, lane, q);
+    sdz.next();
+    s[0] = s[1] = 0.f;
 #pragma unroll
     for (int i = 0; i < NIT; ++i) {
-      float w[V], nv[V], a[V], slope[V], t[V];
-      // y becomes its normed value, nv what the gate sees
-      if (n.post_norm) {
-        p.get(kPostW, i, w);
-        p.get(kPostB, i, t);
-        centre<V>(y[i], means[1], r);
-        vfma<V>(nv, y[i], w, t);
-      } else {
+      float u[V];
+      p.get(2, i, u);
+      centre<V>(h[i], mean[0], r[0]);
+      add(kPreWeight, i, q[i], h[i]);
+      add(kPreBias, i, q[i], 1.f);
+      vmul<V>(q[i], q[i], u);               // 0 behind the row's end
+      s[0] += total<V>(q[i]);
+      vmul<V>(u, q[i], h[i]);
+      s[1] += total<V>(u);
+    }
+    // the next row's means, or mean squares, of h and y
+    sh.next();
+    sy.next();
+    {
+      float t[NIT][V];
+      sh.get(n, at_h + here.bytes, more, lane, t);
+      s[2] = layer ? share<V, NIT, false>(n, lane, t, 0.f) : share<V, NIT, true>(n, lane, t, 0.f);
+      sy.get(n, at_y + here.bytes, more, lane, t);
+      s[3] = layer ? share<V, NIT, false>(n, lane, t, 0.f) : share<V, NIT, true>(n, lane, t, 0.f);
+    }
+    row_sum<4, P>(s, n.width, shared, turn);
+    const float mq = layer ? s[0] * n.inverse_columns : 0.f, mh = s[1] * n.inverse_columns, next_h = s[2], next_y = s[3];
+    sdh.get(n, at_dh + now, live, lane, d);
+    sdh.next();
 #pragma unroll
-        for (int j = 0; j < V; ++j) { nv[j] = y[i][j]; w[j] = 1.f; }
-      }
+    for (int i = 0; i < NIT; ++i) {
+      vfma<V>(h[i], h[i], -mh, q[i]);
+      vadd<V>(h[i], h[i], -mq);
+      vfma<V>(d[i], h[i], r[0], d[i]);
+      dx.put(n, i, lane, live, d[i]);
+    }
+    dx.next();
+    // through the scale, the gate and the norm before
+    float open = 1.f, slope1 = 0.f, sum_gate[1] = {0.f};
+    if (GATE == EPS_B200_GATE_ROW && live) open = activate_one(to_float(*row_gates), n.activation, &slope1);
+    float g[NIT][V];
+    if (GATE == EPS_B200_GATE_ELEMENT) {
+      sg.get(n, at_g + now, live, lane, g);
+      sg.next();
+    }
+    s[0] = s[1] = 0.f;
+#pragma unroll
+    for (int i = 0; i < NIT; ++i) {
+      float nv[V], a[V], slope[V], u[V];
+      p.get(0, i, u);
+      p.get(1, i, nv);
+      centre<V>(y[i], mean[1], r[1]);
+      vfma<V>(nv, y[i], u, nv);             // what the gate sees
       if (GATE == EPS_B200_GATE_ELEMENT) {
         activate<V, true>(g[i], n.activation, a, slope);
         vmul<V>(a, a, d[i]);
       } else {
-        vmul<V>(a, d[i], ra);
+        vmul<V>(a, d[i], open);
       }
-      add(kChannel, i, a, nv);          // without n.scale, which the block's sums take at the end
-      p.get(kScaleC, i, t);
+      add(kChannel, i, a, nv);              // without n.scale, which the block's sums take at the end
+      p.get(3, i, q[i]);
       if (GATE != EPS_B200_GATE_NONE) {
         vmul<V>(nv, nv, d[i]);
-        vmul<V>(nv, nv, t);
+        vmul<V>(nv, nv, q[i]);
         if (GATE == EPS_B200_GATE_ELEMENT) {
           vmul<V>(nv, nv, slope);
-          if (n.dg) put<TY, V, NIT>(n, n.dg, n.dgs, row, i, lane, live, nv);
+          dg.put(n, i, lane, live, nv);
         } else {
-          sum[2] += total<V>(nv);
+          sum_gate[0] += total<V>(nv);
         }
       }
-      vmul<V>(q[i], a, t);
-      if (n.post_norm) {
-        add(kPostWeight, i, q[i], y[i]);
-        add(kPostBias, i, q[i], 1.f);
-        vmul<V>(q[i], q[i], w);
-        sum[0] += total<V>(q[i]);
-        vmul<V>(t, q[i], y[i]);
-        sum[1] += total<V>(t);
-      }
+      vmul<V>(q[i], q[i], a);
+      add(kPostWeight, i, q[i], y[i]);
+      add(kPostBias, i, q[i], 1.f);
+      vmul<V>(q[i], q[i], u);               // 0 behind the row's end
+      s[0] += total<V>(q[i]);
+      vmul<V>(u, q[i], y[i]);
+      s[1] += total<V>(u);
     }
+    dg.next();
     if (GATE == EPS_B200_GATE_ROW) {
-      row_sum<3>(sum, n.width, shared, turn);
-      if (live && lane == 0 && n.dg) static_cast<TY*>(n.dg)[row] = from_float<TY>(sum[2] * rslope);
-    } else if (n.post_norm) {
-      row_sum<2>(reinterpret_cast<float(&)[2]>(sum), n.width, shared, turn);
+      row_sum<1, P>(sum_gate, n.width, shared, turn);
+      if (live && lane == 0 && n.dg) static_cast<TY*>(n.dg)[row_gates - static_cast<const TY*>(n.g)] = from_float<TY>(sum_gate[0] * slope1);
+      row_gates += w.stride;
     }
-    const float mp = n.layer ? sum[0] * n.inverse_columns : 0.f, my = sum[1] * n.inverse_columns;
-    if (n.dy) {
+    const float r_now = r[1];
+    if (layer) {
+      float t[NIT][V];
+      mean[0] = next_h;
+      mean[1] = next_y;
+      sh.get(n, at_h + here.bytes, more, lane, t);
+      s[2] = share<V, NIT, true>(n, lane, t, mean[0]);
+      sy.get(n, at_y + here.bytes, more, lane, t);
+      s[3] = share<V, NIT, true>(n, lane, t, mean[1]);
+      row_sum<4, P>(s, n.width, shared, turn);
+    } else {
+      row_sum<2, P>(reinterpret_cast<float(&)[2]>(s), n.width, shared, turn);
+      s[2] = next_h;
+      s[3] = next_y;
+    }
+    const float mp = layer && post ? s[0] * n.inverse_columns : 0.f, my = post ? s[1] * n.inverse_columns : 0.f;
 #pragma unroll
-      for (int i = 0; i < NIT; ++i) {
-        if (n.post_norm) {
-          vfma<V>(q[i], y[i], -my, q[i]);
-          vadd<V>(q[i], q[i], -mp);
-          vmul<V>(q[i], q[i], r);
-        }
-        put<TY, V, NIT>(n, n.dy, n.dys, row, i, lane, live, q[i]);
-      }
+    for (int i = 0; i < NIT; ++i) {
+      vfma<V>(q[i], y[i], -my, q[i]);
+      vadd<V>(q[i], q[i], -mp);
+      vmul<V>(q[i], q[i], r_now);
+      dy.put(n, i, lane, live, q[i]);
     }
+    dy.next();
+    r[0] = __frsqrt_rn(s[2] + n.epsilon);
+    r[1] = __frsqrt_rn(s[3] + n.epsilon);
+    sh.get(n, at_h + here.bytes, more, lane, h);
+    sy.get(n, at_y + here.bytes, more, lane, y);
   }
-  if constexpr (kRing) asm volatile("cp.async.wait_all;" ::: "memory");
+  if constexpr (kHow == kLanes) asm volatile("cp.async.wait_all;" ::: "memory");
   if (!wanted) return;
   if constexpr (kHeld) {
     __syncthreads();        // the staged parameters and the ring lie there
 #pragma unroll
     for (int k = 0; k < kSums; ++k)
-      if (slot_of[k] >= 0) {
+      if (n.want >> k & 1) {
 #pragma unroll
-        for (int j = 0; j < V; ++j) room[slot_of[k] * cell + j * blockDim.x + threadIdx.x] = held[k][j];
+        for (int j = 0; j < V; ++j) sums[slot_of(k) * cell + j * blockDim.x + threadIdx.x] = held[k][j];
       }
   }
   __syncthreads();
@@ -595,9 +728,9 @@ __global__ void __launch_bounds__(V == 8 ? 512 : 1024) block_norm_gradient(const
     const unsigned at = c / V, i = at / n.width, l = at % n.width, j = c % V;
 #pragma unroll
     for (int k = 0; k < kSums; ++k) {
-      if (slot_of[k] < 0) continue;
+      if (!(n.want >> k & 1)) continue;
       float t = 0.f;
-      for (unsigned g = 0; g < groups; ++g) t += room[slot_of[k] * cell + (i * V + j) * blockDim.x + g * n.width + l];
+      for (unsigned g = 0; g < groups; ++g) t += sums[slot_of(k) * cell + (i * V + j) * blockDim.x + g * n.width + l];
       n.partial[((uint64_t)blockIdx.x * kSums + k) * n.columns + c] = k == kChannel ? t * n.scale : t;
     }
   }
@@ -632,16 +765,24 @@ __global__ void __launch_bounds__(32 * kRuns) block_norm_columns(const Columns p
 // How a row is spread: V elements a lane, `nit` times, over `width` lanes.
 struct Spread { int v, nit; unsigned width, threads; };
 
-Spread spread_of(unsigned columns, bool wide) {
+// The elements of a wide access of these types.
+template <class TX, class TY>
+constexpr int kWide = std::is_same_v<TY, float> ? 4 : 8;
+
+// A lane holds one wide pack where that fits 512 lanes (and, for a float residual
+// of a 16-bit block, the shared memory of 256), else up to sixteen elements; without
+// 16-byte alignment four or sixteen single ones.
+Spread spread_of(unsigned columns, int residual, int type, bool wide) {
   Spread s{};
-  s.v = wide ? 8 : 1;
+  s.v = !wide ? 1 : type == EPS_B200_F32 ? 4 : 8;
   const unsigned packs = (unsigned)ceil_div(columns, s.v);
-  s.nit = wide ? (packs <= 512 ? 1 : 2) : (packs <= 32 ? 1 : packs <= 1024 ? 4 : 8);
+  if (!wide) s.nit = packs <= 32 ? 1 : packs <= 1024 ? 4 : 16;
+  else s.nit = packs <= (residual != type ? 256 : 512) ? 1 : packs <= 1024 ? 2 : 4;
   const unsigned lanes = (unsigned)ceil_div(packs, s.nit);
   if (lanes <= 32) {
     s.width = 1;
     while (s.width < lanes) s.width *= 2;
-    s.threads = 128;
+    s.threads = kLanesThreads;
   } else {
     s.width = s.threads = (unsigned)round_up(lanes, 32);
   }
@@ -653,6 +794,7 @@ constexpr unsigned kMostBlocks = 8 * 160;   // of the gradient: 8 an SM, 160 SMs
 // Blocks that fit the GPU at once, or fewer where the rows need fewer.
 template <class K>
 unsigned resident(K kernel, const Spread& s, size_t shared, uint64_t rows, unsigned sms, unsigned most) {
+  check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)shared), "cudaFuncSetAttribute");
   int each = 0;
   check(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&each, kernel, (int)s.threads, shared), "occupancy");
   need(each > 0, "no room for a block");
@@ -662,24 +804,22 @@ unsigned resident(K kernel, const Spread& s, size_t shared, uint64_t rows, unsig
   return (unsigned)(all < n ? all : n);
 }
 
-template <class TX, class TY, int V, int NIT, int GATE>
+template <class TX, class TY, int V, int NIT, int P, int GATE>
 void forward(const Norm& n, const Spread& s, unsigned sms, cudaStream_t stream) {
-  auto* kernel = block_norm_forward<TX, TY, V, NIT, GATE>;
-  using Sources = ForwardSources<TX, TY, V, NIT>;
-  const unsigned shared = ((V * NIT <= 8 ? kVectors * NIT * V * 4 : 0) + (Sources::kRing ? kSlots * Sources::kSlot : 0)) * s.threads;
-  check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 224 * 1024), "cudaFuncSetAttribute");
-  kernel<<<resident(kernel, s, shared, n.rows, sms, ~0u), s.threads, shared, stream>>>(n);
+  auto* kernel = block_norm_forward<TX, TY, V, NIT, P, GATE>;
+  const unsigned lane = Parameters<TY, V, NIT, V * NIT <= 8, true>::kRecord + (kWay<V, NIT, P> != kDirect ? kSlots * forward_bytes<TX, TY, V>() : 0);
+  kernel<<<resident(kernel, s, lane * s.threads, n.rows, sms, ~0u), s.threads, lane * s.threads, stream>>>(n);
   check(cudaGetLastError(), "block_norm");
 }
 
 // The number of blocks, which is the number of partial sums.
-template <class TX, class TY, int V, int NIT, int GATE>
+template <class TX, class TY, int V, int NIT, int P, int GATE>
 unsigned backward(const Norm& n, const Spread& s, unsigned sms, uint64_t room, cudaStream_t stream) {
-  auto* kernel = block_norm_gradient<TX, TY, V, NIT, GATE>;
-  using Sources = BackwardSources<TX, TY, V, NIT>;
-  const unsigned vectors = Sources::kRing ? kVectors : (unsigned)__builtin_popcount((unsigned)n.want);
-  const unsigned shared = (vectors * NIT * V * 4 + (Sources::kRing ? kSlots * Sources::kSlot : 0)) * s.threads;
-  check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 224 * 1024), "cudaFuncSetAttribute");
+  auto* kernel = block_norm_gradient<TX, TY, V, NIT, P, GATE>;
+  constexpr bool kRing = kWay<V, NIT, P> != kDirect;
+  const unsigned held = (unsigned)__builtin_popcount((unsigned)n.want) * NIT * V * 4;
+  const unsigned walked = kRing ? Parameters<TY, V, NIT, true, false>::kRecord + kSlots * backward_bytes<TX, TY, V>() : 0;
+  const unsigned shared = (walked > held ? walked : held) * s.threads;       // the sums take the others' place in the end
   const unsigned blocks = resident(kernel, s, shared, n.rows, sms, kMostBlocks);
   need(!n.want || room >= (uint64_t)blocks * kSums * n.columns * 4, "block norm workspace too small");
   kernel<<<blocks, s.threads, shared, stream>>>(n);
@@ -695,10 +835,22 @@ void by_gate(int gate, F f) {
                                                                                         : f(Int<EPS_B200_GATE_ELEMENT>{});
 }
 
-template <class F>
+// f(V, NIT, P): P as row_sum has it.
+template <int W, class F>
 void by_spread(const Spread& s, F f) {
-  if (s.v == 8) s.nit == 1 ? f(Int<8>{}, Int<1>{}) : f(Int<8>{}, Int<2>{});
-  else s.nit == 1 ? f(Int<1>{}, Int<1>{}) : s.nit == 4 ? f(Int<1>{}, Int<4>{}) : f(Int<1>{}, Int<8>{});
+  const unsigned warps = s.width / 32;
+  if (s.v == W) {
+    if (s.nit == 4) { if constexpr (W == 4) f(Int<W>{}, Int<4>{}, Int<16>{}); }
+    else if (s.nit == 2) f(Int<W>{}, Int<2>{}, Int<16>{});
+    else if (warps <= 1) f(Int<W>{}, Int<1>{}, Int<1>{});
+    else if (warps <= 4) f(Int<W>{}, Int<1>{}, Int<4>{});
+    else if (warps <= 8) f(Int<W>{}, Int<1>{}, Int<8>{});
+    else f(Int<W>{}, Int<1>{}, Int<16>{});
+  } else {
+    if (s.nit == 1) f(Int<1>{}, Int<1>{}, Int<1>{});
+    else if (s.nit == 16) f(Int<1>{}, Int<16>{}, Int<16>{});
+    else warps <= 1 ? f(Int<1>{}, Int<4>{}, Int<1>{}) : f(Int<1>{}, Int<4>{}, Int<8>{});
+  }
 }
 
 template <class F>
@@ -708,8 +860,7 @@ void by_type(int residual, int type, F f) {
   else residual == EPS_B200_F32 ? f(float{}, f16{}) : f(f16{}, f16{});
 }
 
-// Whether rows at `p` with this stride (elements) and type take 16-byte accesses
-// of eight (or four) elements.
+// Whether rows at `p` with this stride (elements) and type take 16-byte accesses.
 bool rows_wide(const void* p, int64_t stride, int type) {
   return !p || (aligned(p, 16) && stride * (int64_t)size_of(type) % 16 == 0);
 }
@@ -723,7 +874,7 @@ Norm checked(const EpsB200BlockNorm* a) {
   need(a->residual_type == a->type || a->residual_type == EPS_B200_F32, "the residual has the block's type or float32");
   need(a->parameter_type == a->type || a->parameter_type == EPS_B200_F32, "parameters have the block's type or float32");
   need(a->columns > 0 && a->columns <= EPS_B200_BLOCK_NORM_COLUMNS, "columns out of range");
-  need(a->rows < (1ull << 40), "too many rows");
+  need(a->rows < (1ull << 31), "too many rows");
   need(a->epsilon > 0.f && a->epsilon < 1e30f, "epsilon must be positive");
   need(a->scale == a->scale, "the scale is not a number");
   // tensors without rows may have no address
@@ -750,13 +901,15 @@ Norm checked(const EpsB200BlockNorm* a) {
   n.channel = a->channel_scale;
   n.pre_w = a->pre_weight;
   n.pre_b = a->pre_bias;
+  if (!n.post_norm) n.post_w = n.post_b = nullptr;
+  if (!n.y) n.post_b = nullptr;      // then the block adds nothing
   return n;
 }
 
-bool parameters_wide(const Norm& n) {
+bool parameters_wide(const Norm& n, int type) {
   for (const void* p : {n.post_w, n.post_b, n.channel, n.pre_w, n.pre_b})
     if (!aligned(p, 16)) return false;
-  return n.columns % 8 == 0;
+  return n.columns % (type == EPS_B200_F32 ? 4 : 8) == 0;
 }
 
 }  // namespace
@@ -780,15 +933,16 @@ int eps_b200_block_norm(const EpsB200BlockNorm* a, const void* x, int64_t x_stri
     n.out_z = z; n.out_zs = z_stride;
     if (!n.out_h && !n.pre_norm) return;
     OnDevice on(a->device);
-    bool wide = parameters_wide(n) && rows_wide(n.y, n.ys, a->type) && rows_wide(x, x_stride, a->residual_type) &&
+    bool wide = parameters_wide(n, a->type) && rows_wide(n.y, n.ys, a->type) && rows_wide(x, x_stride, a->residual_type) &&
                 rows_wide(h, h_stride, a->residual_type) && rows_wide(z, z_stride, a->type);
     if (n.gate == EPS_B200_GATE_ELEMENT) wide = wide && rows_wide(n.g, n.gs, a->type);
-    const Spread s = spread_of(n.columns, wide);
+    const Spread s = spread_of(n.columns, a->residual_type, a->type, wide);
     n.width = s.width;
     by_type(a->residual_type, a->type, [&](auto tx, auto ty) {
-      by_spread(s, [&](auto v, auto nit) {
+      by_spread<kWide<decltype(tx), decltype(ty)>>(s, [&](auto v, auto nit, auto warps) {
         by_gate(n.gate, [&](auto gate) {
-          forward<decltype(tx), decltype(ty), decltype(v)::value, decltype(nit)::value, decltype(gate)::value>(
+          forward<decltype(tx), decltype(ty), decltype(v)::value, decltype(nit)::value, decltype(warps)::value,
+                  decltype(gate)::value>(
               n, s, sm_count(a->device), static_cast<cudaStream_t>(stream));
         });
       });
@@ -818,6 +972,7 @@ int eps_b200_block_norm_backward(const EpsB200BlockNorm* a, const EpsB200BlockNo
     n.dh = d->dh; n.dhs = d->dh_stride;
     n.dz = d->dz; n.dzs = d->dz_stride;
     n.h = d->h; n.hs = d->h_stride;
+    n.somewhere = n.dz ? n.dz : n.dh ? n.dh : n.y ? n.y : d->dx ? d->dx : d->workspace;
     n.somewhere = n.dz ? n.dz : n.dh ? n.dh : n.y ? n.y : d->dx;
     n.dx = d->dx; n.dxs = d->dx_stride;
     n.dy = d->dy; n.dys = d->dy_stride;
@@ -832,19 +987,21 @@ int eps_b200_block_norm_backward(const EpsB200BlockNorm* a, const EpsB200BlockNo
         if (o) check(cudaMemsetAsync(o, 0, n.columns * 4, st), "cudaMemsetAsync");
       return;
     }
-    bool wide = parameters_wide(n) && rows_wide(n.y, n.ys, a->type) && rows_wide(n.dh, n.dhs, a->residual_type) &&
+    if (!n.somewhere) return;       // nothing comes in and nothing is asked for
+    bool wide = parameters_wide(n, a->type) && rows_wide(n.y, n.ys, a->type) && rows_wide(n.dh, n.dhs, a->residual_type) &&
                 rows_wide(n.dz, n.dzs, a->type) && rows_wide(n.h, n.hs, a->residual_type) &&
                 rows_wide(n.dx, n.dxs, a->residual_type) && rows_wide(n.dy, n.dys, a->type);
     if (n.gate == EPS_B200_GATE_ELEMENT) wide = wide && rows_wide(n.g, n.gs, a->type) && rows_wide(n.dg, n.dgs, a->type);
-    const Spread s = spread_of(n.columns, wide);
+    const Spread s = spread_of(n.columns, a->residual_type, a->type, wide);
     n.width = s.width;
     need(!n.want || (d->workspace && aligned(d->workspace, 16)), "the workspace must be there and 16-byte aligned");
     unsigned blocks = 0;
     n.partial = static_cast<float*>(d->workspace);
     by_type(a->residual_type, a->type, [&](auto tx, auto ty) {
-      by_spread(s, [&](auto v, auto nit) {
+      by_spread<kWide<decltype(tx), decltype(ty)>>(s, [&](auto v, auto nit, auto warps) {
         by_gate(n.gate, [&](auto gate) {
-          blocks = backward<decltype(tx), decltype(ty), decltype(v)::value, decltype(nit)::value, decltype(gate)::value>(
+          blocks = backward<decltype(tx), decltype(ty), decltype(v)::value, decltype(nit)::value, decltype(warps)::value,
+                  decltype(gate)::value>(
               n, s, sm_count(a->device), d->workspace_bytes, st);
         });
       });

@@ -169,46 +169,6 @@ struct MmaShape {
   static constexpr unsigned columns = 2 * BN;                          // of tensor memory
 };
 
-__device__ __forceinline__ void barrier_init(uint64_t* b, unsigned count) {
-  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(shared_at(b)), "r"(count) : "memory");
-}
-
-__device__ __forceinline__ void barrier_arrive(uint64_t* b) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(shared_at(b)) : "memory");
-}
-
-__device__ __forceinline__ void barrier_expect(uint64_t* b, unsigned bytes) {
-  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(shared_at(b)), "r"(bytes) : "memory");
-}
-
-__device__ __forceinline__ uint64_t nanoseconds() {
-  uint64_t t;
-  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-  return t;
-}
-
-// Waits for the phase of this parity to end; false after two seconds, which no
-// working kernel comes near.  The caller then leaves its loop, and the tile's rows
-// become NaN instead of the GPU hanging.
-__device__ __forceinline__ bool barrier_wait(uint64_t* b, unsigned parity) {
-  const unsigned address = shared_at(b);
-  uint64_t start = 0;
-  for (unsigned tries = 1;; ++tries) {
-    unsigned done;
-    asm volatile(
-        "{\n .reg .pred p;\n"
-        " mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
-        " selp.u32 %0, 1, 0, p;\n}\n"
-        : "=r"(done) : "r"(address), "r"(parity) : "memory");
-    if (done) return true;
-    if (tries % 256 == 0) {
-      const uint64_t now = nanoseconds();
-      if (!start) start = now;
-      else if (now - start > 2000000000ull) return false;
-    }
-  }
-}
-
 __device__ __forceinline__ void tma_load(void* to, const CUtensorMap* map, uint64_t* barrier, int x, int y) {
   asm volatile("cp.async.bulk.tensor.2d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
                ::"r"(shared_at(to)), "l"(map), "r"(shared_at(barrier)), "r"(x), "r"(y) : "memory");
