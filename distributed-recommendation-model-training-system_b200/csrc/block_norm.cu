@@ -233,18 +233,28 @@ __device__ __forceinline__ void copy16(unsigned to, const void* from, bool there
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(there ? 16 : 0) : "memory");
 }
 
-// What both directions share: the block's rows, and the lane's.
+// What both directions share: the block's rows, and the lane's.  Where a block has one
+// row at a time, all but `lane` is the same for all threads, and written so that the
+// compiler can tell: it then costs no registers of the lanes.
+template <Way WAY, int P>
 struct Walk {
   unsigned lane, passes, mine;             // passes of the block, and how many of them have a row for this lane
   uint64_t stride, row;
   __device__ __forceinline__ explicit Walk(const Norm& n) {
-    lane = threadIdx.x % n.width;
-    const unsigned groups = blockDim.x / n.width;
-    stride = (uint64_t)gridDim.x * groups;
-    const uint64_t first = (uint64_t)blockIdx.x * groups;     // blocks do not outnumber groups of rows
-    row = first + threadIdx.x / n.width;
-    passes = (unsigned)((n.rows - first + stride - 1) / stride);
-    mine = row < n.rows ? (unsigned)((n.rows - row + stride - 1) / stride) : 0;
+    if constexpr (P > 1) {
+      lane = threadIdx.x;
+      stride = gridDim.x;
+      row = blockIdx.x;
+      passes = mine = (unsigned)((n.rows - row + stride - 1) / stride);
+    } else {
+      lane = threadIdx.x % n.width;
+      const unsigned groups = blockDim.x / n.width;
+      stride = (uint64_t)gridDim.x * groups;
+      const uint64_t first = (uint64_t)blockIdx.x * groups;     // blocks do not outnumber groups of rows
+      row = first + threadIdx.x / n.width;
+      passes = (unsigned)((n.rows - first + stride - 1) / stride);
+      mine = row < n.rows ? (unsigned)((n.rows - row + stride - 1) / stride) : 0;
+    }
   }
 };
 
@@ -253,26 +263,27 @@ struct Walk {
 template <class T, int V, int NIT, Way WAY>
 struct Source {
   static constexpr unsigned kBytes = V * sizeof(T);
-  const char* p;           // kBulk: the next row; else the lane's place in it
+  const char* p;           // the next row
   int64_t step;            // bytes from one row of the walk to the next
-  bool there;              // the tensor is given (and the lane's first pack lies in its row)
+  bool there;              // the tensor is given
 
-  __device__ __forceinline__ Source(const Norm& n, const Walk& w, const void* tensor, int64_t stride) {
-    there = tensor && (WAY == kBulk || w.lane * V < n.columns);
-    const int64_t from = (int64_t)w.row * stride + (WAY == kBulk ? 0 : w.lane * V);
-    p = there ? static_cast<const char*>(tensor) + from * (int64_t)sizeof(T) : static_cast<const char*>(n.somewhere);
+  template <class W>
+  __device__ __forceinline__ Source(const Norm& n, const W& w, const void* tensor, int64_t stride) {
+    there = tensor != nullptr;
+    p = there ? static_cast<const char*>(tensor) + (int64_t)w.row * stride * (int64_t)sizeof(T) : static_cast<const char*>(n.somewhere);
     step = there ? (int64_t)w.stride * stride * (int64_t)sizeof(T) : 0;
   }
   // to: the tensor's bytes in a slot, a shared address
-  __device__ __forceinline__ void ask(unsigned to, bool live) {
+  __device__ __forceinline__ void ask(unsigned to, bool live, unsigned lane) {
 #pragma unroll
-    for (unsigned k = 0; k < kBytes / 16; ++k) copy16(to + (k * kLanesThreads + threadIdx.x) * 16, p + k * 16, live && there);
+    for (unsigned k = 0; k < kBytes / 16; ++k)
+      copy16(to + (k * kLanesThreads + threadIdx.x) * 16, p + (live && there ? lane * kBytes + k * 16 : 0), live && there);
     p += step;
   }
   __device__ __forceinline__ void ask_row(unsigned to, unsigned row_bytes, uint64_t* barrier) {
     if (there) bulk_copy(to, p, row_bytes, barrier);
-    p += step;
   }
+  __device__ __forceinline__ void asked_row() { p += step; }
   __device__ __forceinline__ void get(const Norm& n, unsigned from, bool live, unsigned lane, float (&r)[NIT][V]) {
     if constexpr (WAY != kDirect) {
       Pack<T, V> x;
@@ -286,8 +297,9 @@ struct Source {
     } else {
 #pragma unroll
       for (int i = 0; i < NIT; ++i) {
+        const unsigned c = (i * n.width + lane) * V;
         Pack<T, V> x{};
-        if (live && there && (i * n.width + lane) * V < n.columns) x = load_once<T, V>(reinterpret_cast<const T*>(p) + i * n.width * V);
+        if (live && there && c < n.columns) x = load_once<T, V>(reinterpret_cast<const T*>(p) + c);
         widen(x, r[i]);
       }
     }
@@ -302,15 +314,14 @@ template <class T, int V, int NIT>
 struct Sink {
   char* p;
   int64_t step;
-  bool there;
-  __device__ __forceinline__ Sink(const Norm& n, const Walk& w, void* tensor, int64_t stride) {
-    there = tensor && w.lane * V < n.columns;
-    p = static_cast<char*>(tensor) + (there ? ((int64_t)w.row * stride + w.lane * V) * (int64_t)sizeof(T) : 0);
-    step = there ? (int64_t)w.stride * stride * (int64_t)sizeof(T) : 0;
+  template <class W>
+  __device__ __forceinline__ Sink(const W& w, void* tensor, int64_t stride) {
+    p = static_cast<char*>(tensor) + (tensor ? (int64_t)w.row * stride * (int64_t)sizeof(T) : 0);
+    step = tensor ? (int64_t)w.stride * stride * (int64_t)sizeof(T) : 0;
   }
   __device__ __forceinline__ void put(const Norm& n, int i, unsigned lane, bool live, const float (&v)[V]) const {
-    if (live && there && (i == 0 || (i * n.width + lane) * V < n.columns))
-      store_pack<T, V>(reinterpret_cast<T*>(p) + i * n.width * V, narrow<T, V>(v));
+    const unsigned c = (i * n.width + lane) * V;
+    if (live && p && c < n.columns) store_pack<T, V>(reinterpret_cast<T*>(p) + c, narrow<T, V>(v));
   }
   __device__ __forceinline__ void next() { p += step; }
 };
@@ -361,15 +372,15 @@ __global__ void __launch_bounds__(512) block_norm_forward(const Norm n) {
   clear_row_sums<P>(shared);
   open_ring<kHow>(room + Given::kRecord * blockDim.x, kSlots * slot_bytes, arrived);
   unsigned turn = 0;
-  const Walk w(n);
+  const Walk<kHow, P> w(n);
   const unsigned lane = w.lane;
   // the tensors' places in a slot
   const unsigned at_x = shared_at(room) + Given::kRecord * blockDim.x, at_y = at_x + V * (unsigned)sizeof(TX) * blockDim.x,
                  at_g = at_y + V * (unsigned)sizeof(TY) * blockDim.x;
   Source<TX, V, NIT, kHow> x(n, w, n.x, n.xs);
   Source<TY, V, NIT, kHow> y(n, w, n.y, n.ys), gate(n, w, GATE == EPS_B200_GATE_ELEMENT ? n.g : nullptr, n.gs);
-  Sink<TX, V, NIT> h(n, w, n.out_h, n.out_hs);
-  Sink<TY, V, NIT> z(n, w, n.out_z, n.out_zs);
+  Sink<TX, V, NIT> h(w, n.out_h, n.out_hs);
+  Sink<TY, V, NIT> z(w, n.out_z, n.out_zs);
   unsigned asked = 0;
   Place fill, here;
   auto ask = [&] {
@@ -382,10 +393,13 @@ __global__ void __launch_bounds__(512) block_norm_forward(const Norm n) {
         y.ask_row(at_y + fill.bytes, by, arrived + fill.index);
         if (GATE == EPS_B200_GATE_ELEMENT) gate.ask_row(at_g + fill.bytes, by, arrived + fill.index);
       }
+      x.asked_row();
+      y.asked_row();
+      gate.asked_row();
     } else if constexpr (kHow == kLanes) {
-      x.ask(at_x + fill.bytes, live);
-      y.ask(at_y + fill.bytes, live);
-      if (GATE == EPS_B200_GATE_ELEMENT) gate.ask(at_g + fill.bytes, live);
+      x.ask(at_x + fill.bytes, live && lane * V < n.columns, lane);
+      y.ask(at_y + fill.bytes, live && lane * V < n.columns, lane);
+      if (GATE == EPS_B200_GATE_ELEMENT) gate.ask(at_g + fill.bytes, live && lane * V < n.columns, lane);
       asm volatile("cp.async.commit_group;" ::: "memory");
     }
     fill.next(slot_bytes);
@@ -499,7 +513,7 @@ __global__ void __launch_bounds__(512) block_norm_gradient(const Norm n) {
   clear_row_sums<P>(shared);
   open_ring<kHow>(room + Given::kRecord * blockDim.x, kSlots * slot_bytes, arrived);
   unsigned turn = 0;
-  const Walk w(n);
+  const Walk<kHow, P> w(n);
   const unsigned lane = w.lane, groups = blockDim.x / n.width;
   const unsigned cell = N * blockDim.x;
   const unsigned wanted = __popc(n.want);
@@ -532,8 +546,8 @@ __global__ void __launch_bounds__(512) block_norm_gradient(const Norm n) {
   const unsigned at_dh = shared_at(room) + Given::kRecord * blockDim.x, at_h = at_dh + bx, at_dz = at_h + bx, at_y = at_dz + by, at_g = at_y + by;
   Source<TX, V, NIT, kHow> sdh(n, w, n.dh, n.dhs), sh(n, w, n.dz ? n.h : nullptr, n.hs);
   Source<TY, V, NIT, kHow> sdz(n, w, n.dz, n.dzs), sy(n, w, n.y, n.ys), sg(n, w, GATE == EPS_B200_GATE_ELEMENT ? n.g : nullptr, n.gs);
-  Sink<TX, V, NIT> dx(n, w, n.dx, n.dxs);
-  Sink<TY, V, NIT> dy(n, w, n.dy, n.dys), dg(n, w, GATE == EPS_B200_GATE_ELEMENT ? n.dg : nullptr, n.dgs);
+  Sink<TX, V, NIT> dx(w, n.dx, n.dxs);
+  Sink<TY, V, NIT> dy(w, n.dy, n.dys), dg(w, GATE == EPS_B200_GATE_ELEMENT ? n.dg : nullptr, n.dgs);
   unsigned asked = 0;
   Place fill, here;
   auto ask = [&] {
@@ -549,12 +563,17 @@ __global__ void __launch_bounds__(512) block_norm_gradient(const Norm n) {
         sy.ask_row(at_y + fill.bytes, ry, b);
         if (GATE == EPS_B200_GATE_ELEMENT) sg.ask_row(at_g + fill.bytes, ry, b);
       }
+      sdh.asked_row();
+      sh.asked_row();
+      sdz.asked_row();
+      sy.asked_row();
+      sg.asked_row();
     } else if constexpr (kHow == kLanes) {
-      sdh.ask(at_dh + fill.bytes, live);
-      sh.ask(at_h + fill.bytes, live);
-      sdz.ask(at_dz + fill.bytes, live);
-      sy.ask(at_y + fill.bytes, live);
-      if (GATE == EPS_B200_GATE_ELEMENT) sg.ask(at_g + fill.bytes, live);
+      sdh.ask(at_dh + fill.bytes, live && lane * V < n.columns, lane);
+      sh.ask(at_h + fill.bytes, live && lane * V < n.columns, lane);
+      sdz.ask(at_dz + fill.bytes, live && lane * V < n.columns, lane);
+      sy.ask(at_y + fill.bytes, live && lane * V < n.columns, lane);
+      if (GATE == EPS_B200_GATE_ELEMENT) sg.ask(at_g + fill.bytes, live && lane * V < n.columns, lane);
       asm volatile("cp.async.commit_group;" ::: "memory");
     }
     fill.next(slot_bytes);
@@ -683,12 +702,12 @@ __global__ void __launch_bounds__(512) block_norm_gradient(const Norm n) {
       row_gates += w.stride;
     }
     const float r_now = r[1];
+    sh.get(n, at_h + here.bytes, more, lane, h);
     if (layer) {
       float t[NIT][V];
       mean[0] = next_h;
       mean[1] = next_y;
-      sh.get(n, at_h + here.bytes, more, lane, t);
-      s[2] = share<V, NIT, true>(n, lane, t, mean[0]);
+      s[2] = share<V, NIT, true>(n, lane, h, mean[0]);
       sy.get(n, at_y + here.bytes, more, lane, t);
       s[3] = share<V, NIT, true>(n, lane, t, mean[1]);
       row_sum<4, P>(s, n.width, shared, turn);
@@ -708,7 +727,6 @@ __global__ void __launch_bounds__(512) block_norm_gradient(const Norm n) {
     dy.next();
     r[0] = __frsqrt_rn(s[2] + n.epsilon);
     r[1] = __frsqrt_rn(s[3] + n.epsilon);
-    sh.get(n, at_h + here.bytes, more, lane, h);
     sy.get(n, at_y + here.bytes, more, lane, y);
   }
   if constexpr (kHow == kLanes) asm volatile("cp.async.wait_all;" ::: "memory");
