@@ -13,14 +13,16 @@
 //
 // A warp owns a token; lane l holds experts l * EPL .. l * EPL + EPL - 1.  Ranking is
 // on unsigned images of the keys (`image`), so one warp instruction finds the best
-// key and the lowest lane that holds it owns the lowest index.
+// key and the lowest lane that holds it owns the lowest index.  What bounds it is the
+// number of instructions a token takes (the logits of a batch are a few megabytes):
+// a lane keeps its own best key and looks again only when that has been taken.
 //
 // The sort by expert is a counting sort in three steps.  A tile is the tokens of one
 // block; each of its warps counts its own run of consecutive tokens, whose experts
 // are distinct within a token, so counting needs no atomics and an entry's count
 // before its own increment is its rank in the run.  The block adds up its warps'
-// counts; route_scan turns tile counts into starts; route_place writes.  One tile
-// does all of it in the first launch.
+// counts; route_scan turns tile counts into starts within an expert; route_place adds
+// the experts' starts and writes.  One tile does all of it in the first launch.
 #include <cfloat>
 #include <cmath>
 
@@ -31,7 +33,7 @@ namespace dense {
 namespace {
 
 constexpr unsigned kWarps = 8;             // of a tile
-constexpr unsigned kRun = 16;              // tokens of a warp's run
+constexpr unsigned kRun = 8;               // tokens of a warp's run, where there are several tiles
 constexpr unsigned kTile = kWarps * kRun;
 
 struct Route {
@@ -41,10 +43,10 @@ struct Route {
   int32_t* chosen;
   float* weights;
   int32_t *order, *position, *offsets;
-  uint32_t* counts;                        // [tiles][experts]
+  uint32_t* counts;                        // [tiles][experts]; at the end, the experts' totals
   uint16_t* ranks;                         // [tokens * top_k]
   uint64_t tokens;
-  unsigned experts, top_k, groups, top_groups, per_group, tiles;
+  unsigned experts, top_k, groups, top_groups, per_group, tiles, run;
   int softmax, renormalise, wide;
   float scale;
   const int32_t* given;                    // backward: chosen, dweights -> dlogits
@@ -84,12 +86,22 @@ __device__ __forceinline__ void load_logits(const Route& a, const T* row, unsign
   }
 }
 
+// The sum of n over the lanes up to this one.
+__device__ __forceinline__ unsigned inclusive(unsigned n, unsigned lane) {
+#pragma unroll
+  for (int o = 1; o < 32; o *= 2) {
+    const unsigned up = __shfl_up_sync(~0u, n, o);
+    if (lane >= o) n += up;
+  }
+  return n;
+}
+
 // The scores of a token; lanes past the experts hold 0.
 template <int EPL>
 __device__ __forceinline__ void score(const Route& a, float (&x)[EPL]) {
   if (!a.softmax) {
 #pragma unroll
-    for (int i = 0; i < EPL; ++i) x[i] = __fdiv_rn(1.f, __fadd_rn(1.f, expf(-x[i])));
+    for (int i = 0; i < EPL; ++i) x[i] = __frcp_rn(__fadd_rn(1.f, expf(-x[i])));
     return;
   }
   float top = x[0];
@@ -115,21 +127,62 @@ __device__ __forceinline__ void score(const Route& a, float (&x)[EPL]) {
   for (int i = 0; i < EPL; ++i) x[i] = total == 0.f ? 0.f : __fdiv_rn(x[i], total);
 }
 
-// Shared memory of a warp: the images of its keys, then its groups' scores.
+// Shared memory of a warp: its counts, the chosen of the token at hand, and, for
+// groups that lanes do not divide evenly, its keys and the groups' scores.
 struct Scratch {
+  uint16_t* count;     // [experts]
+  int* expert;         // [32]
+  float* score;        // [32]
   unsigned* keys;      // [experts]
   float* groups;       // [groups]
 };
 
-// Clears the images of experts outside the best groups.
+__host__ __device__ __forceinline__ unsigned scratch_bytes(unsigned experts, unsigned groups, bool spread) {
+  return (experts * 2 + 15) / 16 * 16 + 256 + (spread ? (experts + groups) * 4 : 0);
+}
+
+__device__ __forceinline__ float image_value(unsigned u) { return __uint_as_float(u >> 31 ? u & 0x7FFFFFFFu : ~u); }
+
+// Whether every group is a run of whole lanes, a power of two of them.
+__host__ __device__ __forceinline__ bool lanes_divide(unsigned per_group, unsigned per_lane) {
+  const unsigned lanes = per_group / per_lane;
+  return per_group % per_lane == 0 && (lanes & (lanes - 1)) == 0;
+}
+
+// Clears the images of experts outside the best groups: a group stays if fewer than
+// top_groups come before it.
 template <int EPL>
-__device__ __forceinline__ void keep_groups(const Route& a, const float (&p)[EPL], unsigned (&key)[EPL], unsigned lane, const Scratch& s) {
+__device__ __forceinline__ void keep_groups(const Route& a, unsigned (&key)[EPL], unsigned lane, const Scratch& s) {
   const unsigned e0 = lane * EPL;
+  if (lanes_divide(a.per_group, EPL)) {
+    unsigned first = 0, second = 0;
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) {
+      second = max(second, min(first, key[i]));
+      first = max(first, key[i]);
+    }
+    const unsigned lanes = a.per_group / EPL;
+    for (unsigned o = 1; o < lanes; o *= 2) {
+      const unsigned f = __shfl_xor_sync(~0u, first, o), g = __shfl_xor_sync(~0u, second, o);
+      second = max(max(second, g), min(first, f));
+      first = max(first, f);
+    }
+    const float mine = a.per_group > 1 ? __fadd_rn(image_value(first), image_value(second)) : image_value(first);
+    unsigned before = 0;
+    for (unsigned o = 0; o < a.groups; ++o) {
+      const float v = __shfl_sync(~0u, mine, o * lanes);
+      before += v > mine || (v == mine && o * lanes < (lane & ~(lanes - 1)));
+    }
+    if (before >= a.top_groups) {
+#pragma unroll
+      for (int i = 0; i < EPL; ++i) key[i] = 0;
+    }
+    return;
+  }
 #pragma unroll
   for (int i = 0; i < EPL; ++i)
     if (e0 + i < a.experts) s.keys[e0 + i] = key[i];
   __syncwarp();
-  auto value = [](unsigned u) { return __uint_as_float(u >> 31 ? u & 0x7FFFFFFFu : ~u); };
   for (unsigned g = lane; g < a.groups; g += 32) {
     unsigned first = 0, second = 0;
     for (unsigned i = 0; i < a.per_group; ++i) {
@@ -137,79 +190,90 @@ __device__ __forceinline__ void keep_groups(const Route& a, const float (&p)[EPL
       second = max(second, min(first, k));
       first = max(first, k);
     }
-    s.groups[g] = a.per_group > 1 ? __fadd_rn(value(first), value(second)) : value(first);
+    s.groups[g] = a.per_group > 1 ? __fadd_rn(image_value(first), image_value(second)) : image_value(first);
   }
   __syncwarp();
-  // a group stays if fewer than top_groups come before it
-#pragma unroll
-  for (int i = 0; i < EPL; ++i) {
-    if (e0 + i >= a.experts) continue;
-    const unsigned g = (e0 + i) / a.per_group;
+  for (unsigned g = lane; g < a.groups; g += 32) {
     const float mine = s.groups[g];
     unsigned before = 0;
     for (unsigned o = 0; o < a.groups; ++o) {
       const float v = s.groups[o];
       before += v > mine || (v == mine && o < g);
     }
-    if (before >= a.top_groups) key[i] = 0;
+    s.keys[g] = before < a.top_groups;      // the keys are in registers
   }
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < EPL; ++i)
+    if (e0 + i < a.experts && !s.keys[(e0 + i) / a.per_group]) key[i] = 0;
   __syncwarp();
 }
 
 template <class T, int EPL>
 __global__ void __launch_bounds__(kWarps * 32) route_tokens(const Route a) {
-  extern __shared__ unsigned char raw[];
+  extern __shared__ __align__(16) unsigned char raw[];
   const unsigned lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-  // [kWarps][experts] counts, then each warp's scratch
-  uint16_t* const counts = reinterpret_cast<uint16_t*>(raw);
-  unsigned char* const rest = raw + (kWarps * a.experts * 2 + 15) / 16 * 16 + warp * ((a.experts + a.groups) * 4);
-  const Scratch s{reinterpret_cast<unsigned*>(rest), reinterpret_cast<float*>(rest) + a.experts};
-  uint16_t* const count = counts + warp * a.experts;
+  const bool grouped = a.groups > 1 && a.top_groups < a.groups;
+  const unsigned each = scratch_bytes(a.experts, a.groups, grouped && !lanes_divide(a.per_group, EPL));
+  auto scratch = [&](unsigned w) {
+    unsigned char* const p = raw + w * each;
+    unsigned char* const q = p + (a.experts * 2 + 15) / 16 * 16;
+    return Scratch{reinterpret_cast<uint16_t*>(p), reinterpret_cast<int*>(q), reinterpret_cast<float*>(q) + 32,
+                   reinterpret_cast<unsigned*>(q) + 64, reinterpret_cast<float*>(q) + 64 + a.experts};
+  };
+  const Scratch s = scratch(warp);
   const bool sorting = a.order != nullptr;
   if (sorting)
-    for (unsigned e = lane; e < a.experts; e += 32) count[e] = 0;
+    for (unsigned e = lane; e < a.experts; e += 32) s.count[e] = 0;
+  float bias[EPL];
+#pragma unroll
+  for (int i = 0; i < EPL; ++i) bias[i] = a.bias && lane * EPL + i < a.experts ? a.bias[lane * EPL + i] : 0.f;
   __syncwarp();
 
-  const uint64_t tile = (uint64_t)blockIdx.x * kTile;
-  for (unsigned r = 0; r < kRun; ++r) {
-    const uint64_t token = tile + warp * kRun + r;
-    if (token >= a.tokens) break;
+  const uint64_t tile = (uint64_t)blockIdx.x * kTile, begin = tile + warp * a.run, end = min(begin + a.run, a.tokens);
+  const T* const logits = static_cast<const T*>(a.logits);
+  float next[EPL];
+  if (begin < end) load_logits<T, EPL>(a, logits + begin * a.stride, lane, next);
+  for (uint64_t token = begin; token < end; ++token) {
     float p[EPL];
-    load_logits<T, EPL>(a, static_cast<const T*>(a.logits) + token * a.stride, lane, p);
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) p[i] = next[i];
+    if (token + 1 < end) load_logits<T, EPL>(a, logits + (token + 1) * a.stride, lane, next);
     score<EPL>(a, p);
     unsigned key[EPL];
 #pragma unroll
-    for (int i = 0; i < EPL; ++i) {
-      const unsigned e = lane * EPL + i;
-      key[i] = e < a.experts ? image(a.bias ? __fadd_rn(p[i], a.bias[e]) : p[i]) : 0;
-    }
-    if (a.groups > 1 && a.top_groups < a.groups) keep_groups<EPL>(a, p, key, lane, s);
+    for (int i = 0; i < EPL; ++i) key[i] = lane * EPL + i < a.experts ? image(__fadd_rn(p[i], bias[i])) : 0;
+    if (grouped) keep_groups<EPL>(a, key, lane, s);
 
-    int expert = 0;          // of slot `lane`
-    float weight = 0.f;
-    for (unsigned k = 0; k < a.top_k; ++k) {
-      unsigned best = 0;
+    unsigned best = 0;
 #pragma unroll
-      for (int i = 0; i < EPL; ++i) best = max(best, key[i]);
+    for (int i = 0; i < EPL; ++i) best = max(best, key[i]);
+    for (unsigned k = 0; k < a.top_k; ++k) {
       const unsigned top = __reduce_max_sync(~0u, best);
       const unsigned owner = __ffs(__ballot_sync(~0u, best == top)) - 1;
-      int at = 0;
-      float w = 0.f;
       if (lane == owner) {
-        bool found = false;
+        int at = 0;
 #pragma unroll
-        for (int i = 0; i < EPL; ++i)
-          if (!found && key[i] == top) {
-            found = true;
-            at = lane * EPL + i;
+        for (int i = EPL - 1; i >= 0; --i)
+          if (key[i] == top) at = i;
+        best = 0;
+        float w = 0.f;
+#pragma unroll
+        for (int i = 0; i < EPL; ++i) {
+          if (i == at) {
             w = p[i];
             key[i] = 0;
           }
+          best = max(best, key[i]);
+        }
+        s.expert[k] = (int)(lane * EPL) + at;
+        s.score[k] = w;
       }
-      at = __shfl_sync(~0u, at, owner);
-      w = __shfl_sync(~0u, w, owner);
-      if (lane == k) { expert = at; weight = w; }
     }
+    __syncwarp();
+    const int expert = lane < a.top_k ? s.expert[lane] : 0;
+    float weight = lane < a.top_k ? s.score[lane] : 0.f;
+    __syncwarp();
     float total = 0.f;
     if (a.renormalise) {
       total = weight;
@@ -221,20 +285,21 @@ __global__ void __launch_bounds__(kWarps * 32) route_tokens(const Route a) {
       const uint64_t entry = token * a.top_k + lane;
       a.chosen[entry] = expert;
       a.weights[entry] = weight * a.scale;
-      if (sorting) a.ranks[entry] = count[expert]++;
+      if (sorting) a.ranks[entry] = s.count[expert]++;
     }
     __syncwarp();
   }
   if (!sorting) return;
   __syncthreads();
   // warps' counts to starts within the tile; the tile's totals
-  unsigned* const total = reinterpret_cast<unsigned*>(raw + (kWarps * a.experts * 2 + 15) / 16 * 16);   // the scratch, no longer used
+  unsigned* const total = reinterpret_cast<unsigned*>(raw + kWarps * each);
   for (unsigned e = threadIdx.x; e < a.experts; e += blockDim.x) {
     unsigned before = 0;
 #pragma unroll
     for (unsigned w = 0; w < kWarps; ++w) {
-      const unsigned n = counts[w * a.experts + e];
-      counts[w * a.experts + e] = (uint16_t)before;
+      uint16_t* const c = reinterpret_cast<uint16_t*>(raw + w * each) + e;
+      const unsigned n = *c;
+      *c = (uint16_t)before;
       before += n;
     }
     if (a.tiles > 1) a.counts[(uint64_t)blockIdx.x * a.experts + e] = before;
@@ -246,12 +311,7 @@ __global__ void __launch_bounds__(kWarps * 32) route_tokens(const Route a) {
       unsigned carry = 0;
       for (unsigned e0 = 0; e0 < a.experts; e0 += 32) {
         const unsigned n = e0 + lane < a.experts ? total[e0 + lane] : 0;
-        unsigned sum = n;
-#pragma unroll
-        for (int o = 1; o < 32; o *= 2) {
-          const unsigned up = __shfl_up_sync(~0u, sum, o);
-          if (lane >= o) sum += up;
-        }
+        const unsigned sum = inclusive(n, lane);
         if (e0 + lane < a.experts) {
           total[e0 + lane] = carry + sum - n;
           a.offsets[e0 + lane] = (int32_t)(carry + sum - n);
@@ -264,9 +324,9 @@ __global__ void __launch_bounds__(kWarps * 32) route_tokens(const Route a) {
   }
   const uint64_t first = tile * a.top_k, last = min(tile + kTile, a.tokens) * a.top_k;
   for (uint64_t i = first + threadIdx.x; i < last; i += blockDim.x) {
-    const unsigned w = (unsigned)((i - first) / (kRun * a.top_k));
+    const unsigned w = (unsigned)(i - first) / (a.run * a.top_k);
     const unsigned e = (unsigned)a.chosen[i];
-    const unsigned in_tile = counts[w * a.experts + e] + a.ranks[i];
+    const unsigned in_tile = reinterpret_cast<const uint16_t*>(raw + w * each)[e] + a.ranks[i];
     if (a.tiles > 1) {
       a.ranks[i] = (uint16_t)in_tile;
     } else {
@@ -277,49 +337,68 @@ __global__ void __launch_bounds__(kWarps * 32) route_tokens(const Route a) {
   }
 }
 
-// counts[tile][e] -> entries of expert e before the tile; offsets.  One block; each
-// thread owns one expert at a time.
-__global__ void __launch_bounds__(1024) route_scan(const Route a) {
-  __shared__ unsigned sums[32];
+// counts[tile][e] -> entries of expert e in the tiles before; counts[tiles][e] = all of
+// them.  A block has 32 experts, a warp of it a run of tiles, read twice.
+constexpr unsigned kScanWarps = 32;
+__global__ void __launch_bounds__(32 * kScanWarps) route_scan(const Route a) {
+  __shared__ unsigned sums[kScanWarps][33];
+  const unsigned lane = threadIdx.x % 32, warp = threadIdx.x / 32, e = blockIdx.x * 32 + lane;
+  const unsigned run = (a.tiles + kScanWarps - 1) / kScanWarps, first = warp * run, last = min(first + run, a.tiles);
+  unsigned n = 0;
+  if (e < a.experts) {
+#pragma unroll 8
+    for (unsigned t = first; t < last; ++t) n += a.counts[(uint64_t)t * a.experts + e];
+  }
+  sums[warp][lane] = n;
+  __syncthreads();
+  const unsigned mine = sums[lane][warp], sum = inclusive(mine, lane);     // lane: run of tiles, warp: expert
+  sums[lane][warp] = sum - mine;
+  if (lane == 31 && blockIdx.x * 32 + warp < a.experts) a.counts[(uint64_t)a.tiles * a.experts + blockIdx.x * 32 + warp] = sum;
+  __syncthreads();
+  if (e >= a.experts) return;
+  unsigned before = sums[warp][lane];
+#pragma unroll 8
+  for (unsigned t = first; t < last; ++t) {
+    unsigned* const c = a.counts + (uint64_t)t * a.experts + e;
+    const unsigned here = *c;
+    *c = before;
+    before += here;
+  }
+}
+
+// Every block sums the experts' totals to starts for itself; the first writes them.
+__global__ void __launch_bounds__(256) route_place(const Route a) {
+  __shared__ unsigned starts[EPS_B200_ROUTE_EXPERTS];
+  __shared__ unsigned sums[8];
+  const unsigned lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  const unsigned* const totals = a.counts + (uint64_t)a.tiles * a.experts;
   unsigned carry = 0;
-  for (unsigned e0 = 0; e0 < a.experts; e0 += blockDim.x) {
-    const unsigned e = e0 + threadIdx.x;
-    unsigned n = 0;
-    if (e < a.experts)
-      for (unsigned t = 0; t < a.tiles; ++t) {
-        const unsigned c = a.counts[(uint64_t)t * a.experts + e];
-        a.counts[(uint64_t)t * a.experts + e] = n;
-        n += c;
-      }
-    unsigned sum = n;
-    const unsigned lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-#pragma unroll
-    for (int o = 1; o < 32; o *= 2) {
-      const unsigned up = __shfl_up_sync(~0u, sum, o);
-      if (lane >= o) sum += up;
-    }
+  for (unsigned e0 = 0; e0 < a.experts; e0 += 256) {
+    const unsigned e = e0 + threadIdx.x, n = e < a.experts ? totals[e] : 0, sum = inclusive(n, lane);
     if (lane == 31) sums[warp] = sum;
     __syncthreads();
     unsigned before = carry, all = 0;
-    for (unsigned w = 0; w < blockDim.x / 32; ++w) {
-      if (w < warp) before += sums[w];
+#pragma unroll
+    for (unsigned w = 0; w < 8; ++w) {
+      before += w < warp ? sums[w] : 0;
       all += sums[w];
     }
-    if (e < a.experts) a.offsets[e] = (int32_t)(before + sum - n);
+    if (e < a.experts) starts[e] = before + sum - n;
     carry += all;
     __syncthreads();
   }
-  if (threadIdx.x == 0) a.offsets[a.experts] = (int32_t)carry;
-}
-
-__global__ void __launch_bounds__(256) route_place(const Route a) {
-  const uint64_t i = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x;
-  if (i >= a.tokens * a.top_k) return;
-  const uint64_t tile = i / ((uint64_t)kTile * a.top_k);
-  const unsigned e = (unsigned)a.chosen[i];
-  const unsigned at = (unsigned)a.offsets[e] + a.counts[tile * a.experts + e] + a.ranks[i];
-  a.position[i] = (int32_t)at;
-  a.order[at] = (int32_t)i;
+  if (blockIdx.x == 0) {
+    for (unsigned e = threadIdx.x; e < a.experts; e += 256) a.offsets[e] = (int32_t)starts[e];
+    if (threadIdx.x == 0) a.offsets[a.experts] = (int32_t)carry;
+  }
+  const uint64_t entries = a.tokens * a.top_k;
+  for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < entries; i += (uint64_t)gridDim.x * 256) {
+    const unsigned tile = (unsigned)i / (kTile * a.top_k);
+    const unsigned e = (unsigned)a.chosen[i];
+    const unsigned at = starts[e] + a.counts[(uint64_t)tile * a.experts + e] + a.ranks[i];
+    a.position[i] = (int32_t)at;
+    a.order[at] = (int32_t)i;
+  }
 }
 
 template <class T, int EPL>
@@ -396,6 +475,7 @@ Route checked(const EpsB200RouteExperts* a) {
   r.top_groups = a->top_groups;
   r.per_group = a->experts / a->groups;
   r.tiles = (unsigned)ceil_div(a->tokens, kTile);
+  r.run = r.tiles > 1 ? kRun : (unsigned)ceil_div(a->tokens, kWarps);
   r.softmax = a->score == EPS_B200_SCORE_SOFTMAX;
   r.renormalise = a->renormalise != 0;
   r.scale = a->scale;
@@ -443,7 +523,7 @@ using namespace eps_b200::dense;
 extern "C" {
 
 uint64_t eps_b200_route_experts_workspace(uint64_t tokens, uint32_t experts, uint32_t top_k) {
-  return round_up(tokens * top_k * 2, 16) + ceil_div(tokens, kTile) * experts * 4;
+  return round_up(tokens * top_k * 2, 16) + (ceil_div(tokens, kTile) + 1) * experts * 4;
 }
 
 int eps_b200_route_experts(const EpsB200RouteExperts* a, const float* bias, int32_t* chosen, float* weights,
@@ -473,9 +553,10 @@ int eps_b200_route_experts(const EpsB200RouteExperts* a, const float* bias, int3
     r.position = position;
     r.offsets = offsets;
     r.wide = lanes_wide(r.logits, r.stride, r.experts, a->type);
-    const size_t shared = (kWarps * r.experts * 2 + 15) / 16 * 16 + kWarps * (r.experts + r.groups) * 4;
     by_type(a->type, [&](auto t) {
       by_experts(r.experts, [&](auto epl) {
+        const bool spread = r.groups > 1 && r.top_groups < r.groups && !lanes_divide(r.per_group, decltype(epl)::value);
+        const size_t shared = kWarps * scratch_bytes(r.experts, r.groups, spread) + r.experts * 4;
         auto* kernel = route_tokens<decltype(t), decltype(epl)::value>;
         room(kernel, shared);
         kernel<<<r.tiles, kWarps * 32, shared, st>>>(r);
@@ -483,9 +564,10 @@ int eps_b200_route_experts(const EpsB200RouteExperts* a, const float* bias, int3
     });
     check(cudaGetLastError(), "route_experts");
     if (order && r.tiles > 1) {
-      route_scan<<<1, 1024, 0, st>>>(r);
+      route_scan<<<(unsigned)ceil_div(r.experts, 32), 32 * kScanWarps, 0, st>>>(r);
       check(cudaGetLastError(), "route_scan");
-      route_place<<<(unsigned)ceil_div(r.tokens * r.top_k, 256), 256, 0, st>>>(r);
+      const uint64_t most = (uint64_t)sm_count(a->device) * 8, all = ceil_div(r.tokens * r.top_k, 256);
+      route_place<<<(unsigned)(all < most ? all : most), 256, 0, st>>>(r);
       check(cudaGetLastError(), "route_place");
     }
   });
