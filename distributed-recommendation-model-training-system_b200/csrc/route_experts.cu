@@ -15,7 +15,7 @@
 // on unsigned images of the keys (`image`), so one warp instruction finds the best
 // key and the lowest lane that holds it owns the lowest index.  What bounds it is the
 // number of instructions a token takes (the logits of a batch are a few megabytes):
-// a lane keeps its own best key and looks again only when that has been taken.
+// every lane sorts its own few keys once, and then only offers the best it has left.
 //
 // The sort by expert is a counting sort in three steps.  A tile is the tokens of one
 // block; each of its warps counts its own run of consecutive tokens, whose experts
@@ -60,7 +60,7 @@ struct Route {
 __device__ __forceinline__ unsigned image(float key) {
   if (!(key >= -FLT_MAX)) key = -FLT_MAX;
   const unsigned u = __float_as_uint(key + 0.f);     // -0 is 0
-  return u >> 31 ? ~u : u | 0x80000000u;
+  return u ^ ((unsigned)((int)u >> 31) | 0x80000000u);
 }
 
 __device__ __forceinline__ float warp_max(float v) {
@@ -96,12 +96,36 @@ __device__ __forceinline__ unsigned inclusive(unsigned n, unsigned lane) {
   return n;
 }
 
+// 1 / x, correctly rounded, for x >= 1, infinity and NaN.  One Newton step with fused
+// multiply-adds from the hardware's approximation (P. Markstein, IBM J. Res. Dev. 34,
+// 1990) rounds correctly but where the significand of x is all ones, or where the
+// result or the residual leaves the normal range: those take the library's division,
+// all of a warp together.
+template <int N>
+__device__ __forceinline__ void reciprocals(float (&x)[N]) {
+  bool rare = false;
+#pragma unroll
+  for (int i = 0; i < N; ++i) rare |= !(x[i] < 0x1p100f) || (__float_as_uint(x[i]) & 0x7FFFFFu) == 0x7FFFFFu;
+  if (__any_sync(~0u, rare)) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = __fdiv_rn(1.f, x[i]);
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x[i]));
+    x[i] = fmaf(r, fmaf(-x[i], r, 1.f), r);
+  }
+}
+
 // The scores of a token; lanes past the experts hold 0.
 template <int EPL>
 __device__ __forceinline__ void score(const Route& a, float (&x)[EPL]) {
   if (!a.softmax) {
 #pragma unroll
-    for (int i = 0; i < EPL; ++i) x[i] = __frcp_rn(__fadd_rn(1.f, expf(-x[i])));
+    for (int i = 0; i < EPL; ++i) x[i] = __fadd_rn(1.f, expf(-x[i]));
+    reciprocals<EPL>(x);
     return;
   }
   float top = x[0];
@@ -127,18 +151,37 @@ __device__ __forceinline__ void score(const Route& a, float (&x)[EPL]) {
   for (int i = 0; i < EPL; ++i) x[i] = total == 0.f ? 0.f : __fdiv_rn(x[i], total);
 }
 
-// Shared memory of a warp: its counts, the chosen of the token at hand, and, for
-// groups that lanes do not divide evenly, its keys and the groups' scores.
+// Shared memory of a warp: its counts, its token's scores and sorted keys, and, for
+// groups that lanes do not divide evenly, the keys by expert and the groups' scores.
 struct Scratch {
   uint16_t* count;     // [experts]
-  int* expert;         // [32]
-  float* score;        // [32]
+  int* chosen;         // [32]
+  float* score;        // [32 * EPL]
+  uint64_t* sorted;    // [32][EPL + 2]: an odd number of 16-byte words a lane meets all banks
   unsigned* keys;      // [experts]
   float* groups;       // [groups]
 };
 
-__host__ __device__ __forceinline__ unsigned scratch_bytes(unsigned experts, unsigned groups, bool spread) {
-  return (experts * 2 + 15) / 16 * 16 + 256 + (spread ? (experts + groups) * 4 : 0);
+__host__ __device__ __forceinline__ unsigned scratch_bytes(unsigned experts, unsigned per_lane, unsigned groups, bool spread) {
+  return ((experts * 2 + 15) / 16 * 16 + 128 + 32 * per_lane * 4 + 32 * (per_lane + 2) * 8 + (spread ? (experts + groups) * 4 : 0) + 15) / 16 * 16;
+}
+
+// Descending (K. Batcher's odd-even merge sort), N a power of two.
+template <int N>
+__device__ __forceinline__ void sort(uint64_t (&v)[N]) {
+#pragma unroll
+  for (int p = 1; p < N; p *= 2)
+#pragma unroll
+    for (int k = p; k >= 1; k /= 2)
+#pragma unroll
+      for (int j = k % p; j + k < N; j += 2 * k)
+#pragma unroll
+        for (int i = 0; i < k; ++i)
+          if (i + j + k < N && (i + j) / (2 * p) == (i + j + k) / (2 * p)) {
+            const uint64_t a = v[i + j], b = v[i + j + k];
+            v[i + j] = a > b ? a : b;
+            v[i + j + k] = a > b ? b : a;
+          }
 }
 
 __device__ __forceinline__ float image_value(unsigned u) { return __uint_as_float(u >> 31 ? u & 0x7FFFFFFFu : ~u); }
@@ -210,18 +253,17 @@ __device__ __forceinline__ void keep_groups(const Route& a, unsigned (&key)[EPL]
 }
 
 template <class T, int EPL>
-__global__ void __launch_bounds__(kWarps * 32) route_tokens(const Route a) {
+__global__ void __launch_bounds__(kWarps * 32, EPL <= 8 ? 4 : EPL == 16 ? 2 : 1) route_tokens(const Route a) {
   extern __shared__ __align__(16) unsigned char raw[];
   const unsigned lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   const bool grouped = a.groups > 1 && a.top_groups < a.groups;
-  const unsigned each = scratch_bytes(a.experts, a.groups, grouped && !lanes_divide(a.per_group, EPL));
-  auto scratch = [&](unsigned w) {
-    unsigned char* const p = raw + w * each;
-    unsigned char* const q = p + (a.experts * 2 + 15) / 16 * 16;
-    return Scratch{reinterpret_cast<uint16_t*>(p), reinterpret_cast<int*>(q), reinterpret_cast<float*>(q) + 32,
-                   reinterpret_cast<unsigned*>(q) + 64, reinterpret_cast<float*>(q) + 64 + a.experts};
-  };
-  const Scratch s = scratch(warp);
+  const unsigned each = scratch_bytes(a.experts, EPL, a.groups, grouped && !lanes_divide(a.per_group, EPL));
+  unsigned char* const p0 = raw + warp * each;
+  unsigned char* const p1 = p0 + (a.experts * 2 + 15) / 16 * 16;
+  unsigned char* const p2 = p1 + 128 + 32 * EPL * 4;
+  unsigned char* const p3 = p2 + 32 * (EPL + 2) * 8;
+  const Scratch s{reinterpret_cast<uint16_t*>(p0), reinterpret_cast<int*>(p1), reinterpret_cast<float*>(p1 + 128), reinterpret_cast<uint64_t*>(p2),
+                  reinterpret_cast<unsigned*>(p3), reinterpret_cast<float*>(p3) + a.experts};
   const bool sorting = a.order != nullptr;
   if (sorting)
     for (unsigned e = lane; e < a.experts; e += 32) s.count[e] = 0;
@@ -245,34 +287,31 @@ __global__ void __launch_bounds__(kWarps * 32) route_tokens(const Route a) {
     for (int i = 0; i < EPL; ++i) key[i] = lane * EPL + i < a.experts ? image(__fadd_rn(p[i], bias[i])) : 0;
     if (grouped) keep_groups<EPL>(a, key, lane, s);
 
-    unsigned best = 0;
+    // by key, and the lower index of equal keys first
+    uint64_t order[EPL];
 #pragma unroll
-    for (int i = 0; i < EPL; ++i) best = max(best, key[i]);
+    for (int i = 0; i < EPL; ++i) order[i] = (uint64_t)key[i] << 32 | (unsigned)~(lane * EPL + i);
+    sort<EPL>(order);
+    uint64_t* const mine = s.sorted + lane * (EPL + 2);
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) {
+      mine[i] = order[i];
+      s.score[lane * EPL + i] = p[i];
+    }
+    mine[EPL] = 0;
+    unsigned taken = 0;
+    uint64_t best = order[0];
     for (unsigned k = 0; k < a.top_k; ++k) {
-      const unsigned top = __reduce_max_sync(~0u, best);
-      const unsigned owner = __ffs(__ballot_sync(~0u, best == top)) - 1;
+      const unsigned top = __reduce_max_sync(~0u, (unsigned)(best >> 32));
+      const unsigned owner = __ffs(__ballot_sync(~0u, (unsigned)(best >> 32) == top)) - 1;
       if (lane == owner) {
-        int at = 0;
-#pragma unroll
-        for (int i = EPL - 1; i >= 0; --i)
-          if (key[i] == top) at = i;
-        best = 0;
-        float w = 0.f;
-#pragma unroll
-        for (int i = 0; i < EPL; ++i) {
-          if (i == at) {
-            w = p[i];
-            key[i] = 0;
-          }
-          best = max(best, key[i]);
-        }
-        s.expert[k] = (int)(lane * EPL) + at;
-        s.score[k] = w;
+        s.chosen[k] = (int)~(unsigned)best;
+        best = mine[++taken];
       }
     }
     __syncwarp();
-    const int expert = lane < a.top_k ? s.expert[lane] : 0;
-    float weight = lane < a.top_k ? s.score[lane] : 0.f;
+    const int expert = lane < a.top_k ? s.chosen[lane] : 0;
+    float weight = lane < a.top_k ? s.score[expert] : 0.f;
     __syncwarp();
     float total = 0.f;
     if (a.renormalise) {
@@ -510,8 +549,8 @@ bool lanes_wide(const void* p, int64_t stride, unsigned experts, int type) {
 
 template <class K>
 void room(K kernel, size_t bytes) {
-  if (bytes > 48 * 1024)
-    check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes), "cudaFuncSetAttribute");
+  check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes), "cudaFuncSetAttribute");
+  check(cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, 100), "cudaFuncSetAttribute");
 }
 
 }  // namespace
@@ -556,7 +595,7 @@ int eps_b200_route_experts(const EpsB200RouteExperts* a, const float* bias, int3
     by_type(a->type, [&](auto t) {
       by_experts(r.experts, [&](auto epl) {
         const bool spread = r.groups > 1 && r.top_groups < r.groups && !lanes_divide(r.per_group, decltype(epl)::value);
-        const size_t shared = kWarps * scratch_bytes(r.experts, r.groups, spread) + r.experts * 4;
+        const size_t shared = kWarps * scratch_bytes(r.experts, decltype(epl)::value, r.groups, spread) + r.experts * 4;
         auto* kernel = route_tokens<decltype(t), decltype(epl)::value>;
         room(kernel, shared);
         kernel<<<r.tiles, kWarps * 32, shared, st>>>(r);
