@@ -47,7 +47,7 @@ struct Route {
   uint16_t* ranks;                         // [tokens * top_k]
   uint64_t tokens;
   unsigned experts, top_k, groups, top_groups, per_group, tiles, run;
-  int softmax, renormalise, wide;
+  int softmax, renormalise, wide, wide_out;
   float scale;
   const int32_t* given;                    // backward: chosen, dweights -> dlogits
   const float* dweights;
@@ -55,12 +55,16 @@ struct Route {
   int64_t dstride;
 };
 
+// Orders like the floats, infinities too; 0 is below every one that is not NaN.
+__device__ __forceinline__ unsigned ordered(float v) {
+  const unsigned u = __float_as_uint(v + 0.f);       // -0 is 0
+  return u ^ ((unsigned)((int)u >> 31) | 0x80000000u);
+}
+
 // Orders like the floats, -FLT_MAX and above; 0 is below every image.  NaN and
 // -inf take the place of the lowest finite value.
 __device__ __forceinline__ unsigned image(float key) {
-  if (!(key >= -FLT_MAX)) key = -FLT_MAX;
-  const unsigned u = __float_as_uint(key + 0.f);     // -0 is 0
-  return u ^ ((unsigned)((int)u >> 31) | 0x80000000u);
+  return ordered(key >= -FLT_MAX ? key : -FLT_MAX);
 }
 
 __device__ __forceinline__ float warp_max(float v) {
@@ -103,10 +107,14 @@ __device__ __forceinline__ unsigned inclusive(unsigned n, unsigned lane) {
 // all of a warp together.
 template <int N>
 __device__ __forceinline__ void reciprocals(float (&x)[N]) {
-  bool rare = false;
+  unsigned largest = 0, rest = ~0u;      // as bits: infinity and NaN are above all others
 #pragma unroll
-  for (int i = 0; i < N; ++i) rare |= !(x[i] < 0x1p100f) || (__float_as_uint(x[i]) & 0x7FFFFFu) == 0x7FFFFFu;
-  if (__any_sync(~0u, rare)) {
+  for (int i = 0; i < N; ++i) {
+    const unsigned u = __float_as_uint(x[i]);
+    largest = max(largest, u);
+    rest = min(rest, ~u & 0x7FFFFFu);
+  }
+  if (__any_sync(~0u, largest > 0x71800000u || rest == 0)) {      // 2^100
 #pragma unroll
     for (int i = 0; i < N; ++i) x[i] = __fdiv_rn(1.f, x[i]);
     return;
@@ -120,7 +128,8 @@ __device__ __forceinline__ void reciprocals(float (&x)[N]) {
 }
 
 // The scores of a token; lanes past the experts hold 0.
-template <int EPL>
+// RANKED: with the operations that the ranking is defined by.
+template <int EPL, bool RANKED>
 __device__ __forceinline__ void score(const Route& a, float (&x)[EPL]) {
   if (!a.softmax) {
 #pragma unroll
@@ -138,17 +147,23 @@ __device__ __forceinline__ void score(const Route& a, float (&x)[EPL]) {
   top = warp_max(top);
   nan = __any_sync(~0u, nan);
   if (nan) top = NAN;
-  double sum = 0;
+  std::conditional_t<RANKED, double, float> sum = 0;
 #pragma unroll
   for (int i = 0; i < EPL; ++i) {
     x[i] = top == -INFINITY ? 0.f : expf(__fsub_rn(x[i], top));
-    sum += (double)x[i];
+    sum += x[i];
   }
 #pragma unroll
   for (int o = 16; o; o /= 2) sum += __shfl_xor_sync(~0u, sum, o);
   const float total = (float)sum;
+  if constexpr (RANKED) {
 #pragma unroll
-  for (int i = 0; i < EPL; ++i) x[i] = total == 0.f ? 0.f : __fdiv_rn(x[i], total);
+    for (int i = 0; i < EPL; ++i) x[i] = total == 0.f ? 0.f : __fdiv_rn(x[i], total);
+  } else {
+    const float by = total == 0.f ? 0.f : __fdiv_rn(1.f, total);
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) x[i] *= by;
+  }
 }
 
 // Shared memory of a warp: its counts, its token's scores and sorted keys, and, for
@@ -211,15 +226,17 @@ __device__ __forceinline__ void keep_groups(const Route& a, unsigned (&key)[EPL]
       first = max(first, f);
     }
     const float mine = a.per_group > 1 ? __fadd_rn(image_value(first), image_value(second)) : image_value(first);
-    unsigned before = 0;
-    for (unsigned o = 0; o < a.groups; ++o) {
-      const float v = __shfl_sync(~0u, mine, o * lanes);
-      before += v > mine || (v == mine && o * lanes < (lane & ~(lanes - 1)));
+    // the best of what is left, top_groups times; a group is where its first lane is
+    unsigned left = e0 < a.experts ? ordered(mine) : 0, kept = 0;
+    for (unsigned k = 0; k < a.top_groups; ++k) {
+      const unsigned top = __reduce_max_sync(~0u, left);
+      const unsigned first_lane = __ffs(__ballot_sync(~0u, left == top)) - 1;
+      const unsigned me = (lane ^ first_lane) < lanes;      // same group: the lanes' upper bits agree
+      left = me ? 0 : left;
+      kept |= me;
     }
-    if (before >= a.top_groups) {
 #pragma unroll
-      for (int i = 0; i < EPL; ++i) key[i] = 0;
-    }
+    for (int i = 0; i < EPL; ++i) key[i] = kept ? key[i] : 0;
     return;
   }
 #pragma unroll
@@ -269,7 +286,8 @@ __global__ void __launch_bounds__(kWarps * 32, EPL <= 8 ? 4 : EPL == 16 ? 2 : 1)
     for (unsigned e = lane; e < a.experts; e += 32) s.count[e] = 0;
   float bias[EPL];
 #pragma unroll
-  for (int i = 0; i < EPL; ++i) bias[i] = a.bias && lane * EPL + i < a.experts ? a.bias[lane * EPL + i] : 0.f;
+  for (int i = 0; i < EPL; ++i)       // behind the last expert: a key that every expert's comes before
+    bias[i] = lane * EPL + i >= a.experts ? -INFINITY : a.bias ? a.bias[lane * EPL + i] : 0.f;
   __syncwarp();
 
   const uint64_t tile = (uint64_t)blockIdx.x * kTile, begin = tile + warp * a.run, end = min(begin + a.run, a.tokens);
@@ -281,10 +299,10 @@ __global__ void __launch_bounds__(kWarps * 32, EPL <= 8 ? 4 : EPL == 16 ? 2 : 1)
 #pragma unroll
     for (int i = 0; i < EPL; ++i) p[i] = next[i];
     if (token + 1 < end) load_logits<T, EPL>(a, logits + (token + 1) * a.stride, lane, next);
-    score<EPL>(a, p);
+    score<EPL, true>(a, p);
     unsigned key[EPL];
 #pragma unroll
-    for (int i = 0; i < EPL; ++i) key[i] = lane * EPL + i < a.experts ? image(__fadd_rn(p[i], bias[i])) : 0;
+    for (int i = 0; i < EPL; ++i) key[i] = image(__fadd_rn(p[i], bias[i]));
     if (grouped) keep_groups<EPL>(a, key, lane, s);
 
     // by key, and the lower index of equal keys first
@@ -293,10 +311,17 @@ __global__ void __launch_bounds__(kWarps * 32, EPL <= 8 ? 4 : EPL == 16 ? 2 : 1)
     for (int i = 0; i < EPL; ++i) order[i] = (uint64_t)key[i] << 32 | (unsigned)~(lane * EPL + i);
     sort<EPL>(order);
     uint64_t* const mine = s.sorted + lane * (EPL + 2);
+    if constexpr (EPL >= 4) {
 #pragma unroll
-    for (int i = 0; i < EPL; ++i) {
-      mine[i] = order[i];
-      s.score[lane * EPL + i] = p[i];
+      for (int i = 0; i < EPL; i += 2) *reinterpret_cast<ulonglong2*>(mine + i) = make_ulonglong2(order[i], order[i + 1]);
+#pragma unroll
+      for (int i = 0; i < EPL; i += 4) *reinterpret_cast<float4*>(s.score + lane * EPL + i) = make_float4(p[i], p[i + 1], p[i + 2], p[i + 3]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < EPL; ++i) {
+        mine[i] = order[i];
+        s.score[lane * EPL + i] = p[i];
+      }
     }
     mine[EPL] = 0;
     unsigned taken = 0;
@@ -304,10 +329,9 @@ __global__ void __launch_bounds__(kWarps * 32, EPL <= 8 ? 4 : EPL == 16 ? 2 : 1)
     for (unsigned k = 0; k < a.top_k; ++k) {
       const unsigned top = __reduce_max_sync(~0u, (unsigned)(best >> 32));
       const unsigned owner = __ffs(__ballot_sync(~0u, (unsigned)(best >> 32) == top)) - 1;
-      if (lane == owner) {
-        s.chosen[k] = (int)~(unsigned)best;
-        best = mine[++taken];
-      }
+      if (lane == owner) s.chosen[k] = (int)~(unsigned)best;
+      taken += lane == owner;
+      best = mine[taken];
     }
     __syncwarp();
     const int expert = lane < a.top_k ? s.chosen[lane] : 0;
@@ -440,55 +464,71 @@ __global__ void __launch_bounds__(256) route_place(const Route a) {
   }
 }
 
+// A warp walks tokens, the next one's logits under way.
 template <class T, int EPL>
 __global__ void __launch_bounds__(kWarps * 32) route_gradient(const Route a) {
-  extern __shared__ unsigned char raw[];
+  extern __shared__ __align__(16) unsigned char raw[];
   const unsigned lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-  float* const ds = reinterpret_cast<float*>(raw) + warp * a.experts;
-  const uint64_t token = (uint64_t)blockIdx.x * kWarps + warp;
-  if (token >= a.tokens) return;
-  float p[EPL];
-  load_logits<T, EPL>(a, static_cast<const T*>(a.logits) + token * a.stride, lane, p);
-  score<EPL>(a, p);
+  float* const ds = reinterpret_cast<float*>(raw) + warp * 32 * EPL;      // zeros but while a token's chosen are in it
 #pragma unroll
-  for (int i = 0; i < EPL; ++i)
-    if (lane * EPL + i < a.experts) ds[lane * EPL + i] = p[i];
-  __syncwarp();
-  int expert = -1;
-  float d = 0.f, s = 0.f;
-  if (lane < a.top_k) {
-    expert = a.given[token * a.top_k + lane];
-    if (expert < 0 || (unsigned)expert >= a.experts) expert = -1;
-    if (expert >= 0) {
-      d = a.dweights[token * a.top_k + lane] * a.scale;
-      s = ds[expert];
-    }
-  }
+  for (int i = 0; i < EPL; ++i) ds[i * 32 + lane] = 0.f;
+  const uint64_t stride = (uint64_t)gridDim.x * kWarps;
+  uint64_t token = (uint64_t)blockIdx.x * kWarps + warp;
+  const T* const logits = static_cast<const T*>(a.logits);
+  float next[EPL];
+  if (token < a.tokens) load_logits<T, EPL>(a, logits + token * a.stride, lane, next);
   auto sum = [](float v) {
 #pragma unroll
     for (int o = 16; o; o /= 2) v += __shfl_xor_sync(~0u, v, o);
     return v;
   };
-  if (a.renormalise) {
-    const float total = sum(s);
-    const float mean = sum(d * s) / total;
-    d = total == 0.f || expert < 0 ? 0.f : (d - mean) / total;
-  }
-  const float dot = a.softmax ? sum(d * s) : 0.f;
-  __syncwarp();
+  for (; token < a.tokens; token += stride) {
+    float p[EPL];
 #pragma unroll
-  for (int i = 0; i < EPL; ++i)
-    if (lane * EPL + i < a.experts) ds[lane * EPL + i] = 0.f;
-  __syncwarp();
-  if (expert >= 0) atomicAdd(ds + expert, d);      // distinct experts: no order to depend on
-  __syncwarp();
-  T* const out = static_cast<T*>(a.dlogits) + token * a.dstride;
+    for (int i = 0; i < EPL; ++i) p[i] = next[i];
+    int expert = -1;
+    float d = 0.f;
+    if (lane < a.top_k) {
+      expert = a.given[token * a.top_k + lane];
+      d = a.dweights[token * a.top_k + lane] * a.scale;
+      if ((unsigned)expert >= a.experts) expert = -1;
+    }
+    if (token + stride < a.tokens) load_logits<T, EPL>(a, logits + (token + stride) * a.stride, lane, next);
+    score<EPL, false>(a, p);
+    // the chosen's scores, by way of the lanes that hold them
+    float s = 0.f;
 #pragma unroll
-  for (int i = 0; i < EPL; ++i) {
-    const unsigned e = lane * EPL + i;
-    if (e >= a.experts) continue;
-    const float g = a.softmax ? p[i] * (ds[e] - dot) : ds[e] * p[i] * (1.f - p[i]);
-    out[e] = from_float<T>(g);
+    for (int i = 0; i < EPL; ++i) {
+      const float v = __shfl_sync(~0u, p[i], expert < 0 ? 0 : expert / EPL);
+      if (expert >= 0 && expert % EPL == i) s = v;
+    }
+    if (expert < 0) d = 0.f;
+    if (a.renormalise) {
+      const float total = sum(s), mean = sum(d * s);
+      const float by = total == 0.f ? 0.f : __fdiv_rn(1.f, total);
+      d = expert < 0 ? 0.f : (d - mean * by) * by;
+    }
+    const float dot = a.softmax ? sum(d * s) : 0.f;
+    if (expert >= 0) atomicAdd(ds + expert, d);      // distinct experts: no order to depend on
+    __syncwarp();
+    float g[EPL];
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) g[i] = ds[lane * EPL + i];
+    __syncwarp();
+    if (expert >= 0) ds[expert] = 0.f;
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) g[i] = a.softmax ? p[i] * (g[i] - dot) : g[i] * p[i] * (1.f - p[i]);
+    T* const out = static_cast<T*>(a.dlogits) + token * a.dstride + lane * EPL;
+    if (a.wide_out && (lane + 1) * EPL <= a.experts) {
+      constexpr int W = EPL * sizeof(T) > 16 ? 16 / sizeof(T) : EPL;
+#pragma unroll
+      for (int i = 0; i < EPL; i += W) store_pack<T, W>(out + i, narrow<T, W>(reinterpret_cast<const float(&)[W]>(g[i])));
+    } else {
+#pragma unroll
+      for (int i = 0; i < EPL; ++i)
+        if (lane * EPL + i < a.experts) out[i] = from_float<T>(g[i]);
+    }
   }
 }
 
@@ -624,12 +664,14 @@ int eps_b200_route_experts_backward(const EpsB200RouteExperts* a, const int32_t*
     r.dlogits = dlogits;
     r.dstride = dlogits_stride;
     r.wide = lanes_wide(r.logits, r.stride, r.experts, a->type);
-    const size_t shared = kWarps * r.experts * 4;
+    r.wide_out = lanes_wide(dlogits, dlogits_stride, r.experts, a->type);
+    const uint64_t most = (uint64_t)sm_count(a->device) * 8, all = ceil_div(r.tokens, kWarps);
     by_type(a->type, [&](auto t) {
       by_experts(r.experts, [&](auto epl) {
         auto* kernel = route_gradient<decltype(t), decltype(epl)::value>;
+        const size_t shared = kWarps * 32 * decltype(epl)::value * 4;
         room(kernel, shared);
-        kernel<<<(unsigned)ceil_div(r.tokens, kWarps), kWarps * 32, shared, static_cast<cudaStream_t>(stream)>>>(r);
+        kernel<<<(unsigned)(all < most ? all : most), kWarps * 32, shared, static_cast<cudaStream_t>(stream)>>>(r);
       });
     });
     check(cudaGetLastError(), "route_experts_backward");
