@@ -25,47 +25,94 @@ struct Quantize {
   int8_t* q;
   float* scale;
   int wide;
+  int* clear;              // [count][clear_words] words that the product wants to be 0
+  unsigned clear_words;
 };
 
-// One block a row, two passes over it: the largest magnitude, then the values (the
-// second read comes from L1 or L2).
+// The factor and the scale of a row whose largest magnitude has these bits.
+__device__ __forceinline__ void factors(unsigned top, bool known, float* by, float* scale) {
+  const float amax = __uint_as_float(top);
+  const bool finite = known && top < 0x7F800000u;
+  *by = finite && amax >= 0x1p-120f ? __fmul_rn(127.f, __fdiv_rn(1.f, amax)) : 0.f;
+  *scale = !finite ? NAN : *by == 0.f ? 0.f : __fdiv_rn(amax, 127.f);
+}
+
+// by == 0: nothing but zeros comes out, also of NaN and infinity.
+__device__ __forceinline__ unsigned quantized(float v, float by) {
+  return by == 0.f ? 0u : (unsigned)__float2int_rn(__fmul_rn(v, by)) & 0xFFu;
+}
+
+// Row r's place in x; `known` is false where `rows` points outside.
 template <class T>
-__global__ void __launch_bounds__(256) quantize_rows(const Quantize a) {
-  __shared__ unsigned tops[8];
+__device__ __forceinline__ const T* source_row(const Quantize& a, uint64_t r, bool* known) {
+  const int64_t index = a.rows ? a.rows[r] : (int64_t)r, from = a.rows ? index / (int64_t)a.divisor : index;
+  *known = index >= 0 && (uint64_t)from < a.x_rows;
+  return static_cast<const T*>(a.x) + (*known ? from : 0) * a.stride;
+}
+
+// A block a row.  Rows of up to NIT packs of 16 bytes a thread stay in registers
+// between the search for the largest magnitude and the rounding (one pass over
+// memory, which is what bounds it); NIT == 0 reads a row of any kind twice.
+constexpr unsigned kQuantizeThreads = 128;
+template <class T, int NIT>
+__global__ void __launch_bounds__(kQuantizeThreads) quantize_rows(const Quantize a) {
+  __shared__ unsigned tops[kQuantizeThreads / 32];
+  constexpr int V = 16 / sizeof(T), kHeld = NIT ? NIT : 1;
   const uint64_t r = blockIdx.x;
-  const int64_t from = a.rows ? a.rows[r] / (int64_t)a.divisor : (int64_t)r;
-  const bool known = (!a.rows || a.rows[r] >= 0) && (uint64_t)from < a.x_rows;
-  const T* const x = static_cast<const T*>(a.x) + (known ? from : 0) * a.stride;
-  constexpr int V = 16 / sizeof(T);
+  for (unsigned i = threadIdx.x; i < a.clear_words; i += kQuantizeThreads) a.clear[r * a.clear_words + i] = 0;
+  bool known;
+  const T* const x = source_row<T>(a, r, &known);
   unsigned top = 0;
-  if (known) {
-    if (a.wide) {
-      for (unsigned k = threadIdx.x * V; k < a.inner; k += 256 * V) {
-        const Pack<T, V> p = load_pack<T, V>(x + k);
+  auto look = [&](float v) { top = max(top, __float_as_uint(v) & 0x7FFFFFFFu); };
+  Pack<T, V> held[kHeld];
+  if constexpr (NIT > 0) {
 #pragma unroll
-        for (int j = 0; j < V; ++j) top = max(top, __float_as_uint(to_float(p.v[j])) & 0x7FFFFFFFu);
-      }
-    } else {
-      for (unsigned k = threadIdx.x; k < a.inner; k += 256) top = max(top, __float_as_uint(to_float(x[k])) & 0x7FFFFFFFu);
+    for (int i = 0; i < NIT; ++i) {
+      const unsigned k = (i * kQuantizeThreads + threadIdx.x) * V;
+      held[i] = Pack<T, V>{};
+      if (known && k < a.inner) held[i] = load_once<T, V>(x + k);
     }
+#pragma unroll
+    for (int i = 0; i < NIT; ++i) {
+      float v[V];
+      widen(held[i], v);
+#pragma unroll
+      for (int j = 0; j < V; ++j) look(v[j]);
+    }
+  } else if (known) {
+    for (unsigned k = threadIdx.x; k < a.inner; k += kQuantizeThreads) look(to_float(x[k]));
   }
   top = __reduce_max_sync(~0u, top);
   if (threadIdx.x % 32 == 0) tops[threadIdx.x / 32] = top;
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < 8; ++w) top = max(top, tops[w]);
-  const float amax = __uint_as_float(top);
-  const bool finite = known && top < 0x7F800000u;
-  const float by = finite && amax >= 0x1p-120f ? __fmul_rn(127.f, __fdiv_rn(1.f, amax)) : 0.f;
-  if (threadIdx.x == 0) a.scale[r] = !finite ? NAN : by == 0.f ? 0.f : __fdiv_rn(amax, 127.f);
+  for (unsigned w = 0; w < kQuantizeThreads / 32; ++w) top = max(top, tops[w]);
+  float by, scale;
+  factors(top, known, &by, &scale);
+  if (threadIdx.x == 0) a.scale[r] = scale;
   int8_t* const q = a.q + r * a.padded;
-  auto round = [by](float v) { return by == 0.f ? 0 : __float2int_rn(__fmul_rn(v, by)); };
-  for (unsigned k = threadIdx.x * 4; k < a.padded; k += 256 * 4) {
-    unsigned word = 0;
+  if constexpr (NIT > 0) {
 #pragma unroll
-    for (unsigned j = 0; j < 4; ++j)
-      if (k + j < a.inner) word |= ((unsigned)round(to_float(x[k + j])) & 0xFFu) << 8 * j;
-    *reinterpret_cast<unsigned*>(q + k) = word;
+    for (int i = 0; i < NIT; ++i) {
+      const unsigned k = (i * kQuantizeThreads + threadIdx.x) * V;
+      if (k >= a.padded) continue;           // behind `inner` the packs hold zeros
+      float v[V];
+      widen(held[i], v);
+      unsigned words[V / 4];
+#pragma unroll
+      for (int w = 0; w < V / 4; ++w)
+        words[w] = quantized(v[4 * w], by) | quantized(v[4 * w + 1], by) << 8 | quantized(v[4 * w + 2], by) << 16 | quantized(v[4 * w + 3], by) << 24;
+      if constexpr (V == 8) *reinterpret_cast<uint2*>(q + k) = make_uint2(words[0], words[1]);
+      else *reinterpret_cast<unsigned*>(q + k) = words[0];
+    }
+  } else {
+    for (unsigned k = threadIdx.x * 4; k < a.padded; k += kQuantizeThreads * 4) {
+      unsigned word = 0;
+#pragma unroll
+      for (unsigned j = 0; j < 4; ++j)
+        if (k + j < a.inner) word |= quantized(to_float(x[k + j]), by) << 8 * j;
+      *reinterpret_cast<unsigned*>(q + k) = word;
+    }
   }
 }
 
@@ -75,9 +122,22 @@ struct Product {
   const int32_t* offsets;
   void* out;
   unsigned rows, experts, channels, padded;
+  int* sums;               // [rows, channels], zeros: where parts of the tensor cores' sums meet; or NULL
 };
 
 struct Tile { unsigned expert, row, rows; };   // rows == 0: there is no such tile
+
+// Expert e's run of rows, clamped to what there is.
+__device__ __forceinline__ void run_of(const Product& a, unsigned e, unsigned* begin, unsigned* end) {
+  *begin = (unsigned)min(max(a.offsets[e], 0), (int)a.rows);
+  *end = (unsigned)min(max(a.offsets[e + 1], 0), (int)a.rows);
+}
+
+__device__ __forceinline__ unsigned tiles_of(const Product& a, unsigned e, unsigned tile_rows) {
+  unsigned begin, end;
+  run_of(a, e, &begin, &end);
+  return end > begin ? (end - begin + tile_rows - 1) / tile_rows : 0;
+}
 
 // The index-th tile of `tile_rows` rows, expert after expert; called by a whole warp.
 __device__ __forceinline__ Tile locate(const Product& a, unsigned tile_rows, unsigned index) {
@@ -89,10 +149,7 @@ __device__ __forceinline__ Tile locate(const Product& a, unsigned tile_rows, uns
   unsigned before = 0;
   for (unsigned e0 = 0; e0 < a.experts; e0 += 32) {
     unsigned begin = 0, end = 0;
-    if (e0 + lane < a.experts) {
-      begin = (unsigned)min(max(a.offsets[e0 + lane], 0), (int)a.rows);
-      end = (unsigned)min(max(a.offsets[e0 + lane + 1], 0), (int)a.rows);
-    }
+    if (e0 + lane < a.experts) run_of(a, e0 + lane, &begin, &end);
     const unsigned n = end > begin ? (end - begin + tile_rows - 1) / tile_rows : 0;
     unsigned sum = n;
 #pragma unroll
@@ -112,36 +169,117 @@ __device__ __forceinline__ Tile locate(const Product& a, unsigned tile_rows, uns
   return {0, 0, 0};
 }
 
-// A warp a channel, RT rows at once, the weights streamed past them.
-template <class T, int RT>
-__global__ void __launch_bounds__(256) product_rows(const Product a, unsigned channel_blocks) {
-  const unsigned lane = threadIdx.x % 32;
+// Few rows: the weights' bytes are all there is.  A warp has a channel, asks for its
+// first weights, and while they come the block quantizes its RT rows into shared
+// memory for all its warps (every block does that again: the rows are a few kilobytes
+// in L2, and a launch before this one would take longer).
+constexpr unsigned kRowsThreads = 256, kRowsAhead = 8;
+template <class T, int RT, bool QUANTIZE>
+__global__ void __launch_bounds__(kRowsThreads) product_rows(const Product a, const Quantize z, unsigned channel_blocks) {
+  extern __shared__ __align__(16) int8_t staged[];      // QUANTIZE: [RT][padded]
+  __shared__ unsigned tops[RT][kRowsThreads / 32];
+  constexpr int kV = 16 / sizeof(T);
+  const unsigned lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   const Tile t = locate(a, RT, blockIdx.x / channel_blocks);
-  const unsigned n = blockIdx.x % channel_blocks * 8 + threadIdx.x / 32;
-  if (!t.rows || n >= a.channels) return;
-  const int8_t* const w = a.weight + ((uint64_t)t.expert * a.channels + n) * a.padded;
-  const int8_t* const q = a.q + (uint64_t)t.row * a.padded;
+  if (!t.rows) return;
+  const unsigned n = blockIdx.x % channel_blocks * (kRowsThreads / 32) + warp;
+  const bool in = n < a.channels;
+  const int8_t* const w = a.weight + ((uint64_t)t.expert * a.channels + (in ? n : 0)) * a.padded;
+  int4 ahead[kRowsAhead];
+#pragma unroll
+  for (unsigned i = 0; i < kRowsAhead; ++i) {
+    const unsigned k = (i * 32 + lane) * 16;
+    ahead[i] = make_int4(0, 0, 0, 0);
+    if (in && k < a.padded) ahead[i] = __ldcs(reinterpret_cast<const int4*>(w + k));
+  }
+  float scale[RT];
+  if constexpr (QUANTIZE) {
+    // rows in turn: a row's values a thread holds are every kRowsThreads-th
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+      bool known = false;
+      unsigned top = 0;
+      if (r < t.rows) {
+        const T* const x = source_row<T>(z, t.row + r, &known);
+        if (known && z.wide) {
+#pragma unroll 2
+          for (unsigned k = threadIdx.x * kV; k < z.inner; k += kRowsThreads * kV) {
+            float v[kV];
+            widen(load_pack<T, kV>(x + k), v);
+#pragma unroll
+            for (int j = 0; j < kV; ++j) top = max(top, __float_as_uint(v[j]) & 0x7FFFFFFFu);
+          }
+        } else if (known) {
+          for (unsigned k = threadIdx.x; k < z.inner; k += kRowsThreads) top = max(top, __float_as_uint(to_float(x[k])) & 0x7FFFFFFFu);
+        }
+      }
+      top = __reduce_max_sync(~0u, top);
+      if (lane == 0) tops[r][warp] = top;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+      scale[r] = 0.f;
+      if (r >= t.rows) continue;
+      bool known;
+      const T* const x = source_row<T>(z, t.row + r, &known);
+      unsigned top = 0;
+#pragma unroll
+      for (unsigned i = 0; i < kRowsThreads / 32; ++i) top = max(top, tops[r][i]);
+      float by;
+      factors(top, known, &by, &scale[r]);
+      if (known && z.wide) {
+        for (unsigned k = threadIdx.x * kV; k < a.padded; k += kRowsThreads * kV) {
+          float v[kV] = {};
+          if (k < z.inner) widen(load_pack<T, kV>(x + k), v);
+#pragma unroll
+          for (int j = 0; j < kV; j += 4)
+            *reinterpret_cast<unsigned*>(staged + r * a.padded + k + j) =
+                quantized(v[j], by) | quantized(v[j + 1], by) << 8 | quantized(v[j + 2], by) << 16 | quantized(v[j + 3], by) << 24;
+        }
+      } else {
+        for (unsigned k = threadIdx.x; k < a.padded; k += kRowsThreads)
+          staged[r * a.padded + k] = k < z.inner ? (int8_t)quantized(to_float(x[k]), by) : 0;
+      }
+    }
+    __syncthreads();
+  } else {
+#pragma unroll
+    for (int r = 0; r < RT; ++r) scale[r] = r < t.rows ? a.scale[t.row + r] : 0.f;
+  }
+  if (!in) return;
+  const int8_t* const q = QUANTIZE ? staged : a.q + (uint64_t)t.row * a.padded;
   int acc[RT];
 #pragma unroll
   for (int r = 0; r < RT; ++r) acc[r] = 0;
-  for (unsigned k = lane * 16; k < a.padded; k += 512) {
-    const int4 x = *reinterpret_cast<const int4*>(w + k);
+  for (unsigned k0 = 0; k0 < a.padded; k0 += kRowsAhead * 512) {
+    int4 now[kRowsAhead];
 #pragma unroll
-    for (int r = 0; r < RT; ++r) {
-      if (r >= t.rows) continue;
-      const int4 y = *reinterpret_cast<const int4*>(q + (uint64_t)r * a.padded + k);
-      acc[r] = __dp4a(x.x, y.x, __dp4a(x.y, y.y, __dp4a(x.z, y.z, __dp4a(x.w, y.w, acc[r]))));
+    for (unsigned i = 0; i < kRowsAhead; ++i) {
+      now[i] = ahead[i];
+      const unsigned k = k0 + kRowsAhead * 512 + (i * 32 + lane) * 16;
+      ahead[i] = make_int4(0, 0, 0, 0);
+      if (k < a.padded) ahead[i] = __ldcs(reinterpret_cast<const int4*>(w + k));
+    }
+#pragma unroll
+    for (unsigned i = 0; i < kRowsAhead; ++i) {
+      const unsigned k = k0 + (i * 32 + lane) * 16;
+      if (k >= a.padded) break;
+#pragma unroll
+      for (int r = 0; r < RT; ++r) {
+        if (r >= t.rows) continue;
+        const int4 y = *reinterpret_cast<const int4*>(q + (uint64_t)r * a.padded + k);
+        acc[r] = __dp4a(now[i].x, y.x, __dp4a(now[i].y, y.y, __dp4a(now[i].z, y.z, __dp4a(now[i].w, y.w, acc[r]))));
+      }
     }
   }
+  const uint64_t c = (uint64_t)t.expert * a.channels + n;
+  const float ws = a.weight_scale[c], b = a.bias ? a.bias[c] : 0.f;
 #pragma unroll
   for (int r = 0; r < RT; ++r) {
     const int sum = __reduce_add_sync(~0u, acc[r]);
-    if (lane == r && r < t.rows) {
-      const uint64_t c = (uint64_t)t.expert * a.channels + n;
-      float v = (float)sum * (a.scale[t.row + r] * a.weight_scale[c]);
-      if (a.bias) v += a.bias[c];
-      static_cast<T*>(a.out)[(uint64_t)(t.row + r) * a.channels + n] = from_float<T>(v);
-    }
+    if (lane == 0 && r < t.rows)
+      static_cast<T*>(a.out)[(uint64_t)(t.row + r) * a.channels + n] = from_float<T>(fmaf((float)sum, scale[r] * ws, b));
   }
 }
 
@@ -154,7 +292,8 @@ __global__ void __launch_bounds__(256) product_rows(const Product a, unsigned ch
 // matrix instruction reads; out-of-range rows and bytes arrive as zeros, and rows of
 // the next expert or channel group, which a ragged tile also covers, are not stored.
 //
-// One block an SM walks the tiles: warp 0 fills the stages, warp 1 issues
+// With few tiles the blocks share the stages of all tiles evenly (see Deal).  One block
+// an SM walks its parts of the tiles: warp 0 fills the stages, warp 1 issues
 // tcgen05.mma (kind::i8, 32-bit sums in tensor memory), warps 4..7 scale, round and
 // store the tile before while the next is being summed (two halves of tensor memory).
 constexpr int kMmaThreads = 256;
@@ -169,29 +308,60 @@ struct MmaShape {
   static constexpr unsigned columns = 2 * BN;                          // of tensor memory
 };
 
-__device__ __forceinline__ void tma_load(void* to, const CUtensorMap* map, uint64_t* barrier, int x, int y) {
+// The same for a whole warp, which stays together.
+// `b` is a shared address.
+__device__ __forceinline__ bool warp_wait(unsigned b, unsigned parity) {
+  uint64_t start = 0;
+  for (unsigned tries = 1;; ++tries) {
+    unsigned done;
+    asm volatile(
+        "{\n .reg .pred p;\n"
+        " mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+        " selp.u32 %0, 1, 0, p;\n}\n"
+        : "=r"(done) : "r"(b), "r"(parity) : "memory");
+    if (__all_sync(~0u, done)) return true;
+    if (tries % 256 == 0) {
+      const uint64_t now = nanoseconds();
+      if (!start) start = now;
+      else if (__any_sync(~0u, now - start > 2000000000ull)) return false;
+    }
+  }
+}
+
+// One lane of a warp that is together, always the same.
+__device__ __forceinline__ bool elected() {
+  unsigned one;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xFFFFFFFF;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(one));
+  return one;
+}
+
+__device__ __forceinline__ void expect(unsigned barrier, unsigned bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(barrier), "r"(bytes) : "memory");
+}
+
+__device__ __forceinline__ void tma_load(unsigned to, const CUtensorMap* map, unsigned barrier, int x, int y) {
   asm volatile("cp.async.bulk.tensor.2d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
-               ::"r"(shared_at(to)), "l"(map), "r"(shared_at(barrier)), "r"(x), "r"(y) : "memory");
+               ::"r"(to), "l"(map), "r"(barrier), "r"(x), "r"(y) : "memory");
 }
 
 // Shared-memory descriptor of a K-major operand in the 128-byte swizzle: rows of 128
-// bytes, groups of eight rows 1024 bytes apart.
-__device__ __forceinline__ uint64_t operand(const void* p) {
-  return (uint64_t)(shared_at(p) >> 4 & 0x3FFF) | 1ull << 16 | (uint64_t)(1024 >> 4) << 32 | 1ull << 46 | 2ull << 61;
-}
+// bytes, groups of eight rows 1024 bytes apart.  Its upper word is a constant, its
+// lower one moves with the address; kept apart they stay in uniform registers.
+constexpr unsigned kOperandHigh = 1024 >> 4 | 1u << 14 | 2u << 29;
+__device__ __forceinline__ unsigned operand_low(unsigned address) { return (address >> 4 & 0x3FFF) | 1u << 16; }
 
 template <int BN>
-__device__ __forceinline__ void mma_i8(unsigned d, uint64_t a, uint64_t b, bool accumulate) {
+__device__ __forceinline__ void mma_i8(unsigned d, unsigned a, unsigned b, bool accumulate) {
   // 32-bit signed sums, signed 8-bit operands, both K-major, N = BN, M = 128
   constexpr unsigned shape = 2u << 4 | 1u << 7 | 1u << 10 | (unsigned)(BN / 8) << 17 | (kTileM / 16) << 24;
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n}\n"
-      ::"r"(d), "l"(a), "l"(b), "r"(shape), "r"((unsigned)accumulate) : "memory");
+      "{\n .reg .pred p;\n .reg .b64 a, b;\n setp.ne.u32 p, %4, 0;\n mov.b64 a, {%1, %5};\n mov.b64 b, {%2, %5};\n"
+      " tcgen05.mma.cta_group::1.kind::i8 [%0], a, b, %3, p;\n}\n"
+      ::"r"(d), "r"(a), "r"(b), "r"(shape), "r"((unsigned)accumulate), "r"(kOperandHigh) : "memory");
 }
 
-__device__ __forceinline__ void mma_commit(uint64_t* barrier) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(shared_at(barrier)) : "memory");
+__device__ __forceinline__ void mma_commit(unsigned barrier) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(barrier) : "memory");
 }
 
 // 32 lanes x 32 columns of tensor memory: lane l of the warp gets its 32 columns.
@@ -208,6 +378,61 @@ __device__ __forceinline__ void tensor_load(unsigned address, int (&v)[32]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
 
+// The parts of the work that a block does, one after the other: `steps` stages of
+// inner size of a tile each.  With few tiles (`sums` given) all stages of all tiles are
+// dealt out evenly, in runs that may begin and end inside a tile, and added up in
+// `sums`; otherwise a block takes every grid-th whole tile.
+struct Part {
+  Tile tile;
+  unsigned channel_tile;
+  unsigned first, last;        // stages of the tile
+};
+
+struct Deal {
+  const Product& a;
+  unsigned tile_rows, channel_tiles, steps;
+  uint64_t at, end;            // sums given: stages; otherwise tiles
+
+  // The stages of all tiles; called by a whole warp.
+  static __device__ __forceinline__ uint64_t stages_of(const Product& a, unsigned tile_rows, unsigned channel_tiles, unsigned steps) {
+    const unsigned lane = threadIdx.x % 32;
+    uint64_t tiles = 0;
+    if (!a.offsets) {
+      tiles = (a.rows + tile_rows - 1) / tile_rows;
+    } else {
+      for (unsigned e0 = 0; e0 < a.experts; e0 += 32) {
+        unsigned n = 0;
+        if (e0 + lane < a.experts) n = tiles_of(a, e0 + lane, tile_rows);
+        tiles += __reduce_add_sync(~0u, n);
+      }
+    }
+    return tiles * channel_tiles * steps;
+  }
+  __device__ __forceinline__ Deal(const Product& p, unsigned rows, unsigned channels, unsigned s, uint64_t all)
+      : a(p), tile_rows(rows), channel_tiles(channels), steps(s) {
+    at = a.sums ? all * blockIdx.x / gridDim.x : blockIdx.x;
+    end = a.sums ? all * (blockIdx.x + 1) / gridDim.x : ~0ull;
+  }
+  __device__ __forceinline__ bool next(Part* p) {
+    if (at >= end) return false;
+    const uint64_t index = a.sums ? at / steps : at;
+    p->tile = locate(a, tile_rows, (unsigned)(index / channel_tiles));
+    if (!p->tile.rows) return false;
+    p->channel_tile = (unsigned)(index % channel_tiles);
+    p->first = 0;
+    p->last = steps;
+    if (a.sums) {
+      p->first = (unsigned)(at - index * steps);
+      const uint64_t left = end - at;
+      if (p->first + left < steps) p->last = p->first + (unsigned)left;
+      at += p->last - p->first;
+    } else {
+      at += gridDim.x;
+    }
+    return true;
+  }
+};
+
 template <class T, int BN>
 __global__ void __launch_bounds__(kMmaThreads, 1)
     product_tiles(const Product a, const __grid_constant__ CUtensorMap weights, const __grid_constant__ CUtensorMap rows,
@@ -216,7 +441,8 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
   extern __shared__ unsigned char raw[];
   __shared__ uint64_t full[Shape::stages], empty[Shape::stages], summed[2], drained[2];
   __shared__ unsigned tensor_base;
-  unsigned char* const stages = raw + (1024 - shared_at(raw) % 1024) % 1024;
+  const unsigned at_stages = (shared_at(raw) + 1023) / 1024 * 1024, at_full = shared_at(full), at_empty = shared_at(empty);
+  const unsigned low_operand = operand_low(at_stages);
   const unsigned warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   if (threadIdx.x == 0) {
     for (unsigned s = 0; s < Shape::stages; ++s) {
@@ -241,81 +467,92 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const unsigned base = tensor_base;
   const unsigned steps = (a.padded + kStageK - 1) / kStageK;
+  const uint64_t all = a.sums ? Deal::stages_of(a, BN, channel_tiles, steps) : 0;
+  Deal deal(a, BN, channel_tiles, steps, all);
+  Part part;
 
   if (warp == 0) {
     unsigned stage = 0, phase = 0, filled = 0;
     bool ok = true;
-    for (unsigned t = blockIdx.x; ok; t += gridDim.x) {
-      const Tile tile = locate(a, BN, t / channel_tiles);
-      if (!tile.rows) break;
-      if (lane == 0) {
-        const int y = (int)(tile.expert * a.channels + t % channel_tiles * kTileM);
-        for (unsigned k = 0; k < steps; ++k) {
-          if (!(ok = barrier_wait(empty + stage, phase ^ 1))) break;
-          unsigned char* const p = stages + stage * Shape::stage_bytes;
-          barrier_expect(full + stage, Shape::stage_bytes);
-          tma_load(p, &weights, full + stage, (int)(k * kStageK), y);
-          tma_load(p + kTileM * kStageK, &rows, full + stage, (int)(k * kStageK), (int)tile.row);
-          if (++filled > Shape::stages) filled = Shape::stages;
-          if (++stage == Shape::stages) { stage = 0; phase ^= 1; }
+    while (ok && deal.next(&part)) {
+      const int y = (int)(part.tile.expert * a.channels + part.channel_tile * kTileM);
+      for (unsigned k = part.first; k < part.last; ++k) {
+        if (!(ok = warp_wait(at_empty + stage * 8, phase ^ 1))) break;
+        const unsigned to = at_stages + stage * Shape::stage_bytes, barrier = at_full + stage * 8;
+        if (elected()) {
+          expect(barrier, Shape::stage_bytes);
+          tma_load(to, &weights, barrier, (int)(k * kStageK), y);
+          tma_load(to + kTileM * kStageK, &rows, barrier, (int)(k * kStageK), (int)part.tile.row);
         }
+        if (++filled > Shape::stages) filled = Shape::stages;
+        if (++stage == Shape::stages) { stage = 0; phase ^= 1; }
       }
-      ok = __shfl_sync(~0u, ok, 0);
     }
     // no block ends with copies into its shared memory in flight
-    if (lane == 0 && !ok)
+    if (!ok)
       for (unsigned n = 0; n < filled; ++n) {
         stage = stage ? stage - 1 : Shape::stages - 1;
         if (stage == Shape::stages - 1) phase ^= 1;
-        barrier_wait(full + stage, phase);
+        warp_wait(at_full + stage * 8, phase);
       }
   } else if (warp == 1) {
     unsigned stage = 0, phase = 0, half = 0, turn = 0;
     bool ok = true;
-    for (unsigned t = blockIdx.x; ok; t += gridDim.x) {
-      if (!locate(a, BN, t / channel_tiles).rows) break;
-      if (lane == 0) {
-        ok = barrier_wait(drained + half, turn ^ 1);
+    while (ok && deal.next(&part)) {
+      ok = warp_wait(shared_at(drained) + half * 8, turn ^ 1);
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      for (unsigned k = part.first; ok && k < part.last; ++k) {
+        if (!(ok = warp_wait(at_full + stage * 8, phase))) break;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        for (unsigned k = 0; ok && k < steps; ++k) {
-          if (!(ok = barrier_wait(full + stage, phase))) break;
-          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-          const unsigned char* const p = stages + stage * Shape::stage_bytes;
-          const uint64_t w = operand(p), q = operand(p + kTileM * kStageK);
+        const unsigned w = low_operand + stage * (Shape::stage_bytes / 16), q = w + kTileM * kStageK / 16, d = base + half * BN;
+        if (elected()) {
 #pragma unroll
-          for (unsigned i = 0; i < kStageK / 32; ++i) mma_i8<BN>(base + half * BN, w + 2 * i, q + 2 * i, k || i);
-          mma_commit(empty + stage);
-          if (++stage == Shape::stages) { stage = 0; phase ^= 1; }
+          for (unsigned i = 0; i < kStageK / 32; ++i) mma_i8<BN>(d, w + 2 * i, q + 2 * i, k != part.first || i);
+          mma_commit(at_empty + stage * 8);
         }
-        if (ok) mma_commit(summed + half);
+        if (++stage == Shape::stages) { stage = 0; phase ^= 1; }
       }
-      ok = __shfl_sync(~0u, ok, 0);
+      if (ok && elected()) mma_commit(shared_at(summed) + half * 8);
+      __syncwarp();
       half ^= 1;
       turn ^= half == 0;
     }
   } else if (warp >= 4) {
     unsigned half = 0, turn = 0;
     bool ok = true;
-    for (unsigned t = blockIdx.x; ok; t += gridDim.x) {
-      const Tile tile = locate(a, BN, t / channel_tiles);
-      if (!tile.rows) break;
-      const unsigned n = t % channel_tiles * kTileM + (warp - 4) * 32 + lane;
+    while (ok && deal.next(&part)) {
+      const Tile tile = part.tile;
+      const unsigned l = (warp - 4) * 32 + lane, n = part.channel_tile * kTileM + l;
       const uint64_t c = (uint64_t)tile.expert * a.channels + n;
       const bool in = n < a.channels;
       const float ws = in ? a.weight_scale[c] : 0.f, b = in && a.bias ? a.bias[c] : 0.f;
-      ok = __all_sync(~0u, barrier_wait(summed + half, turn));
+      ok = warp_wait(shared_at(summed) + half * 8, turn);
+      if (!ok && a.sums)           // the rows whose sums are lost
+        for (unsigned r = lane; r < tile.rows; r += 32) const_cast<float*>(a.scale)[tile.row + r] = NAN;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       T* const out = static_cast<T*>(a.out) + (uint64_t)tile.row * a.channels + n;
-#pragma unroll 1
-      for (unsigned r0 = 0; r0 < tile.rows; r0 += 32) {
-        int v[32];
-        tensor_load(base + half * BN + r0 + ((warp - 4) * 32 << 16), v);
+      const unsigned from = base + half * BN + ((warp - 4) * 32 << 16);
+      auto finish = [&](unsigned r0, const int (&v)[32]) {
         const float mine = r0 + lane < tile.rows ? a.scale[tile.row + r0 + lane] : 0.f;
 #pragma unroll
         for (unsigned j = 0; j < 32; ++j) {
           const float s = __shfl_sync(~0u, mine, j);
           const float value = ok ? fmaf((float)v[j], s * ws, b) : NAN;
           if (in && r0 + j < tile.rows) out[(uint64_t)(r0 + j) * a.channels] = from_float<T>(value);
+        }
+      };
+#pragma unroll 1
+      for (unsigned r0 = 0; r0 < tile.rows; r0 += 32) {
+        int v[32];
+        tensor_load(from + r0, v);
+        if (!a.sums) {
+          finish(r0, v);
+        } else {
+          // a part of the sum: 32-bit integers may be added in any order
+          int* const s = a.sums + (uint64_t)(tile.row + r0) * a.channels + n;
+#pragma unroll
+          for (unsigned j = 0; j < 32; ++j)
+            if (in && r0 + j < tile.rows) atomicAdd(s + (uint64_t)j * a.channels, v[j]);
         }
       }
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -332,6 +569,23 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(base), "r"(Shape::columns) : "memory");
 }
 
+// The tiles' sums, scaled: 32 rows of a tile a block.
+template <class T>
+__global__ void __launch_bounds__(256) product_finish(const Product a, unsigned tile_rows, unsigned channel_tiles) {
+  const Tile tile = locate(a, tile_rows, blockIdx.x / channel_tiles);
+  const unsigned n = blockIdx.x % channel_tiles * kTileM + threadIdx.x % kTileM, r0 = blockIdx.y * 32 + threadIdx.x / kTileM;
+  if (r0 >= tile.rows || n >= a.channels) return;
+  const uint64_t c = (uint64_t)tile.expert * a.channels + n;
+  const float ws = a.weight_scale[c], b = a.bias ? a.bias[c] : 0.f;
+#pragma unroll
+  for (unsigned j = 0; j < 32; j += 2) {
+    const unsigned r = r0 + j;
+    if (r >= tile.rows) break;
+    const uint64_t at = (uint64_t)(tile.row + r) * a.channels + n;
+    static_cast<T*>(a.out)[at] = from_float<T>(fmaf((float)__ldcg(a.sums + at), a.scale[tile.row + r] * ws, b));
+  }
+}
+
 template <class F>
 void by_type(int type, F f) {
   if (type == EPS_B200_F32) f(float{});
@@ -341,7 +595,16 @@ void by_type(int type, F f) {
 
 void quantize(int type, const Quantize& a, cudaStream_t stream) {
   need(a.count < (1ull << 31), "too many rows");
-  by_type(type, [&](auto t) { quantize_rows<decltype(t)><<<(unsigned)a.count, 256, 0, stream>>>(a); });
+  by_type(type, [&](auto t) {
+    using T = decltype(t);
+    const unsigned blocks = (unsigned)a.count;
+    const uint64_t packs = ceil_div(a.inner * sizeof(T), 16 * kQuantizeThreads);
+    if (!a.wide || packs > 8) quantize_rows<T, 0><<<blocks, kQuantizeThreads, 0, stream>>>(a);
+    else if (packs <= 1) quantize_rows<T, 1><<<blocks, kQuantizeThreads, 0, stream>>>(a);
+    else if (packs <= 2) quantize_rows<T, 2><<<blocks, kQuantizeThreads, 0, stream>>>(a);
+    else if (packs <= 4) quantize_rows<T, 4><<<blocks, kQuantizeThreads, 0, stream>>>(a);
+    else quantize_rows<T, 8><<<blocks, kQuantizeThreads, 0, stream>>>(a);
+  });
   check(cudaGetLastError(), "int8_quantize");
 }
 
@@ -381,6 +644,22 @@ uint64_t tile_bound(const Product& a, unsigned tile_rows) {
   return ceil_div(a.rows, tile_rows) + extra;
 }
 
+// Which kernel a product takes, by the rows of an expert on average (the host does not
+// know the groups), and its tile's rows.
+unsigned tile_rows_of(uint64_t rows, uint64_t experts) {
+  const uint64_t each = ceil_div(rows, experts);
+  if (rows <= 8 || each <= 2) return 0;
+  return each > 128 ? 256 : each > 64 ? 128 : each > 32 ? 64 : 32;
+}
+
+// Whether the blocks share the tiles' stages: whole tiles would leave most SMs idle,
+// while sums in memory cost four bytes an output twice over L2.  The bound stands for
+// two rounds of a B200's 148 SMs.
+constexpr uint64_t kFewTiles = 296;
+bool shares(const Product& a, unsigned tile_rows) {
+  return tile_rows && tile_bound(a, tile_rows) * ceil_div(a.channels, kTileM) < kFewTiles;
+}
+
 template <int BN>
 void tiles(int type, const Product& a, unsigned sms, cudaStream_t stream) {
   using Shape = MmaShape<BN>;
@@ -389,29 +668,52 @@ void tiles(int type, const Product& a, unsigned sms, cudaStream_t stream) {
   const unsigned channel_tiles = (unsigned)ceil_div(a.channels, kTileM);
   const uint64_t most = tile_bound(a, BN) * channel_tiles;
   need(most < (1ull << 31), "too many rows");
+  const unsigned blocks = a.sums || most > sms ? sms : (unsigned)most;
   by_type(type, [&](auto t) {
     auto* kernel = product_tiles<decltype(t), BN>;
     check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Shape::shared), "cudaFuncSetAttribute");
-    kernel<<<(unsigned)(most < sms ? most : sms), kMmaThreads, Shape::shared, stream>>>(a, w, q, channel_tiles);
+    kernel<<<blocks, kMmaThreads, Shape::shared, stream>>>(a, w, q, channel_tiles);
+    check(cudaGetLastError(), "int8_product");
+    if (a.sums) product_finish<decltype(t)><<<dim3((unsigned)most, BN / 32), 256, 0, stream>>>(a, BN, channel_tiles);
   });
   check(cudaGetLastError(), "int8_product");
 }
 
-void product(int type, const Product& a, unsigned sms, cudaStream_t stream) {
-  const uint64_t each = ceil_div(a.rows, a.experts);      // rows of an expert, on average
-  if (a.rows > 8 && each > 2) {
-    need((uint64_t)a.experts * a.channels < (1ull << 31), "too many channels");
-    if (each > 128) tiles<256>(type, a, sms, stream);
-    else if (each > 64) tiles<128>(type, a, sms, stream);
-    else if (each > 32) tiles<64>(type, a, sms, stream);
-    else tiles<32>(type, a, sms, stream);
-    return;
+void product_by_tiles(int type, const Product& a, unsigned sms, cudaStream_t stream) {
+  need((uint64_t)a.experts * a.channels < (1ull << 31), "too many channels");
+  switch (tile_rows_of(a.rows, a.experts)) {
+    case 256: return tiles<256>(type, a, sms, stream);
+    case 128: return tiles<128>(type, a, sms, stream);
+    case 64: return tiles<64>(type, a, sms, stream);
+    default: return tiles<32>(type, a, sms, stream);
   }
-  const unsigned channel_blocks = (unsigned)ceil_div(a.channels, 8);
-  const uint64_t most = tile_bound(a, 8) * channel_blocks;
+}
+
+// z: quantize on the way; nullptr: a.q and a.scale are given.
+template <int RT>
+void rows_at_once(int type, const Product& a, const Quantize* z, cudaStream_t stream) {
+  const unsigned channel_blocks = (unsigned)ceil_div(a.channels, kRowsThreads / 32);
+  const uint64_t most = tile_bound(a, RT) * channel_blocks;
   need(most < (1ull << 31), "too many rows");
-  by_type(type, [&](auto t) { product_rows<decltype(t), 8><<<(unsigned)most, 256, 0, stream>>>(a, channel_blocks); });
+  by_type(type, [&](auto t) {
+    if (z) {
+      auto* kernel = product_rows<decltype(t), RT, true>;
+      const unsigned shared = RT * a.padded;
+      check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)shared), "cudaFuncSetAttribute");
+      kernel<<<(unsigned)most, kRowsThreads, shared, stream>>>(a, *z, channel_blocks);
+    } else {
+      product_rows<decltype(t), RT, false><<<(unsigned)most, kRowsThreads, 0, stream>>>(a, Quantize{}, channel_blocks);
+    }
+  });
   check(cudaGetLastError(), "int8_product");
+}
+
+void product_by_rows(int type, const Product& a, const Quantize* z, cudaStream_t stream) {
+  const uint64_t each = ceil_div(a.rows, a.experts);
+  if (a.rows == 1) rows_at_once<1>(type, a, z, stream);
+  else if (a.rows == 2 || each <= 2) rows_at_once<2>(type, a, z, stream);
+  else if (a.rows <= 4) rows_at_once<4>(type, a, z, stream);
+  else rows_at_once<8>(type, a, z, stream);
 }
 
 Quantize quantize_args(int type, const void* x, int64_t x_stride, uint64_t x_rows, unsigned inner, const int32_t* rows,
@@ -422,7 +724,7 @@ Quantize quantize_args(int type, const void* x, int64_t x_stride, uint64_t x_row
   need(!count || (q && scale && (x || !x_rows)), "null input or output");
   need(aligned(q, 16), "q must be 16-byte aligned");
   return Quantize{x, x_stride, x_rows, count, inner, (unsigned)eps_b200_int8_stride(inner), divisor, rows, q, scale,
-                  aligned(x, 16) && x_stride * (int64_t)size_of(type) % 16 == 0 && inner * size_of(type) % 16 == 0};
+                  aligned(x, 16) && x_stride * (int64_t)size_of(type) % 16 == 0 && inner * size_of(type) % 16 == 0, nullptr, 0};
 }
 
 Product product_args(const EpsB200Int8Product* a) {
@@ -469,9 +771,18 @@ int eps_b200_int8_quantize(int32_t device, int32_t type, const void* x, int64_t 
 }
 
 uint64_t eps_b200_int8_product_workspace(uint64_t rows, uint32_t experts, uint32_t channels, uint32_t inner) {
-  (void)experts;
-  (void)channels;
-  return rows * eps_b200_int8_stride(inner) + round_up(rows * 4, 16);
+  Product p{};
+  static const int32_t grouped = 0;       // any address: the bound for groups is the larger one
+  p.rows = (unsigned)rows;
+  p.experts = experts ? experts : 1;
+  p.channels = channels;
+  const unsigned tile_rows = tile_rows_of(rows, p.experts);
+  bool sums = shares(p, tile_rows);
+  if (p.experts > 1) {
+    p.offsets = &grouped;
+    sums = shares(p, tile_rows);
+  }
+  return rows * eps_b200_int8_stride(inner) + round_up(rows * 4, 16) + (sums ? rows * channels * 4 : 0);
 }
 
 int eps_b200_int8_product(const EpsB200Int8Product* a, const int8_t* q, const float* scale, void* stream,
@@ -483,8 +794,20 @@ int eps_b200_int8_product(const EpsB200Int8Product* a, const int8_t* q, const fl
     if (!p.rows) return;
     p.q = q;
     p.scale = scale;
+    const auto st = static_cast<cudaStream_t>(stream);
+    const unsigned tile_rows = tile_rows_of(p.rows, p.experts);
+    if (!tile_rows) {
+      OnDevice on(a->device);
+      return product_by_rows(a->type, p, nullptr, st);
+    }
     OnDevice on(a->device);
-    product(a->type, p, sm_count(a->device), static_cast<cudaStream_t>(stream));
+    if (shares(p, tile_rows)) {
+      const uint64_t bytes = (uint64_t)p.rows * p.channels * 4;
+      need(a->workspace && a->workspace_bytes >= bytes, "int8 workspace too small");
+      p.sums = static_cast<int*>(a->workspace);
+      check(cudaMemsetAsync(p.sums, 0, bytes, st), "cudaMemsetAsync");
+    }
+    product_by_tiles(a->type, p, sm_count(a->device), st);
   });
 }
 
@@ -497,13 +820,20 @@ int eps_b200_int8_linear(const EpsB200Int8Product* a, const void* x, int64_t x_s
          "int8 workspace too small");
     auto* q = static_cast<int8_t*>(a->workspace);
     auto* scale = reinterpret_cast<float*>(q + (uint64_t)p.rows * p.padded);
-    const Quantize z = quantize_args(a->type, x, x_stride, x_rows, a->inner, rows, a->rows_divisor, a->rows, q, scale);
+    Quantize z = quantize_args(a->type, x, x_stride, x_rows, a->inner, rows, a->rows_divisor, a->rows, q, scale);
     p.q = q;
     p.scale = scale;
-    OnDevice on(a->device);
     const auto st = static_cast<cudaStream_t>(stream);
+    const unsigned tile_rows = tile_rows_of(p.rows, p.experts);
+    OnDevice on(a->device);
+    if (!tile_rows && p.padded <= 24 * 1024) return product_by_rows(a->type, p, &z, st);       // eight rows fit shared memory
+    if (shares(p, tile_rows)) {
+      p.sums = z.clear = reinterpret_cast<int*>(reinterpret_cast<char*>(scale) + round_up(p.rows * 4ull, 16));
+      z.clear_words = p.channels;
+    }
     quantize(a->type, z, st);
-    product(a->type, p, sm_count(a->device), st);
+    if (tile_rows) product_by_tiles(a->type, p, sm_count(a->device), st);
+    else product_by_rows(a->type, p, nullptr, st);
   });
 }
 

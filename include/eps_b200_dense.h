@@ -153,7 +153,8 @@ EPS_B200_EXPORT int eps_b200_int8_quantize(int32_t device, int32_t type, const v
  * read as clamped to [0, rows] and a run that ends before it begins as empty; rows
  * of no run are not written.  q, weight and out 16-byte aligned; q and weight have
  * row strides of eps_b200_int8_stride(inner) with zeros behind `inner` (at most
- * EPS_B200_INT8_INNER, so that the sum fits 32 bits), out is contiguous. */
+ * EPS_B200_INT8_INNER, so that the sum fits 32 bits), out is contiguous.  The
+ * workspace has eps_b200_int8_product_workspace() bytes. */
 #define EPS_B200_INT8_INNER 131072u
 typedef struct {
   int32_t device;
