@@ -810,37 +810,34 @@ Spread spread_of(unsigned columns, int residual, int type, bool wide) {
 constexpr unsigned kMostBlocks = 8 * 160;   // of the gradient: 8 an SM, 160 SMs
 
 // Blocks that fit the GPU at once, or fewer where the rows need fewer.
-template <class K>
-unsigned resident(K kernel, const Spread& s, size_t shared, uint64_t rows, unsigned sms, unsigned most) {
-  check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)shared), "cudaFuncSetAttribute");
-  int each = 0;
-  check(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&each, kernel, (int)s.threads, shared), "occupancy");
-  need(each > 0, "no room for a block");
-  uint64_t n = (uint64_t)sms * (unsigned)each;
+template <auto Kernel>
+unsigned resident(int device, const Spread& s, size_t shared, uint64_t rows, unsigned most) {
+  room<Kernel>(device, shared);
+  uint64_t n = (uint64_t)sm_count(device) * blocks_each<Kernel>(device, s.threads, shared);
   if (n > most) n = most;
   const uint64_t all = ceil_div(rows, s.threads / s.width);
   return (unsigned)(all < n ? all : n);
 }
 
 template <class TX, class TY, int V, int NIT, int P, int GATE>
-void forward(const Norm& n, const Spread& s, unsigned sms, cudaStream_t stream) {
-  auto* kernel = block_norm_forward<TX, TY, V, NIT, P, GATE>;
+void forward(const Norm& n, const Spread& s, int device, cudaStream_t stream) {
+  constexpr auto kKernel = block_norm_forward<TX, TY, V, NIT, P, GATE>;
   const unsigned lane = Parameters<TY, V, NIT, V * NIT <= 8, true>::kRecord + (kWay<V, NIT, P> != kDirect ? kSlots * forward_bytes<TX, TY, V>() : 0);
-  kernel<<<resident(kernel, s, lane * s.threads, n.rows, sms, ~0u), s.threads, lane * s.threads, stream>>>(n);
+  kKernel<<<resident<kKernel>(device, s, lane * s.threads, n.rows, ~0u), s.threads, lane * s.threads, stream>>>(n);
   check(cudaGetLastError(), "block_norm");
 }
 
 // The number of blocks, which is the number of partial sums.
 template <class TX, class TY, int V, int NIT, int P, int GATE>
-unsigned backward(const Norm& n, const Spread& s, unsigned sms, uint64_t room, cudaStream_t stream) {
-  auto* kernel = block_norm_gradient<TX, TY, V, NIT, P, GATE>;
+unsigned backward(const Norm& n, const Spread& s, int device, uint64_t space, cudaStream_t stream) {
+  constexpr auto kKernel = block_norm_gradient<TX, TY, V, NIT, P, GATE>;
   constexpr bool kRing = kWay<V, NIT, P> != kDirect;
   const unsigned held = (unsigned)__builtin_popcount((unsigned)n.want) * NIT * V * 4;
   const unsigned walked = kRing ? Parameters<TY, V, NIT, true, false>::kRecord + kSlots * backward_bytes<TX, TY, V>() : 0;
   const unsigned shared = (walked > held ? walked : held) * s.threads;       // the sums take the others' place in the end
-  const unsigned blocks = resident(kernel, s, shared, n.rows, sms, kMostBlocks);
-  need(!n.want || room >= (uint64_t)blocks * kSums * n.columns * 4, "block norm workspace too small");
-  kernel<<<blocks, s.threads, shared, stream>>>(n);
+  const unsigned blocks = resident<kKernel>(device, s, shared, n.rows, kMostBlocks);
+  need(!n.want || space >= (uint64_t)blocks * kSums * n.columns * 4, "block norm workspace too small");
+  kKernel<<<blocks, s.threads, shared, stream>>>(n);
   check(cudaGetLastError(), "block_norm_backward");
   return blocks;
 }
@@ -961,7 +958,7 @@ int eps_b200_block_norm(const EpsB200BlockNorm* a, const void* x, int64_t x_stri
         by_gate(n.gate, [&](auto gate) {
           forward<decltype(tx), decltype(ty), decltype(v)::value, decltype(nit)::value, decltype(warps)::value,
                   decltype(gate)::value>(
-              n, s, sm_count(a->device), static_cast<cudaStream_t>(stream));
+              n, s, a->device, static_cast<cudaStream_t>(stream));
         });
       });
     });
@@ -1020,7 +1017,7 @@ int eps_b200_block_norm_backward(const EpsB200BlockNorm* a, const EpsB200BlockNo
         by_gate(n.gate, [&](auto gate) {
           blocks = backward<decltype(tx), decltype(ty), decltype(v)::value, decltype(nit)::value, decltype(warps)::value,
                   decltype(gate)::value>(
-              n, s, sm_count(a->device), d->workspace_bytes, st);
+              n, s, a->device, d->workspace_bytes, st);
         });
       });
     });

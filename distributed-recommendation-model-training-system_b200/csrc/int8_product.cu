@@ -661,7 +661,8 @@ bool shares(const Product& a, unsigned tile_rows) {
 }
 
 template <int BN>
-void tiles(int type, const Product& a, unsigned sms, cudaStream_t stream) {
+void tiles(int type, const Product& a, int device, cudaStream_t stream) {
+  const unsigned sms = sm_count(device);
   using Shape = MmaShape<BN>;
   const CUtensorMap w = tensor_map(a.weight, (uint64_t)a.experts * a.channels, a.padded, kTileM);
   const CUtensorMap q = tensor_map(a.q, a.rows, a.padded, BN);
@@ -670,8 +671,8 @@ void tiles(int type, const Product& a, unsigned sms, cudaStream_t stream) {
   need(most < (1ull << 31), "too many rows");
   const unsigned blocks = a.sums || most > sms ? sms : (unsigned)most;
   by_type(type, [&](auto t) {
-    auto* kernel = product_tiles<decltype(t), BN>;
-    check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Shape::shared), "cudaFuncSetAttribute");
+    constexpr auto kernel = product_tiles<decltype(t), BN>;
+    room<kernel>(device, Shape::shared);
     kernel<<<blocks, kMmaThreads, Shape::shared, stream>>>(a, w, q, channel_tiles);
     check(cudaGetLastError(), "int8_product");
     if (a.sums) product_finish<decltype(t)><<<dim3((unsigned)most, BN / 32), 256, 0, stream>>>(a, BN, channel_tiles);
@@ -679,27 +680,27 @@ void tiles(int type, const Product& a, unsigned sms, cudaStream_t stream) {
   check(cudaGetLastError(), "int8_product");
 }
 
-void product_by_tiles(int type, const Product& a, unsigned sms, cudaStream_t stream) {
+void product_by_tiles(int type, const Product& a, int device, cudaStream_t stream) {
   need((uint64_t)a.experts * a.channels < (1ull << 31), "too many channels");
   switch (tile_rows_of(a.rows, a.experts)) {
-    case 256: return tiles<256>(type, a, sms, stream);
-    case 128: return tiles<128>(type, a, sms, stream);
-    case 64: return tiles<64>(type, a, sms, stream);
-    default: return tiles<32>(type, a, sms, stream);
+    case 256: return tiles<256>(type, a, device, stream);
+    case 128: return tiles<128>(type, a, device, stream);
+    case 64: return tiles<64>(type, a, device, stream);
+    default: return tiles<32>(type, a, device, stream);
   }
 }
 
 // z: quantize on the way; nullptr: a.q and a.scale are given.
 template <int RT>
-void rows_at_once(int type, const Product& a, const Quantize* z, cudaStream_t stream) {
+void rows_at_once(int type, const Product& a, const Quantize* z, int device, cudaStream_t stream) {
   const unsigned channel_blocks = (unsigned)ceil_div(a.channels, kRowsThreads / 32);
   const uint64_t most = tile_bound(a, RT) * channel_blocks;
   need(most < (1ull << 31), "too many rows");
   by_type(type, [&](auto t) {
     if (z) {
-      auto* kernel = product_rows<decltype(t), RT, true>;
+      constexpr auto kernel = product_rows<decltype(t), RT, true>;
       const unsigned shared = RT * a.padded;
-      check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)shared), "cudaFuncSetAttribute");
+      room<kernel>(device, shared);
       kernel<<<(unsigned)most, kRowsThreads, shared, stream>>>(a, *z, channel_blocks);
     } else {
       product_rows<decltype(t), RT, false><<<(unsigned)most, kRowsThreads, 0, stream>>>(a, Quantize{}, channel_blocks);
@@ -708,12 +709,12 @@ void rows_at_once(int type, const Product& a, const Quantize* z, cudaStream_t st
   check(cudaGetLastError(), "int8_product");
 }
 
-void product_by_rows(int type, const Product& a, const Quantize* z, cudaStream_t stream) {
+void product_by_rows(int type, const Product& a, const Quantize* z, int device, cudaStream_t stream) {
   const uint64_t each = ceil_div(a.rows, a.experts);
-  if (a.rows == 1) rows_at_once<1>(type, a, z, stream);
-  else if (a.rows == 2 || each <= 2) rows_at_once<2>(type, a, z, stream);
-  else if (a.rows <= 4) rows_at_once<4>(type, a, z, stream);
-  else rows_at_once<8>(type, a, z, stream);
+  if (a.rows == 1) rows_at_once<1>(type, a, z, device, stream);
+  else if (a.rows == 2 || each <= 2) rows_at_once<2>(type, a, z, device, stream);
+  else if (a.rows <= 4) rows_at_once<4>(type, a, z, device, stream);
+  else rows_at_once<8>(type, a, z, device, stream);
 }
 
 Quantize quantize_args(int type, const void* x, int64_t x_stride, uint64_t x_rows, unsigned inner, const int32_t* rows,
@@ -798,7 +799,7 @@ int eps_b200_int8_product(const EpsB200Int8Product* a, const int8_t* q, const fl
     const unsigned tile_rows = tile_rows_of(p.rows, p.experts);
     if (!tile_rows) {
       OnDevice on(a->device);
-      return product_by_rows(a->type, p, nullptr, st);
+      return product_by_rows(a->type, p, nullptr, a->device, st);
     }
     OnDevice on(a->device);
     if (shares(p, tile_rows)) {
@@ -807,7 +808,7 @@ int eps_b200_int8_product(const EpsB200Int8Product* a, const int8_t* q, const fl
       p.sums = static_cast<int*>(a->workspace);
       check(cudaMemsetAsync(p.sums, 0, bytes, st), "cudaMemsetAsync");
     }
-    product_by_tiles(a->type, p, sm_count(a->device), st);
+    product_by_tiles(a->type, p, a->device, st);
   });
 }
 
@@ -826,14 +827,14 @@ int eps_b200_int8_linear(const EpsB200Int8Product* a, const void* x, int64_t x_s
     const auto st = static_cast<cudaStream_t>(stream);
     const unsigned tile_rows = tile_rows_of(p.rows, p.experts);
     OnDevice on(a->device);
-    if (!tile_rows && p.padded <= 24 * 1024) return product_by_rows(a->type, p, &z, st);       // eight rows fit shared memory
+    if (!tile_rows && p.padded <= 24 * 1024) return product_by_rows(a->type, p, &z, a->device, st);       // eight rows fit shared memory
     if (shares(p, tile_rows)) {
       p.sums = z.clear = reinterpret_cast<int*>(reinterpret_cast<char*>(scale) + round_up(p.rows * 4ull, 16));
       z.clear_words = p.channels;
     }
     quantize(a->type, z, st);
-    if (tile_rows) product_by_tiles(a->type, p, sm_count(a->device), st);
-    else product_by_rows(a->type, p, nullptr, st);
+    if (tile_rows) product_by_tiles(a->type, p, a->device, st);
+    else product_by_rows(a->type, p, nullptr, a->device, st);
   });
 }
 

@@ -587,12 +587,6 @@ bool lanes_wide(const void* p, int64_t stride, unsigned experts, int type) {
   return aligned(p, bytes) && stride * (int64_t)size_of(type) % (int64_t)bytes == 0;
 }
 
-template <class K>
-void room(K kernel, size_t bytes) {
-  check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes), "cudaFuncSetAttribute");
-  check(cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, 100), "cudaFuncSetAttribute");
-}
-
 }  // namespace
 }  // namespace dense
 }  // namespace eps_b200
@@ -636,8 +630,8 @@ int eps_b200_route_experts(const EpsB200RouteExperts* a, const float* bias, int3
       by_experts(r.experts, [&](auto epl) {
         const bool spread = r.groups > 1 && r.top_groups < r.groups && !lanes_divide(r.per_group, decltype(epl)::value);
         const size_t shared = kWarps * scratch_bytes(r.experts, decltype(epl)::value, r.groups, spread) + r.experts * 4;
-        auto* kernel = route_tokens<decltype(t), decltype(epl)::value>;
-        room(kernel, shared);
+        constexpr auto kernel = route_tokens<decltype(t), decltype(epl)::value>;
+        room<kernel>(a->device, shared);
         kernel<<<r.tiles, kWarps * 32, shared, st>>>(r);
       });
     });
@@ -668,9 +662,9 @@ int eps_b200_route_experts_backward(const EpsB200RouteExperts* a, const int32_t*
     const uint64_t most = (uint64_t)sm_count(a->device) * 8, all = ceil_div(r.tokens, kWarps);
     by_type(a->type, [&](auto t) {
       by_experts(r.experts, [&](auto epl) {
-        auto* kernel = route_gradient<decltype(t), decltype(epl)::value>;
+        constexpr auto kernel = route_gradient<decltype(t), decltype(epl)::value>;
         const size_t shared = kWarps * 32 * decltype(epl)::value * 4;
-        room(kernel, shared);
+        room<kernel>(a->device, shared);
         kernel<<<(unsigned)(all < most ? all : most), kWarps * 32, shared, static_cast<cudaStream_t>(stream)>>>(r);
       });
     });

@@ -18,6 +18,7 @@ have any stride.  Element types are float32, bfloat16 and float16.
 from __future__ import annotations
 
 import ctypes as C
+import struct
 import threading
 from typing import NamedTuple, Sequence
 
@@ -95,20 +96,21 @@ class AdamWArgs(C.Structure):
 
 
 def _bind():
+    # the structs that are packed for each call go in as bytes of the same layout
     lib, P, vp, i64, u64, u32, i32 = (load_library(), C.POINTER, C.c_void_p, C.c_int64, C.c_uint64,
                                       C.c_uint32, C.c_int32)
     st = P(Status)
-    lib.eps_b200_block_norm.argtypes = [P(BlockNorm), vp, i64, vp, i64, vp, i64, vp, st]
+    lib.eps_b200_block_norm.argtypes = [C.c_char_p, vp, i64, vp, i64, vp, i64, vp, st]
     lib.eps_b200_block_norm_workspace.argtypes = [u64, u32]
-    lib.eps_b200_block_norm_backward.argtypes = [P(BlockNorm), P(BlockNormGradientArgs), vp, st]
+    lib.eps_b200_block_norm_backward.argtypes = [C.c_char_p, C.c_char_p, vp, st]
     lib.eps_b200_route_experts_workspace.argtypes = [u64, u32, u32]
-    lib.eps_b200_route_experts.argtypes = [P(RouteExperts), vp, vp, vp, vp, vp, vp, vp, u64, vp, st]
-    lib.eps_b200_route_experts_backward.argtypes = [P(RouteExperts), vp, vp, vp, i64, vp, st]
+    lib.eps_b200_route_experts.argtypes = [C.c_char_p, vp, vp, vp, vp, vp, vp, vp, u64, vp, st]
+    lib.eps_b200_route_experts_backward.argtypes = [C.c_char_p, vp, vp, vp, i64, vp, st]
     lib.eps_b200_int8_stride.argtypes = [u32]
     lib.eps_b200_int8_quantize.argtypes = [i32, i32, vp, i64, u64, u32, vp, u32, u64, vp, vp, vp, st]
     lib.eps_b200_int8_product_workspace.argtypes = [u64, u32, u32, u32]
-    lib.eps_b200_int8_product.argtypes = [P(Int8Product), vp, vp, vp, st]
-    lib.eps_b200_int8_linear.argtypes = [P(Int8Product), vp, i64, u64, vp, vp, st]
+    lib.eps_b200_int8_product.argtypes = [C.c_char_p, vp, vp, vp, st]
+    lib.eps_b200_int8_linear.argtypes = [C.c_char_p, vp, i64, u64, vp, vp, st]
     lib.eps_b200_adamw_plan_bytes.argtypes = [P(AdamWTensor), u64]
     lib.eps_b200_adamw_plan.argtypes = [P(AdamWTensor), u64, vp, u64, P(u64), st]
     lib.eps_b200_adamw.argtypes = [P(AdamWArgs), vp, u64, u64, vp, st]
@@ -148,47 +150,64 @@ def _choice(table, value, what):
         _refuse(f"{what} is one of {', '.join(map(str, table))}: got {value!r}")
 
 
-def _stream(device):
-    return torch.cuda.current_stream(device).cuda_stream
+# A call of a small size takes the host longer than the GPU, so what follows is written
+# for few and cheap steps: device indices instead of device objects, the stream's raw
+# handle, and argument structs packed in one go.
+_stream = torch._C._cuda_getCurrentRawStream      # of a device index
 
 
-def _tensor(t, what, like=None):
-    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+def _tensor(t, what, device=None):
+    """t's device index; refuses what is no CUDA tensor, or on another device."""
+    index = t.get_device() if isinstance(t, torch.Tensor) else -1
+    if index < 0:
         _refuse(f"{what} must be a CUDA tensor")
-    if like is not None and t.device != like.device:
-        _refuse(f"{what} is on {t.device}, not on {like.device}")
-    return t
+    if device is not None and index != device:
+        _refuse(f"{what} is on cuda:{index}, not on cuda:{device}")
+    return index
 
 
-def _matrix(t, what, like=None, columns=None, rows=None):
-    """(t as rows by columns, its row stride); its last axis contiguous."""
-    _tensor(t, what, like)
+def _matrix(t, what, device=None, columns=None, rows=None):
+    """(t as rows by columns, its row stride, rows, columns); its last axis contiguous."""
+    _tensor(t, what, device)
     if t.dtype not in _TYPES:
         _refuse(f"{what} must be float32, bfloat16 or float16")
-    if t.dim() < 1:
-        _refuse(f"{what} must have a last axis")
     if t.dim() != 2:
+        if t.dim() < 1:
+            _refuse(f"{what} must have a last axis")
         try:
             t = t.view(-1, t.shape[-1]) if t.numel() else t.reshape(0, t.shape[-1])
         except RuntimeError:
             _refuse(f"{what}: its leading axes cannot be seen as one")
-    if columns is not None and t.shape[1] != columns:
-        _refuse(f"{what} has {t.shape[1]} columns, not {columns}")
-    if rows is not None and t.shape[0] != rows:
-        _refuse(f"{what} has {t.shape[0]} rows, not {rows}")
-    if t.shape[1] > 1 and t.stride(1) != 1:
+    n, width = t.shape
+    if columns is not None and width != columns:
+        _refuse(f"{what} has {width} columns, not {columns}")
+    if rows is not None and n != rows:
+        _refuse(f"{what} has {n} rows, not {rows}")
+    stride, inner = t.stride()
+    if inner != 1 and width > 1:
         _refuse(f"the last axis of {what} must be contiguous")
-    return t, t.stride(0)
+    return t, stride, n, width
 
 
-def _vector(t, what, like, n, dtype):
-    """The address of a contiguous vector of n elements, or None."""
+def _vector(t, what, device, n, dtype):
+    """The address of a contiguous vector of n elements; 0 for None."""
     if t is None:
-        return None
-    _tensor(t, what, like)
+        return 0
+    _tensor(t, what, device)
     if t.dtype != dtype or t.numel() != n or not t.is_contiguous():
         _refuse(f"{what} must be a contiguous {dtype} vector of {n}")
     return t.data_ptr()
+
+
+def _ptr(t):
+    return 0 if t is None else t.data_ptr()
+
+
+def _pack(fields, *values):
+    try:
+        return fields.pack(*values)
+    except (struct.error, TypeError, OverflowError) as e:
+        _refuse(f"an argument is out of range: {e}")
 
 
 # ------------------------------------------------------------ norms and gate
@@ -204,40 +223,55 @@ class BlockNormGradients(NamedTuple):
     pre_bias: torch.Tensor | None
 
 
-def _block_norm_args(residual, y, gate, post_weight, post_bias, pre_weight, pre_bias, channel_scale,
-                     scale, kind, activation, epsilon, post_norm, pre_norm, dtype):
-    """(C struct, y, gate) for a residual given as rows by columns."""
-    rows, columns = residual.shape
-    parameters = [p for p in (post_weight, post_bias, channel_scale, pre_weight, pre_bias) if p is not None]
-    ptype = parameters[0].dtype if parameters else torch.float32
+_BLOCK_NORM = struct.Struct("@9iIQ2f2P2q5P")           # BlockNorm
+_BLOCK_NORM_GRADIENTS = struct.Struct("@3P3q3P3q6PQ")    # BlockNormGradientArgs
+
+
+def _block_norm_args(device, rows, columns, rtype, y, gate, post_weight, post_bias, pre_weight, pre_bias,
+                     channel_scale, scale, kind, activation, epsilon, post_norm, pre_norm, dtype):
+    """The packed struct for a residual of rows by columns."""
+    ptype = torch.float32
+    for p in (post_weight, pre_weight, channel_scale, post_bias, pre_bias):
+        if p is not None:
+            ptype = p.dtype if isinstance(p, torch.Tensor) else None
+            break
     if ptype != torch.float32 and ptype != dtype:
         _refuse("weights, biases and channel_scale have the block's type or float32, all the same")
     y_stride = gate_stride = gate_kind = 0
     if y is not None:
-        y, y_stride = _matrix(y, "y", residual, columns, rows)
+        y, y_stride, _, _ = _matrix(y, "y", device, columns, rows)
     if gate is not None:
         if y is None:
             _refuse("a gate needs a block output y")
-        _tensor(gate, "gate", residual)
+        _tensor(gate, "gate", device)
         if gate.dtype != dtype:
             _refuse("the gate has the type of y")
         # one value a row: [rows] or [..., 1]; a matrix of one column is an element gate where D is 1
-        if gate.numel() == rows and columns > 1:
+        if columns > 1 and gate.numel() == rows:
             gate_kind = 1
             if not gate.is_contiguous():
                 _refuse("a gate of one value a row must be contiguous")
         else:
             gate_kind = 2
-            gate, gate_stride = _matrix(gate, "gate", residual, columns, rows)
-    vectors = [_vector(p, what, residual, columns, ptype) for p, what in (
-        (post_weight, "post_weight"), (post_bias, "post_bias"), (channel_scale, "channel_scale"),
-        (pre_weight, "pre_weight"), (pre_bias, "pre_bias"))]
-    args = BlockNorm(residual.device.index, _choice(_KINDS, kind, "kind"), gate_kind,
-                     _choice(_ACTIVATIONS, activation, "activation"), bool(post_norm), bool(pre_norm),
-                     _TYPES[dtype], _TYPES[residual.dtype], _TYPES[ptype], columns, rows, epsilon, scale,
-                     None if y is None else y.data_ptr(), None if gate is None else gate.data_ptr(),
-                     y_stride, gate_stride, *vectors)
-    return args, y, gate
+            gate, gate_stride, _, _ = _matrix(gate, "gate", device, columns, rows)
+    return _pack(_BLOCK_NORM, device, _choice(_KINDS, kind, "kind"), gate_kind,
+                 _choice(_ACTIVATIONS, activation, "activation"), bool(post_norm), bool(pre_norm),
+                 _TYPES[dtype], _TYPES[rtype], _TYPES[ptype], columns, rows, epsilon, scale,
+                 _ptr(y), _ptr(gate), y_stride, gate_stride,
+                 _vector(post_weight, "post_weight", device, columns, ptype),
+                 _vector(post_bias, "post_bias", device, columns, ptype),
+                 _vector(channel_scale, "channel_scale", device, columns, ptype),
+                 _vector(pre_weight, "pre_weight", device, columns, ptype),
+                 _vector(pre_bias, "pre_bias", device, columns, ptype))
+
+
+def _block_type(residual, y, device):
+    if y is None:
+        return residual.dtype
+    _tensor(y, "y", device)
+    if y.dtype not in _TYPES:
+        _refuse("y must be float32, bfloat16 or float16")
+    return y.dtype
 
 
 def block_norm(x, y=None, gate=None, *, post_weight=None, post_bias=None, pre_weight=None,
@@ -255,17 +289,18 @@ def block_norm(x, y=None, gate=None, *, post_weight=None, post_bias=None, pre_we
     "layer"; activation "none", "sigmoid", "silu" or "tanh".  Weights, biases and
     channel_scale are vectors of D, all float32 or all of y's type.  D is at most
     8192.  Returns (h, z), z None without pre_norm."""
-    residual, x_stride = _matrix(x, "x")
-    dtype = residual.dtype if y is None else _tensor(y, "y", residual).dtype
-    args, y2, g2 = _block_norm_args(residual, y, gate, post_weight, post_bias, pre_weight, pre_bias,
-                                    channel_scale, scale, kind, activation, epsilon, post_norm, pre_norm,
-                                    dtype)
-    columns = residual.shape[1]
-    h = x if y is None else torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    z = torch.empty(x.shape, dtype=dtype, device=x.device) if pre_norm else None
-    _call(_lib.eps_b200_block_norm, C.byref(args), residual.data_ptr(), x_stride,
-          None if y is None else h.data_ptr(), columns, None if z is None else z.data_ptr(), columns,
-          _stream(residual.device))
+    residual, x_stride, rows, columns = _matrix(x, "x")
+    device = residual.get_device()
+    dtype = _block_type(residual, y, device)
+    args = _block_norm_args(device, rows, columns, residual.dtype, y, gate, post_weight, post_bias, pre_weight,
+                            pre_bias, channel_scale, scale, kind, activation, epsilon, post_norm, pre_norm, dtype)
+    dense = torch.contiguous_format
+    h = x if y is None else torch.empty_like(x, memory_format=dense)
+    z = None
+    if pre_norm:
+        z = torch.empty_like(x, memory_format=dense) if dtype == x.dtype else torch.empty_like(x, dtype=dtype, memory_format=dense)
+    _call(_lib.eps_b200_block_norm, args, residual.data_ptr(), x_stride, 0 if y is None else h.data_ptr(), columns,
+          _ptr(z), columns, _stream(device))
     return h, z
 
 
@@ -279,38 +314,39 @@ def block_norm_backward(dh, dz, h, y=None, gate=None, *, post_weight=None, post_
     computed again from h and y.  Gradients of x, y and gate have their types,
     gradients of weights, biases and channel_scale are float32.  Sums over rows are
     taken in a fixed order."""
-    residual, h_stride = _matrix(h, "h")
-    rows, columns = residual.shape
-    dtype = residual.dtype if y is None else _tensor(y, "y", residual).dtype
-    args, y2, g2 = _block_norm_args(residual, y, gate, post_weight, post_bias, pre_weight, pre_bias,
-                                    channel_scale, scale, kind, activation, epsilon, post_norm, pre_norm,
-                                    dtype)
+    residual, h_stride, rows, columns = _matrix(h, "h")
+    device = residual.get_device()
+    dtype = _block_type(residual, y, device)
+    args = _block_norm_args(device, rows, columns, residual.dtype, y, gate, post_weight, post_bias, pre_weight,
+                            pre_bias, channel_scale, scale, kind, activation, epsilon, post_norm, pre_norm, dtype)
     if dz is not None and not pre_norm:
         _refuse("dz needs pre_norm")
-    dh2, dh_stride = (None, 0) if dh is None else _matrix(dh, "dh", residual, columns, rows)
-    dz2, dz_stride = (None, 0) if dz is None else _matrix(dz, "dz", residual, columns, rows)
-    if dh2 is not None and dh2.dtype != residual.dtype:
-        _refuse("dh has the type of h")
-    if dz2 is not None and dz2.dtype != dtype:
-        _refuse("dz has the type of y")
-    device = residual.device
-    dx = torch.empty(h.shape, dtype=h.dtype, device=device)
-    dy = None if y is None else torch.empty(y.shape, dtype=dtype, device=device)
-    dgate = None if gate is None else torch.empty(gate.shape, dtype=dtype, device=device)
+    dh_stride = dz_stride = 0
+    if dh is not None:
+        dh, dh_stride, _, _ = _matrix(dh, "dh", device, columns, rows)
+        if dh.dtype != residual.dtype:
+            _refuse("dh has the type of h")
+    if dz is not None:
+        dz, dz_stride, _, _ = _matrix(dz, "dz", device, columns, rows)
+        if dz.dtype != dtype:
+            _refuse("dz has the type of y")
+    dense = torch.contiguous_format
+    dx = torch.empty_like(h, memory_format=dense)
+    dy = None if y is None else torch.empty_like(y, memory_format=dense)
+    dgate = None if gate is None else torch.empty_like(gate, memory_format=dense)
     post, pre = y is not None and post_norm, pre_norm
-    wanted = [post_weight is not None and post, post_bias is not None and post,
-              channel_scale is not None and y is not None, pre_weight is not None and pre,
-              pre_bias is not None and pre]
-    sums = torch.empty((sum(wanted), columns), dtype=torch.float32, device=device)
-    rest = iter(sums)
-    vectors = [next(rest) if w else None for w in wanted]
-    space = _lib.eps_b200_block_norm_workspace(rows, columns) if any(wanted) else 0
-    workspace = torch.empty(space, dtype=torch.uint8, device=device)
-    ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
-    grads = BlockNormGradientArgs(ptr(dh2), ptr(dz2), residual.data_ptr(), dh_stride, dz_stride, h_stride,
-                                  dx.data_ptr(), ptr(dy), ptr(dgate), columns, columns, columns,
-                                  *[ptr(v) for v in vectors], workspace.data_ptr(), space)
-    _call(_lib.eps_b200_block_norm_backward, C.byref(args), C.byref(grads), _stream(device))
+    wanted = (post and post_weight is not None, post and post_bias is not None,
+              y is not None and channel_scale is not None, pre and pre_weight is not None,
+              pre and pre_bias is not None)
+    vectors, space, workspace = [None] * 5, 0, None
+    if any(wanted):
+        rest = iter(torch.empty((sum(wanted), columns), dtype=torch.float32, device=h.device).unbind())
+        vectors = [next(rest) if w else None for w in wanted]
+        space = _lib.eps_b200_block_norm_workspace(rows, columns)
+        workspace = torch.empty(space, dtype=torch.uint8, device=h.device)
+    grads = _pack(_BLOCK_NORM_GRADIENTS, _ptr(dh), _ptr(dz), residual.data_ptr(), dh_stride, dz_stride, h_stride,
+                  dx.data_ptr(), _ptr(dy), _ptr(dgate), columns, columns, columns, *map(_ptr, vectors), _ptr(workspace), space)
+    _call(_lib.eps_b200_block_norm_backward, args, grads, _stream(device))
     return BlockNormGradients(dx, dy, dgate, *vectors)
 
 
@@ -327,10 +363,12 @@ class Routing(NamedTuple):
     offsets: torch.Tensor | None
 
 
-def _route_args(logits, stride, top_k, score, renormalise, scale, groups, top_groups):
-    return RouteExperts(logits.device.index, _TYPES[logits.dtype], _choice(_SCORES, score, "score"),
-                        bool(renormalise), logits.shape[1], top_k, groups, top_groups, logits.shape[0],
-                        scale, 0, logits.data_ptr(), stride)
+_ROUTE = struct.Struct("@4i4IQfiPq")          # RouteExperts
+
+
+def _route_args(logits, stride, tokens, experts, top_k, score, renormalise, scale, groups, top_groups):
+    return _pack(_ROUTE, logits.get_device(), _TYPES[logits.dtype], _choice(_SCORES, score, "score"),
+                 bool(renormalise), experts, top_k, groups, top_groups, tokens, scale, 0, logits.data_ptr(), stride)
 
 
 def route(logits, top_k: int, *, score: str = "softmax", bias=None, groups: int = 1,
@@ -345,29 +383,27 @@ def route(logits, top_k: int, *, score: str = "softmax", bias=None, groups: int 
     `renormalise`, times `scale`.  Equal keys go to the lower index; a masked logit
     is -inf.  At most 1024 experts and top_k 32.  With `sort`, the entries sorted
     by expert come too."""
-    logits, stride = _matrix(logits, "logits")
-    if min(top_k, groups, groups if top_groups is None else top_groups) <= 0:
+    logits, stride, tokens, experts = _matrix(logits, "logits")
+    top_groups = groups if top_groups is None else top_groups
+    if top_k <= 0 or groups <= 0 or top_groups <= 0:
         _refuse("top_k, groups and top_groups are positive")
-    tokens, experts = logits.shape
-    args = _route_args(logits, stride, top_k, score, renormalise, scale, groups,
-                       groups if top_groups is None else top_groups)
-    device = logits.device
-    b = _vector(bias, "bias", logits, experts, torch.float32)
+    args = _route_args(logits, stride, tokens, experts, top_k, score, renormalise, scale, groups, top_groups)
+    index, device = logits.get_device(), logits.device
+    b = _vector(bias, "bias", index, experts, torch.float32)
     chosen = torch.empty((tokens, top_k), dtype=torch.int32, device=device)
-    weights = torch.empty((tokens, top_k), dtype=torch.float32, device=device)
+    weights = torch.empty_like(chosen, dtype=torch.float32)
     if not sort:
-        _call(_lib.eps_b200_route_experts, C.byref(args), b, chosen.data_ptr(), weights.data_ptr(), None, None, None,
-              None, 0, _stream(device))
+        _call(_lib.eps_b200_route_experts, args, b, chosen.data_ptr(), weights.data_ptr(), 0, 0, 0, 0, 0, _stream(index))
         return Routing(chosen, weights, None, None, None)
-    order = torch.empty(tokens * top_k, dtype=torch.int32, device=device)
-    position = torch.empty((tokens, top_k), dtype=torch.int32, device=device)
+    position = torch.empty_like(chosen)
+    order = torch.empty_like(chosen).view(-1)
     offsets = torch.empty(experts + 1, dtype=torch.int32, device=device)
     space = _lib.eps_b200_route_experts_workspace(tokens, experts, top_k)
     workspace = torch.empty(space, dtype=torch.uint8, device=device)
     # an empty tensor has no address, yet it is asked for
-    _call(_lib.eps_b200_route_experts, C.byref(args), b, chosen.data_ptr(), weights.data_ptr(),
+    _call(_lib.eps_b200_route_experts, args, b, chosen.data_ptr(), weights.data_ptr(),
           order.data_ptr() or offsets.data_ptr(), position.data_ptr() or offsets.data_ptr(), offsets.data_ptr(),
-          workspace.data_ptr(), space, _stream(device))
+          workspace.data_ptr(), space, _stream(index))
     return Routing(chosen, weights, order, position, offsets)
 
 
@@ -375,28 +411,28 @@ def route_backward(logits, experts, dweights, *, score: str = "softmax", renorma
                    scale: float = 1.0):
     """The logits' gradient from that of route's weights, for the experts it chose;
     the choice itself, the bias and the groups take none."""
-    flat, stride = _matrix(logits, "logits")
-    _tensor(experts, "experts", flat)
-    _tensor(dweights, "dweights", flat)
+    flat, stride, tokens, count = _matrix(logits, "logits")
+    index = flat.get_device()
+    _tensor(experts, "experts", index)
+    _tensor(dweights, "dweights", index)
     if experts.dim() < 1 or experts.shape[-1] == 0 or experts.dtype != torch.int32 or not experts.is_contiguous():
         _refuse("experts must be a contiguous int32 tensor, as route gives it")
     top_k = experts.shape[-1]
-    if experts.numel() != flat.shape[0] * top_k:
+    if experts.numel() != tokens * top_k:
         _refuse("experts and logits have different numbers of tokens")
     if dweights.dtype != torch.float32 or dweights.numel() != experts.numel() or not dweights.is_contiguous():
         _refuse("dweights must be contiguous float32, in the shape of experts")
-    args = _route_args(flat, stride, top_k, score, renormalise, scale, 1, 1)
-    out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-    _call(_lib.eps_b200_route_experts_backward, C.byref(args), experts.data_ptr(), dweights.data_ptr(), out.data_ptr(),
-          flat.shape[1], _stream(flat.device))
+    args = _route_args(flat, stride, tokens, count, top_k, score, renormalise, scale, 1, 1)
+    out = torch.empty_like(logits, memory_format=torch.contiguous_format)
+    _call(_lib.eps_b200_route_experts_backward, args, experts.data_ptr(), dweights.data_ptr(), out.data_ptr(), count, _stream(index))
     return out
 
 
 # ------------------------------------------------------------- 8-bit products
-def _row_index(rows, rows_divisor, like):
+def _row_index(rows, rows_divisor, device):
     if rows is None:
-        return None
-    _tensor(rows, "rows", like)
+        return 0
+    _tensor(rows, "rows", device)
     if rows.dtype != torch.int32 or rows.dim() != 1 or not rows.is_contiguous():
         _refuse("rows must be a contiguous int32 vector")
     if rows_divisor <= 0:
@@ -408,15 +444,19 @@ def quantize_rows(x, rows=None, rows_divisor: int = 1):
     """x [..., inner] in 8-bit integers with one scale a row: (q, scale) with q
     [n, stride] int8, zeros behind `inner`, and scale [n] float32.  Row r is
     x[rows[r] // rows_divisor], or x[r] without `rows`."""
-    x, stride = _matrix(x, "x")
-    index = _row_index(rows, rows_divisor, x)
-    n, inner = x.shape[0] if rows is None else rows.shape[0], x.shape[1]
+    x, stride, x_rows, inner = _matrix(x, "x")
+    device = x.get_device()
+    index = _row_index(rows, rows_divisor, device)
+    n = x_rows if rows is None else rows.shape[0]
     padded = _lib.eps_b200_int8_stride(inner)
     q = torch.empty((n, padded), dtype=torch.int8, device=x.device)
     scale = torch.empty(n, dtype=torch.float32, device=x.device)
-    _call(_lib.eps_b200_int8_quantize, x.device.index, _TYPES[x.dtype], x.data_ptr(), stride, x.shape[0], inner,
-          index, rows_divisor, n, q.data_ptr(), scale.data_ptr(), _stream(x.device))
+    _call(_lib.eps_b200_int8_quantize, device, _TYPES[x.dtype], x.data_ptr(), stride, x_rows, inner,
+          index, rows_divisor, n, q.data_ptr(), scale.data_ptr(), _stream(device))
     return q, scale
+
+
+_INT8_PRODUCT = struct.Struct("@2i4IQ6PQ")          # Int8Product
 
 
 class QuantizedExperts:
@@ -434,7 +474,7 @@ class QuantizedExperts:
         self.device = weight.device
         n = self.experts * self.channels
         for t, what in ((scale, "scale"), (bias, "bias")):
-            _vector(t, what, weight, n, torch.float32)
+            _vector(t, what, weight.get_device(), n, torch.float32)
         if scale is None:
             _refuse("the weights need their scales")
         self.stride = _lib.eps_b200_int8_stride(self.inner)
@@ -461,13 +501,12 @@ class QuantizedExperts:
         (may be left out with one expert).  rows int32 [n]: row r of the product is
         made from x[rows[r] // rows_divisor] -- a Routing's `order` with rows_divisor
         = top_k; without it from x[r].  Rows in no expert's run are left unwritten."""
-        flat, stride = _matrix(x, "x", columns=self.inner)
-        if flat.device != self.device:
-            _refuse(f"x is on {flat.device}, not on {self.device}")
-        index = _row_index(rows, rows_divisor, flat)
-        n = flat.shape[0] if rows is None else rows.shape[0]
+        device = self.device.index
+        flat, stride, x_rows, _ = _matrix(x, "x", device, self.inner)
+        index = _row_index(rows, rows_divisor, device)
+        n = x_rows if rows is None else rows.shape[0]
         if offsets is not None:
-            _tensor(offsets, "offsets", flat)
+            _tensor(offsets, "offsets", device)
             if offsets.dtype != torch.int32 or offsets.numel() != self.experts + 1 or not offsets.is_contiguous():
                 _refuse("offsets must be a contiguous int32 vector of experts + 1")
         elif self.experts != 1:
@@ -476,12 +515,10 @@ class QuantizedExperts:
         out = torch.empty(shape, dtype=flat.dtype, device=self.device)
         space = _lib.eps_b200_int8_product_workspace(n, self.experts, self.channels, self.inner)
         workspace = torch.empty(space, dtype=torch.uint8, device=self.device)
-        args = Int8Product(self.device.index, _TYPES[flat.dtype], self.experts, self.channels, self.inner,
-                           rows_divisor, n, self.weight.data_ptr(), self.scale.data_ptr(),
-                           None if self.bias is None else self.bias.data_ptr(),
-                           None if offsets is None else offsets.data_ptr(), out.data_ptr(), workspace.data_ptr(), space)
-        _call(_lib.eps_b200_int8_linear, C.byref(args), flat.data_ptr(), stride, flat.shape[0], index,
-              _stream(self.device))
+        args = _pack(_INT8_PRODUCT, device, _TYPES[flat.dtype], self.experts, self.channels, self.inner, rows_divisor, n,
+                     self.weight.data_ptr(), self.scale.data_ptr(), _ptr(self.bias), _ptr(offsets), out.data_ptr(),
+                     workspace.data_ptr(), space)
+        _call(_lib.eps_b200_int8_linear, args, flat.data_ptr(), stride, x_rows, index, _stream(device))
         return out
 
 
@@ -511,11 +548,12 @@ class AdamW:
         self.parameters = list(parameters)
         if not self.parameters:
             _refuse("no parameters")
-        head = _tensor(self.parameters[0], "a parameter")
+        head = self.parameters[0]
+        index = _tensor(head, "a parameter")
         if head.dtype not in _TYPES:
             _refuse("parameters are float32, bfloat16 or float16")
         for p in self.parameters:
-            _tensor(p, "a parameter", head)
+            _tensor(p, "a parameter", index)
             if p.dtype != head.dtype or not p.is_contiguous():
                 _refuse("parameters are contiguous and of one type")
         if state_bits not in (8, 32):
@@ -564,7 +602,7 @@ class AdamW:
             _refuse("gradients have the parameters' type or float32")
         tensors = (AdamWTensor * len(gradients))()
         for i, (p, g, a) in enumerate(zip(self.parameters, gradients, self.starts)):
-            _tensor(g, "a gradient", p)
+            _tensor(g, "a gradient", self.device.index)
             if g.dtype != dtype or g.shape != p.shape or not g.is_contiguous():
                 _refuse("gradients are contiguous, of one type and of the parameters' shapes")
             tensors[i] = AdamWTensor(p.data_ptr(), g.data_ptr(), p.numel(), a)
@@ -587,10 +625,11 @@ class AdamW:
         _, plan, blocks, gtype = self._bound
         a = self._args
         a.gradient_type = gtype
-        a.gradient_scale = _vector(gradient_scale, "gradient_scale", self.first, 1, torch.float32)
-        a.skip = _vector(skip, "skip", self.first, 1, torch.int32)
+        device = self.device.index
+        a.gradient_scale = _vector(gradient_scale, "gradient_scale", device, 1, torch.float32)
+        a.skip = _vector(skip, "skip", device, 1, torch.int32)
         a.step = self.steps + 1
-        _call(_lib.eps_b200_adamw, C.byref(a), plan.data_ptr(), len(self.parameters), blocks, _stream(self.device))
+        _call(_lib.eps_b200_adamw, C.byref(a), plan.data_ptr(), len(self.parameters), blocks, _stream(device))
         self.steps += 1
 
     def state(self) -> dict:

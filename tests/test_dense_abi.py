@@ -3,6 +3,7 @@ arguments before they look for a GPU."""
 import ctypes as C
 import os
 import re
+import struct
 import subprocess
 
 import pytest
@@ -39,6 +40,12 @@ def test_struct_layouts_match_the_header(tmp_path):
     for _, py in pairs:
         want += [C.sizeof(py)] + [getattr(py, f[0]).offset for f in py._fields_]
     assert got == want
+    for packed, py in ((dense._BLOCK_NORM, dense.BlockNorm), (dense._BLOCK_NORM_GRADIENTS, dense.BlockNormGradientArgs),
+                       (dense._ROUTE, dense.RouteExperts), (dense._INT8_PRODUCT, dense.Int8Product)):
+        assert packed.size == C.sizeof(py)
+        codes = {C.c_int32: "i", C.c_uint32: "I", C.c_uint64: "L", C.c_int64: "l", C.c_float: "f", C.c_void_p: "P"}
+        plain = "".join(codes[f[1]] for f in py._fields_)
+        assert struct.calcsize("@" + plain) == packed.size and len(packed.unpack(bytes(packed.size))) == len(py._fields_)
 
 
 def refused(fn, *args):
@@ -54,7 +61,7 @@ A = 1 << 20      # an address that is only looked at, never read, by a call that
 def norm(**change):
     fields = dict(device=0, kind=0, gate_kind=2, activation=1, post_norm=1, pre_norm=1, type=1, residual_type=1, parameter_type=0,
                   columns=64, rows=4, epsilon=1e-6, scale=1.0, y=A, gate=A, y_stride=64, gate_stride=64)
-    return C.byref(dense.BlockNorm(**{**fields, **change}))
+    return bytes(dense.BlockNorm(**{**fields, **change}))
 
 
 @pytest.mark.parametrize("change", [dict(kind=2), dict(gate_kind=3), dict(gate_kind=0), dict(activation=4), dict(type=3), dict(residual_type=2),
@@ -63,13 +70,13 @@ def norm(**change):
 def test_block_norm_refuses(change):
     assert refused(LIB.eps_b200_block_norm, norm(**change), A, 64, A, 64, A, 64, None) == eps.INVALID_ARGUMENT
     g = dense.BlockNormGradientArgs(dz=A, h=A, dx=A)
-    assert refused(LIB.eps_b200_block_norm_backward, norm(**change), C.byref(g), None) == eps.INVALID_ARGUMENT
+    assert refused(LIB.eps_b200_block_norm_backward, norm(**change), bytes(g), None) == eps.INVALID_ARGUMENT
 
 
 def test_block_norm_refuses_missing_tensors():
     call = lambda x, h, z: refused(LIB.eps_b200_block_norm, norm(), x, 64, h, 64, z, 64, None)  # noqa: E731
     assert call(None, A, A) == call(A, None, A) == call(A, A, None) == eps.INVALID_ARGUMENT
-    back = lambda args, **g: refused(LIB.eps_b200_block_norm_backward, args, C.byref(dense.BlockNormGradientArgs(**g)), None)  # noqa: E731
+    back = lambda args, **g: refused(LIB.eps_b200_block_norm_backward, args, bytes(dense.BlockNormGradientArgs(**g)), None)  # noqa: E731
     assert back(norm(), dz=A) == eps.INVALID_ARGUMENT
     assert back(norm(pre_norm=0), dz=A, h=A) == eps.INVALID_ARGUMENT
     assert back(norm(y=None, gate=None, gate_kind=0), dh=A, dy=A) == eps.INVALID_ARGUMENT
@@ -81,7 +88,7 @@ def test_block_norm_refuses_missing_tensors():
 def routing(**change):
     fields = dict(device=0, type=0, score=0, renormalise=1, experts=16, top_k=2, groups=4, top_groups=2, tokens=8, scale=1.0,
                   logits=A, logits_stride=16)
-    return C.byref(dense.RouteExperts(**{**fields, **change}))
+    return bytes(dense.RouteExperts(**{**fields, **change}))
 
 
 @pytest.mark.parametrize("change", [dict(type=5), dict(score=2), dict(experts=0), dict(experts=1025), dict(groups=0), dict(groups=3),
@@ -101,7 +108,7 @@ def test_routing_refuses_missing_tensors():
 def linear(**change):
     fields = dict(device=0, type=1, experts=2, channels=32, inner=64, rows_divisor=1, rows=4, weight=A, weight_scale=A, offsets=A, out=A,
                   workspace=A, workspace_bytes=1 << 20)
-    return C.byref(dense.Int8Product(**{**fields, **change}))
+    return bytes(dense.Int8Product(**{**fields, **change}))
 
 
 @pytest.mark.parametrize("change", [dict(type=7), dict(experts=0), dict(channels=0), dict(inner=0), dict(inner=131073), dict(rows=1 << 31),
