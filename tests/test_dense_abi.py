@@ -147,12 +147,12 @@ def test_adamw_plan():
     plan, blocks = (C.c_uint8 * size)(), C.c_uint64()
     assert refused(LIB.eps_b200_adamw_plan, t, 3, plan, size, C.byref(blocks)) == 0
     chunks = (C.c_uint32 * (2 * blocks.value)).from_buffer(plan, 3 * C.sizeof(dense.AdamWTensor))
-    elements = lambda c: 4096 * c[1]  # noqa: E731
+    elements = lambda c: 2048 * c[1]  # noqa: E731
     seen = [(chunks[2 * i], chunks[2 * i + 1]) for i in range(blocks.value)]
     assert size == 3 * C.sizeof(dense.AdamWTensor) + 8 * blocks.value
     for tensor, n in ((0, 10000), (1, 0), (2, 4096)):
         mine = [elements(c) for c in seen if c[0] == tensor]
-        assert mine == list(range(0, n, 4096))
+        assert mine == list(range(0, n, 2048))
     assert refused(LIB.eps_b200_adamw_plan, t, 3, plan, size - 1, C.byref(blocks)) == eps.INVALID_ARGUMENT
     t[2].state_begin = 10241
     assert refused(LIB.eps_b200_adamw_plan, t, 3, plan, size, C.byref(blocks)) == eps.INVALID_ARGUMENT
