@@ -175,6 +175,48 @@ def test_8bit_step(dtype, master):
         assert bool((decoded(opt.second, opt.second_scale)[torch.cat([torch.nn.functional.pad(v, (0, -v.numel() % 256)) for v in plain.v]) > 0] > 0).all())
 
 
+def mixed(h):
+    h = ((h ^ (h >> 16)) * 0x85EBCA6B) & 0xFFFFFFFF
+    h = ((h ^ (h >> 13)) * 0xC2B2AE35) & 0xFFFFFFFF
+    return h ^ (h >> 16)
+
+
+@gpu
+def test_8bit_codes_are_those_of_the_formula():
+    """The codes and scales of several steps bit for bit, from a float32 restatement whose every operation
+    is rounded by itself."""
+    params = tensors(1, SIZES, 0.1)
+    opt = dense.AdamW(params, state_bits=8, seed=77, **HYPER)
+    n = opt.first.numel()
+    m, r = torch.zeros(n, device="cuda"), torch.zeros(n, device="cuda")
+    for k in range(5):
+        grads = tensors(40 + k, SIZES, 1e-2)
+        opt.step(grads)
+        g = torch.zeros(n, device="cuda")
+        for x, a in zip(grads, opt.starts):
+            g[a:a + x.numel()] = x
+        m = 0.9 * m + (1 - 0.9) * g
+        root = torch.sqrt(0.98 * (r * r) + (1 - 0.98) * g * g)
+        key = mixed(torch.tensor(77, device="cuda") ^ mixed(torch.tensor(k + 1, device="cuda")))
+        h = mixed((torch.arange(n // 2, device="cuda") * 0x9E3779B1 + key) & 0xFFFFFFFF)
+        u = torch.stack([h & 0xFFFF, h >> 16], -1).view(-1)
+        out = []
+        for v in (m, root):
+            scale = v.view(-1, 256).abs().amax(-1) * torch.tensor(1 / 448, device="cuda")
+            x = (v.view(-1, 256) * torch.where(scale == 0, 0.0, 1 / scale)[:, None]).view(-1)
+            out.append((x, scale))
+        (xm, sm), (xr, sr) = out
+        coarse = ((xr.view(torch.int32) + (u.int() << 4)) & -0x100000).view(torch.float32)
+        fine = torch.floor(xr * 512 + u.float() / 65536) / 512
+        xr = torch.where(xr > 0, torch.where(xr < 2.0 ** -6, fine, coarse).clamp(2.0 ** -9, 448), xr)
+        cm, cr = xm.clamp(-448, 448).to(torch.float8_e4m3fn), xr.to(torch.float8_e4m3fn)
+        assert torch.equal(opt.first_scale, sm) and torch.equal(opt.second_scale, sr)
+        assert torch.equal(opt.first.view(torch.uint8), cm.view(torch.uint8))
+        assert torch.equal(opt.second.view(torch.uint8), cr.view(torch.uint8))
+        m = (cm.float().view(-1, 256) * sm[:, None]).view(-1)
+        r = (cr.float().view(-1, 256) * sr[:, None]).view(-1)
+
+
 @gpu
 def test_8bit_roots_are_right_on_average():
     """The same moments rounded at many places: their mean is the value, although a step moves it by far
