@@ -253,14 +253,6 @@ __global__ void __launch_bounds__(kRowsThreads) product_rows(const Product a, co
 #pragma unroll
   for (int r = 0; r < RT; ++r) acc[r] = 0;
   for (unsigned k0 = 0; k0 < a.padded; k0 += kRowsAhead * 512) {
-    int4 now[kRowsAhead];
-#pragma unroll
-    for (unsigned i = 0; i < kRowsAhead; ++i) {
-      now[i] = ahead[i];
-      const unsigned k = k0 + kRowsAhead * 512 + (i * 32 + lane) * 16;
-      ahead[i] = make_int4(0, 0, 0, 0);
-      if (k < a.padded) ahead[i] = __ldcs(reinterpret_cast<const int4*>(w + k));
-    }
 #pragma unroll
     for (unsigned i = 0; i < kRowsAhead; ++i) {
       const unsigned k = k0 + (i * 32 + lane) * 16;
@@ -269,8 +261,10 @@ __global__ void __launch_bounds__(kRowsThreads) product_rows(const Product a, co
       for (int r = 0; r < RT; ++r) {
         if (r >= t.rows) continue;
         const int4 y = *reinterpret_cast<const int4*>(q + (uint64_t)r * a.padded + k);
-        acc[r] = __dp4a(now[i].x, y.x, __dp4a(now[i].y, y.y, __dp4a(now[i].z, y.z, __dp4a(now[i].w, y.w, acc[r]))));
+        acc[r] = __dp4a(ahead[i].x, y.x, __dp4a(ahead[i].y, y.y, __dp4a(ahead[i].z, y.z, __dp4a(ahead[i].w, y.w, acc[r]))));
       }
+      const unsigned next = k + kRowsAhead * 512;
+      if (next < a.padded) ahead[i] = __ldcs(reinterpret_cast<const int4*>(w + next));
     }
   }
   const uint64_t c = (uint64_t)t.expert * a.channels + n;
@@ -652,6 +646,9 @@ unsigned tile_rows_of(uint64_t rows, uint64_t experts) {
   return each > 128 ? 256 : each > 64 ? 128 : each > 32 ? 64 : 32;
 }
 
+// Whether rows are quantized where they are used: few of them, eight of which fit shared memory.
+bool on_the_way(unsigned tile_rows, uint64_t padded) { return !tile_rows && padded <= 24 * 1024; }
+
 // Whether the blocks share the tiles' stages: whole tiles would leave most SMs idle,
 // while sums in memory cost four bytes an output twice over L2.  The bound stands for
 // two rounds of a B200's 148 SMs.
@@ -718,11 +715,11 @@ void product_by_rows(int type, const Product& a, const Quantize* z, int device, 
 }
 
 Quantize quantize_args(int type, const void* x, int64_t x_stride, uint64_t x_rows, unsigned inner, const int32_t* rows,
-                       unsigned divisor, uint64_t count, int8_t* q, float* scale) {
+                       unsigned divisor, uint64_t count, int8_t* q, float* scale, bool kept = true) {
   need(known_type(type), "unknown element type");
   need(inner > 0 && inner <= EPS_B200_INT8_INNER, "inner size out of range");
   need(rows ? divisor > 0 : count <= x_rows, "more rows than x has");
-  need(!count || (q && scale && (x || !x_rows)), "null input or output");
+  need(!count || (!kept || (q && scale)) && (x || !x_rows), "null input or output");
   need(aligned(q, 16), "q must be 16-byte aligned");
   return Quantize{x, x_stride, x_rows, count, inner, (unsigned)eps_b200_int8_stride(inner), divisor, rows, q, scale,
                   aligned(x, 16) && x_stride * (int64_t)size_of(type) % 16 == 0 && inner * size_of(type) % 16 == 0, nullptr, 0};
@@ -778,6 +775,7 @@ uint64_t eps_b200_int8_product_workspace(uint64_t rows, uint32_t experts, uint32
   p.experts = experts ? experts : 1;
   p.channels = channels;
   const unsigned tile_rows = tile_rows_of(rows, p.experts);
+  if (on_the_way(tile_rows, eps_b200_int8_stride(inner))) return 0;
   bool sums = shares(p, tile_rows);
   if (p.experts > 1) {
     p.offsets = &grouped;
@@ -817,17 +815,19 @@ int eps_b200_int8_linear(const EpsB200Int8Product* a, const void* x, int64_t x_s
   return guard(status, [&] {
     Product p = product_args(a);
     if (!p.rows) return;
-    need(a->workspace && a->workspace_bytes >= eps_b200_int8_product_workspace(a->rows, a->experts, a->channels, a->inner),
-         "int8 workspace too small");
+    const uint64_t bytes = eps_b200_int8_product_workspace(a->rows, a->experts, a->channels, a->inner);
+    need(!bytes || (a->workspace && a->workspace_bytes >= bytes), "int8 workspace too small");
     auto* q = static_cast<int8_t*>(a->workspace);
     auto* scale = reinterpret_cast<float*>(q + (uint64_t)p.rows * p.padded);
-    Quantize z = quantize_args(a->type, x, x_stride, x_rows, a->inner, rows, a->rows_divisor, a->rows, q, scale);
+    const unsigned tile_rows = tile_rows_of(p.rows, p.experts);
+    const bool direct = on_the_way(tile_rows, p.padded);
+    need(direct || q, "null workspace");
+    Quantize z = quantize_args(a->type, x, x_stride, x_rows, a->inner, rows, a->rows_divisor, a->rows, q, scale, !direct);
     p.q = q;
     p.scale = scale;
     const auto st = static_cast<cudaStream_t>(stream);
-    const unsigned tile_rows = tile_rows_of(p.rows, p.experts);
     OnDevice on(a->device);
-    if (!tile_rows && p.padded <= 24 * 1024) return product_by_rows(a->type, p, &z, a->device, st);       // eight rows fit shared memory
+    if (direct) return product_by_rows(a->type, p, &z, a->device, st);
     if (shares(p, tile_rows)) {
       p.sums = z.clear = reinterpret_cast<int*>(reinterpret_cast<char*>(scale) + round_up(p.rows * 4ull, 16));
       z.clear_words = p.channels;

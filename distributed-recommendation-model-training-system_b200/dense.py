@@ -482,6 +482,7 @@ class QuantizedExperts:
         self.weight[..., : self.inner] = weight
         self.scale = scale.reshape(self.experts, self.channels)
         self.bias = None if bias is None else bias.reshape(self.experts, self.channels)
+        self._index, self._fixed = self.device.index, (self.weight.data_ptr(), self.scale.data_ptr(), _ptr(self.bias))
 
     @classmethod
     def from_weights(cls, weight, bias=None):
@@ -501,7 +502,7 @@ class QuantizedExperts:
         (may be left out with one expert).  rows int32 [n]: row r of the product is
         made from x[rows[r] // rows_divisor] -- a Routing's `order` with rows_divisor
         = top_k; without it from x[r].  Rows in no expert's run are left unwritten."""
-        device = self.device.index
+        device = self._index
         flat, stride, x_rows, _ = _matrix(x, "x", device, self.inner)
         index = _row_index(rows, rows_divisor, device)
         n = x_rows if rows is None else rows.shape[0]
@@ -514,10 +515,10 @@ class QuantizedExperts:
         shape = (*x.shape[:-1], self.channels) if rows is None else (n, self.channels)
         out = torch.empty(shape, dtype=flat.dtype, device=self.device)
         space = _lib.eps_b200_int8_product_workspace(n, self.experts, self.channels, self.inner)
-        workspace = torch.empty(space, dtype=torch.uint8, device=self.device)
+        workspace = torch.empty(space, dtype=torch.uint8, device=self.device) if space else None
         args = _pack(_INT8_PRODUCT, device, _TYPES[flat.dtype], self.experts, self.channels, self.inner, rows_divisor, n,
-                     self.weight.data_ptr(), self.scale.data_ptr(), _ptr(self.bias), _ptr(offsets), out.data_ptr(),
-                     workspace.data_ptr(), space)
+                     *self._fixed, _ptr(offsets), out.data_ptr(),
+                     _ptr(workspace), space)
         _call(_lib.eps_b200_int8_linear, args, flat.data_ptr(), stride, x_rows, index, _stream(device))
         return out
 

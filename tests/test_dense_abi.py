@@ -122,7 +122,7 @@ def test_int8_refuses(change):
 def test_int8_refuses_missing_tensors():
     assert refused(LIB.eps_b200_int8_product, linear(), None, A, None) == eps.INVALID_ARGUMENT
     assert refused(LIB.eps_b200_int8_product, linear(), A + 1, A, None) == eps.INVALID_ARGUMENT
-    assert refused(LIB.eps_b200_int8_linear, linear(workspace_bytes=8), A, 64, 4, None, None) == eps.INVALID_ARGUMENT
+    assert refused(LIB.eps_b200_int8_linear, linear(rows=400, workspace_bytes=8), A, 64, 400, None, None) == eps.INVALID_ARGUMENT
     assert refused(LIB.eps_b200_int8_linear, linear(), A, 64, 3, None, None) == eps.INVALID_ARGUMENT        # fewer rows than asked for
     assert refused(LIB.eps_b200_int8_linear, linear(rows_divisor=0), A, 64, 3, A, None) == eps.INVALID_ARGUMENT
     assert refused(LIB.eps_b200_int8_quantize, 0, 0, A, 64, 4, 64, None, 1, 4, None, A, None) == eps.INVALID_ARGUMENT
