@@ -173,11 +173,12 @@ __device__ __forceinline__ Tile locate(const Product& a, unsigned tile_rows, uns
 // first weights, and while they come the block quantizes its RT rows into shared
 // memory for all its warps (every block does that again: the rows are a few kilobytes
 // in L2, and a launch before this one would take longer).
-constexpr unsigned kRowsThreads = 256, kRowsAhead = 8;
+constexpr unsigned kRowsThreads = 512, kRowsAhead = 8;
 template <class T, int RT, bool QUANTIZE>
 __global__ void __launch_bounds__(kRowsThreads) product_rows(const Product a, const Quantize z, unsigned channel_blocks) {
   extern __shared__ __align__(16) int8_t staged[];      // QUANTIZE: [RT][padded]
-  __shared__ unsigned tops[RT][kRowsThreads / 32];
+  __shared__ unsigned tops[kRowsThreads / 32];
+  __shared__ float scales[RT];
   constexpr int kV = 16 / sizeof(T);
   const unsigned lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   const Tile t = locate(a, RT, blockIdx.x / channel_blocks);
@@ -194,55 +195,48 @@ __global__ void __launch_bounds__(kRowsThreads) product_rows(const Product a, co
   }
   float scale[RT];
   if constexpr (QUANTIZE) {
-    // rows in turn: a row's values a thread holds are every kRowsThreads-th
+    // the block's warps share the rows: all rows are read at once
+    constexpr unsigned kEach = kRowsThreads / RT;
+    const unsigned r = threadIdx.x / kEach, thread = threadIdx.x % kEach;
+    bool known = false;
+    const T* const x = r < t.rows ? source_row<T>(z, t.row + r, &known) : nullptr;
+    unsigned top = 0;
+    if (known && z.wide) {
+#pragma unroll 4
+      for (unsigned k = thread * kV; k < z.inner; k += kEach * kV) {
+        float v[kV];
+        widen(load_pack<T, kV>(x + k), v);
 #pragma unroll
-    for (int r = 0; r < RT; ++r) {
-      bool known = false;
-      unsigned top = 0;
-      if (r < t.rows) {
-        const T* const x = source_row<T>(z, t.row + r, &known);
-        if (known && z.wide) {
-#pragma unroll 2
-          for (unsigned k = threadIdx.x * kV; k < z.inner; k += kRowsThreads * kV) {
-            float v[kV];
-            widen(load_pack<T, kV>(x + k), v);
-#pragma unroll
-            for (int j = 0; j < kV; ++j) top = max(top, __float_as_uint(v[j]) & 0x7FFFFFFFu);
-          }
-        } else if (known) {
-          for (unsigned k = threadIdx.x; k < z.inner; k += kRowsThreads) top = max(top, __float_as_uint(to_float(x[k])) & 0x7FFFFFFFu);
-        }
+        for (int j = 0; j < kV; ++j) top = max(top, __float_as_uint(v[j]) & 0x7FFFFFFFu);
       }
-      top = __reduce_max_sync(~0u, top);
-      if (lane == 0) tops[r][warp] = top;
+    } else if (known) {
+#pragma unroll 4
+      for (unsigned k = thread; k < z.inner; k += kEach) top = max(top, __float_as_uint(to_float(x[k])) & 0x7FFFFFFFu);
+    }
+    top = __reduce_max_sync(~0u, top);
+    if (lane == 0) tops[warp] = top;
+    __syncthreads();
+#pragma unroll
+    for (unsigned i = 0; i < kEach / 32; ++i) top = max(top, tops[r * (kEach / 32) + i]);
+    float by, mine;
+    factors(top, known, &by, &mine);
+    if (thread == 0) scales[r] = mine;
+    int8_t* const s = staged + r * a.padded;
+    if (known && z.wide) {
+      for (unsigned k = thread * kV; k < a.padded; k += kEach * kV) {
+        float v[kV] = {};
+        if (k < z.inner) widen(load_pack<T, kV>(x + k), v);
+#pragma unroll
+        for (int j = 0; j < kV; j += 4)
+          *reinterpret_cast<unsigned*>(s + k + j) =
+              quantized(v[j], by) | quantized(v[j + 1], by) << 8 | quantized(v[j + 2], by) << 16 | quantized(v[j + 3], by) << 24;
+      }
+    } else if (r < t.rows) {
+      for (unsigned k = thread; k < a.padded; k += kEach) s[k] = known && k < z.inner ? (int8_t)quantized(to_float(x[k]), by) : 0;
     }
     __syncthreads();
 #pragma unroll
-    for (int r = 0; r < RT; ++r) {
-      scale[r] = 0.f;
-      if (r >= t.rows) continue;
-      bool known;
-      const T* const x = source_row<T>(z, t.row + r, &known);
-      unsigned top = 0;
-#pragma unroll
-      for (unsigned i = 0; i < kRowsThreads / 32; ++i) top = max(top, tops[r][i]);
-      float by;
-      factors(top, known, &by, &scale[r]);
-      if (known && z.wide) {
-        for (unsigned k = threadIdx.x * kV; k < a.padded; k += kRowsThreads * kV) {
-          float v[kV] = {};
-          if (k < z.inner) widen(load_pack<T, kV>(x + k), v);
-#pragma unroll
-          for (int j = 0; j < kV; j += 4)
-            *reinterpret_cast<unsigned*>(staged + r * a.padded + k + j) =
-                quantized(v[j], by) | quantized(v[j + 1], by) << 8 | quantized(v[j + 2], by) << 16 | quantized(v[j + 3], by) << 24;
-        }
-      } else {
-        for (unsigned k = threadIdx.x; k < a.padded; k += kRowsThreads)
-          staged[r * a.padded + k] = k < z.inner ? (int8_t)quantized(to_float(x[k]), by) : 0;
-      }
-    }
-    __syncthreads();
+    for (int i = 0; i < RT; ++i) scale[i] = scales[i];
   } else {
 #pragma unroll
     for (int r = 0; r < RT; ++r) scale[r] = r < t.rows ? a.scale[t.row + r] : 0.f;
