@@ -25,8 +25,6 @@ struct Quantize {
   int8_t* q;
   float* scale;
   int wide;
-  int* clear;              // [count][clear_words] words that the product wants to be 0
-  unsigned clear_words;
 };
 
 // The factor and the scale of a row whose largest magnitude has these bits.
@@ -59,7 +57,6 @@ __global__ void __launch_bounds__(kQuantizeThreads) quantize_rows(const Quantize
   __shared__ unsigned tops[kQuantizeThreads / 32];
   constexpr int V = 16 / sizeof(T), kHeld = NIT ? NIT : 1;
   const uint64_t r = blockIdx.x;
-  for (unsigned i = threadIdx.x; i < a.clear_words; i += kQuantizeThreads) a.clear[r * a.clear_words + i] = 0;
   bool known;
   const T* const x = source_row<T>(a, r, &known);
   unsigned top = 0;
@@ -122,7 +119,6 @@ struct Product {
   const int32_t* offsets;
   void* out;
   unsigned rows, experts, channels, padded;
-  int* sums;               // [rows, channels], zeros: where parts of the tensor cores' sums meet; or NULL
 };
 
 struct Tile { unsigned expert, row, rows; };   // rows == 0: there is no such tile
@@ -280,8 +276,7 @@ __global__ void __launch_bounds__(kRowsThreads) product_rows(const Product a, co
 // matrix instruction reads; out-of-range rows and bytes arrive as zeros, and rows of
 // the next expert or channel group, which a ragged tile also covers, are not stored.
 //
-// With few tiles the blocks share the stages of all tiles evenly (see Deal).  One block
-// an SM walks its parts of the tiles: warp 0 fills the stages, warp 1 issues
+// One block an SM walks the tiles: warp 0 fills the stages, warp 1 issues
 // tcgen05.mma (kind::i8, 32-bit sums in tensor memory), warps 4..7 scale, round and
 // store the tile before while the next is being summed (two halves of tensor memory).
 constexpr int kMmaThreads = 256;
@@ -366,58 +361,19 @@ __device__ __forceinline__ void tensor_load(unsigned address, int (&v)[32]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
 
-// The parts of the work that a block does, one after the other: `steps` stages of
-// inner size of a tile each.  With few tiles (`sums` given) all stages of all tiles are
-// dealt out evenly, in runs that may begin and end inside a tile, and added up in
-// `sums`; otherwise a block takes every grid-th whole tile.
-struct Part {
+// The tiles that a block does, one after the other: every grid-th.  Called by a whole warp.
+struct Walk {
+  const Product& a;
+  unsigned tile_rows, channel_tiles, at;
   Tile tile;
   unsigned channel_tile;
-  unsigned first, last;        // stages of the tile
-};
 
-struct Deal {
-  const Product& a;
-  unsigned tile_rows, channel_tiles, steps;
-  uint64_t at, end;            // sums given: stages; otherwise tiles
-
-  // The stages of all tiles; called by a whole warp.
-  static __device__ __forceinline__ uint64_t stages_of(const Product& a, unsigned tile_rows, unsigned channel_tiles, unsigned steps) {
-    const unsigned lane = threadIdx.x % 32;
-    uint64_t tiles = 0;
-    if (!a.offsets) {
-      tiles = (a.rows + tile_rows - 1) / tile_rows;
-    } else {
-      for (unsigned e0 = 0; e0 < a.experts; e0 += 32) {
-        unsigned n = 0;
-        if (e0 + lane < a.experts) n = tiles_of(a, e0 + lane, tile_rows);
-        tiles += __reduce_add_sync(~0u, n);
-      }
-    }
-    return tiles * channel_tiles * steps;
-  }
-  __device__ __forceinline__ Deal(const Product& p, unsigned rows, unsigned channels, unsigned s, uint64_t all)
-      : a(p), tile_rows(rows), channel_tiles(channels), steps(s) {
-    at = a.sums ? all * blockIdx.x / gridDim.x : blockIdx.x;
-    end = a.sums ? all * (blockIdx.x + 1) / gridDim.x : ~0ull;
-  }
-  __device__ __forceinline__ bool next(Part* p) {
-    if (at >= end) return false;
-    const uint64_t index = a.sums ? at / steps : at;
-    p->tile = locate(a, tile_rows, (unsigned)(index / channel_tiles));
-    if (!p->tile.rows) return false;
-    p->channel_tile = (unsigned)(index % channel_tiles);
-    p->first = 0;
-    p->last = steps;
-    if (a.sums) {
-      p->first = (unsigned)(at - index * steps);
-      const uint64_t left = end - at;
-      if (p->first + left < steps) p->last = p->first + (unsigned)left;
-      at += p->last - p->first;
-    } else {
-      at += gridDim.x;
-    }
-    return true;
+  __device__ __forceinline__ Walk(const Product& p, unsigned rows, unsigned channels) : a(p), tile_rows(rows), channel_tiles(channels), at(blockIdx.x) {}
+  __device__ __forceinline__ bool next() {
+    tile = locate(a, tile_rows, at / channel_tiles);
+    channel_tile = at % channel_tiles;
+    at += gridDim.x;
+    return tile.rows;
   }
 };
 
@@ -455,22 +411,20 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const unsigned base = tensor_base;
   const unsigned steps = (a.padded + kStageK - 1) / kStageK;
-  const uint64_t all = a.sums ? Deal::stages_of(a, BN, channel_tiles, steps) : 0;
-  Deal deal(a, BN, channel_tiles, steps, all);
-  Part part;
+  Walk walk(a, BN, channel_tiles);
 
   if (warp == 0) {
     unsigned stage = 0, phase = 0, filled = 0;
     bool ok = true;
-    while (ok && deal.next(&part)) {
-      const int y = (int)(part.tile.expert * a.channels + part.channel_tile * kTileM);
-      for (unsigned k = part.first; k < part.last; ++k) {
+    while (ok && walk.next()) {
+      const int y = (int)(walk.tile.expert * a.channels + walk.channel_tile * kTileM);
+      for (unsigned k = 0; k < steps; ++k) {
         if (!(ok = warp_wait(at_empty + stage * 8, phase ^ 1))) break;
         const unsigned to = at_stages + stage * Shape::stage_bytes, barrier = at_full + stage * 8;
         if (elected()) {
           expect(barrier, Shape::stage_bytes);
           tma_load(to, &weights, barrier, (int)(k * kStageK), y);
-          tma_load(to + kTileM * kStageK, &rows, barrier, (int)(k * kStageK), (int)part.tile.row);
+          tma_load(to + kTileM * kStageK, &rows, barrier, (int)(k * kStageK), (int)walk.tile.row);
         }
         if (++filled > Shape::stages) filled = Shape::stages;
         if (++stage == Shape::stages) { stage = 0; phase ^= 1; }
@@ -486,16 +440,16 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
   } else if (warp == 1) {
     unsigned stage = 0, phase = 0, half = 0, turn = 0;
     bool ok = true;
-    while (ok && deal.next(&part)) {
+    while (ok && walk.next()) {
       ok = warp_wait(shared_at(drained) + half * 8, turn ^ 1);
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      for (unsigned k = part.first; ok && k < part.last; ++k) {
+      for (unsigned k = 0; ok && k < steps; ++k) {
         if (!(ok = warp_wait(at_full + stage * 8, phase))) break;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         const unsigned w = low_operand + stage * (Shape::stage_bytes / 16), q = w + kTileM * kStageK / 16, d = base + half * BN;
         if (elected()) {
 #pragma unroll
-          for (unsigned i = 0; i < kStageK / 32; ++i) mma_i8<BN>(d, w + 2 * i, q + 2 * i, k != part.first || i);
+          for (unsigned i = 0; i < kStageK / 32; ++i) mma_i8<BN>(d, w + 2 * i, q + 2 * i, k || i);
           mma_commit(at_empty + stage * 8);
         }
         if (++stage == Shape::stages) { stage = 0; phase ^= 1; }
@@ -508,39 +462,26 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
   } else if (warp >= 4) {
     unsigned half = 0, turn = 0;
     bool ok = true;
-    while (ok && deal.next(&part)) {
-      const Tile tile = part.tile;
-      const unsigned l = (warp - 4) * 32 + lane, n = part.channel_tile * kTileM + l;
+    while (ok && walk.next()) {
+      const Tile tile = walk.tile;
+      const unsigned l = (warp - 4) * 32 + lane, n = walk.channel_tile * kTileM + l;
       const uint64_t c = (uint64_t)tile.expert * a.channels + n;
       const bool in = n < a.channels;
       const float ws = in ? a.weight_scale[c] : 0.f, b = in && a.bias ? a.bias[c] : 0.f;
       ok = warp_wait(shared_at(summed) + half * 8, turn);
-      if (!ok && a.sums)           // the rows whose sums are lost
-        for (unsigned r = lane; r < tile.rows; r += 32) const_cast<float*>(a.scale)[tile.row + r] = NAN;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       T* const out = static_cast<T*>(a.out) + (uint64_t)tile.row * a.channels + n;
       const unsigned from = base + half * BN + ((warp - 4) * 32 << 16);
-      auto finish = [&](unsigned r0, const int (&v)[32]) {
+#pragma unroll 1
+      for (unsigned r0 = 0; r0 < tile.rows; r0 += 32) {
+        int v[32];
+        tensor_load(from + r0, v);
         const float mine = r0 + lane < tile.rows ? a.scale[tile.row + r0 + lane] : 0.f;
 #pragma unroll
         for (unsigned j = 0; j < 32; ++j) {
           const float s = __shfl_sync(~0u, mine, j);
           const float value = ok ? fmaf((float)v[j], s * ws, b) : NAN;
           if (in && r0 + j < tile.rows) out[(uint64_t)(r0 + j) * a.channels] = from_float<T>(value);
-        }
-      };
-#pragma unroll 1
-      for (unsigned r0 = 0; r0 < tile.rows; r0 += 32) {
-        int v[32];
-        tensor_load(from + r0, v);
-        if (!a.sums) {
-          finish(r0, v);
-        } else {
-          // a part of the sum: 32-bit integers may be added in any order
-          int* const s = a.sums + (uint64_t)(tile.row + r0) * a.channels + n;
-#pragma unroll
-          for (unsigned j = 0; j < 32; ++j)
-            if (in && r0 + j < tile.rows) atomicAdd(s + (uint64_t)j * a.channels, v[j]);
         }
       }
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -555,23 +496,6 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   if (warp == 2)
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(base), "r"(Shape::columns) : "memory");
-}
-
-// The tiles' sums, scaled: 32 rows of a tile a block.
-template <class T>
-__global__ void __launch_bounds__(256) product_finish(const Product a, unsigned tile_rows, unsigned channel_tiles) {
-  const Tile tile = locate(a, tile_rows, blockIdx.x / channel_tiles);
-  const unsigned n = blockIdx.x % channel_tiles * kTileM + threadIdx.x % kTileM, r0 = blockIdx.y * 32 + threadIdx.x / kTileM;
-  if (r0 >= tile.rows || n >= a.channels) return;
-  const uint64_t c = (uint64_t)tile.expert * a.channels + n;
-  const float ws = a.weight_scale[c], b = a.bias ? a.bias[c] : 0.f;
-#pragma unroll
-  for (unsigned j = 0; j < 32; j += 2) {
-    const unsigned r = r0 + j;
-    if (r >= tile.rows) break;
-    const uint64_t at = (uint64_t)(tile.row + r) * a.channels + n;
-    static_cast<T*>(a.out)[at] = from_float<T>(fmaf((float)__ldcg(a.sums + at), a.scale[tile.row + r] * ws, b));
-  }
 }
 
 template <class F>
@@ -632,24 +556,32 @@ uint64_t tile_bound(const Product& a, unsigned tile_rows) {
   return ceil_div(a.rows, tile_rows) + extra;
 }
 
-// Which kernel a product takes, by the rows of an expert on average (the host does not
-// know the groups), and its tile's rows.
-unsigned tile_rows_of(uint64_t rows, uint64_t experts) {
+// Which kernel a product takes, and its tile's rows: 0 for product_rows.  The host does
+// not know the groups, so it goes by the rows of an expert on average.
+//
+// A block takes its tiles in rounds, and a stage takes much the same time whatever the
+// tile's rows (0.42 us at 32 and 64, 0.45 at 128, 0.52 at 256, from 24, 200, 1531 and
+// 8189 rows), so the tile is the one whose rounds of a B200's 148 SMs cost least, the
+// smaller of equals: 200 rows x 4096 channels make 32 tiles of 256 rows or 128 of 64.
+unsigned tile_rows_of(uint64_t rows, uint64_t experts, uint64_t channels) {
   const uint64_t each = ceil_div(rows, experts);
   if (rows <= 8 || each <= 2) return 0;
-  return each > 128 ? 256 : each > 64 ? 128 : each > 32 ? 64 : 32;
+  static const struct { unsigned rows; uint64_t cost; } shapes[] = {{32, 42}, {64, 42}, {128, 45}, {256, 52}};
+  unsigned best = 0;
+  uint64_t least = ~0ull;
+  for (const auto& s : shapes) {
+    const uint64_t tiles = ceil_div(each, s.rows) * (experts < rows ? experts : rows) * ceil_div(channels, kTileM);
+    const uint64_t cost = ceil_div(tiles, 148) * s.cost;
+    if (cost < least) {
+      least = cost;
+      best = s.rows;
+    }
+  }
+  return best;
 }
 
 // Whether rows are quantized where they are used: few of them, eight of which fit shared memory.
 bool on_the_way(unsigned tile_rows, uint64_t padded) { return !tile_rows && padded <= 24 * 1024; }
-
-// Whether the blocks share the tiles' stages: whole tiles would leave most SMs idle,
-// while sums in memory cost four bytes an output twice over L2.  The bound stands for
-// two rounds of a B200's 148 SMs.
-constexpr uint64_t kFewTiles = 296;
-bool shares(const Product& a, unsigned tile_rows) {
-  return tile_rows && tile_bound(a, tile_rows) * ceil_div(a.channels, kTileM) < kFewTiles;
-}
 
 template <int BN>
 void tiles(int type, const Product& a, int device, cudaStream_t stream) {
@@ -660,20 +592,18 @@ void tiles(int type, const Product& a, int device, cudaStream_t stream) {
   const unsigned channel_tiles = (unsigned)ceil_div(a.channels, kTileM);
   const uint64_t most = tile_bound(a, BN) * channel_tiles;
   need(most < (1ull << 31), "too many rows");
-  const unsigned blocks = a.sums || most > sms ? sms : (unsigned)most;
+  const unsigned blocks = most > sms ? sms : (unsigned)most;
   by_type(type, [&](auto t) {
     constexpr auto kernel = product_tiles<decltype(t), BN>;
     room<kernel>(device, Shape::shared);
     kernel<<<blocks, kMmaThreads, Shape::shared, stream>>>(a, w, q, channel_tiles);
-    check(cudaGetLastError(), "int8_product");
-    if (a.sums) product_finish<decltype(t)><<<dim3((unsigned)most, BN / 32), 256, 0, stream>>>(a, BN, channel_tiles);
   });
   check(cudaGetLastError(), "int8_product");
 }
 
 void product_by_tiles(int type, const Product& a, int device, cudaStream_t stream) {
   need((uint64_t)a.experts * a.channels < (1ull << 31), "too many channels");
-  switch (tile_rows_of(a.rows, a.experts)) {
+  switch (tile_rows_of(a.rows, a.experts, a.channels)) {
     case 256: return tiles<256>(type, a, device, stream);
     case 128: return tiles<128>(type, a, device, stream);
     case 64: return tiles<64>(type, a, device, stream);
@@ -716,7 +646,7 @@ Quantize quantize_args(int type, const void* x, int64_t x_stride, uint64_t x_row
   need(!count || (!kept || (q && scale)) && (x || !x_rows), "null input or output");
   need(aligned(q, 16), "q must be 16-byte aligned");
   return Quantize{x, x_stride, x_rows, count, inner, (unsigned)eps_b200_int8_stride(inner), divisor, rows, q, scale,
-                  aligned(x, 16) && x_stride * (int64_t)size_of(type) % 16 == 0 && inner * size_of(type) % 16 == 0, nullptr, 0};
+                  aligned(x, 16) && x_stride * (int64_t)size_of(type) % 16 == 0 && inner * size_of(type) % 16 == 0};
 }
 
 Product product_args(const EpsB200Int8Product* a) {
@@ -763,19 +693,8 @@ int eps_b200_int8_quantize(int32_t device, int32_t type, const void* x, int64_t 
 }
 
 uint64_t eps_b200_int8_product_workspace(uint64_t rows, uint32_t experts, uint32_t channels, uint32_t inner) {
-  Product p{};
-  static const int32_t grouped = 0;       // any address: the bound for groups is the larger one
-  p.rows = (unsigned)rows;
-  p.experts = experts ? experts : 1;
-  p.channels = channels;
-  const unsigned tile_rows = tile_rows_of(rows, p.experts);
-  if (on_the_way(tile_rows, eps_b200_int8_stride(inner))) return 0;
-  bool sums = shares(p, tile_rows);
-  if (p.experts > 1) {
-    p.offsets = &grouped;
-    sums = shares(p, tile_rows);
-  }
-  return rows * eps_b200_int8_stride(inner) + round_up(rows * 4, 16) + (sums ? rows * channels * 4 : 0);
+  if (on_the_way(tile_rows_of(rows, experts ? experts : 1, channels), eps_b200_int8_stride(inner))) return 0;
+  return rows * eps_b200_int8_stride(inner) + round_up(rows * 4, 16);
 }
 
 int eps_b200_int8_product(const EpsB200Int8Product* a, const int8_t* q, const float* scale, void* stream,
@@ -788,18 +707,12 @@ int eps_b200_int8_product(const EpsB200Int8Product* a, const int8_t* q, const fl
     p.q = q;
     p.scale = scale;
     const auto st = static_cast<cudaStream_t>(stream);
-    const unsigned tile_rows = tile_rows_of(p.rows, p.experts);
+    const unsigned tile_rows = tile_rows_of(p.rows, p.experts, p.channels);
     if (!tile_rows) {
       OnDevice on(a->device);
       return product_by_rows(a->type, p, nullptr, a->device, st);
     }
     OnDevice on(a->device);
-    if (shares(p, tile_rows)) {
-      const uint64_t bytes = (uint64_t)p.rows * p.channels * 4;
-      need(a->workspace && a->workspace_bytes >= bytes, "int8 workspace too small");
-      p.sums = static_cast<int*>(a->workspace);
-      check(cudaMemsetAsync(p.sums, 0, bytes, st), "cudaMemsetAsync");
-    }
     product_by_tiles(a->type, p, a->device, st);
   });
 }
@@ -813,19 +726,15 @@ int eps_b200_int8_linear(const EpsB200Int8Product* a, const void* x, int64_t x_s
     need(!bytes || (a->workspace && a->workspace_bytes >= bytes), "int8 workspace too small");
     auto* q = static_cast<int8_t*>(a->workspace);
     auto* scale = reinterpret_cast<float*>(q + (uint64_t)p.rows * p.padded);
-    const unsigned tile_rows = tile_rows_of(p.rows, p.experts);
+    const unsigned tile_rows = tile_rows_of(p.rows, p.experts, p.channels);
     const bool direct = on_the_way(tile_rows, p.padded);
     need(direct || q, "null workspace");
-    Quantize z = quantize_args(a->type, x, x_stride, x_rows, a->inner, rows, a->rows_divisor, a->rows, q, scale, !direct);
+    const Quantize z = quantize_args(a->type, x, x_stride, x_rows, a->inner, rows, a->rows_divisor, a->rows, q, scale, !direct);
     p.q = q;
     p.scale = scale;
     const auto st = static_cast<cudaStream_t>(stream);
     OnDevice on(a->device);
     if (direct) return product_by_rows(a->type, p, &z, a->device, st);
-    if (shares(p, tile_rows)) {
-      p.sums = z.clear = reinterpret_cast<int*>(reinterpret_cast<char*>(scale) + round_up(p.rows * 4ull, 16));
-      z.clear_words = p.channels;
-    }
     quantize(a->type, z, st);
     if (tile_rows) product_by_tiles(a->type, p, a->device, st);
     else product_by_rows(a->type, p, nullptr, a->device, st);

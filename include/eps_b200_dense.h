@@ -153,8 +153,7 @@ EPS_B200_EXPORT int eps_b200_int8_quantize(int32_t device, int32_t type, const v
  * read as clamped to [0, rows] and a run that ends before it begins as empty; rows
  * of no run are not written.  q, weight and out 16-byte aligned; q and weight have
  * row strides of eps_b200_int8_stride(inner) with zeros behind `inner` (at most
- * EPS_B200_INT8_INNER, so that the sum fits 32 bits), out is contiguous.  The
- * workspace has eps_b200_int8_product_workspace() bytes. */
+ * EPS_B200_INT8_INNER, so that the sum fits 32 bits), out is contiguous. */
 #define EPS_B200_INT8_INNER 131072u
 typedef struct {
   int32_t device;
@@ -174,7 +173,8 @@ EPS_B200_EXPORT uint64_t eps_b200_int8_product_workspace(uint64_t rows, uint32_t
                                                          uint32_t channels, uint32_t inner);
 EPS_B200_EXPORT int eps_b200_int8_product(const EpsB200Int8Product* args, const int8_t* q,
                                           const float* scale, void* stream, EpsB200Status* status);
-/* quantize and product in one call, q and scale in the workspace. */
+/* quantize and product in one call, q and scale in the workspace of
+ * eps_b200_int8_product_workspace() bytes (0 for few rows: then they need none). */
 EPS_B200_EXPORT int eps_b200_int8_linear(const EpsB200Int8Product* args, const void* x,
                                          int64_t x_stride, uint64_t x_rows, const int32_t* rows,
                                          void* stream, EpsB200Status* status);
