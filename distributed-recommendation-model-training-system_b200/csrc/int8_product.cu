@@ -271,21 +271,33 @@ __global__ void __launch_bounds__(kRowsThreads) product_rows(const Product a, co
 //
 // A tile is 128 channels x BN rows of one expert: D[channel, row] = W q^T, so the
 // channels lie on the lanes of tensor memory and a store of a warp covers 32
-// neighbouring channels of one output row.  Both operands are K-major int8, 128
-// bytes of inner size a stage, brought by TMA with the 128-byte swizzle that the
-// matrix instruction reads; out-of-range rows and bytes arrive as zeros, and rows of
+// neighbouring channels of one output row.  Both operands are K-major int8, brought by
+// TMA in spans of 128 bytes of inner size with the 128-byte swizzle that the matrix
+// instruction reads; a stage is one span, or two for tiles of up to 128 rows, since a
+// stage's hand-over between the warps takes as long (some 430 cycles) whatever it holds
+// (200 rows x 4096 x 4096: 15.6 us with one span a stage, 14.2 with two, 15.5 with four,
+// which leave too few stages);
+// out-of-range rows and bytes arrive as zeros, and rows of
 // the next expert or channel group, which a ragged tile also covers, are not stored.
 //
 // One block an SM walks the tiles: warp 0 fills the stages, warp 1 issues
 // tcgen05.mma (kind::i8, 32-bit sums in tensor memory), warps 4..7 scale, round and
 // store the tile before while the next is being summed (two halves of tensor memory).
+//
+// What bounds it: a large product (8189 x 8192 x 4096: 243 us, 2.26e15 operations a
+// second, the tensor pipe busy 53 % of the time) by what the SMs bring in, 48 KB for
+// every 512 cycles of matrix instructions, 13 TB/s over the GPU out of L2; a pair of
+// SMs on one tile would halve half of that.  Few rows: by the weights' way through one
+// SM's copies (64 GB/s) where there are fewer tiles than SMs.
 constexpr int kMmaThreads = 256;
-constexpr unsigned kStageK = 128;          // bytes of inner size a stage
+constexpr unsigned kSpan = 128;            // bytes of inner size that one swizzled copy covers
 constexpr unsigned kTileM = 128;           // channels of a tile
 
 template <int BN>
 struct MmaShape {
-  static constexpr unsigned stage_bytes = (kTileM + BN) * kStageK;
+  static constexpr unsigned spans = BN < 256 ? 2 : 1;                  // of a stage: see above
+  static constexpr unsigned span_bytes = (kTileM + BN) * kSpan;        // of both operands
+  static constexpr unsigned stage_bytes = spans * span_bytes;
   static constexpr unsigned stages = 196608 / stage_bytes < 8 ? 196608 / stage_bytes : 8;
   static constexpr unsigned shared = stages * stage_bytes + 1024;      // and room to align
   static constexpr unsigned columns = 2 * BN;                          // of tensor memory
@@ -410,7 +422,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
   __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const unsigned base = tensor_base;
-  const unsigned steps = (a.padded + kStageK - 1) / kStageK;
+  const unsigned steps = (a.padded + Shape::spans * kSpan - 1) / (Shape::spans * kSpan);
   Walk walk(a, BN, channel_tiles);
 
   if (warp == 0) {
@@ -423,8 +435,12 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
         const unsigned to = at_stages + stage * Shape::stage_bytes, barrier = at_full + stage * 8;
         if (elected()) {
           expect(barrier, Shape::stage_bytes);
-          tma_load(to, &weights, barrier, (int)(k * kStageK), y);
-          tma_load(to + kTileM * kStageK, &rows, barrier, (int)(k * kStageK), (int)walk.tile.row);
+#pragma unroll
+          for (unsigned s = 0; s < Shape::spans; ++s) {
+            const int x = (int)((k * Shape::spans + s) * kSpan);      // behind the inner size zeros arrive
+            tma_load(to + s * Shape::span_bytes, &weights, barrier, x, y);
+            tma_load(to + s * Shape::span_bytes + kTileM * kSpan, &rows, barrier, x, (int)walk.tile.row);
+          }
         }
         if (++filled > Shape::stages) filled = Shape::stages;
         if (++stage == Shape::stages) { stage = 0; phase ^= 1; }
@@ -446,10 +462,16 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
       for (unsigned k = 0; ok && k < steps; ++k) {
         if (!(ok = warp_wait(at_full + stage * 8, phase))) break;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        const unsigned w = low_operand + stage * (Shape::stage_bytes / 16), q = w + kTileM * kStageK / 16, d = base + half * BN;
+        const unsigned w = low_operand + stage * (Shape::stage_bytes / 16), q = w + kTileM * kSpan / 16, d = base + half * BN;
         if (elected()) {
 #pragma unroll
-          for (unsigned i = 0; i < kStageK / 32; ++i) mma_i8<BN>(d, w + 2 * i, q + 2 * i, k || i);
+          for (unsigned s = 0; s < Shape::spans; ++s) {
+#pragma unroll
+            for (unsigned i = 0; i < kSpan / 32; ++i) {
+              const unsigned at = s * (Shape::span_bytes / 16) + 2 * i;
+              mma_i8<BN>(d, w + at, q + at, k || s || i);
+            }
+          }
           mma_commit(at_empty + stage * 8);
         }
         if (++stage == Shape::stages) { stage = 0; phase ^= 1; }
@@ -542,7 +564,7 @@ Encode encoder() {
 CUtensorMap tensor_map(const void* p, uint64_t rows, unsigned padded, unsigned box_rows) {
   CUtensorMap m;
   const cuuint64_t dims[2] = {padded, rows}, strides[1] = {padded};
-  const cuuint32_t box[2] = {kStageK, box_rows}, step[2] = {1, 1};
+  const cuuint32_t box[2] = {kSpan, box_rows}, step[2] = {1, 1};
   const CUresult r = encoder()(&m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(p), dims, strides, box, step,
                                CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);

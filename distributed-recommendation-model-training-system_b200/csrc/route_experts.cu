@@ -282,6 +282,7 @@ __global__ void __launch_bounds__(kWarps * 32, EPL <= 8 ? 4 : EPL == 16 ? 2 : 1)
   const Scratch s{reinterpret_cast<uint16_t*>(p0), reinterpret_cast<int*>(p1), reinterpret_cast<float*>(p1 + 128), reinterpret_cast<uint64_t*>(p2),
                   reinterpret_cast<unsigned*>(p3), reinterpret_cast<float*>(p3) + a.experts};
   const bool sorting = a.order != nullptr;
+  uint16_t* const ranks = reinterpret_cast<uint16_t*>(raw + kWarps * each + a.experts * 4);     // of the tile's entries in their warp's run
   if (sorting)
     for (unsigned e = lane; e < a.experts; e += 32) s.count[e] = 0;
   float bias[EPL];
@@ -348,7 +349,7 @@ __global__ void __launch_bounds__(kWarps * 32, EPL <= 8 ? 4 : EPL == 16 ? 2 : 1)
       const uint64_t entry = token * a.top_k + lane;
       a.chosen[entry] = expert;
       a.weights[entry] = weight * a.scale;
-      if (sorting) a.ranks[entry] = s.count[expert]++;
+      if (sorting) ranks[entry - tile * a.top_k] = s.count[expert]++;
     }
     __syncwarp();
   }
@@ -389,7 +390,7 @@ __global__ void __launch_bounds__(kWarps * 32, EPL <= 8 ? 4 : EPL == 16 ? 2 : 1)
   for (uint64_t i = first + threadIdx.x; i < last; i += blockDim.x) {
     const unsigned w = (unsigned)(i - first) / (a.run * a.top_k);
     const unsigned e = (unsigned)a.chosen[i];
-    const unsigned in_tile = reinterpret_cast<const uint16_t*>(raw + w * each)[e] + a.ranks[i];
+    const unsigned in_tile = reinterpret_cast<const uint16_t*>(raw + w * each)[e] + ranks[i - first];
     if (a.tiles > 1) {
       a.ranks[i] = (uint16_t)in_tile;
     } else {
@@ -596,6 +597,7 @@ using namespace eps_b200::dense;
 extern "C" {
 
 uint64_t eps_b200_route_experts_workspace(uint64_t tokens, uint32_t experts, uint32_t top_k) {
+  if (tokens <= kTile) return 0;
   return round_up(tokens * top_k * 2, 16) + (ceil_div(tokens, kTile) + 1) * experts * 4;
 }
 
@@ -613,7 +615,7 @@ int eps_b200_route_experts(const EpsB200RouteExperts* a, const float* bias, int3
       if (offsets) check(cudaMemsetAsync(offsets, 0, (r.experts + 1) * 4, st), "cudaMemsetAsync");
       return;
     }
-    if (order) {
+    if (order && r.tiles > 1) {
       need(workspace && workspace_bytes >= eps_b200_route_experts_workspace(r.tokens, r.experts, r.top_k) &&
                aligned(workspace, 16), "routing workspace too small or not 16-byte aligned");
       r.ranks = static_cast<uint16_t*>(workspace);
@@ -629,7 +631,7 @@ int eps_b200_route_experts(const EpsB200RouteExperts* a, const float* bias, int3
     by_type(a->type, [&](auto t) {
       by_experts(r.experts, [&](auto epl) {
         const bool spread = r.groups > 1 && r.top_groups < r.groups && !lanes_divide(r.per_group, decltype(epl)::value);
-        const size_t shared = kWarps * scratch_bytes(r.experts, decltype(epl)::value, r.groups, spread) + r.experts * 4;
+        const size_t shared = kWarps * scratch_bytes(r.experts, decltype(epl)::value, r.groups, spread) + r.experts * 4 + (order ? kTile * r.top_k * 2 : 0);
         constexpr auto kernel = route_tokens<decltype(t), decltype(epl)::value>;
         room<kernel>(a->device, shared);
         kernel<<<r.tiles, kWarps * 32, shared, st>>>(r);

@@ -399,11 +399,11 @@ def route(logits, top_k: int, *, score: str = "softmax", bias=None, groups: int 
     order = torch.empty_like(chosen).view(-1)
     offsets = torch.empty(experts + 1, dtype=torch.int32, device=device)
     space = _lib.eps_b200_route_experts_workspace(tokens, experts, top_k)
-    workspace = torch.empty(space, dtype=torch.uint8, device=device)
+    workspace = torch.empty(space, dtype=torch.uint8, device=device) if space else None
     # an empty tensor has no address, yet it is asked for
     _call(_lib.eps_b200_route_experts, args, b, chosen.data_ptr(), weights.data_ptr(),
           order.data_ptr() or offsets.data_ptr(), position.data_ptr() or offsets.data_ptr(), offsets.data_ptr(),
-          workspace.data_ptr(), space, _stream(index))
+          _ptr(workspace), space, _stream(index))
     return Routing(chosen, weights, order, position, offsets)
 
 

@@ -101,7 +101,8 @@ EPS_B200_EXPORT int eps_b200_block_norm_backward(const EpsB200BlockNorm* args,
  *
  * With `order` given, the entries (token * top_k + slot) sorted by expert, equal
  * experts in entry order, their inverse `position`, and offsets[e] .. offsets[e + 1],
- * the run of expert e in `order`.  Needs eps_b200_route_experts_workspace() bytes. */
+ * the run of expert e in `order`.  Needs eps_b200_route_experts_workspace() bytes (0 for
+ * one tile of tokens). */
 enum { EPS_B200_SCORE_SOFTMAX = 0, EPS_B200_SCORE_SIGMOID = 1 };
 #define EPS_B200_ROUTE_EXPERTS 1024u       /* most experts */
 #define EPS_B200_ROUTE_TOP_K 32u           /* most experts of a token */
