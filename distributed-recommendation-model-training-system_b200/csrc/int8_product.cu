@@ -373,16 +373,66 @@ __device__ __forceinline__ void tensor_load(unsigned address, int (&v)[32]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
 
+// The groups' tiles, counted once a block: `locate` reads offsets from memory for every
+// tile, some thousand cycles in each of a block's roles, and this one a few words of
+// shared memory.
+constexpr unsigned kListed = 256;           // experts that are listed; more are located in memory
+struct Groups {
+  unsigned last[kListed];                   // tiles up to and with this expert
+  unsigned begin[kListed], end[kListed];    // its rows
+};
+
+// By one whole warp, before a barrier of the block.
+__device__ __forceinline__ void list_groups(const Product& a, unsigned tile_rows, Groups& g) {
+  const unsigned lane = threadIdx.x % 32;
+  unsigned before = 0;
+  if (!a.offsets || a.experts > kListed) return;
+  for (unsigned e0 = 0; e0 < a.experts; e0 += 32) {
+    const unsigned e = e0 + lane;
+    unsigned begin = 0, end = 0;
+    if (e < a.experts) run_of(a, e, &begin, &end);
+    unsigned sum = end > begin ? (end - begin + tile_rows - 1) / tile_rows : 0;
+#pragma unroll
+    for (int o = 1; o < 32; o *= 2) {
+      const unsigned up = __shfl_up_sync(~0u, sum, o);
+      if (lane >= o) sum += up;
+    }
+    if (e < a.experts) {
+      g.last[e] = before + sum;
+      g.begin[e] = begin;
+      g.end[e] = end;
+    }
+    before += __shfl_sync(~0u, sum, 31);
+  }
+}
+
+// As `locate`, with the groups listed.
+__device__ __forceinline__ Tile look_up(const Product& a, const Groups& g, unsigned tile_rows, unsigned index) {
+  if (!a.offsets || a.experts > kListed) return locate(a, tile_rows, index);
+  const unsigned lane = threadIdx.x % 32;
+  for (unsigned e0 = 0; e0 < a.experts; e0 += 32) {
+    const unsigned e = e0 + lane;
+    const unsigned here = __ballot_sync(~0u, e < a.experts && index < g.last[e]);
+    if (!here) continue;
+    const unsigned owner = e0 + __ffs(here) - 1;
+    const unsigned row = g.begin[owner] + (index - (owner ? g.last[owner - 1] : 0)) * tile_rows;
+    return {owner, row, min(tile_rows, g.end[owner] - row)};
+  }
+  return {0, 0, 0};
+}
+
 // The tiles that a block does, one after the other: every grid-th.  Called by a whole warp.
 struct Walk {
   const Product& a;
+  const Groups& groups;
   unsigned tile_rows, channel_tiles, at;
   Tile tile;
   unsigned channel_tile;
 
-  __device__ __forceinline__ Walk(const Product& p, unsigned rows, unsigned channels) : a(p), tile_rows(rows), channel_tiles(channels), at(blockIdx.x) {}
+  __device__ __forceinline__ Walk(const Product& p, const Groups& g, unsigned rows, unsigned channels)
+      : a(p), groups(g), tile_rows(rows), channel_tiles(channels), at(blockIdx.x) {}
   __device__ __forceinline__ bool next() {
-    tile = locate(a, tile_rows, at / channel_tiles);
+    tile = look_up(a, groups, tile_rows, at / channel_tiles);
     channel_tile = at % channel_tiles;
     at += gridDim.x;
     return tile.rows;
@@ -397,6 +447,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
   extern __shared__ unsigned char raw[];
   __shared__ uint64_t full[Shape::stages], empty[Shape::stages], summed[2], drained[2];
   __shared__ unsigned tensor_base;
+  __shared__ Groups groups;
   const unsigned at_stages = (shared_at(raw) + 1023) / 1024 * 1024, at_full = shared_at(full), at_empty = shared_at(empty);
   const unsigned low_operand = operand_low(at_stages);
   const unsigned warp = threadIdx.x / 32, lane = threadIdx.x % 32;
@@ -418,12 +469,13 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
                  "r"(Shape::columns) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
+  if (warp == 3) list_groups(a, BN, groups);
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const unsigned base = tensor_base;
   const unsigned steps = (a.padded + Shape::spans * kSpan - 1) / (Shape::spans * kSpan);
-  Walk walk(a, BN, channel_tiles);
+  Walk walk(a, groups, BN, channel_tiles);
 
   if (warp == 0) {
     unsigned stage = 0, phase = 0, filled = 0;
@@ -490,6 +542,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
       const uint64_t c = (uint64_t)tile.expert * a.channels + n;
       const bool in = n < a.channels;
       const float ws = in ? a.weight_scale[c] : 0.f, b = in && a.bias ? a.bias[c] : 0.f;
+      float mine = lane < tile.rows ? a.scale[tile.row + lane] : 0.f;      // of the first 32 rows
       ok = warp_wait(shared_at(summed) + half * 8, turn);
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       T* const out = static_cast<T*>(a.out) + (uint64_t)tile.row * a.channels + n;
@@ -498,13 +551,14 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
       for (unsigned r0 = 0; r0 < tile.rows; r0 += 32) {
         int v[32];
         tensor_load(from + r0, v);
-        const float mine = r0 + lane < tile.rows ? a.scale[tile.row + r0 + lane] : 0.f;
+        const float next = r0 + 32 + lane < tile.rows ? a.scale[tile.row + r0 + 32 + lane] : 0.f;
 #pragma unroll
         for (unsigned j = 0; j < 32; ++j) {
           const float s = __shfl_sync(~0u, mine, j);
           const float value = ok ? fmaf((float)v[j], s * ws, b) : NAN;
           if (in && r0 + j < tile.rows) out[(uint64_t)(r0 + j) * a.channels] = from_float<T>(value);
         }
+        mine = next;
       }
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       __syncwarp();
