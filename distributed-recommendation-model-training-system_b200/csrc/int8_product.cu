@@ -281,7 +281,7 @@ __global__ void __launch_bounds__(kRowsThreads) product_rows(const Product a, co
 // the next expert or channel group, which a ragged tile also covers, are not stored.
 //
 // One block an SM walks the tiles: warp 0 fills the stages, warp 1 issues
-// tcgen05.mma (kind::i8, 32-bit sums in tensor memory), warps 4..7 scale, round and
+// tcgen05.mma (kind::i8, 32-bit sums in tensor memory), warps 4..11 scale, round and
 // store the tile before while the next is being summed (two halves of tensor memory).
 //
 // What bounds it: a large product (8189 x 8192 x 4096: 243 us, 2.26e15 operations a
@@ -289,7 +289,7 @@ __global__ void __launch_bounds__(kRowsThreads) product_rows(const Product a, co
 // every 512 cycles of matrix instructions, 13 TB/s over the GPU out of L2; a pair of
 // SMs on one tile would halve half of that.  Few rows: by the weights' way through one
 // SM's copies (64 GB/s) where there are fewer tiles than SMs.
-constexpr int kMmaThreads = 256;
+constexpr int kMmaThreads = 384;            // four warps that feed, eight that store
 constexpr unsigned kSpan = 128;            // bytes of inner size that one swizzled copy covers
 constexpr unsigned kTileM = 128;           // channels of a tile
 
@@ -458,7 +458,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
     }
     for (int s = 0; s < 2; ++s) {
       barrier_init(summed + s, 1);
-      barrier_init(drained + s, 4);
+      barrier_init(drained + s, 8);
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&weights) : "memory");
@@ -538,26 +538,31 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
     bool ok = true;
     while (ok && walk.next()) {
       const Tile tile = walk.tile;
-      const unsigned l = (warp - 4) * 32 + lane, n = walk.channel_tile * kTileM + l;
+      // a quarter of the channels, and every second 32 of the rows
+      const unsigned quarter = warp % 4, odd = (warp - 4) / 4 * 32;
+      const unsigned n = walk.channel_tile * kTileM + quarter * 32 + lane;
       const uint64_t c = (uint64_t)tile.expert * a.channels + n;
       const bool in = n < a.channels;
       const float ws = in ? a.weight_scale[c] : 0.f, b = in && a.bias ? a.bias[c] : 0.f;
-      float mine = lane < tile.rows ? a.scale[tile.row + lane] : 0.f;      // of the first 32 rows
+      float mine = odd + lane < tile.rows ? a.scale[tile.row + odd + lane] : 0.f;      // of the first 32 rows
       ok = warp_wait(shared_at(summed) + half * 8, turn);
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      T* const out = static_cast<T*>(a.out) + (uint64_t)tile.row * a.channels + n;
-      const unsigned from = base + half * BN + ((warp - 4) * 32 << 16);
+      T* out = static_cast<T*>(a.out) + (uint64_t)(tile.row + odd) * a.channels + n;
+      const unsigned from = base + half * BN + (quarter * 32 << 16);
 #pragma unroll 1
-      for (unsigned r0 = 0; r0 < tile.rows; r0 += 32) {
+      for (unsigned r0 = odd; r0 < tile.rows; r0 += 64) {
         int v[32];
         tensor_load(from + r0, v);
-        const float next = r0 + 32 + lane < tile.rows ? a.scale[tile.row + r0 + 32 + lane] : 0.f;
+        const float next = r0 + 64 + lane < tile.rows ? a.scale[tile.row + r0 + 64 + lane] : 0.f;
+        const unsigned rows_left = in ? tile.rows - r0 : 0;
 #pragma unroll
         for (unsigned j = 0; j < 32; ++j) {
           const float s = __shfl_sync(~0u, mine, j);
           const float value = ok ? fmaf((float)v[j], s * ws, b) : NAN;
-          if (in && r0 + j < tile.rows) out[(uint64_t)(r0 + j) * a.channels] = from_float<T>(value);
+          if (j < rows_left) *out = from_float<T>(value);
+          out += a.channels;
         }
+        out += (uint64_t)32 * a.channels;
         mine = next;
       }
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");

@@ -74,7 +74,7 @@ def test_types_with_bias(dtype):
 
 @gpu
 @pytest.mark.parametrize("sizes", [[0, 0, 7], [1, 0, 2, 0], [130, 0, 1, 64, 300, 0, 17, 128], [0, 0, 0], [3] * 40, [257, 511],
-                                   [1] * 100 + [900]])
+                                   [1] * 100 + [900], [5] * 300 + [0] * 20 + [70], [0] * 299 + [400]])
 def test_ragged_groups(sizes):
     check(sizes, 136, 200, bias=True)
     check(sizes, 64, 64, BF16)
