@@ -284,11 +284,11 @@ __global__ void __launch_bounds__(kRowsThreads) product_rows(const Product a, co
 // tcgen05.mma (kind::i8, 32-bit sums in tensor memory), warps 4..11 scale, round and
 // store the tile before while the next is being summed (two halves of tensor memory).
 //
-// What bounds it: a large product (8189 x 8192 x 4096: 243 us, 2.26e15 operations a
-// second, the tensor pipe busy 53 % of the time) by what the SMs bring in, 48 KB for
-// every 512 cycles of matrix instructions, 13 TB/s over the GPU out of L2; a pair of
-// SMs on one tile would halve half of that.  Few rows: by the weights' way through one
-// SM's copies (64 GB/s) where there are fewer tiles than SMs.
+// What bounds it: a large product (8189 x 8192 x 4096: 179 us, 3.07e15 operations a
+// second) by the hand-over of its stages and by what the SMs bring in, 48 KB for every
+// 512 cycles of matrix instructions, 18 TB/s over the GPU out of L2; a pair of SMs on one
+// tile would take a third off that.  Four warps storing instead of eight took 225 us:
+// the next tile but one waited for them.
 constexpr int kMmaThreads = 384;            // four warps that feed, eight that store
 constexpr unsigned kSpan = 128;            // bytes of inner size that one swizzled copy covers
 constexpr unsigned kTileM = 128;           // channels of a tile
@@ -640,18 +640,21 @@ uint64_t tile_bound(const Product& a, unsigned tile_rows) {
 // Which kernel a product takes, and its tile's rows: 0 for product_rows.  The host does
 // not know the groups, so it goes by the rows of an expert on average.
 //
-// A block takes its tiles in rounds, and a stage takes much the same time whatever the
-// tile's rows (0.42 us at 32 and 64, 0.45 at 128, 0.52 at 256, from 24, 200, 1531 and
-// 8189 rows), so the tile is the one whose rounds of a B200's 148 SMs cost least, the
-// smaller of equals: 200 rows x 4096 channels make 32 tiles of 256 rows or 128 of 64.
+// A block takes its tiles in rounds, and 128 bytes of inner size take a tile 0.23, 0.35
+// or 0.44 us at 64, 128 or 256 rows (from 500 and 2000 rows x 4096 x 4096; tiles of 32
+// rows took 0.24), so the tile is the one whose rounds of a B200's 148 SMs cost least,
+// the smaller of equals: 500 rows take 17.5 us by 64, 14.2 by 128 and 17.8 by 256; 2000 rows 48.6 by 64
+// and 30.4 by 256.  A group's last tile is half empty on average.
 unsigned tile_rows_of(uint64_t rows, uint64_t experts, uint64_t channels) {
   const uint64_t each = ceil_div(rows, experts);
   if (rows <= 8 || each <= 2) return 0;
-  static const struct { unsigned rows; uint64_t cost; } shapes[] = {{32, 42}, {64, 42}, {128, 45}, {256, 52}};
+  const uint64_t groups = experts < rows ? experts : rows;
+  static const struct { unsigned rows; uint64_t cost; } shapes[] = {{64, 23}, {128, 35}, {256, 44}};
   unsigned best = 0;
   uint64_t least = ~0ull;
   for (const auto& s : shapes) {
-    const uint64_t tiles = ceil_div(each, s.rows) * (experts < rows ? experts : rows) * ceil_div(channels, kTileM);
+    const uint64_t row_tiles = experts == 1 ? ceil_div(rows, s.rows) : ceil_div(2 * rows + groups * s.rows, 2 * s.rows);
+    const uint64_t tiles = row_tiles * ceil_div(channels, kTileM);
     const uint64_t cost = ceil_div(tiles, 148) * s.cost;
     if (cost < least) {
       least = cost;
@@ -687,8 +690,7 @@ void product_by_tiles(int type, const Product& a, int device, cudaStream_t strea
   switch (tile_rows_of(a.rows, a.experts, a.channels)) {
     case 256: return tiles<256>(type, a, device, stream);
     case 128: return tiles<128>(type, a, device, stream);
-    case 64: return tiles<64>(type, a, device, stream);
-    default: return tiles<32>(type, a, device, stream);
+    default: return tiles<64>(type, a, device, stream);
   }
 }
 
