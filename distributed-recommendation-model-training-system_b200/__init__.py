@@ -14,6 +14,7 @@ Host (numpy) and device (torch CUDA tensor) inputs are both accepted; the
 library itself runs only the hand-written sm_100a kernels.  There is no CPU
 fallback: importing this package fails loudly if the native library is missing,
 and every call fails with the library's own error when no GPU is present.
+The operators of the dense model on top of the pooled rows are in ``dense``.
 Errors raise ``EpsError`` whose ``code`` is eps::Error::Code + 1
 (include/eps/types.hpp:17-25).
 """

@@ -49,8 +49,9 @@ __device__ __forceinline__ const T* source_row(const Quantize& a, uint64_t r, bo
 }
 
 // A block a row.  Rows of up to NIT packs of 16 bytes a thread stay in registers
-// between the search for the largest magnitude and the rounding (one pass over
-// memory, which is what bounds it); NIT == 0 reads a row of any kind twice.
+// between the search for the largest magnitude and the rounding: one pass over memory,
+// which is what bounds it (8189 x 4096 bf16: 19 us, 5.3 TB/s; 33 when rows were read
+// twice).  NIT == 0 reads a row of any kind twice.
 constexpr unsigned kQuantizeThreads = 128;
 template <class T, int NIT>
 __global__ void __launch_bounds__(kQuantizeThreads) quantize_rows(const Quantize a) {
@@ -168,7 +169,9 @@ __device__ __forceinline__ Tile locate(const Product& a, unsigned tile_rows, uns
 // Few rows: the weights' bytes are all there is.  A warp has a channel, asks for its
 // first weights, and while they come the block quantizes its RT rows into shared
 // memory for all its warps (every block does that again: the rows are a few kilobytes
-// in L2, and a launch before this one would take longer).
+// in L2, and a launch before this one would take longer).  1 x 4096 x 4096 takes 8.9 us,
+// 13 with a launch of its own to quantize, against a floor of 2.6: what is left is the
+// wait for the row before anything can be summed.
 constexpr unsigned kRowsThreads = 512, kRowsAhead = 8;
 template <class T, int RT, bool QUANTIZE>
 __global__ void __launch_bounds__(kRowsThreads) product_rows(const Product a, const Quantize z, unsigned channel_blocks) {

@@ -16,6 +16,9 @@
 // key and the lowest lane that holds it owns the lowest index.  What bounds it is the
 // number of instructions a token takes (the logits of a batch are a few megabytes):
 // every lane sorts its own few keys once, and then only offers the best it has left.
+// Measured at 32771 x 256 floats, top 8 of the best 4 of 8 groups: 44 us (850
+// instructions a token; 132 with the best key searched anew each time and groups scored
+// lane by lane), 6 to scan the tiles and 5 to place; the gradient at 32771 x 96 bf16 19.
 //
 // The sort by expert is a counting sort in three steps.  A tile is the tokens of one
 // block; each of its warps counts its own run of consecutive tokens, whose experts

@@ -153,6 +153,24 @@ def test_quantize_rows():
 
 
 @gpu
+@pytest.mark.parametrize("n", [0, 3, 60, 400])
+def test_product_of_quantized_rows(n):
+    """eps_b200_int8_product on rows that were quantized before gives what the one call gives."""
+    import ctypes as C
+    import eps_b200
+    layer = dense.QuantizedExperts.from_weights(torch.randn(2, 200, 144, generator=gen(20), device="cuda"))
+    x = torch.randn(n, 144, generator=gen(21), device="cuda")
+    off = offsets_of([n // 3, n - n // 3])
+    q, s = dense.quantize_rows(x)
+    out = torch.empty(n, 200, device="cuda")
+    args = bytes(dense.Int8Product(device=0, type=0, experts=2, channels=200, inner=144, rows_divisor=1, rows=n, weight=layer.weight.data_ptr(),
+                                   weight_scale=layer.scale.data_ptr(), offsets=off.data_ptr(), out=out.data_ptr()))
+    st = eps_b200.Status()
+    assert dense._lib.eps_b200_int8_product(args, q.data_ptr(), s.data_ptr(), torch.cuda.current_stream().cuda_stream, C.byref(st)) == 0, st.message
+    assert torch.equal(out, layer.product(x, offsets=off))
+
+
+@gpu
 def test_a_bad_row_stays_alone():
     for n in (6, 300):
         x = torch.randn(n, 96, generator=gen(10), device="cuda")
