@@ -305,7 +305,7 @@ struct Source {
       for (int i = 0; i < NIT; ++i) {
         const unsigned c = (i * n.width + lane) * V;
         Pack<T, V> x{};
-        if (live && there && c < n.columns) x = load_once<T, V>(reinterpret_cast<const T*>(p) + c);
+        if (live && there && c < n.columns) x = load_pack<T, V>(reinterpret_cast<const T*>(p) + c);      // read again: kept in L1
         widen(x, r[i]);
       }
     }
@@ -504,12 +504,13 @@ __global__ void __launch_bounds__(512) block_norm_forward(const Norm n) {
 
 // The column sums of a lane stay in registers where a lane has few columns, else in
 // shared memory (each lane its own columns: no conflict, no atomic).  They leave a
-// block once; block_norm_columns adds the blocks up in order.
+// block once; block_norm_columns adds the blocks up in order.  Single elements are read
+// as needed, so a second block an SM hides their latency (572 -> 284 us at 27148 x 1207).
 template <class TX, class TY, int V, int NIT, int P, int GATE>
-__global__ void __launch_bounds__(512) block_norm_gradient(const Norm n) {
+__global__ void __launch_bounds__(512, V == 1 && NIT <= 4 ? 2 : 1) block_norm_gradient(const Norm n) {
   constexpr int N = V * NIT;
   constexpr Way kHow = kWay<V, NIT, P>;
-  constexpr bool kHeld = kHow != kDirect;
+  constexpr bool kHeld = N <= 8;
   using Given = Parameters<TY, V, NIT, kHeld, false>;
   extern __shared__ __align__(16) char room[];      // the staged parameters, then the ring; in the end the sums
   float* const sums = reinterpret_cast<float*>(room);      // [wanted][N][blockDim.x]
@@ -524,12 +525,12 @@ __global__ void __launch_bounds__(512) block_norm_gradient(const Norm n) {
   const unsigned cell = N * blockDim.x;
   const unsigned wanted = __popc(n.want);
   auto slot_of = [&](int k) { return __popc(n.want & ((1 << k) - 1)); };      // of a wanted sum
-  float held[kHeld ? kSums : 1][V];
+  float held[kHeld ? kSums : 1][kHeld ? NIT : 1][V];
   if constexpr (kHeld) {
 #pragma unroll
     for (int k = 0; k < kSums; ++k)
 #pragma unroll
-      for (int j = 0; j < V; ++j) held[k][j] = 0.f;
+      for (int j = 0; j < N; ++j) held[k][j / V][j % V] = 0.f;
   } else {
     for (unsigned i = threadIdx.x; i < wanted * cell; i += blockDim.x) sums[i] = 0.f;
     __syncthreads();
@@ -537,8 +538,8 @@ __global__ void __launch_bounds__(512) block_norm_gradient(const Norm n) {
   // column sums k of the lane's pack i grow by a * b, or by a
   auto add = [&](int k, int i, const auto& a, const auto& b) {
     if constexpr (kHeld) {
-      if constexpr (std::is_same_v<std::decay_t<decltype(b)>, float>) vadd<V>(held[k], held[k], a);
-      else vfma<V>(held[k], a, b, held[k]);
+      if constexpr (std::is_same_v<std::decay_t<decltype(b)>, float>) vadd<V>(held[k][i], held[k][i], a);
+      else vfma<V>(held[k][i], a, b, held[k][i]);
     } else if (n.want >> k & 1) {
 #pragma unroll
       for (int j = 0; j < V; ++j) {
@@ -743,7 +744,7 @@ __global__ void __launch_bounds__(512) block_norm_gradient(const Norm n) {
     for (int k = 0; k < kSums; ++k)
       if (n.want >> k & 1) {
 #pragma unroll
-        for (int j = 0; j < V; ++j) sums[slot_of(k) * cell + j * blockDim.x + threadIdx.x] = held[k][j];
+        for (int j = 0; j < N; ++j) sums[slot_of(k) * cell + j * blockDim.x + threadIdx.x] = held[k][j / V][j % V];
       }
   }
   __syncthreads();
@@ -795,12 +796,14 @@ constexpr int kWide = std::is_same_v<TY, float> ? 4 : 8;
 
 // A lane holds one wide pack where that fits 512 lanes (and, for a float residual
 // of a 16-bit block, the shared memory of 256), else up to sixteen elements; without
-// 16-byte alignment four or sixteen single ones.
+// 16-byte alignment four single ones up to 2048 columns, where the column sums still
+// fit registers and two blocks an SM (27148 x 1207 bfloat16, backward: 284 us, against
+// 663 with sixteen a lane and the sums in shared memory), and sixteen beyond.
 Spread spread_of(unsigned columns, int residual, int type, bool wide) {
   Spread s{};
   s.v = !wide ? 1 : type == EPS_B200_F32 ? 4 : 8;
   const unsigned packs = (unsigned)ceil_div(columns, s.v);
-  if (!wide) s.nit = packs <= 32 ? 1 : packs <= 1024 ? 4 : 16;
+  if (!wide) s.nit = packs <= 32 ? 1 : packs <= 2048 ? 4 : 16;
   else s.nit = packs <= (residual != type ? 256 : 512) ? 1 : packs <= 1024 ? 2 : 4;
   const unsigned lanes = (unsigned)ceil_div(packs, s.nit);
   if (lanes <= 32) {
@@ -839,7 +842,7 @@ unsigned backward(const Norm& n, const Spread& s, int device, uint64_t space, cu
   constexpr auto kKernel = block_norm_gradient<TX, TY, V, NIT, P, GATE>;
   constexpr bool kRing = kWay<V, NIT, P> != kDirect;
   const unsigned held = (unsigned)__builtin_popcount((unsigned)n.want) * NIT * V * 4;
-  const unsigned walked = kRing ? Parameters<TY, V, NIT, true, false>::kRecord + kSlots * backward_bytes<TX, TY, V>() : 0;
+  const unsigned walked = Parameters<TY, V, NIT, V * NIT <= 8, false>::kRecord + (kRing ? kSlots * backward_bytes<TX, TY, V>() : 0);
   const unsigned shared = (walked > held ? walked : held) * s.threads;       // the sums take the others' place in the end
   const unsigned blocks = resident<kKernel>(device, s, shared, n.rows, kMostBlocks);
   need(!n.want || space >= (uint64_t)blocks * kSums * n.columns * 4, "block norm workspace too small");
@@ -870,7 +873,8 @@ void by_spread(const Spread& s, F f) {
   } else {
     if (s.nit == 1) f(Int<1>{}, Int<1>{}, Int<1>{});
     else if (s.nit == 16) f(Int<1>{}, Int<16>{}, Int<16>{});
-    else warps <= 1 ? f(Int<1>{}, Int<4>{}, Int<1>{}) : f(Int<1>{}, Int<4>{}, Int<8>{});
+    else if (warps <= 1) f(Int<1>{}, Int<4>{}, Int<1>{});
+    else warps <= 8 ? f(Int<1>{}, Int<4>{}, Int<8>{}) : f(Int<1>{}, Int<4>{}, Int<16>{});
   }
 }
 
