@@ -30,7 +30,8 @@ parity : one round from freshly initialised tables checked against the
          rows with <= 64 occurrences bit-exact, longer rows within 1e-6 of their
          sum of |terms|; at N = 1 also the bit-exact mode
          (EPS_B200_FLAG_REFERENCE_ORDER), every row bit-exact.  Runs after all
-         timing, never inside a timed region.
+         timing, never inside a timed region; "unavailable" where that build is
+         missing.
 cpu_baseline / --impl reference: the UNMODIFIED reference CPU parameter server
          (oracle/_ref, compiled from its own sources) with one shard per host
          core behind its DistributedClient, timed wall-clock on the same job.
@@ -1018,8 +1019,11 @@ def run_b200(args):
         del flush
 
     # ---- parity: one round from fresh tables against the reference (checker only)
+    from oracle_lib import reference_available
     parity = None
-    if not args.no_check:
+    if not args.no_check and not reference_available():
+        parity = {"unavailable": "reference CPU build oracle/_ref/libeps_ref.so is missing"}
+    elif not args.no_check:
         reports = parity_check(eps, torch, wl, args, parts, rank, world, dev, comms,
                                bitexact=not args.no_bitexact)
         ok = all(r["parity"] for r in reports)
