@@ -3,6 +3,7 @@
 //
 // Mathematics: s = softmax(l) or 1 / (1 + exp(-l)); key = s + bias; the best groups
 // by the sum of their two best keys; the k best keys in them; w = s / sum(s) * scale.
+// A masked expert (l = -inf) has the lowest key there is: its bias does not bring it back.
 // Backward, over the chosen c with d = dw * scale:
 //   ds_c = (d_c - sum_j d_j s_j / S) / S   (renormalised, S = sum_j s_j; else d_c)
 //   softmax: dl_e = s_e (ds_e - sum_c ds_c s_c),   sigmoid: dl_e = ds_e s_e (1 - s_e)
@@ -303,10 +304,22 @@ __global__ void __launch_bounds__(kWarps * 32, EPL <= 8 ? 4 : EPL == 16 ? 2 : 1)
 #pragma unroll
     for (int i = 0; i < EPL; ++i) p[i] = next[i];
     if (token + 1 < end) load_logits<T, EPL>(a, logits + (token + 1) * a.stride, lane, next);
+    float lowest = p[0];
+#pragma unroll
+    for (int i = 1; i < EPL; ++i) lowest = fminf(lowest, p[i]);
+    unsigned masked = 0;                // bit i: the lane's expert i is masked
+    if (lowest == -INFINITY) {
+#pragma unroll
+      for (int i = 0; i < EPL; ++i) masked |= (unsigned)(p[i] == -INFINITY) << i;
+    }
     score<EPL, true>(a, p);
     unsigned key[EPL];
 #pragma unroll
     for (int i = 0; i < EPL; ++i) key[i] = image(__fadd_rn(p[i], bias[i]));
+    if (masked) {
+#pragma unroll
+      for (int i = 0; i < EPL; ++i) key[i] = masked >> i & 1 ? image(-INFINITY) : key[i];
+    }
     if (grouped) keep_groups<EPL>(a, key, lane, s);
 
     // by key, and the lower index of equal keys first

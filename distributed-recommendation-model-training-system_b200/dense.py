@@ -381,8 +381,8 @@ def route(logits, top_k: int, *, score: str = "softmax", bias=None, groups: int 
     the top_groups best of `groups` equal runs are eligible, a group counting the sum
     of its two best keys.  Weights are the chosen scores, divided by their sum if
     `renormalise`, times `scale`.  Equal keys go to the lower index; a masked logit
-    is -inf.  At most 1024 experts and top_k 32.  With `sort`, the entries sorted
-    by expert come too."""
+    is -inf, and ranks last whatever its bias.  At most 1024 experts and top_k 32.
+    With `sort`, the entries sorted by expert come too."""
     logits, stride, tokens, experts = _matrix(logits, "logits")
     top_groups = groups if top_groups is None else top_groups
     if top_k <= 0 or groups <= 0 or top_groups <= 0:

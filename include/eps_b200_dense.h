@@ -91,13 +91,15 @@ EPS_B200_EXPORT int eps_b200_block_norm_backward(const EpsB200BlockNorm* args,
 
 /* ---- Routing of tokens to experts.
  *   s = softmax(logits) or sigmoid(logits)      a row of -inf alone has s = 0
- *   key = s + bias[e]                           the bias ranks, it does not weigh
+ *   key = s + bias[e]                           the bias ranks, it does not weigh;
+ *                                               the lowest where the logit is -inf
  *   the `top_groups` best of `groups` equal runs of experts, by the sum of their
  *   two best keys (their only key in groups of one expert);
  *   the `top_k` best keys of those groups, best first;
  *   weight = s (divided by their sum if `renormalise`; 0 if that is 0) * scale.
- * Equal keys and equal groups go to the lower index.  A key that is NaN or -inf
- * ranks as the lowest finite value; a NaN score stays NaN in its weight.
+ * Equal keys and equal groups go to the lower index.  A key that is NaN or -inf, and
+ * that of a masked expert (logit -inf) whatever its bias, ranks as the lowest finite
+ * value; a NaN score stays NaN in its weight.
  *
  * With `order` given, the entries (token * top_k + slot) sorted by expert, equal
  * experts in entry order, their inverse `position`, and offsets[e] .. offsets[e + 1],
