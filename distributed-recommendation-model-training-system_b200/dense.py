@@ -9,7 +9,7 @@
 Every tensor is a torch CUDA tensor; work goes to torch's current stream of the
 tensors' device and is asynchronous, results and workspaces come from torch's
 allocator, and nothing is kept between calls but what the two classes hold.  Calls
-can be captured in a CUDA graph.  There is no CPU fallback; a refused call raises
+can be captured in a CUDA graph; a captured AdamW step counts its replays.  There is no CPU fallback; a refused call raises
 ``EpsError`` with ``code`` INVALID_ARGUMENT before anything is launched.
 
 Leading axes of a tensor count as rows; the last axis must be contiguous, rows may
@@ -18,6 +18,7 @@ have any stride.  Element types are float32, bfloat16 and float16.
 from __future__ import annotations
 
 import ctypes as C
+import math
 import struct
 import threading
 from typing import NamedTuple, Sequence
@@ -34,7 +35,7 @@ ENTRY_POINTS = ("eps_b200_block_norm", "eps_b200_block_norm_workspace",
                 "eps_b200_route_experts", "eps_b200_route_experts_backward",
                 "eps_b200_int8_stride", "eps_b200_int8_quantize",
                 "eps_b200_int8_product_workspace", "eps_b200_int8_product", "eps_b200_int8_linear",
-                "eps_b200_adamw_plan_bytes", "eps_b200_adamw_plan", "eps_b200_adamw")
+                "eps_b200_adamw_plan_bytes", "eps_b200_adamw_plan", "eps_b200_adamw", "eps_b200_adamw_counted")
 
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _KINDS = {"rms": 0, "layer": 1}
@@ -95,6 +96,11 @@ class AdamWArgs(C.Structure):
                 ("weight_decay", C.c_double), ("step", C.c_uint64), ("seed", C.c_uint64)]
 
 
+class AdamWClock(C.Structure):
+    _fields_ = [("taken", C.c_int64), ("learning_rate", C.c_double), ("decay", C.c_float), ("rate", C.c_float),
+                ("inverse_root", C.c_float), ("key", C.c_uint32)]
+
+
 def _bind():
     # the structs that are packed for each call go in as bytes of the same layout
     lib, P, vp, i64, u64, u32, i32 = (load_library(), C.POINTER, C.c_void_p, C.c_int64, C.c_uint64,
@@ -114,6 +120,7 @@ def _bind():
     lib.eps_b200_adamw_plan_bytes.argtypes = [P(AdamWTensor), u64]
     lib.eps_b200_adamw_plan.argtypes = [P(AdamWTensor), u64, vp, u64, P(u64), st]
     lib.eps_b200_adamw.argtypes = [P(AdamWArgs), vp, u64, u64, vp, st]
+    lib.eps_b200_adamw_counted.argtypes = [P(AdamWArgs), vp, u64, u64, vp, vp, st]
     for name in ENTRY_POINTS:
         sized = name.endswith(("_workspace", "_bytes", "_stride"))
         getattr(lib, name).restype = u64 if sized else C.c_int
@@ -154,6 +161,14 @@ def _choice(table, value, what):
 # for few and cheap steps: device indices instead of device objects, the stream's raw
 # handle, and argument structs packed in one go.
 _stream = torch._C._cuda_getCurrentRawStream      # of a device index
+
+
+def _capturing(device):
+    """Whether the current stream of a device index is being captured in a graph."""
+    if torch._C._cuda_getDevice() != device:
+        with torch.cuda.device(device):
+            return torch._C._cuda_isCurrentStreamCapturing()
+    return torch._C._cuda_isCurrentStreamCapturing()
 
 
 def _tensor(t, what, device=None):
@@ -540,7 +555,13 @@ class AdamW:
 
     The moments lie one tensor after the other in `first` and `second` (and `master`),
     tensor i from element starts[i] on; `first_scale` and `second_scale` hold the
-    scales of 8-bit moments."""
+    scales of 8-bit moments.
+
+    A step that is captured in a CUDA graph counts itself: each replay is a step of its
+    own.  From the first capture on, the number of steps is held on the GPU (`steps`
+    waits for the current stream to read it), and learning_rate is set in the order of
+    the current stream.  Gradients are bound before a capture; a captured step keeps
+    those it reads alive, and the optimizer has to outlive the graph."""
 
     def __init__(self, parameters: Sequence[torch.Tensor], gradients: Sequence[torch.Tensor] | None = None, *,
                  learning_rate: float = 1e-3, beta1: float = 0.9, beta2: float = 0.999,
@@ -561,7 +582,7 @@ class AdamW:
             _refuse("moments have 32 or 8 bits")
         if master and head.dtype == torch.float32:
             _refuse("float32 parameters take no master copy")
-        self.device, self.state_bits, self.steps = head.device, state_bits, 0
+        self.device, self.state_bits, self._steps = head.device, state_bits, 0
         self.starts, total = [], 0
         for p in self.parameters:
             self.starts.append(total)
@@ -580,9 +601,24 @@ class AdamW:
         self._args = AdamWArgs(self.device.index, _TYPES[head.dtype], 0, state_bits, ptr(self.master),
                                ptr(self.first), ptr(self.second), ptr(self.first_scale), ptr(self.second_scale),
                                None, None, learning_rate, beta1, beta2, epsilon, weight_decay, 0, seed)
+        # an AdamWClock: no step taken, no rate of its own; used from the first captured step on
+        self._clock = torch.tensor(list(struct.unpack("@4q", bytes(AdamWClock(0, -1.0)))), device=self.device)
+        self._counted, self._kept = False, []
         self._bound = None
         if gradients is not None:
             self.bind(gradients)
+
+    @property
+    def steps(self) -> int:
+        """The number of steps taken."""
+        return self._steps + (int(self._clock[0].item()) if self._counted else 0)
+
+    @steps.setter
+    def steps(self, value: int):
+        if self._counted:
+            self._clock[0] = value - self._steps     # graphs hold the sum's other part
+        else:
+            self._steps = value
 
     @property
     def learning_rate(self) -> float:
@@ -590,6 +626,10 @@ class AdamW:
 
     @learning_rate.setter
     def learning_rate(self, value: float):
+        if self._counted:
+            if not 0 <= value < math.inf:
+                _refuse("invalid learning rate")
+            self._clock[1:2].view(torch.float64).fill_(value)
         self._args.learning_rate = value
 
     def bind(self, gradients: Sequence[torch.Tensor]):
@@ -598,6 +638,8 @@ class AdamW:
         gradients = list(gradients)
         if len(gradients) != len(self.parameters):
             _refuse("a gradient for each parameter")
+        if _capturing(self.device.index):
+            _refuse("gradients are bound before a capture")
         dtype = gradients[0].dtype if isinstance(gradients[0], torch.Tensor) else None
         if dtype not in (self.parameters[0].dtype, torch.float32):
             _refuse("gradients have the parameters' type or float32")
@@ -627,11 +669,19 @@ class AdamW:
         a = self._args
         a.gradient_type = gtype
         device = self.device.index
+        capturing = _capturing(device)
         a.gradient_scale = _vector(gradient_scale, "gradient_scale", device, 1, torch.float32)
         a.skip = _vector(skip, "skip", device, 1, torch.int32)
-        a.step = self.steps + 1
-        _call(_lib.eps_b200_adamw, C.byref(a), plan.data_ptr(), len(self.parameters), blocks, _stream(device))
-        self.steps += 1
+        a.step = self._steps + 1
+        if capturing or self._counted:
+            _call(_lib.eps_b200_adamw_counted, C.byref(a), plan.data_ptr(), len(self.parameters), blocks,
+                  self._clock.data_ptr(), _stream(device))
+            self._counted = True
+            if capturing and not any(kept is self._bound for kept in self._kept):
+                self._kept.append(self._bound)
+        else:
+            _call(_lib.eps_b200_adamw, C.byref(a), plan.data_ptr(), len(self.parameters), blocks, _stream(device))
+            self._steps += 1
 
     def state(self) -> dict:
         """What load_state takes, by reference."""

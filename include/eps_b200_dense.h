@@ -15,7 +15,8 @@
  *    and workspaces are the caller's, and may be reused once the stream has
  *    passed the call;
  *  - `stream` is a cudaStream_t (NULL = the legacy default stream).  Calls are
- *    asynchronous, keep nothing between calls, and can be captured in a graph;
+ *    asynchronous, keep nothing between calls, and can be captured in a graph (an
+ *    AdamW step as eps_b200_adamw_counted);
  *  - an element type is EPS_B200_F32, _BF16 or _F16.  Sums, statistics and
  *    scores are held in 32 bits or more whatever the type;
  *  - the last axis of every tensor is contiguous; a row stride is given in
@@ -233,6 +234,23 @@ EPS_B200_EXPORT int eps_b200_adamw_plan(const EpsB200AdamWTensor* tensors, uint6
                                         EpsB200Status* status);
 EPS_B200_EXPORT int eps_b200_adamw(const EpsB200AdamW* args, const void* plan, uint64_t count,
                                    uint64_t blocks, void* stream, EpsB200Status* status);
+
+/* The step for a captured graph.  eps_b200_adamw takes its number by value, and with it
+ * the bias corrections, the learning rate and the random bits: every replay would be the
+ * same step again.  This one reads them from `clock`, in device memory of the caller's
+ * that lives between the calls: the step's number is args->step + taken, and each call or
+ * replay adds 1 to taken (a skipped step too).  A learning_rate of 0 or more there takes
+ * the place of args->learning_rate; below 0 the latter holds.  The other members are
+ * written by the call. */
+typedef struct {
+  int64_t taken;
+  double learning_rate;
+  float decay, rate, inverse_root;
+  uint32_t key;
+} EpsB200AdamWClock;
+EPS_B200_EXPORT int eps_b200_adamw_counted(const EpsB200AdamW* args, const void* plan, uint64_t count,
+                                           uint64_t blocks, EpsB200AdamWClock* clock, void* stream,
+                                           EpsB200Status* status);
 
 #ifdef __cplusplus
 }
