@@ -187,9 +187,9 @@ EPS_B200_EXPORT int eps_b200_int8_linear(const EpsB200Int8Product* args, const v
  *   g = gradient * *gradient_scale              (1 if NULL)
  *   m = beta1 m + (1 - beta1) g,   v = beta2 v + (1 - beta2) g^2
  *   p = p (1 - lr * weight_decay) - lr / (1 - beta1^step) * m / (sqrt(v / (1 - beta2^step)) + epsilon)
- * all in 32 bits.  A step whose *skip is nonzero changes nothing.  Unlike the
- * store's LazyAdam, epsilon is added after the bias correction and every element
- * moves at every step.
+ * all in 32 bits; an epsilon below the smallest normal float counts as that.  A step
+ * whose *skip is nonzero changes nothing.  Unlike the store's LazyAdam, epsilon is
+ * added after the bias correction and every element moves at every step.
  *
  * The moments of all tensors lie in one buffer each, tensor i from element
  * state_begin[i], a multiple of EPS_B200_ADAMW_BLOCK.  state_bits == 32: float.
