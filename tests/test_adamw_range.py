@@ -1,4 +1,5 @@
-"""AdamW at the ends of its range: moments below float32's normal numbers and the smallest epsilons."""
+"""AdamW at the ends of its range: moments below float32's normal numbers, the smallest epsilons, and
+tensors without elements."""
 import pytest
 import torch
 
@@ -35,3 +36,12 @@ def test_no_gradient_under_the_smallest_epsilons(bits, epsilon):
     p, g = torch.ones(300, device="cuda"), torch.zeros(300, device="cuda")
     dense.AdamW([p], [g], state_bits=bits, epsilon=epsilon, weight_decay=0.0).step()
     assert bool((p == 1).all())
+
+
+@gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_nothing_to_update(bits):
+    p = [torch.empty(0, device="cuda"), torch.empty(0, 4, device="cuda")]
+    opt = dense.AdamW(p, [torch.empty_like(t) for t in p], state_bits=bits)
+    opt.step()
+    assert opt.steps == 1
