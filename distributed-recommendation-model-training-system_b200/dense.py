@@ -218,6 +218,22 @@ def _ptr(t):
     return 0 if t is None else t.data_ptr()
 
 
+class _Streams:
+    """The streams on which tensors that the package holds are used.  torch's allocator hands
+    freed memory out again in the order of the stream that it was made on; it has to hear of
+    the others, or what is dropped here could be overwritten under a running kernel."""
+
+    def __init__(self, device, *tensors):
+        self.seen, self.tensors = {_stream(device)}, [t for t in tensors if t is not None]
+
+    def use(self, stream, device):
+        if stream not in self.seen:
+            current = torch.cuda.current_stream(device)
+            for t in self.tensors:
+                t.record_stream(current)
+            self.seen.add(stream)
+
+
 def _pack(fields, *values):
     try:
         return fields.pack(*values)
@@ -498,6 +514,7 @@ class QuantizedExperts:
         self.scale = scale.reshape(self.experts, self.channels)
         self.bias = None if bias is None else bias.reshape(self.experts, self.channels)
         self._index, self._fixed = self.device.index, (self.weight.data_ptr(), self.scale.data_ptr(), _ptr(self.bias))
+        self._streams = _Streams(self._index, self.weight, self.scale, self.bias)
 
     @classmethod
     def from_weights(cls, weight, bias=None):
@@ -518,7 +535,7 @@ class QuantizedExperts:
         made from x[rows[r] // rows_divisor] -- a Routing's `order` with rows_divisor
         = top_k; without it from x[r].  Rows in no expert's run are left unwritten."""
         device = self._index
-        flat, stride, x_rows, _ = _matrix(x, "x", device, self.inner)
+        flat, x_stride, x_rows, _ = _matrix(x, "x", device, self.inner)
         index = _row_index(rows, rows_divisor, device)
         n = x_rows if rows is None else rows.shape[0]
         if offsets is not None:
@@ -534,7 +551,9 @@ class QuantizedExperts:
         args = _pack(_INT8_PRODUCT, device, _TYPES[flat.dtype], self.experts, self.channels, self.inner, rows_divisor, n,
                      *self._fixed, _ptr(offsets), out.data_ptr(),
                      _ptr(workspace), space)
-        _call(_lib.eps_b200_int8_linear, args, flat.data_ptr(), stride, x_rows, index, _stream(device))
+        stream = _stream(device)
+        self._streams.use(stream, device)
+        _call(_lib.eps_b200_int8_linear, args, flat.data_ptr(), x_stride, x_rows, index, stream)
         return out
 
 
@@ -604,6 +623,7 @@ class AdamW:
         # an AdamWClock: no step taken, no rate of its own; used from the first captured step on
         self._clock = torch.tensor(list(struct.unpack("@4q", bytes(AdamWClock(0, -1.0)))), device=self.device)
         self._counted, self._kept = False, []
+        self._streams = _Streams(index, self.first, self.second, self.first_scale, self.second_scale, self.master, self._clock)
         self._bound = None
         if gradients is not None:
             self.bind(gradients)
@@ -654,7 +674,7 @@ class AdamW:
         blocks = C.c_uint64(0)
         _call(_lib.eps_b200_adamw_plan, tensors, len(gradients), host.data_ptr(), size, C.byref(blocks))
         plan = host.to(self.device)
-        self._bound = (gradients, plan, blocks.value, _TYPES[dtype])
+        self._bound = (gradients, plan, blocks.value, _TYPES[dtype], _Streams(self.device.index, plan, *gradients))
 
     def step(self, gradients: Sequence[torch.Tensor] | None = None, *, gradient_scale=None, skip=None):
         """One step.  gradient_scale: a float32 scalar on the GPU that multiplies
@@ -665,7 +685,7 @@ class AdamW:
             self.bind(gradients)
         if self._bound is None:
             _refuse("no gradients: give them to AdamW, bind or step")
-        _, plan, blocks, gtype = self._bound
+        _, plan, blocks, gtype, streams = self._bound
         a = self._args
         a.gradient_type = gtype
         device = self.device.index
@@ -673,14 +693,17 @@ class AdamW:
         a.gradient_scale = _vector(gradient_scale, "gradient_scale", device, 1, torch.float32)
         a.skip = _vector(skip, "skip", device, 1, torch.int32)
         a.step = self._steps + 1
+        stream = _stream(device)
+        streams.use(stream, device)
+        self._streams.use(stream, device)
         if capturing or self._counted:
             _call(_lib.eps_b200_adamw_counted, C.byref(a), plan.data_ptr(), len(self.parameters), blocks,
-                  self._clock.data_ptr(), _stream(device))
+                  self._clock.data_ptr(), stream)
             self._counted = True
             if capturing and not any(kept is self._bound for kept in self._kept):
                 self._kept.append(self._bound)
         else:
-            _call(_lib.eps_b200_adamw, C.byref(a), plan.data_ptr(), len(self.parameters), blocks, _stream(device))
+            _call(_lib.eps_b200_adamw, C.byref(a), plan.data_ptr(), len(self.parameters), blocks, stream)
             self._steps += 1
 
     def state(self) -> dict:
