@@ -821,7 +821,7 @@ constexpr unsigned kMostBlocks = 8 * 160;   // of the gradient: 8 an SM, 160 SMs
 // Blocks that fit the GPU at once, or fewer where the rows need fewer.
 template <auto Kernel>
 unsigned resident(int device, const Spread& s, size_t shared, uint64_t rows, unsigned most) {
-  room<Kernel>(device, shared);
+  room<Kernel>(device);
   uint64_t n = (uint64_t)sm_count(device) * blocks_each<Kernel>(device, s.threads, shared);
   if (n > most) n = most;
   const uint64_t all = ceil_div(rows, s.threads / s.width);

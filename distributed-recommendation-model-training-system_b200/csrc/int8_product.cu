@@ -682,7 +682,7 @@ void tiles(int type, const Product& a, int device, cudaStream_t stream) {
   const unsigned blocks = most > sms ? sms : (unsigned)most;
   by_type(type, [&](auto t) {
     constexpr auto kernel = product_tiles<decltype(t), BN>;
-    room<kernel>(device, Shape::shared);
+    room<kernel>(device);
     kernel<<<blocks, kMmaThreads, Shape::shared, stream>>>(a, w, q, channel_tiles);
   });
   check(cudaGetLastError(), "int8_product");
@@ -707,7 +707,7 @@ void rows_at_once(int type, const Product& a, const Quantize* z, int device, cud
     if (z) {
       constexpr auto kernel = product_rows<decltype(t), RT, true>;
       const unsigned shared = RT * a.padded;
-      room<kernel>(device, shared);
+      room<kernel>(device);
       kernel<<<(unsigned)most, kRowsThreads, shared, stream>>>(a, *z, channel_blocks);
     } else {
       product_rows<decltype(t), RT, false><<<(unsigned)most, kRowsThreads, 0, stream>>>(a, Quantize{}, channel_blocks);

@@ -649,7 +649,7 @@ int eps_b200_route_experts(const EpsB200RouteExperts* a, const float* bias, int3
         const bool spread = r.groups > 1 && r.top_groups < r.groups && !lanes_divide(r.per_group, decltype(epl)::value);
         const size_t shared = kWarps * scratch_bytes(r.experts, decltype(epl)::value, r.groups, spread) + r.experts * 4 + (order ? kTile * r.top_k * 2 : 0);
         constexpr auto kernel = route_tokens<decltype(t), decltype(epl)::value>;
-        room<kernel>(a->device, shared);
+        room<kernel>(a->device);
         kernel<<<r.tiles, kWarps * 32, shared, st>>>(r);
       });
     });
@@ -682,7 +682,7 @@ int eps_b200_route_experts_backward(const EpsB200RouteExperts* a, const int32_t*
       by_experts(r.experts, [&](auto epl) {
         constexpr auto kernel = route_gradient<decltype(t), decltype(epl)::value>;
         const size_t shared = kWarps * 32 * decltype(epl)::value * 4;
-        room<kernel>(a->device, shared);
+        room<kernel>(a->device);
         kernel<<<(unsigned)(all < most ? all : most), kWarps * 32, shared, static_cast<cudaStream_t>(stream)>>>(r);
       });
     });
