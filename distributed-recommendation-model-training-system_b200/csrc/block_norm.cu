@@ -997,8 +997,6 @@ int eps_b200_block_norm_backward(const EpsB200BlockNorm* a, const EpsB200BlockNo
     n.dh = d->dh; n.dhs = d->dh_stride;
     n.dz = d->dz; n.dzs = d->dz_stride;
     n.h = d->h; n.hs = d->h_stride;
-    n.somewhere = n.dz ? n.dz : n.dh ? n.dh : n.y ? n.y : d->dx ? d->dx : d->workspace;
-    n.somewhere = n.dz ? n.dz : n.dh ? n.dh : n.y ? n.y : d->dx;
     n.dx = d->dx; n.dxs = d->dx_stride;
     n.dy = d->dy; n.dys = d->dy_stride;
     n.dg = d->dgate; n.dgs = d->dgate_stride;
@@ -1012,6 +1010,8 @@ int eps_b200_block_norm_backward(const EpsB200BlockNorm* a, const EpsB200BlockNo
         if (o) check(cudaMemsetAsync(o, 0, n.columns * 4, st), "cudaMemsetAsync");
       return;
     }
+    need(!n.want || (d->workspace && aligned(d->workspace, 16)), "the workspace must be there and 16-byte aligned");
+    n.somewhere = n.dz ? n.dz : n.dh ? n.dh : n.y ? n.y : d->dx ? d->dx : n.want ? d->workspace : nullptr;
     if (!n.somewhere) return;       // nothing comes in and nothing is asked for
     bool wide = parameters_wide(n, a->type) && rows_wide(n.y, n.ys, a->type) && rows_wide(n.dh, n.dhs, a->residual_type) &&
                 rows_wide(n.dz, n.dzs, a->type) && rows_wide(n.h, n.hs, a->residual_type) &&
@@ -1019,7 +1019,6 @@ int eps_b200_block_norm_backward(const EpsB200BlockNorm* a, const EpsB200BlockNo
     if (n.gate == EPS_B200_GATE_ELEMENT) wide = wide && rows_wide(n.g, n.gs, a->type) && rows_wide(n.dg, n.dgs, a->type);
     const Spread s = spread_of(n.columns, a->residual_type, a->type, wide);
     n.width = s.width;
-    need(!n.want || (d->workspace && aligned(d->workspace, 16)), "the workspace must be there and 16-byte aligned");
     unsigned blocks = 0;
     n.partial = static_cast<float*>(d->workspace);
     by_type(a->residual_type, a->type, [&](auto tx, auto ty) {

@@ -1,0 +1,41 @@
+"""block_norm where tensors are not given: what is wanted is written all the same."""
+import ctypes as C
+
+import pytest
+import torch
+
+from conftest import import_package
+from test_block_norm import values
+
+eps = import_package()
+from eps_b200 import dense  # noqa: E402
+
+gpu = pytest.mark.gpu
+
+
+def backward(args, **gradients):
+    st = eps.Status()
+    given = {k: v.data_ptr() if torch.is_tensor(v) else v for k, v in gradients.items()}
+    rc = dense._lib.eps_b200_block_norm_backward(bytes(args), bytes(dense.BlockNormGradientArgs(**given)),
+                                                 torch.cuda.current_stream().cuda_stream, C.byref(st))
+    return rc, st.message
+
+
+@gpu
+@pytest.mark.parametrize("columns", [40, 33, 2048])
+@pytest.mark.parametrize("kind", [0, 1])
+def test_wanted_gradients_are_written_where_nothing_comes_in(columns, kind):
+    """Without dh and dz the gradients of the norm's weight and bias are zeros, whatever else is asked for."""
+    rows = 7
+    args = dense.BlockNorm(device=0, kind=kind, pre_norm=1, type=0, residual_type=0, parameter_type=0, columns=columns, rows=rows, epsilon=1e-5, scale=1.0)
+    h = values(1, rows, columns)
+    space = dense._lib.eps_b200_block_norm_workspace(rows, columns)
+    workspace = torch.empty(space, dtype=torch.uint8, device="cuda")
+    for more in ({}, {"h": h, "h_stride": columns}):
+        w, b = (torch.full((columns,), 7.0, device="cuda") for _ in range(2))
+        rc, message = backward(args, dpre_weight=w, dpre_bias=b, workspace=workspace, workspace_bytes=space, **more)
+        assert rc == 0, message
+        assert not w.any() and not b.any()
+    rc, _ = backward(args, dpre_weight=w)
+    assert rc == eps.INVALID_ARGUMENT              # sums need their workspace
+    assert backward(args)[0] == 0                  # nothing comes in and nothing is asked for
