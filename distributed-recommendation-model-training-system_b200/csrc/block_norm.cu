@@ -927,7 +927,10 @@ Norm checked(const EpsB200BlockNorm* a) {
   n.pre_w = a->pre_weight;
   n.pre_b = a->pre_bias;
   if (!n.post_norm) n.post_w = n.post_b = nullptr;
-  if (!n.y) n.post_b = nullptr;      // then the block adds nothing
+  if (!n.y) {      // then the block adds nothing: zeros, times what is finite
+    n.post_w = n.post_b = n.channel = nullptr;
+    n.scale = 1.f;
+  }
   return n;
 }
 
@@ -996,6 +999,7 @@ int eps_b200_block_norm_backward(const EpsB200BlockNorm* a, const EpsB200BlockNo
     need((!d->dpre_weight && !d->dpre_bias) || n.pre_norm, "gradients of a norm that is not there");
     n.dh = d->dh; n.dhs = d->dh_stride;
     n.dz = d->dz; n.dzs = d->dz_stride;
+    if (!n.dz) n.pre_w = nullptr;        // zeros come in that way, whatever the weight is
     n.h = d->h; n.hs = d->h_stride;
     n.dx = d->dx; n.dxs = d->dx_stride;
     n.dy = d->dy; n.dys = d->dy_stride;

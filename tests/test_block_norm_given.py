@@ -1,5 +1,7 @@
-"""block_norm where tensors are not given: what is wanted is written all the same."""
+"""block_norm where tensors are not given: what is wanted is written all the same, and what belongs to the
+missing tensors leaves no trace."""
 import ctypes as C
+import math
 
 import pytest
 import torch
@@ -39,3 +41,27 @@ def test_wanted_gradients_are_written_where_nothing_comes_in(columns, kind):
     rc, _ = backward(args, dpre_weight=w)
     assert rc == eps.INVALID_ARGUMENT              # sums need their workspace
     assert backward(args)[0] == 0                  # nothing comes in and nothing is asked for
+
+
+@gpu
+@pytest.mark.parametrize("columns", [48, 33, 1024])
+@pytest.mark.parametrize("kind", ["rms", "layer"])
+def test_what_belongs_to_missing_tensors_leaves_no_trace(columns, kind):
+    x, y, g = values(1, 5, columns), values(2, 5, columns), values(3, 5, columns)
+    bad = torch.ones(columns, device="cuda")
+    bad[3], bad[4] = math.inf, math.nan
+    # no block output: its scale and weights do not matter
+    want = dense.block_norm(x, kind=kind)
+    for more in (dict(scale=math.inf), dict(channel_scale=bad), dict(post_weight=bad, post_bias=bad), dict(activation="silu")):
+        h, z = dense.block_norm(x, kind=kind, **more)
+        assert h is x and torch.equal(z, want[1])
+        got = dense.block_norm_backward(x, g, x, kind=kind, **more)
+        assert torch.equal(got.x, dense.block_norm_backward(x, g, x, kind=kind).x)
+    # no gradient by way of the norm after: its weight does not matter
+    want = dense.block_norm_backward(g, None, x, y, g, kind=kind, pre_weight=torch.ones(columns, device="cuda"))
+    got = dense.block_norm_backward(g, None, x, y, g, kind=kind, pre_weight=bad, pre_bias=bad)
+    assert torch.equal(got.x, g) and torch.equal(got.y, want.y) and torch.equal(got.gate, want.gate)
+    assert not got.pre_weight.any() and not got.pre_bias.any()
+    # a norm that is left out, with weights
+    h, z = dense.block_norm(x, y, post_norm=False, pre_norm=False, post_weight=bad, pre_weight=bad)
+    assert z is None and torch.equal(h, x + y)
