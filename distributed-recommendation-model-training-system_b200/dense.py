@@ -277,8 +277,8 @@ def _block_norm_args(device, rows, columns, rtype, y, gate, post_weight, post_bi
         _tensor(gate, "gate", device)
         if gate.dtype != dtype:
             _refuse("the gate has the type of y")
-        # one value a row: [rows] or [..., 1]; a matrix of one column is an element gate where D is 1
-        if columns > 1 and gate.numel() == rows:
+        # one value a row: [rows] or [..., 1]; where D is 1 that is an element gate too, but not without its last axis
+        if gate.numel() == rows and (columns > 1 or gate.dim() == 1):
             gate_kind = 1
             if not gate.is_contiguous():
                 _refuse("a gate of one value a row must be contiguous")

@@ -1,11 +1,12 @@
 """block_norm where tensors are not given: what is wanted is written all the same, and what belongs to the
-missing tensors leaves no trace."""
+missing tensors leaves no trace.  One column with a gate for each row."""
 import ctypes as C
 import math
 
 import pytest
 import torch
 
+import dense_reference as ref
 from conftest import import_package
 from test_block_norm import values
 
@@ -65,3 +66,15 @@ def test_what_belongs_to_missing_tensors_leaves_no_trace(columns, kind):
     # a norm that is left out, with weights
     h, z = dense.block_norm(x, y, post_norm=False, pre_norm=False, post_weight=bad, pre_weight=bad)
     assert z is None and torch.equal(h, x + y)
+
+
+@gpu
+def test_one_column_with_a_gate_for_each_row():
+    x, y, g = values(1, 6, 1), values(2, 6, 1), values(3, 6)
+    w = values(4, 1)
+    how = dict(post_norm=False, pre_norm=False, channel_scale=w, scale=0.5)
+    h, _ = dense.block_norm(x, y, g, **how)
+    assert torch.equal(h, dense.block_norm(x, y, g[:, None], **how)[0])
+    ref.close(h, x.double() + 0.5 * w.double() * torch.sigmoid(g.double())[:, None] * y.double(), x.abs() + y.abs())
+    got, want = (dense.block_norm_backward(x, None, h, y, gate, **how) for gate in (g, g[:, None]))
+    assert got.gate.shape == (6,) and torch.equal(got.gate, want.gate[:, 0]) and torch.equal(got.y, want.y)
