@@ -448,7 +448,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
                   unsigned channel_tiles) {
   using Shape = MmaShape<BN>;
   extern __shared__ unsigned char raw[];
-  __shared__ uint64_t full[Shape::stages], empty[Shape::stages], summed[2], drained[2];
+  __shared__ uint64_t full[Shape::stages], empty[Shape::stages], summed[2], drained[2], issued;
   __shared__ unsigned tensor_base;
   __shared__ Groups groups;
   const unsigned at_stages = (shared_at(raw) + 1023) / 1024 * 1024, at_full = shared_at(full), at_empty = shared_at(empty);
@@ -463,6 +463,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
       barrier_init(summed + s, 1);
       barrier_init(drained + s, 8);
     }
+    barrier_init(&issued, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&weights) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&rows) : "memory");
@@ -536,10 +537,15 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
       half ^= 1;
       turn ^= half == 0;
     }
+    // nor with matrix instructions that still write to the tensor memory it gives back
+    if (!ok) {
+      if (elected()) mma_commit(shared_at(&issued));
+      warp_wait(shared_at(&issued), 0);
+    }
   } else if (warp >= 4) {
     unsigned half = 0, turn = 0;
     bool ok = true;
-    while (ok && walk.next()) {
+    while (walk.next()) {        // after a wait that ran out: no more waits, and NaN for all tiles that are left
       const Tile tile = walk.tile;
       // a quarter of the channels, and every second 32 of the rows
       const unsigned quarter = warp % 4, odd = (warp - 4) / 4 * 32;
@@ -548,14 +554,14 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
       const bool in = n < a.channels;
       const float ws = in ? a.weight_scale[c] : 0.f, b = in && a.bias ? a.bias[c] : 0.f;
       float mine = odd + lane < tile.rows ? a.scale[tile.row + odd + lane] : 0.f;      // of the first 32 rows
-      ok = warp_wait(shared_at(summed) + half * 8, turn);
+      ok = ok && warp_wait(shared_at(summed) + half * 8, turn);
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       T* out = static_cast<T*>(a.out) + (uint64_t)(tile.row + odd) * a.channels + n;
       const unsigned from = base + half * BN + (quarter * 32 << 16);
 #pragma unroll 1
       for (unsigned r0 = odd; r0 < tile.rows; r0 += 64) {
         int v[32];
-        tensor_load(from + r0, v);
+        tensor_load(from + r0, v);        // what lies there, where the sums never came
         const float next = r0 + 64 + lane < tile.rows ? a.scale[tile.row + r0 + 64 + lane] : 0.f;
         const unsigned rows_left = in ? tile.rows - r0 : 0;
 #pragma unroll
@@ -570,7 +576,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
       }
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       __syncwarp();
-      if (lane == 0) barrier_arrive(drained + half);
+      if (ok && lane == 0) barrier_arrive(drained + half);
       half ^= 1;
       turn ^= half == 0;
     }
