@@ -361,6 +361,17 @@ __device__ __forceinline__ bool arrive(uint64_t (&arrived)[kSlots], const Place&
   return true;
 }
 
+// No block ends, or writes to the ring, with copies into it in flight.  Where no wait ran
+// out, all rows that were asked for have arrived.
+template <Way WAY>
+__device__ __forceinline__ void close_ring(uint64_t (&arrived)[kSlots], bool good, unsigned asked) {
+  if constexpr (WAY == kLanes) asm volatile("cp.async.wait_all;" ::: "memory");
+  if constexpr (WAY == kBulk) {
+    if (good || threadIdx.x != 0) return;
+    for (unsigned i = asked > kSlots ? asked - kSlots : 0; i < asked; ++i) barrier_wait(arrived + i % kSlots, i / kSlots & 1);
+  }
+}
+
 template <class TX, class TY, int V>
 __host__ __device__ constexpr unsigned forward_bytes() { return V * (sizeof(TX) + 2 * sizeof(TY)); }     // of a thread in a slot
 template <class TX, class TY, int V>
@@ -387,10 +398,12 @@ __global__ void __launch_bounds__(512) block_norm_forward(const Norm n) {
   Source<TY, V, NIT, kHow> y(n, w, n.y, n.ys), gate(n, w, GATE == EPS_B200_GATE_ELEMENT ? n.g : nullptr, n.gs);
   Sink<TX, V, NIT> h(w, n.out_h, n.out_hs);
   Sink<TY, V, NIT> z(w, n.out_z, n.out_zs);
+  bool good = true;          // no wait has run out; after one that has, nothing is copied or waited for, and results are NaN
   unsigned asked = 0;
   Place fill, here;
   auto ask = [&] {
-    const bool live = asked++ < w.mine;
+    const bool live = good && asked < w.mine;
+    asked += live;
     if constexpr (kHow == kBulk) {
       if (threadIdx.x == 0 && live) {
         const unsigned bx = n.columns * (unsigned)sizeof(TX), by = n.columns * (unsigned)sizeof(TY);
@@ -418,7 +431,7 @@ __global__ void __launch_bounds__(512) block_norm_forward(const Norm n) {
 
   // the first row's y and its statistics
   float v[NIT][V], mean = 0.f, r = 1.f;
-  bool good = arrive<kHow>(arrived, here, true);
+  good = arrive<kHow>(arrived, here, true);
   y.get(n, at_y, 0 < w.mine, lane, v);
   y.next();
   {
@@ -469,7 +482,7 @@ __global__ void __launch_bounds__(512) block_norm_forward(const Norm n) {
     h.next();
     // the next row's y; its statistics together with this row's h's
     here.next(slot_bytes);
-    good = arrive<kHow>(arrived, here, pass + 1 < w.passes);
+    good = good && arrive<kHow>(arrived, here, pass + 1 < w.passes);
     y.get(n, at_y + here.bytes, pass + 1 < w.mine, lane, t);
     y.next();
     float s[2], m = 0.f;
@@ -499,7 +512,7 @@ __global__ void __launch_bounds__(512) block_norm_forward(const Norm n) {
     }
     z.next();
   }
-  if constexpr (kHow == kLanes) asm volatile("cp.async.wait_all;" ::: "memory");
+  close_ring<kHow>(arrived, good, asked);
 }
 
 // The column sums of a lane stay in registers where a lane has few columns, else in
@@ -555,10 +568,12 @@ __global__ void __launch_bounds__(512, V == 1 && NIT <= 4 ? 2 : 1) block_norm_gr
   Source<TY, V, NIT, kHow> sdz(n, w, n.dz, n.dzs), sy(n, w, n.y, n.ys), sg(n, w, GATE == EPS_B200_GATE_ELEMENT ? n.g : nullptr, n.gs);
   Sink<TX, V, NIT> dx(w, n.dx, n.dxs);
   Sink<TY, V, NIT> dy(w, n.dy, n.dys), dg(w, GATE == EPS_B200_GATE_ELEMENT ? n.dg : nullptr, n.dgs);
+  bool good = true;          // no wait has run out; after one that has, nothing is copied or waited for, and results are NaN
   unsigned asked = 0;
   Place fill, here;
   auto ask = [&] {
-    const bool live = asked++ < w.mine;
+    const bool live = good && asked < w.mine;
+    asked += live;
     if constexpr (kHow == kBulk) {
       if (threadIdx.x == 0 && live) {
         const unsigned rx = n.columns * (unsigned)sizeof(TX), ry = n.columns * (unsigned)sizeof(TY);
@@ -594,7 +609,7 @@ __global__ void __launch_bounds__(512, V == 1 && NIT <= 4 ? 2 : 1) block_norm_gr
   // the first row's statistics, of h and of y
   float mean[2] = {0.f, 0.f}, r[2];
   float h[NIT][V], y[NIT][V];
-  bool good = arrive<kHow>(arrived, here, true);
+  good = arrive<kHow>(arrived, here, true);
   sh.get(n, at_h, 0 < w.mine, lane, h);
   sy.get(n, at_y, 0 < w.mine, lane, y);
   {
@@ -620,7 +635,7 @@ __global__ void __launch_bounds__(512, V == 1 && NIT <= 4 ? 2 : 1) block_norm_gr
     if constexpr (kHow != kDirect) ask();
     const unsigned now = here.bytes;
     here.next(slot_bytes);
-    good = arrive<kHow>(arrived, here, pass + 1 < w.passes);
+    good = good && arrive<kHow>(arrived, here, pass + 1 < w.passes);
     float d[NIT][V], q[NIT][V], s[4];
     // through the norm after
     sdz.get(n, at_dz + now, live, lane, q);
@@ -736,7 +751,7 @@ __global__ void __launch_bounds__(512, V == 1 && NIT <= 4 ? 2 : 1) block_norm_gr
     r[1] = __frsqrt_rn(s[3] + n.epsilon);
     sy.get(n, at_y + here.bytes, more, lane, y);
   }
-  if constexpr (kHow == kLanes) asm volatile("cp.async.wait_all;" ::: "memory");
+  close_ring<kHow>(arrived, good, asked);
   if (!wanted) return;
   if constexpr (kHeld) {
     __syncthreads();        // the staged parameters and the ring lie there
