@@ -104,33 +104,6 @@ __device__ __forceinline__ unsigned inclusive(unsigned n, unsigned lane) {
   return n;
 }
 
-// 1 / x, correctly rounded, for x >= 1, infinity and NaN.  One Newton step with fused
-// multiply-adds from the hardware's approximation (P. Markstein, IBM J. Res. Dev. 34,
-// 1990) rounds correctly but where the significand of x is all ones, or where the
-// result or the residual leaves the normal range: those take the library's division,
-// all of a warp together.
-template <int N>
-__device__ __forceinline__ void reciprocals(float (&x)[N]) {
-  unsigned largest = 0, rest = ~0u;      // as bits: infinity and NaN are above all others
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const unsigned u = __float_as_uint(x[i]);
-    largest = max(largest, u);
-    rest = min(rest, ~u & 0x7FFFFFu);
-  }
-  if (__any_sync(~0u, largest > 0x71800000u || rest == 0)) {      // 2^100
-#pragma unroll
-    for (int i = 0; i < N; ++i) x[i] = __fdiv_rn(1.f, x[i]);
-    return;
-  }
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    float r;
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x[i]));
-    x[i] = fmaf(r, fmaf(-x[i], r, 1.f), r);
-  }
-}
-
 // The scores of a token; lanes past the experts hold 0.
 // RANKED: with the operations that the ranking is defined by.
 template <int EPL, bool RANKED>
