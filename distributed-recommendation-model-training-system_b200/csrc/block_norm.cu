@@ -355,9 +355,9 @@ struct Place {
 
 // Whether the row at `at` has arrived; what a lane reads then is its own row's.
 template <Way WAY>
-__device__ __forceinline__ bool arrive(uint64_t (&arrived)[kSlots], const Place& at, bool expected) {
+__device__ __forceinline__ bool arrive(uint64_t (&arrived)[kSlots], const Place& at, bool expected, bool gave_up) {
   if constexpr (WAY == kLanes) asm volatile("cp.async.wait_group %0;" ::"n"(kAhead - 1) : "memory");
-  if constexpr (WAY == kBulk) return !expected || barrier_wait(arrived + at.index, at.phase);
+  if constexpr (WAY == kBulk) return !expected || barrier_wait(arrived + at.index, at.phase, gave_up);
   return true;
 }
 
@@ -398,7 +398,7 @@ __global__ void __launch_bounds__(512) block_norm_forward(const Norm n) {
   Source<TY, V, NIT, kHow> y(n, w, n.y, n.ys), gate(n, w, GATE == EPS_B200_GATE_ELEMENT ? n.g : nullptr, n.gs);
   Sink<TX, V, NIT> h(w, n.out_h, n.out_hs);
   Sink<TY, V, NIT> z(w, n.out_z, n.out_zs);
-  bool good = true;          // no wait has run out; after one that has, nothing is copied or waited for, and results are NaN
+  bool good = true;          // no wait has run out; after one that has, nothing is copied or waited for long, and results are NaN
   unsigned asked = 0;
   Place fill, here;
   auto ask = [&] {
@@ -431,7 +431,7 @@ __global__ void __launch_bounds__(512) block_norm_forward(const Norm n) {
 
   // the first row's y and its statistics
   float v[NIT][V], mean = 0.f, r = 1.f;
-  good = arrive<kHow>(arrived, here, true);
+  good = arrive<kHow>(arrived, here, true, false);
   y.get(n, at_y, 0 < w.mine, lane, v);
   y.next();
   {
@@ -482,7 +482,7 @@ __global__ void __launch_bounds__(512) block_norm_forward(const Norm n) {
     h.next();
     // the next row's y; its statistics together with this row's h's
     here.next(slot_bytes);
-    good = good && arrive<kHow>(arrived, here, pass + 1 < w.passes);
+    good &= arrive<kHow>(arrived, here, pass + 1 < w.passes, !good);
     y.get(n, at_y + here.bytes, pass + 1 < w.mine, lane, t);
     y.next();
     float s[2], m = 0.f;
@@ -568,7 +568,7 @@ __global__ void __launch_bounds__(512, V == 1 && NIT <= 4 ? 2 : 1) block_norm_gr
   Source<TY, V, NIT, kHow> sdz(n, w, n.dz, n.dzs), sy(n, w, n.y, n.ys), sg(n, w, GATE == EPS_B200_GATE_ELEMENT ? n.g : nullptr, n.gs);
   Sink<TX, V, NIT> dx(w, n.dx, n.dxs);
   Sink<TY, V, NIT> dy(w, n.dy, n.dys), dg(w, GATE == EPS_B200_GATE_ELEMENT ? n.dg : nullptr, n.dgs);
-  bool good = true;          // no wait has run out; after one that has, nothing is copied or waited for, and results are NaN
+  bool good = true;          // no wait has run out; after one that has, nothing is copied or waited for long, and results are NaN
   unsigned asked = 0;
   Place fill, here;
   auto ask = [&] {
@@ -609,7 +609,7 @@ __global__ void __launch_bounds__(512, V == 1 && NIT <= 4 ? 2 : 1) block_norm_gr
   // the first row's statistics, of h and of y
   float mean[2] = {0.f, 0.f}, r[2];
   float h[NIT][V], y[NIT][V];
-  good = arrive<kHow>(arrived, here, true);
+  good = arrive<kHow>(arrived, here, true, false);
   sh.get(n, at_h, 0 < w.mine, lane, h);
   sy.get(n, at_y, 0 < w.mine, lane, y);
   {
@@ -635,7 +635,7 @@ __global__ void __launch_bounds__(512, V == 1 && NIT <= 4 ? 2 : 1) block_norm_gr
     if constexpr (kHow != kDirect) ask();
     const unsigned now = here.bytes;
     here.next(slot_bytes);
-    good = good && arrive<kHow>(arrived, here, pass + 1 < w.passes);
+    good &= arrive<kHow>(arrived, here, pass + 1 < w.passes, !good);
     float d[NIT][V], q[NIT][V], s[4];
     // through the norm after
     sdz.get(n, at_dz + now, live, lane, q);
