@@ -56,31 +56,45 @@ struct Norm {
 // The column sums of the backward pass, in this order in `partial`.
 enum { kPostWeight, kPostBias, kChannel, kPreWeight, kPreBias, kSums };
 
-// 1 / (1 + 2^(-g log2 e)): two instructions of the special-function unit, each good
-// to two units of the last place; subnormal powers count as 0, which 1 + hides.
-template <int V>
+// 1 / (1 + 2^-t) with t = g log2 e: two instructions of the special-function unit, each
+// good to two units of the last place; subnormal powers count as 0, which 1 + hides.
+// Rounding t costs another |g| / 2 units.  Gates of 16 bits have a unit 2^13 or 2^16 as
+// large and go without (a gate of -20 is off by some ten units of float); a float block
+// takes what t lost, e = t - g log2 e, into account as 2^e = 1 + e ln 2.  Where t is
+// not finite, or so large that the result is 0 or 1, there is nothing to add.
+template <int V, bool FINE>
 __device__ __forceinline__ void sigmoid(const float (&g)[V], float (&s)[V]) {
-  vmul<V>(s, g, -1.4426950408889634f);
+  constexpr float kLog = 1.4426950408889634f, kLogRest = 1.925963e-8f;      // log2 e and what its float lacks
+  vmul<V>(s, g, kLog);
+  [[maybe_unused]] float e[V];
+  if constexpr (FINE) {
+    vfma<V>(e, g, -kLog, s);
+    vfma<V>(e, g, -kLogRest, e);
+    vfma<V>(e, e, 0.6931471805599453f, 1.f);
 #pragma unroll
-  for (int j = 0; j < V; ++j) asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(s[j]));
-  vadd<V>(s, s, 1.f);
+    for (int j = 0; j < V; ++j) e[j] = fabsf(s[j]) < 256.f ? e[j] : 1.f;
+  }
+#pragma unroll
+  for (int j = 0; j < V; ++j) asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(s[j]) : "f"(-s[j]));
+  if constexpr (FINE) vfma<V>(s, s, e, 1.f);
+  else vadd<V>(s, s, 1.f);
 #pragma unroll
   for (int j = 0; j < V; ++j) asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(s[j]));
 }
 
 // act(g) and, where SLOPE, its derivative for V values; the choice is made once for
 // all of them.
-template <int V, bool SLOPE>
+template <int V, bool SLOPE, bool FINE>
 __device__ __forceinline__ void activate(const float (&g)[V], int activation, float (&a)[V], float (&slope)[V]) {
   if (activation == EPS_B200_ACT_SIGMOID) {
-    sigmoid<V>(g, a);
+    sigmoid<V, FINE>(g, a);
     if (SLOPE) {
 #pragma unroll
       for (int j = 0; j < V; ++j) slope[j] = fmaf(-a[j], a[j], a[j]);
     }
   } else if (activation == EPS_B200_ACT_SILU) {
     float s[V];
-    sigmoid<V>(g, s);
+    sigmoid<V, FINE>(g, s);
     vmul<V>(a, g, s);
     if (SLOPE) {
 #pragma unroll
@@ -101,9 +115,10 @@ __device__ __forceinline__ void activate(const float (&g)[V], int activation, fl
   }
 }
 
+template <bool FINE>
 __device__ __forceinline__ float activate_one(float g, int activation, float* slope) {
   float v[1] = {g}, a[1], s[1];
-  activate<1, true>(v, activation, a, s);
+  activate<1, true, FINE>(v, activation, a, s);
   *slope = s[0];
   return a[0];
 }
@@ -380,7 +395,7 @@ __host__ __device__ constexpr unsigned backward_bytes() { return V * (2 * sizeof
 template <class TX, class TY, int V, int NIT, int P, int GATE>
 __global__ void __launch_bounds__(512) block_norm_forward(const Norm n) {
   constexpr Way kHow = kWay<V, NIT, P>;
-  constexpr bool kStaged = V * NIT <= 8;
+  constexpr bool kStaged = V * NIT <= 8, kFine = std::is_same_v<TY, float>;
   using Given = Parameters<TY, V, NIT, kStaged, true>;
   extern __shared__ __align__(16) char room[];       // the staged parameters, then the ring
   __shared__ float shared[kRowSumShared];
@@ -456,7 +471,7 @@ __global__ void __launch_bounds__(512) block_norm_forward(const Norm n) {
     x.next();
     float open = 1.f, unused;
     if (GATE == EPS_B200_GATE_ROW) {
-      if (live) open = activate_one(to_float(*row_gates), n.activation, &unused);
+      if (live) open = activate_one<kFine>(to_float(*row_gates), n.activation, &unused);
       row_gates += w.stride;
     }
     float g[NIT][V];
@@ -472,7 +487,7 @@ __global__ void __launch_bounds__(512) block_norm_forward(const Norm n) {
       centre<V>(v[i], mean, r);
       vfma<V>(v[i], v[i], a, b);
       if (GATE == EPS_B200_GATE_ELEMENT) {
-        activate<V, false>(g[i], n.activation, a, b);
+        activate<V, false, kFine>(g[i], n.activation, a, b);
         vfma<V>(v[i], v[i], a, t[i]);
       } else {
         vfma<V>(v[i], v[i], open, t[i]);
@@ -523,7 +538,7 @@ template <class TX, class TY, int V, int NIT, int P, int GATE>
 __global__ void __launch_bounds__(512, V == 1 && NIT <= 4 ? 2 : 1) block_norm_gradient(const Norm n) {
   constexpr int N = V * NIT;
   constexpr Way kHow = kWay<V, NIT, P>;
-  constexpr bool kHeld = N <= 8;
+  constexpr bool kHeld = N <= 8, kFine = std::is_same_v<TY, float>;
   using Given = Parameters<TY, V, NIT, kHeld, false>;
   extern __shared__ __align__(16) char room[];      // the staged parameters, then the ring; in the end the sums
   float* const sums = reinterpret_cast<float*>(room);      // [wanted][N][blockDim.x]
@@ -677,7 +692,7 @@ __global__ void __launch_bounds__(512, V == 1 && NIT <= 4 ? 2 : 1) block_norm_gr
     dx.next();
     // through the scale, the gate and the norm before
     float open = 1.f, slope1 = 0.f, sum_gate[1] = {0.f};
-    if (GATE == EPS_B200_GATE_ROW && live) open = activate_one(to_float(*row_gates), n.activation, &slope1);
+    if (GATE == EPS_B200_GATE_ROW && live) open = activate_one<kFine>(to_float(*row_gates), n.activation, &slope1);
     float g[NIT][V];
     if (GATE == EPS_B200_GATE_ELEMENT) {
       sg.get(n, at_g + now, live, lane, g);
@@ -692,7 +707,7 @@ __global__ void __launch_bounds__(512, V == 1 && NIT <= 4 ? 2 : 1) block_norm_gr
       centre<V>(y[i], mean[1], r[1]);
       vfma<V>(nv, y[i], u, nv);             // what the gate sees
       if (GATE == EPS_B200_GATE_ELEMENT) {
-        activate<V, true>(g[i], n.activation, a, slope);
+        activate<V, true, kFine>(g[i], n.activation, a, slope);
         vmul<V>(a, a, d[i]);
       } else {
         vmul<V>(a, d[i], open);
