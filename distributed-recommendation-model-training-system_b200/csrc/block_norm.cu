@@ -22,9 +22,9 @@
 // A row belongs to a group of lanes (a power of two up to a warp, or a whole block),
 // V consecutive elements a lane NIT times.
 //
-// Measured at 16381 x 2048 bf16: forward (rms, element gate) 67 us, 5.0 TB/s; backward
-// (layer norm, every gradient) 143 us, 3.7 TB/s, and 8 us to add up the blocks' column
-// sums.  Forward before its rows were copied ahead: 127 us; with the copies but two
+// Measured at 16381 x 2048 bf16: forward (rms, element gate) 69 us, 4.9 TB/s; backward
+// (layer norm, every gradient) 145 us, 3.7 TB/s, and 8 us to add up the blocks' column
+// sums; in float 109 us, 6.2 TB/s, and (rms) 213 us, 5.0 TB/s, both with the sums.  Forward before its rows were copied ahead: 127 us; with the copies but two
 // barriers more a row, 97.  Backward is bound by instructions at 16 warps an SM, whose
 // registers the 40 column sums of a lane fill.
 #include <cmath>

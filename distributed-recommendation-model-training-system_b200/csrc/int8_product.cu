@@ -287,10 +287,10 @@ __global__ void __launch_bounds__(kRowsThreads) product_rows(const Product a, co
 // tcgen05.mma (kind::i8, 32-bit sums in tensor memory), warps 4..11 scale, round and
 // store the tile before while the next is being summed (two halves of tensor memory).
 //
-// What bounds it: a large product (8189 x 8192 x 4096: 179 us, 3.07e15 operations a
-// second) by the hand-over of its stages and by what the SMs bring in, 48 KB for every
+// What bounds it: a large product (8189 x 8192 x 4096: 175 us alone, 3.15e15 operations a
+// second; some 220 one after another, where the power cap holds it) by the hand-over of its stages and by what the SMs bring in, 48 KB for every
 // 512 cycles of matrix instructions, 18 TB/s over the GPU out of L2; a pair of SMs on one
-// tile would take a third off that.  Four warps storing instead of eight took 225 us:
+// tile would take a third off that.  Four warps storing instead of eight took 225 us (and eight 179):
 // the next tile but one waited for them.
 constexpr int kMmaThreads = 384;            // four warps that feed, eight that store
 constexpr unsigned kSpan = 128;            // bytes of inner size that one swizzled copy covers

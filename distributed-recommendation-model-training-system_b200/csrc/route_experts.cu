@@ -16,8 +16,9 @@
 // on unsigned images of the keys (`image`), so one warp instruction finds the best
 // key and the lowest lane that holds it owns the lowest index.  What bounds it is the
 // number of instructions a token takes (the logits of a batch are a few megabytes):
-// every lane sorts its own few keys once, and then only offers the best it has left.
-// Measured at 32771 x 256 floats, top 8 of the best 4 of 8 groups: 44 us (850
+// every lane sorts its own few keys once, and then only offers the best it has left (in
+// registers up to 8 keys a lane; the 16 or 32 of more than 256 experts lie in local memory).
+// Measured at 32771 x 256 floats, top 8 of the best 4 of 8 groups: 46 us (850
 // instructions a token; 132 with the best key searched anew each time and groups scored
 // lane by lane), 6 to scan the tiles and 5 to place; the gradient at 32771 x 96 bf16 19.
 //
@@ -105,7 +106,8 @@ __device__ __forceinline__ unsigned inclusive(unsigned n, unsigned lane) {
 }
 
 // The scores of a token; lanes past the experts hold 0.
-// RANKED: with the operations that the ranking is defined by.
+// RANKED: with the operations that the ranking is defined by.  The gradient, which ranks
+// nothing, multiplies by the reciprocal of a sum in 32 bits: one rounding more a score.
 template <int EPL, bool RANKED>
 __device__ __forceinline__ void score(const Route& a, float (&x)[EPL]) {
   if (!a.softmax) {

@@ -12,6 +12,9 @@ allocator, and nothing is kept between calls but what the two classes hold.  Cal
 can be captured in a CUDA graph; a captured AdamW step counts its replays.  There is no CPU fallback; a refused call raises
 ``EpsError`` with ``code`` INVALID_ARGUMENT before anything is launched.
 
+Results carry no autograd history, whether their inputs require gradients or not:
+gradients come from the *_backward functions.
+
 Leading axes of a tensor count as rows; the last axis must be contiguous, rows may
 have any stride.  Element types are float32, bfloat16 and float16.
 """

@@ -19,6 +19,8 @@
  *    AdamW step as eps_b200_adamw_counted);
  *  - an element type is EPS_B200_F32, _BF16 or _F16.  Sums, statistics and
  *    scores are held in 32 bits or more whatever the type;
+ *  - no kernel waits longer than two seconds for a copy or a sum; where one gives up,
+ *    what it still had to write becomes NaN;
  *  - the last axis of every tensor is contiguous; a row stride is given in
  *    elements.  Any alignment of the element type is accepted (16-byte aligned
  *    rows take wider loads).
