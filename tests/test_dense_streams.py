@@ -16,7 +16,7 @@ def held_up(call):
     s = torch.cuda.Stream()
     s.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(s):
-        torch.cuda._sleep(400_000_000)
+        torch.cuda._sleep(1_000_000_000)
         call()
         done = torch.cuda.Event()
         done.record()
