@@ -24,7 +24,8 @@ LIB = os.path.join(HERE, "libeps_b200.so")
 
 SOURCES = ["store.cu", "lookup.cu", "sort.cu", "push.cu", "route.cu", "noalloc.cu", "runtime.cu",
            "comm.cu", "client.cu", "sync.cu", "runtime_api.cu",
-           "block_norm.cu", "route_experts.cu", "int8_product.cu", "adamw.cu"]
+           "block_norm.cu", "route_experts.cu", "int8_product.cu", "adamw.cu",
+           "gradient_norm.cu", "balance_loss.cu", "low_rank.cu"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-std=c++17", "-lineinfo", "--fmad=false", "-Xcompiler", "-fPIC",
          "-Xcompiler", "-fvisibility=hidden", "-I", CSRC, "-I", INCLUDE]

@@ -4,11 +4,14 @@
     routing = dense.route(logits, top_k=8, score="sigmoid", bias=balance)
     experts = dense.QuantizedExperts.from_weights(weight)          # [experts, channels, inner]
     out = experts.product(z, offsets=routing.offsets, rows=routing.order, rows_divisor=8)
-    dense.AdamW(parameters, gradients, state_bits=8).step()
+    out = dense.Adapters(down, up).product(x, ids, base=layer.product(x))
+    balance = dense.balance_loss(logits, routing.experts)
+    clip = dense.GradientNorm(gradients).measure(max_norm=1.0)
+    dense.AdamW(parameters, gradients, state_bits=8).step(gradient_scale=clip.scale, skip=clip.skip)
 
 Every tensor is a torch CUDA tensor; work goes to torch's current stream of the
 tensors' device and is asynchronous, results and workspaces come from torch's
-allocator, and nothing is kept between calls but what the two classes hold.  Calls
+allocator, and nothing is kept between calls but what the classes hold.  Calls
 can be captured in a CUDA graph; a captured AdamW step counts its replays.  There is no CPU fallback; a refused call raises
 ``EpsError`` with ``code`` INVALID_ARGUMENT before anything is launched.
 
@@ -31,19 +34,25 @@ import torch
 from . import EpsError, INVALID_ARGUMENT, Status, load_library
 
 __all__ = ["block_norm", "block_norm_backward", "BlockNormGradients", "route", "route_backward",
-           "Routing", "quantize_rows", "QuantizedExperts", "AdamW", "ENTRY_POINTS"]
+           "Routing", "balance_loss", "balance_loss_backward", "BalanceLoss", "quantize_rows", "QuantizedExperts",
+           "Adapters", "GradientNorm", "GradientMeasure", "AdamW", "ENTRY_POINTS"]
 
 ENTRY_POINTS = ("eps_b200_block_norm", "eps_b200_block_norm_workspace",
                 "eps_b200_block_norm_backward", "eps_b200_route_experts_workspace",
                 "eps_b200_route_experts", "eps_b200_route_experts_backward",
                 "eps_b200_int8_stride", "eps_b200_int8_quantize",
                 "eps_b200_int8_product_workspace", "eps_b200_int8_product", "eps_b200_int8_linear",
-                "eps_b200_adamw_plan_bytes", "eps_b200_adamw_plan", "eps_b200_adamw", "eps_b200_adamw_counted")
+                "eps_b200_adamw_plan_bytes", "eps_b200_adamw_plan", "eps_b200_adamw", "eps_b200_adamw_counted",
+                "eps_b200_gradient_norm_plan_bytes", "eps_b200_gradient_norm_plan",
+                "eps_b200_gradient_norm_workspace", "eps_b200_gradient_norm",
+                "eps_b200_balance_loss_workspace", "eps_b200_balance_loss", "eps_b200_balance_loss_backward",
+                "eps_b200_low_rank_rank", "eps_b200_low_rank_inner", "eps_b200_low_rank_workspace", "eps_b200_low_rank")
 
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _KINDS = {"rms": 0, "layer": 1}
 _ACTIVATIONS = {"none": 0, "sigmoid": 1, "silu": 2, "tanh": 3}
 _SCORES = {"softmax": 0, "sigmoid": 1}
+_NORMS = {"l2": 0, "max": 1}
 ADAMW_BLOCK = 256           # elements of a tensor that share a scale (EPS_B200_ADAMW_BLOCK)
 
 
@@ -104,6 +113,33 @@ class AdamWClock(C.Structure):
                 ("inverse_root", C.c_float), ("key", C.c_uint32)]
 
 
+class Gradient(C.Structure):
+    _fields_ = [("gradient", C.c_void_p), ("elements", C.c_uint64), ("type", C.c_int32), ("reserved", C.c_int32)]
+
+
+class GradientNormArgs(C.Structure):
+    _fields_ = [("device", C.c_int32), ("kind", C.c_int32), ("clip", C.c_int32), ("reserved", C.c_int32),
+                ("plan", C.c_void_p), ("blocks", C.c_uint64), ("gradient_scale", C.c_void_p),
+                ("max_norm", C.c_double), ("result", C.c_void_p), ("workspace", C.c_void_p),
+                ("workspace_bytes", C.c_uint64)]
+
+
+class BalanceLossArgs(C.Structure):
+    _fields_ = [("device", C.c_int32), ("type", C.c_int32), ("score", C.c_int32),
+                ("normalise", C.c_int32), ("experts", C.c_uint32), ("top_k", C.c_uint32),
+                ("tokens", C.c_uint64), ("weight", C.c_float), ("reserved", C.c_int32),
+                ("logits", C.c_void_p), ("logits_stride", C.c_int64), ("mask", C.c_void_p)]
+
+
+class LowRank(C.Structure):
+    _fields_ = [("device", C.c_int32), ("type", C.c_int32), ("adapters", C.c_uint32),
+                ("rank", C.c_uint32), ("inner", C.c_uint32), ("channels", C.c_uint32),
+                ("rows", C.c_uint64)] + \
+               [(n, C.c_void_p) for n in ("down", "up", "scale", "ids", "x", "base", "out")] + \
+               [(n, C.c_int64) for n in ("x_stride", "base_stride", "out_stride")] + \
+               [("workspace", C.c_void_p), ("workspace_bytes", C.c_uint64)]
+
+
 def _bind():
     # the structs that are packed for each call go in as bytes of the same layout
     lib, P, vp, i64, u64, u32, i32 = (load_library(), C.POINTER, C.c_void_p, C.c_int64, C.c_uint64,
@@ -124,8 +160,19 @@ def _bind():
     lib.eps_b200_adamw_plan.argtypes = [P(AdamWTensor), u64, vp, u64, P(u64), st]
     lib.eps_b200_adamw.argtypes = [P(AdamWArgs), vp, u64, u64, vp, st]
     lib.eps_b200_adamw_counted.argtypes = [P(AdamWArgs), vp, u64, u64, vp, vp, st]
+    lib.eps_b200_gradient_norm_plan_bytes.argtypes = [P(Gradient), u64]
+    lib.eps_b200_gradient_norm_plan.argtypes = [P(Gradient), u64, vp, u64, P(u64), st]
+    lib.eps_b200_gradient_norm_workspace.argtypes = [u64]
+    lib.eps_b200_gradient_norm.argtypes = [C.c_char_p, vp, st]
+    lib.eps_b200_balance_loss_workspace.argtypes = [u64, u32]
+    lib.eps_b200_balance_loss.argtypes = [C.c_char_p, vp, vp, vp, vp, vp, vp, u64, vp, st]
+    lib.eps_b200_balance_loss_backward.argtypes = [C.c_char_p, vp, vp, vp, vp, i64, vp, i64, vp, st]
+    lib.eps_b200_low_rank_rank.argtypes = [u32]
+    lib.eps_b200_low_rank_inner.argtypes = [u32]
+    lib.eps_b200_low_rank_workspace.argtypes = [u64, u32]
+    lib.eps_b200_low_rank.argtypes = [C.c_char_p, vp, st]
     for name in ENTRY_POINTS:
-        sized = name.endswith(("_workspace", "_bytes", "_stride"))
+        sized = name.endswith(("_workspace", "_bytes", "_stride", "_low_rank_rank", "_inner"))
         getattr(lib, name).restype = u64 if sized else C.c_int
     return lib
 
@@ -462,6 +509,87 @@ def route_backward(logits, experts, dweights, *, score: str = "softmax", renorma
     return out
 
 
+# -------------------------------------------------------------- balance loss
+class BalanceLoss(NamedTuple):
+    """loss, a float32 scalar; counts [experts] int32, each expert's entries; mass [experts]
+    float32, the sum of its p over the tokens; tokens, an int32 scalar, how many were
+    counted.  Of several ranks with a batch each, counts, mass and tokens add up to those
+    of the joint batch."""
+    loss: torch.Tensor
+    counts: torch.Tensor
+    mass: torch.Tensor
+    tokens: torch.Tensor
+
+
+_BALANCE = struct.Struct("@4i2IQfiPqP")          # BalanceLossArgs
+
+
+def _balance_args(logits, stride, tokens, experts, top_k, score, normalise, mask, weight):
+    index, at = logits.get_device(), 0
+    if mask is not None:
+        _tensor(mask, "mask", index)
+        if mask.dtype != torch.bool or mask.numel() != tokens or not mask.is_contiguous():
+            _refuse("mask must be contiguous bool, a value for each token")
+        at = mask.data_ptr()
+    return _pack(_BALANCE, index, _TYPES[logits.dtype], _choice(_SCORES, score, "score"), bool(normalise), experts, top_k,
+                 tokens, weight, 0, logits.data_ptr(), stride, at)
+
+
+def balance_loss(logits, experts, *, score: str = "softmax", normalise: bool = True, mask=None,
+                 weight: float = 1.0) -> BalanceLoss:
+    """The loss that balances a router's experts, and how many entries each has.
+
+        p = softmax(logits) or sigmoid(logits), the latter divided by its sum if `normalise`
+        loss = weight * E / (top_k * n^2) * sum_e counts[e] * mass[e],  mass[e] = sum_t p[t, e]
+
+    logits [tokens, E]; experts [tokens, top_k] int32, as route gives them (entries outside
+    [0, E) count for none).  mask [tokens] bool: only these n tokens count, the others'
+    logits are not read.  A row of masked logits (-inf) alone has p = 0; without a token the
+    loss is 0.  At most 1024 experts and top_k 32."""
+    logits, stride, tokens, count = _matrix(logits, "logits")
+    index, device = logits.get_device(), logits.device
+    _tensor(experts, "experts", index)
+    if experts.dim() < 1 or experts.shape[-1] == 0 or experts.dtype != torch.int32 or not experts.is_contiguous():
+        _refuse("experts must be a contiguous int32 tensor, as route gives it")
+    top_k = experts.shape[-1]
+    if experts.numel() != tokens * top_k:
+        _refuse("experts and logits have different numbers of tokens")
+    args = _balance_args(logits, stride, tokens, count, top_k, score, normalise, mask, weight)
+    loss = torch.empty((), dtype=torch.float32, device=device)
+    counted = torch.empty((), dtype=torch.int32, device=device)
+    counts = torch.empty(count, dtype=torch.int32, device=device)
+    mass = torch.empty(count, dtype=torch.float32, device=device)
+    space = _lib.eps_b200_balance_loss_workspace(tokens, count)
+    workspace = torch.empty(space, dtype=torch.uint8, device=device) if space else None
+    _call(_lib.eps_b200_balance_loss, args, experts.data_ptr(), loss.data_ptr(), counts.data_ptr(), mass.data_ptr(),
+          counted.data_ptr(), _ptr(workspace), space, _stream(index))
+    return BalanceLoss(loss, counts, mass, counted)
+
+
+def balance_loss_backward(logits, counts, tokens, top_k: int, *, score: str = "softmax", normalise: bool = True,
+                          mask=None, weight: float = 1.0, dloss=None, add=None):
+    """The logits' gradient from that of balance_loss (dloss, a float32 scalar on the GPU;
+    None: 1), in the logits' type.  counts and tokens are the forward's, or their sums over
+    ranks; the counts take no gradient.  `add`, a gradient of the logits that comes another
+    way (route_backward's), is added before the one rounding; masked tokens get it alone."""
+    flat, stride, rows, count = _matrix(logits, "logits")
+    index = flat.get_device()
+    if top_k <= 0:
+        _refuse("top_k is positive")
+    at = _vector(counts, "counts", index, count, torch.int32)
+    n = _vector(tokens, "tokens", index, 1, torch.int32)
+    d = _vector(dloss, "dloss", index, 1, torch.float32)
+    add_stride = 0
+    if add is not None:
+        add, add_stride, _, _ = _matrix(add, "add", index, count, rows)
+        if add.dtype != flat.dtype:
+            _refuse("add has the type of the logits")
+    args = _balance_args(flat, stride, rows, count, top_k, score, normalise, mask, weight)
+    out = torch.empty_like(logits, memory_format=torch.contiguous_format)
+    _call(_lib.eps_b200_balance_loss_backward, args, at, n, d, _ptr(add), add_stride, out.data_ptr(), count, _stream(index))
+    return out
+
+
 # ------------------------------------------------------------- 8-bit products
 def _row_index(rows, rows_divisor, device):
     if rows is None:
@@ -558,6 +686,183 @@ class QuantizedExperts:
         self._streams.use(stream, device)
         _call(_lib.eps_b200_int8_linear, args, flat.data_ptr(), x_stride, x_rows, index, stream)
         return out
+
+
+# ------------------------------------------------------------------ adapters
+_LOW_RANK = struct.Struct("@2i4IQ7P3qPQ")          # LowRank
+
+
+class Adapters:
+    """Low-rank adapters beside a linear layer that many requests share, each row with its
+    own: out[t] = base[t] + scale[a] * up[a] (down[a] x[t]) for a = ids[t].
+
+    Laid out once; load() puts another adapter in the place of one."""
+
+    def __init__(self, down, up, scale=None):
+        """down [adapters, rank, inner] and up [adapters, channels, rank] of one type
+        (float32, bfloat16 or float16), copied; scale float32 [adapters] (None: 1).
+        Ranks are at most 128, adapters 16384."""
+        index = _tensor(down, "down")
+        _tensor(up, "up", index)
+        if down.dim() != 3 or up.dim() != 3 or 0 in down.shape or 0 in up.shape:
+            _refuse("down must be [adapters, rank, inner] and up [adapters, channels, rank]")
+        self.adapters, self.rank, self.inner = down.shape
+        self.channels = up.shape[1]
+        if up.shape[0] != self.adapters or up.shape[2] != self.rank:
+            _refuse("down and up have different numbers of adapters or ranks")
+        if down.dtype not in _TYPES or up.dtype != down.dtype:
+            _refuse("down and up must be float32, bfloat16 or float16, both the same")
+        if self.rank > 128 or self.adapters > 16384:
+            _refuse("ranks are at most 128, adapters 16384")
+        _vector(scale, "scale", index, self.adapters, torch.float32)
+        self.device, self.dtype = down.device, down.dtype
+        rank, inner = _lib.eps_b200_low_rank_rank(self.rank), _lib.eps_b200_low_rank_inner(self.inner)
+        self.down = torch.zeros((self.adapters, rank, inner), dtype=self.dtype, device=self.device)
+        self.up = torch.zeros((self.adapters, self.channels, rank), dtype=self.dtype, device=self.device)
+        self.down[:, : self.rank, : self.inner] = down.detach()
+        self.up[..., : self.rank] = up.detach()
+        self.scale = torch.ones(self.adapters, device=self.device) if scale is None else scale.detach().reshape(-1).clone()
+        self._index, self._fixed = index, (self.down.data_ptr(), self.up.data_ptr(), self.scale.data_ptr())
+        self._streams = _Streams(index, self.down, self.up, self.scale)
+
+    def load(self, adapter: int, down, up, scale: float = 1.0):
+        """Puts an adapter (down [rank, inner], up [channels, rank], of this rank or a lower
+        one) in the place of number `adapter`, in the order of the current stream: what
+        reads the old one on another stream has to be waited for."""
+        if not 0 <= adapter < self.adapters:
+            _refuse(f"adapters are 0 to {self.adapters - 1}")
+        _tensor(down, "down", self._index)
+        _tensor(up, "up", self._index)
+        rank = down.shape[0] if down.dim() == 2 else 0
+        if not 0 < rank <= self.rank or down.shape != (rank, self.inner) or up.shape != (self.channels, rank):
+            _refuse(f"down must be [rank, {self.inner}] and up [{self.channels}, rank], with a rank of 1 to {self.rank}")
+        if down.dtype != self.dtype or up.dtype != self.dtype:
+            _refuse(f"down and up must be {self.dtype}")
+        self._streams.use(_stream(self._index), self._index)
+        self.down[adapter, :rank, : self.inner] = down.detach()
+        self.down[adapter, rank:] = 0
+        self.up[adapter, :, :rank] = up.detach()
+        self.up[adapter, :, rank:] = 0
+        self.scale[adapter] = scale
+        return self
+
+    def product(self, x, ids, base=None, out=None):
+        """base + scale * up (down x) for x [..., inner], each row with the adapter that
+        ids (int32, one a row) names: [..., channels] in x's type.  An id outside
+        [0, adapters), such as -1, is no adapter: the row is base's.  base [..., channels]
+        (None: 0), the shared layer's output; a row of stride 0 stands for all.  out: where
+        the result goes, base itself for one; it may not overlap x, nor base otherwise.
+        All have the adapters' type."""
+        device = self._index
+        flat, x_stride, rows, _ = _matrix(x, "x", device, self.inner)
+        if flat.dtype != self.dtype:
+            _refuse(f"x must be {self.dtype}, as the adapters are")
+        _tensor(ids, "ids", device)
+        if ids.dtype != torch.int32 or ids.numel() != rows or not ids.is_contiguous():
+            _refuse("ids must be contiguous int32, one for each row of x")
+        base_stride = 0
+        if base is not None:
+            base, base_stride, _, _ = _matrix(base, "base", device, self.channels, rows)
+            if base.dtype != self.dtype:
+                _refuse("base has the type of x")
+        if out is None:
+            result = out = torch.empty((*x.shape[:-1], self.channels), dtype=self.dtype, device=self.device)
+            out_stride = self.channels
+        else:
+            result = out
+            out, out_stride, _, _ = _matrix(out, "out", device, self.channels, rows)
+            if out.dtype != self.dtype:
+                _refuse("out has the type of x")
+        space = _lib.eps_b200_low_rank_workspace(rows, self.adapters)
+        workspace = torch.empty(space, dtype=torch.uint8, device=self.device) if space else None
+        args = _pack(_LOW_RANK, device, _TYPES[self.dtype], self.adapters, self.rank, self.inner, self.channels, rows, *self._fixed,
+                     ids.data_ptr(), flat.data_ptr(), _ptr(base), out.data_ptr(), x_stride, base_stride, out_stride,
+                     _ptr(workspace), space)
+        stream = _stream(device)
+        self._streams.use(stream, device)
+        _call(_lib.eps_b200_low_rank, args, stream)
+        return result
+
+
+# ------------------------------------------------------------- gradient norm
+class GradientMeasure(NamedTuple):
+    """norm and scale, float32 scalars on the GPU, and skip, an int32 one.  scale and skip
+    are what AdamW.step takes: the factor that clips (times the given gradient_scale), and
+    whether the norm is not finite (scale is 0 then)."""
+    norm: torch.Tensor
+    scale: torch.Tensor
+    skip: torch.Tensor
+
+
+_GRADIENT_NORM = struct.Struct("@4iPQPdPPQ")          # GradientNormArgs
+
+
+class GradientNorm:
+    """The norm over many gradients, and clipping by it.
+
+        norm = |gradient_scale| * sqrt(sum g^2)                 kind "l2"; "max": max |g|
+        scale = gradient_scale * min(1, max_norm / norm)
+
+    `gradients` are contiguous float32, bfloat16 or float16 tensors of one device, each of
+    its own type, no two of which overlap (the buffers of one AdamW or of several): their
+    addresses go to the GPU now, their values are read by each call.  Sums are held in 64
+    bits and taken in a fixed order.  A captured call keeps the buffers it reads alive; the
+    object has to outlive the graph."""
+
+    def __init__(self, gradients: Sequence[torch.Tensor], *, kind: str = "l2"):
+        self._kind, self._kept = _choice(_NORMS, kind, "kind"), []
+        self.bind(gradients)
+
+    def bind(self, gradients: Sequence[torch.Tensor]):
+        """Makes these the buffers that are measured."""
+        gradients = list(gradients)
+        if not gradients:
+            _refuse("no gradients")
+        index = _tensor(gradients[0], "a gradient")
+        if _capturing(index):
+            _refuse("gradients are bound before a capture")
+        tensors = (Gradient * len(gradients))()
+        for i, g in enumerate(gradients):
+            _tensor(g, "a gradient", index)
+            if g.dtype not in _TYPES or not g.is_contiguous():
+                _refuse("gradients are contiguous, of float32, bfloat16 or float16")
+            tensors[i] = Gradient(g.data_ptr(), g.numel(), _TYPES[g.dtype], 0)
+        size = _lib.eps_b200_gradient_norm_plan_bytes(tensors, len(gradients))
+        host = torch.empty(size, dtype=torch.uint8)
+        blocks = C.c_uint64(0)
+        _call(_lib.eps_b200_gradient_norm_plan, tensors, len(gradients), host.data_ptr(), size, C.byref(blocks))
+        device = gradients[0].device
+        plan = host.to(device)
+        self.device, self.gradients = device, gradients
+        self._bound = (gradients, plan, blocks.value, _lib.eps_b200_gradient_norm_workspace(blocks.value),
+                       _Streams(index, plan, *gradients))
+
+    def _run(self, clip, max_norm, gradient_scale):
+        _, plan, blocks, space, streams = self._bound
+        device = self.device.index
+        scale = _vector(gradient_scale, "gradient_scale", device, 1, torch.float32)
+        result = torch.empty(3, dtype=torch.float32, device=self.device)
+        workspace = torch.empty(space, dtype=torch.uint8, device=self.device) if space else None
+        args = _pack(_GRADIENT_NORM, device, self._kind, clip, 0, plan.data_ptr(), blocks, scale, max_norm, result.data_ptr(),
+                     _ptr(workspace), space)
+        stream = _stream(device)
+        streams.use(stream, device)
+        _call(_lib.eps_b200_gradient_norm, args, stream)
+        if _capturing(device) and not any(kept is self._bound for kept in self._kept):
+            self._kept.append(self._bound)
+        norm, factor, skip = result.unbind()
+        return GradientMeasure(norm, factor, skip.view(torch.int32))
+
+    def measure(self, max_norm: float = math.inf, *, gradient_scale=None) -> GradientMeasure:
+        """The norm and the factor that brings it to max_norm at most; the gradients stay
+        as they are.  gradient_scale: a float32 scalar on the GPU that the gradients are to
+        be multiplied by anyway (one over a loss scale)."""
+        return self._run(0, max_norm, gradient_scale)
+
+    def clip(self, max_norm: float, *, gradient_scale=None) -> GradientMeasure:
+        """measure(), and every gradient times that factor in place, rounded once; where
+        the norm is not finite they stay as they are."""
+        return self._run(1, max_norm, gradient_scale)
 
 
 # --------------------------------------------------------------------- AdamW

@@ -254,6 +254,122 @@ EPS_B200_EXPORT int eps_b200_adamw_counted(const EpsB200AdamW* args, const void*
                                            uint64_t blocks, EpsB200AdamWClock* clock, void* stream,
                                            EpsB200Status* status);
 
+/* ---- The norm over many gradients, the factor that clips it, and clipping in place.
+ *   u = *gradient_scale                          1 if NULL
+ *   norm = |u| sqrt(sum g^2)                     EPS_B200_GRADIENT_L2
+ *   norm = |u| max |g|                           EPS_B200_GRADIENT_MAX
+ *   scale = u * min(1, max_norm / norm)          u where norm is 0
+ * Where norm is not finite (as a float) skip is 1 and scale 0; else skip is 0.  scale
+ * and skip are what eps_b200_adamw takes.  With `clip` every gradient becomes
+ * gradient * scale, rounded once, and stays as it is where skip is 1.  Sums are taken
+ * in 64 bits, in an order that only the sizes and the GPU decide, so results repeat
+ * exactly. */
+enum { EPS_B200_GRADIENT_L2 = 0, EPS_B200_GRADIENT_MAX = 1 };
+
+typedef struct {
+  void* gradient;
+  uint64_t elements;
+  int32_t type;                  /* each tensor has its own */
+  int32_t reserved;
+} EpsB200Gradient;
+
+typedef struct {
+  float norm, scale;
+  int32_t skip;
+} EpsB200GradientResult;
+
+/* Lays the tensors out for eps_b200_gradient_norm, as eps_b200_adamw_plan does for
+ * AdamW: `plan` (host, eps_b200_gradient_norm_plan_bytes() bytes) is to be copied to
+ * the device by the caller, 16-byte aligned, and *blocks_out receives its block count.
+ * Tensors that overlap are refused. */
+EPS_B200_EXPORT uint64_t eps_b200_gradient_norm_plan_bytes(const EpsB200Gradient* tensors, uint64_t count);
+EPS_B200_EXPORT int eps_b200_gradient_norm_plan(const EpsB200Gradient* tensors, uint64_t count, void* plan,
+                                                uint64_t plan_bytes, uint64_t* blocks_out,
+                                                EpsB200Status* status);
+typedef struct {
+  int32_t device;
+  int32_t kind, clip;
+  int32_t reserved;
+  const void* plan;
+  uint64_t blocks;
+  const float* gradient_scale;   /* device scalar or NULL */
+  double max_norm;               /* >= 0; infinity: nothing is clipped */
+  EpsB200GradientResult* result; /* device */
+  void* workspace;
+  uint64_t workspace_bytes;
+} EpsB200GradientNorm;
+EPS_B200_EXPORT uint64_t eps_b200_gradient_norm_workspace(uint64_t blocks);
+EPS_B200_EXPORT int eps_b200_gradient_norm(const EpsB200GradientNorm* args, void* stream, EpsB200Status* status);
+
+/* ---- A loss that balances the experts, and how many entries each has.
+ *   s = softmax(logits) or sigmoid(logits)       a row of -inf alone has s = 0
+ *   p = s / sum_e s                              s itself if not `normalise` (0 if the
+ *                                                sum is 0; a softmax is normalised as it is)
+ * over the tokens whose mask is not 0 (all without a mask), n of them:
+ *   counts[e] = entries of chosen[t, :] that are e; entries outside [0, experts) count for none
+ *   mass[e] = sum_t p[t, e]
+ *   loss = weight * experts / (top_k * n^2) * sum_e counts[e] * mass[e]     0 if n is 0
+ * What masked tokens hold is read by no sum.  Sums over tokens are taken in an order
+ * that only the sizes and the GPU decide.  Of several ranks with a batch each, counts,
+ * mass and counted add up to those of the joint batch; backward takes the sums. */
+typedef struct {
+  int32_t device;
+  int32_t type;                  /* of logits, add and dlogits */
+  int32_t score, normalise;
+  uint32_t experts, top_k;       /* at most EPS_B200_ROUTE_EXPERTS and EPS_B200_ROUTE_TOP_K */
+  uint64_t tokens;               /* tokens * top_k < 2^31 */
+  float weight;
+  int32_t reserved;
+  const void* logits;            /* [tokens, experts] */
+  int64_t logits_stride;
+  const uint8_t* mask;           /* [tokens] or NULL */
+} EpsB200BalanceLoss;
+
+EPS_B200_EXPORT uint64_t eps_b200_balance_loss_workspace(uint64_t tokens, uint32_t experts);
+EPS_B200_EXPORT int eps_b200_balance_loss(const EpsB200BalanceLoss* args, const int32_t* chosen,
+                                          float* loss, int32_t* counts, float* mass, int32_t* counted,
+                                          void* workspace, uint64_t workspace_bytes,
+                                          void* stream, EpsB200Status* status);
+/* dlogits = *dloss * (the loss's gradient) + add, rounded once; masked tokens get `add`
+ * alone.  dloss NULL: 1; add NULL: 0; dlogits may be `add` itself.  The counts take no
+ * gradient. */
+EPS_B200_EXPORT int eps_b200_balance_loss_backward(const EpsB200BalanceLoss* args, const int32_t* counts,
+                                                   const int32_t* counted, const float* dloss,
+                                                   const void* add, int64_t add_stride,
+                                                   void* dlogits, int64_t dlogits_stride,
+                                                   void* stream, EpsB200Status* status);
+
+/* ---- Low-rank adapters of many requests at once, beside a layer that they share.
+ *   a = ids[t];  out[t] = base[t] + scale[a] * up[a] (down[a] x[t])
+ * An id outside [0, adapters) is no adapter: out[t] is base[t].  base NULL: 0; out may
+ * be base itself.  out must not overlap x.  down [adapters, R, K'] and up [adapters,
+ * channels, R] are contiguous and 16-byte aligned, with R = eps_b200_low_rank_rank(rank)
+ * and K' = eps_b200_low_rank_inner(inner), and zeros behind `rank` and `inner`.  All
+ * have one type.  Products are exact and sums are held in 32 bits; down[a] x[t] is
+ * kept to 16 bits of mantissa or more (24 with float, where infinity, NaN or a magnitude
+ * from 3.38e38 on in x[t], down, up or a sum makes what it enters NaN).  A row's result
+ * does not depend on the other rows' values. */
+#define EPS_B200_LOW_RANK 128u             /* most ranks */
+#define EPS_B200_LOW_RANK_ADAPTERS 16384u  /* most adapters */
+typedef struct {
+  int32_t device;
+  int32_t type;
+  uint32_t adapters, rank, inner, channels;
+  uint64_t rows;                 /* < 2^31 */
+  const void *down, *up;
+  const float* scale;            /* [adapters] or NULL: 1 */
+  const int32_t* ids;            /* [rows] */
+  const void *x, *base;          /* [rows, inner], [rows, channels] */
+  void* out;                     /* [rows, channels] */
+  int64_t x_stride, base_stride, out_stride;
+  void* workspace;
+  uint64_t workspace_bytes;
+} EpsB200LowRank;
+EPS_B200_EXPORT uint64_t eps_b200_low_rank_rank(uint32_t rank);
+EPS_B200_EXPORT uint64_t eps_b200_low_rank_inner(uint32_t inner);
+EPS_B200_EXPORT uint64_t eps_b200_low_rank_workspace(uint64_t rows, uint32_t adapters);
+EPS_B200_EXPORT int eps_b200_low_rank(const EpsB200LowRank* args, void* stream, EpsB200Status* status);
+
 #ifdef __cplusplus
 }
 #endif
