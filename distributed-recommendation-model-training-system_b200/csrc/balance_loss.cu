@@ -17,8 +17,6 @@
 // cover it) hold it in registers between its reductions and the next row is under way
 // meanwhile; each lane sums its columns over all of its rows.  Blocks leave their sums,
 // which a cluster adds up in block order: no float atomics, so results repeat exactly.
-#include <cooperative_groups.h>
-
 #include <algorithm>
 #include <cmath>
 
@@ -31,8 +29,9 @@ namespace {
 constexpr unsigned kThreads = 256, kWarps = kThreads / 32;
 // Blocks an SM, by the columns of a lane: what their registers leave room for.
 constexpr unsigned blocks_an_sm(int columns) { return columns <= 8 ? 4 : columns <= 16 ? 2 : 1; }
-constexpr unsigned kMost = 1024;          // most blocks that leave sums
-constexpr unsigned kFinish = 8;           // blocks that add them up
+constexpr unsigned kTogether = 4;         // blocks whose sums are added before they leave them
+constexpr unsigned kMost = 1024;          // most blocks
+constexpr unsigned kFinish = 8, kFinishThreads = 512, kFinishWarps = kFinishThreads / 32;      // blocks that add up what is left
 
 struct Rows {
   const void* logits;
@@ -50,7 +49,7 @@ struct Forward : Rows {
   int32_t* counts;
   float* mass;
   int32_t* counted;
-  uint32_t* sums;            // a block's mass, counts and counted tokens: 2 E + 1 words
+  uint32_t* sums;            // a cluster's mass, counts and counted tokens: 2 E + 1 words
 };
 
 struct Backward : Rows {
@@ -150,7 +149,8 @@ __device__ __forceinline__ double warp_sum(double v) {
   return v;
 }
 
-// Sums of a block's run of tokens: [tokens * b / blocks, tokens * (b + 1) / blocks).
+// Sums of a block's run of tokens, [tokens * b / blocks, tokens * (b + 1) / blocks), added
+// over a cluster; one block alone finishes by itself.
 template <class T, int V, int J, bool SIGMOID>
 __global__ void __launch_bounds__(kThreads, blocks_an_sm(J * V)) balance_forward(Forward f) {
   extern __shared__ uint32_t shared[];
@@ -158,9 +158,15 @@ __global__ void __launch_bounds__(kThreads, blocks_an_sm(J * V)) balance_forward
   float* const mass = reinterpret_cast<float*>(shared);       // [kWarps][E]
   uint32_t* const counts = shared + kWarps * E;                 // [E], and the counted tokens behind them
   asm volatile("griddepcontrol.launch_dependents;");
+  const unsigned begin = (uint64_t)f.tokens * blockIdx.x / gridDim.x, end = (uint64_t)f.tokens * (blockIdx.x + 1) / gridDim.x;
+  const unsigned step = kWarps * (32 / width), first = lane % width * V;
+  const T* const logits = static_cast<const T*>(f.logits);
+  Held<T, V, J> now, next;
+  unsigned row = begin + warp * (32 / width) + lane / width;
+  bool there = row < end && (!f.mask || f.mask[row]);
+  now.load(logits + (int64_t)row * f.stride, first, width, E, there);
   for (unsigned i = threadIdx.x; i <= E; i += kThreads) counts[i] = 0;
   __syncthreads();
-  const unsigned begin = (uint64_t)f.tokens * blockIdx.x / gridDim.x, end = (uint64_t)f.tokens * (blockIdx.x + 1) / gridDim.x;
   // entries and counted tokens
   for (unsigned i = begin * f.top_k + threadIdx.x; i < end * f.top_k; i += kThreads) {
     const unsigned e = (unsigned)f.chosen[i];
@@ -175,13 +181,7 @@ __global__ void __launch_bounds__(kThreads, blocks_an_sm(J * V)) balance_forward
     counts[E] = end - begin;
   }
   // mass
-  const unsigned step = kWarps * (32 / width), first = lane % width * V;
-  const T* const logits = static_cast<const T*>(f.logits);
   float sum[J * V] = {};
-  Held<T, V, J> now, next;
-  unsigned row = begin + warp * (32 / width) + lane / width;
-  bool there = row < end && (!f.mask || f.mask[row]);
-  now.load(logits + (int64_t)row * f.stride, first, width, E, there);
   while (__any_sync(~0u, row < end)) {
     const unsigned after = row + step;
     const bool more = after < end && (!f.mask || f.mask[after]);
@@ -213,15 +213,26 @@ __global__ void __launch_bounds__(kThreads, blocks_an_sm(J * V)) balance_forward
   }
   __syncthreads();
   if (gridDim.x > 1) {
-    uint32_t* const mine = f.sums + (size_t)blockIdx.x * (2 * E + 1);
     for (unsigned e = threadIdx.x; e < E; e += kThreads) {
       float s = 0.f;
 #pragma unroll
       for (unsigned w = 0; w < kWarps; ++w) s += mass[w * E + e];
-      mine[e] = __float_as_uint(s);
-      mine[E + e] = counts[e];
+      mass[e] = s;
     }
-    if (threadIdx.x == 0) mine[2 * E] = counts[E];
+    cluster_sync();
+    uint32_t* const mine = f.sums + (size_t)(blockIdx.x / kTogether) * (2 * E + 1);
+    for (unsigned e = threadIdx.x * kTogether + cluster_rank(); e <= E; e += kThreads * kTogether) {
+      float s = 0.f;
+      uint32_t n = 0;
+#pragma unroll
+      for (unsigned r = 0; r < kTogether; ++r) {
+        if (e < E) s += cluster_load(mass + e, r);
+        n += cluster_load(counts + e, r);
+      }
+      if (e < E) mine[e] = __float_as_uint(s);
+      mine[E + e] = n;
+    }
+    cluster_sync();                      // no block leaves while another reads from it
     return;
   }
   double dot = 0;
@@ -245,13 +256,12 @@ __global__ void __launch_bounds__(kThreads, blocks_an_sm(J * V)) balance_forward
   }
 }
 
-// Adds the blocks' sums up, one cluster: each of its blocks takes some experts, 32 lanes
-// a run of them, its warps the blocks in turn.
-__global__ void __cluster_dims__(kFinish) __launch_bounds__(kThreads) balance_finish(Forward f, unsigned blocks) {
-  namespace cg = cooperative_groups;
-  __shared__ double mass[kWarps][32];
-  __shared__ uint32_t counts[kWarps][32];
-  __shared__ uint32_t tokens[kWarps];
+// Adds the clusters' sums up, one cluster: each of its blocks takes some experts, 32 lanes
+// a run of them, its warps the sums in turn.
+__global__ void __cluster_dims__(kFinish) __launch_bounds__(kFinishThreads) balance_finish(Forward f, unsigned sums) {
+  __shared__ double mass[kFinishWarps][32];
+  __shared__ uint32_t counts[kFinishWarps][32];
+  __shared__ uint32_t tokens[kFinishWarps];
   __shared__ double mine;
   const unsigned E = f.experts, lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -261,7 +271,8 @@ __global__ void __cluster_dims__(kFinish) __launch_bounds__(kThreads) balance_fi
     double m = 0;
     uint32_t n = 0;
     if (e < E)
-      for (unsigned b = warp; b < blocks; b += kWarps) {
+#pragma unroll 5
+      for (unsigned b = warp; b < sums; b += kFinishWarps) {
         m += (double)__uint_as_float(f.sums[(size_t)b * (2 * E + 1) + e]);
         n += f.sums[(size_t)b * (2 * E + 1) + E + e];
       }
@@ -271,7 +282,7 @@ __global__ void __cluster_dims__(kFinish) __launch_bounds__(kThreads) balance_fi
     if (warp == 0 && e < E) {
       m = 0;
       n = 0;
-      for (unsigned w = 0; w < kWarps; ++w) {
+      for (unsigned w = 0; w < kFinishWarps; ++w) {
         m += mass[w][lane];
         n += counts[w][lane];
       }
@@ -283,7 +294,7 @@ __global__ void __cluster_dims__(kFinish) __launch_bounds__(kThreads) balance_fi
   }
   uint32_t n = 0;
   if (blockIdx.x == 0) {
-    for (unsigned b = threadIdx.x; b < blocks; b += kThreads) n += f.sums[(size_t)b * (2 * E + 1) + 2 * E];
+    for (unsigned b = threadIdx.x; b < sums; b += kFinishThreads) n += f.sums[(size_t)b * (2 * E + 1) + 2 * E];
     n = __reduce_add_sync(~0u, n);
     if (lane == 0) tokens[warp] = n;
   }
@@ -291,17 +302,16 @@ __global__ void __cluster_dims__(kFinish) __launch_bounds__(kThreads) balance_fi
     dot = warp_sum(dot);
     if (lane == 0) mine = dot;
   }
-  cg::cluster_group cluster = cg::this_cluster();
-  cluster.sync();
+  cluster_sync();
   if (blockIdx.x == 0 && threadIdx.x == 0) {
     dot = 0;
-    for (unsigned r = 0; r < kFinish; ++r) dot += *cluster.map_shared_rank(&mine, r);
+    for (unsigned r = 0; r < kFinish; ++r) dot += cluster_load(&mine, r);
     n = 0;
-    for (unsigned w = 0; w < kWarps; ++w) n += tokens[w];
+    for (unsigned w = 0; w < kFinishWarps; ++w) n += tokens[w];
     *f.counted = (int32_t)n;
     *f.loss = loss_of(dot, n, f);
   }
-  cluster.sync();                        // no block leaves while the first reads from it
+  cluster_sync();                        // no block leaves while the first reads from it
 }
 
 template <class T, int V, int J, bool SIGMOID>
@@ -408,24 +418,34 @@ void forward(Forward f, bool wide, bool sigmoid, unsigned grid, int device, cuda
       auto go = [&](auto s) {
         constexpr bool S = decltype(s)::value;
         room<balance_forward<T, V, J, S>>(device);
-        balance_forward<T, V, J, S><<<grid, kThreads, bytes, stream>>>(f);
+        cudaLaunchAttribute together{};
+        together.id = cudaLaunchAttributeClusterDimension;
+        together.val.clusterDim.x = grid == 1 ? 1 : kTogether;
+        together.val.clusterDim.y = together.val.clusterDim.z = 1;
+        cudaLaunchConfig_t config{};
+        config.gridDim = grid;
+        config.blockDim = kThreads;
+        config.dynamicSmemBytes = bytes;
+        config.stream = stream;
+        config.attrs = &together;
+        config.numAttrs = 1;
+        check(cudaLaunchKernelEx(&config, balance_forward<T, V, J, S>, f), "balance_forward");
       };
       sigmoid ? go(std::true_type{}) : go(std::false_type{});
     });
   };
   wide ? run(std::integral_constant<int, 16 / sizeof(T)>{}) : run(std::integral_constant<int, 1>{});
-  check(cudaGetLastError(), "balance_forward");
   if (grid == 1) return;
   cudaLaunchAttribute early{};
   early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   early.val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t config{};
   config.gridDim = kFinish;
-  config.blockDim = kThreads;
+  config.blockDim = kFinishThreads;
   config.stream = stream;
   config.attrs = &early;
   config.numAttrs = 1;
-  check(cudaLaunchKernelEx(&config, balance_finish, f, grid), "balance_finish");
+  check(cudaLaunchKernelEx(&config, balance_finish, f, grid / kTogether), "balance_finish");
 }
 
 template <class T>
@@ -444,9 +464,11 @@ void backward(Backward b, bool wide, bool sigmoid, int device, cudaStream_t stre
   check(cudaGetLastError(), "balance_backward");
 }
 
-// Blocks of the forward pass: some 8192 values each, so that a small batch takes one.
+// Blocks of the forward pass: some 8192 values each, so that a small batch takes one;
+// more come in clusters.
 unsigned forward_blocks(uint64_t tokens, uint32_t experts, unsigned sms) {
-  return (unsigned)std::max<uint64_t>(1, std::min<uint64_t>(ceil_div(tokens * experts, 8192), std::min(sms * 4, kMost)));
+  const uint64_t n = ceil_div(tokens * experts, 8192);
+  return n <= 1 ? 1 : (unsigned)std::min<uint64_t>(round_up(n, kTogether), std::min(sms * 4, kMost) / kTogether * kTogether);
 }
 
 bool wide_rows(const void* p, int64_t stride, size_t size) { return aligned(p, 16) && stride * (int64_t)size % 16 == 0; }
@@ -482,7 +504,7 @@ extern "C" {
 
 uint64_t eps_b200_balance_loss_workspace(uint64_t tokens, uint32_t experts) {
   const unsigned blocks = forward_blocks(tokens, experts, kMost);
-  return blocks == 1 ? 0 : (uint64_t)blocks * (2 * (uint64_t)experts + 1) * 4;
+  return blocks == 1 ? 0 : (uint64_t)blocks / kTogether * (2 * (uint64_t)experts + 1) * 4;
 }
 
 int eps_b200_balance_loss(const EpsB200BalanceLoss* a, const int32_t* chosen, float* loss, int32_t* counts, float* mass, int32_t* counted,

@@ -12,8 +12,6 @@
 // spans of 16 KB, each with its address, so one launch walks tensors of any size and
 // type.  Blocks leave one sum each and the next launch adds them, in the same order in
 // every block: no atomics, so results repeat exactly.
-#include <cooperative_groups.h>
-
 #include <algorithm>
 #include <cfloat>
 #include <cmath>
@@ -193,16 +191,15 @@ __global__ void __launch_bounds__(kThreads, kBlocksEach) gradient_finish(Call c,
 constexpr unsigned kCluster = 8, kClusterThreads = 1024, kClusterSpans = 96;
 template <int KIND, bool CLIP>
 __global__ void __cluster_dims__(kCluster) __launch_bounds__(kClusterThreads) gradient_few(Call c) {
-  namespace cg = cooperative_groups;
   using V = typename Gather<KIND>::V;
   __shared__ V mine;
   const V v = gather_spans<KIND>(c);
   if (threadIdx.x == 0) mine = v;
-  cg::cluster_group cluster = cg::this_cluster();
-  cluster.sync();
+  cluster_sync();
   V all = 0;
-  for (unsigned r = 0; r < kCluster; ++r) all = Gather<KIND>::join(all, *cluster.map_shared_rank(&mine, r));
-  cluster.sync();                        // no block leaves while another reads from it
+#pragma unroll
+  for (unsigned r = 0; r < kCluster; ++r) all = Gather<KIND>::join(all, cluster_load(&mine, r));
+  cluster_sync();                        // no block leaves while another reads from it
   const float scale = conclude(c, Gather<KIND>::norm(all), blockIdx.x == 0);
   if constexpr (CLIP) clip_spans(c, scale);
 }

@@ -12,10 +12,13 @@
 // memory, over the blocks; then its warps share out the channels.  One launch, no u in
 // memory; a launch before it sorts many rows by adapter.
 //
-// Fragments come straight from memory: a sum over k may take its terms in any order, so
-// each lane of a matrix instruction's row reads 16 consecutive bytes and gives them to
+// Fragments need no exchange between lanes: a sum over k may take its terms in any order,
+// so each lane of a matrix instruction's row takes 16 consecutive bytes and gives them to
 // the places that the instruction has for it, the same for both operands.  In the second
-// product the columns are dealt so that a lane ends up with 8 consecutive channels.
+// product the columns are dealt so that a lane ends up with 16 bytes of consecutive
+// channels.  So every lane copies what it needs itself, asynchronously and some turns
+// ahead, into shared memory that no other lane reads; the copies of base go on while u is
+// still being added up.
 //
 // Precision: 16-bit products are exact and summed in float.  u is not rounded to 16
 // bits: it goes on as the sum of two 16-bit values (float16: under a power of two of the
@@ -35,7 +38,7 @@ constexpr unsigned kThreads = 256, kWarps = kThreads / 32;
 constexpr unsigned kFew = 64;             // rows that the units are found for without a sort
 constexpr unsigned kUnitTiles = 4;        // 16-row tiles of a unit of sorted rows
 constexpr unsigned kUnit = kUnitTiles * 16;
-constexpr unsigned kSortThreads = 1024;
+constexpr unsigned kSortThreads = 1024, kSortBatch = 8;      // ids of a thread that are asked for at once
 
 struct Unit {
   int32_t adapter;                        // -1: none
@@ -80,26 +83,51 @@ __device__ __forceinline__ void cut(float a, float b, uint32_t (&p)[3]) {
 // The products of cut operands that count, small ones first: (plane of a, plane of b).
 __device__ constexpr int kTerms[6][2] = {{0, 2}, {2, 0}, {1, 1}, {0, 1}, {1, 0}, {0, 0}};
 
-// V values from p; those from `left` on are 0.  WIDE: all or none are there.
-template <class T, int V, bool WIDE>
-__device__ __forceinline__ Pack<T, V> load_part(const T* p, int left, bool once) {
-  Pack<T, V> r;
-  if constexpr (WIDE) {
-    if (left > 0) {
-      r = once ? load_once<T, V>(p) : load_pack<T, V>(p);
-    } else {
-#pragma unroll
-      for (int i = 0; i < V; ++i) r.v[i] = from_float<T>(0.f);
-    }
+// BYTES from p to this lane's place in shared memory, or zeros.
+template <int BYTES>
+__device__ __forceinline__ void copy_ahead(unsigned to, const void* p, bool there) {
+  if constexpr (BYTES == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(p), "r"(there ? 16 : 0) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(to), "l"(p), "n"(BYTES), "r"(there ? BYTES : 0) : "memory");
+}
+__device__ __forceinline__ void copies_end() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int LEFT>
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory"); }
+template <class P>
+__device__ __forceinline__ P own_shared(unsigned at) {
+  P r;
+  if constexpr (sizeof(P) == 16) {
+    uint4& x = reinterpret_cast<uint4&>(r);
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w) : "r"(at) : "memory");
+  } else if constexpr (sizeof(P) == 8) {
+    uint2& x = reinterpret_cast<uint2&>(r);
+    asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(x.x), "=r"(x.y) : "r"(at) : "memory");
   } else {
-#pragma unroll
-    for (int i = 0; i < V; ++i) r.v[i] = i < left ? p[i] : from_float<T>(0.f);
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(reinterpret_cast<uint32_t&>(r)) : "r"(at) : "memory");
   }
   return r;
 }
 
-template <class T, int V, bool WIDE>
-__device__ __forceinline__ void store_part(T* p, int left, const Pack<T, V>& r) {
+// 16 bytes of a row from p on, of which the first `left` values are there; the others are
+// 0.  WIDE: rows begin and end on 16 bytes.
+template <class T, bool WIDE>
+__device__ __forceinline__ void copy_row(unsigned to, const T* p, int left) {
+  constexpr int V = 16 / sizeof(T);
+  if constexpr (WIDE) {
+    copy_ahead<16>(to, p, left > 0);
+  } else {
+    Pack<T, V> r;
+#pragma unroll
+    for (int i = 0; i < V; ++i) r.v[i] = i < left ? p[i] : from_float<T>(0.f);
+    const uint4& x = reinterpret_cast<const uint4&>(r);
+    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(x.x), "r"(x.y), "r"(x.z), "r"(x.w) : "memory");
+  }
+}
+
+template <class T, bool WIDE>
+__device__ __forceinline__ void store_row(T* p, int left, const Pack<T, 16 / sizeof(T)>& r) {
+  constexpr int V = 16 / sizeof(T);
   if constexpr (WIDE) {
     if (left > 0) store_pack<T, V>(p, r);
   } else {
@@ -126,11 +154,24 @@ struct Shape {
   static constexpr int kPairsInOne = !kFloat && R == 8;          // both parts of u in one instruction
   static constexpr int kMultiplies = kPairsInOne || kRanks <= 4 ? kLoads : 2 * kLoads;
   static constexpr int kParts = kFloat ? 3 : kPairsInOne ? 1 : 2;
+  static constexpr int kRun = 4 * kEach;                         // channels that a warp takes at once
+  static constexpr int kMatrices = kEach / 2;                    // of 8 channels
   static constexpr bool kKeep = R * sizeof(T) <= 256;            // up's fragments stay in registers for all tiles
-  static constexpr size_t kSums = (size_t)kAlong * M * 16 * R * 4;
-  static constexpr size_t kFragments = (size_t)M * kMultiplies * kParts * 512;
+  // a warp's copies under way: pieces of a lane's 16 bytes of x and down, or of base and up
+  static constexpr bool kWeights = R * sizeof(T) <= 64;          // down and up are copied ahead too
+  static constexpr int kRows = (kTiles > M ? kTiles : M) * 2 * 512;
+  static constexpr int kDown = kWeights ? R / 8 * 512 : 0;
+  static constexpr int kUpPiece = kRanks * sizeof(T);
+  static constexpr int kUp = kWeights ? kMatrices * kLoads * kUpPiece * 32 : 0;
+  static constexpr int kSlot = kRows + (kDown > kUp ? kDown : kUp);
+  static constexpr int kAhead = M == 1 ? 4 : 2;
+  static constexpr size_t kCopies = (size_t)kWarps * kAhead * kSlot;
+  // the warps' sums, in two rounds; the first becomes the block's part, the others u's fragments
   static constexpr size_t kPart = (size_t)M * 16 * R * 4;
-  static constexpr size_t kBytes = (kSums > kFragments ? kSums : kFragments) + kPart;
+  static constexpr size_t kFragments = (size_t)M * kMultiplies * kParts * 512;
+  static constexpr int kRounds = kAlong > 1 ? 2 : 1;
+  static constexpr size_t kSums = kAlong / kRounds * kPart;
+  static constexpr size_t kBytes = kCopies + (kSums > kPart + kFragments ? kSums : kPart + kFragments);
 };
 
 // A unit's rows, as every block of the cluster finds them.
@@ -197,112 +238,180 @@ __device__ __forceinline__ bool find_sorted(const Call& c, unsigned number, Foun
   return true;
 }
 
-__device__ __forceinline__ unsigned cluster_rank() { unsigned r; asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
-__device__ __forceinline__ unsigned cluster_size() { unsigned r; asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(r)); return r; }
-__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive;" ::: "memory"); }
-__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait;" ::: "memory"); }
-__device__ __forceinline__ float2 cluster_load(const float* p, unsigned rank) {
-  unsigned at;
-  float2 v;
-  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(shared_at(p)), "r"(rank));
-  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(at));
-  return v;
-}
+// ----------------------------------------------------------------- a warp's turns
+// The turns of a warp's lane: steps along the inner size, then runs of channels.  Turn i's
+// copies lie in slot i % kAhead.
+template <class T, int R, int M, bool WIDE>
+struct Turns {
+  using S = Shape<T, R, M>;
+  const Call& c;
+  const Found<M>& f;
+  unsigned tiles, across, step, steps, run, runs, slots;     // first step and number of steps, first run and number of runs
+  const T *down, *up;
+
+  __device__ __forceinline__ Turns(const Call& c, const Found<M>& f, unsigned rank, unsigned blocks, unsigned shared) : c(c), f(f) {
+    const unsigned lane = threadIdx.x % 32, warp = threadIdx.x / 32, g = lane / 4, quad = lane % 4;
+    const unsigned along = warp / S::kAcross;
+    across = warp % S::kAcross;
+    tiles = (f.count + 15) / 16;
+    const unsigned all = c.padded / S::kStep, share = rank * S::kAlong + along, shares = blocks * S::kAlong;
+    step = (unsigned)((uint64_t)all * share / shares);
+    steps = across * S::kTiles < tiles ? (unsigned)((uint64_t)all * (share + 1) / shares) - step : 0;
+    const unsigned every = (c.channels + S::kRun - 1) / S::kRun;
+    run = (unsigned)((uint64_t)every * rank / blocks) + warp;
+    const unsigned end = (unsigned)((uint64_t)every * (rank + 1) / blocks);
+    runs = run < end ? (end - run + kWarps - 1) / kWarps : 0;
+    slots = shared + warp * S::kAhead * S::kSlot + lane * 16;
+    down = static_cast<const T*>(c.down) + ((uint64_t)f.adapter * R + g) * c.padded + quad * S::kEach;
+    up = static_cast<const T*>(c.up) + (uint64_t)f.adapter * c.channels * R + quad * S::kRanks;
+  }
+  __device__ __forceinline__ unsigned slot(unsigned i) const { return slots + i % S::kAhead * S::kSlot; }
+  __device__ __forceinline__ unsigned upper(unsigned i) const { return slot(i) + S::kRows; }
+  // where a lane's smaller pieces lie, one lane's next to the other's
+  __device__ __forceinline__ unsigned up_piece(unsigned i, int k) const {
+    return upper(i) - threadIdx.x % 32 * (16 - S::kUpPiece) + k * S::kUpPiece * 32;
+  }
+  __device__ __forceinline__ const T* down_at(unsigned i, int n) const { return down + (size_t)n * 8 * c.padded + (step + i) * S::kStep; }
+  // column g of matrix j is channel kEach (g / 2) + 2 j + g % 2 of the run
+  __device__ __forceinline__ const T* up_at(unsigned i, int j, int l) const {
+    const unsigned g = threadIdx.x % 32 / 4;
+    const unsigned channel = (run + (i - steps) * kWarps) * S::kRun + g / 2 * S::kEach + 2 * j + g % 2;
+    return up + (size_t)min(channel, c.channels - 1) * R + l * 4 * S::kRanks;
+  }
+
+  __device__ __forceinline__ void copy(unsigned i) const {
+    const unsigned lane = threadIdx.x % 32, g = lane / 4, quad = lane % 4;
+    if (i < steps) {
+      const unsigned k = (step + i) * S::kStep + quad * S::kEach;
+      const int left = (int)c.inner - (int)k;
+#pragma unroll
+      for (int m = 0; m < S::kTiles; ++m)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const unsigned r = (across * S::kTiles + m) * 16 + h * 8 + g;
+          const bool there = r < f.count;        // a row behind the unit's last counts as zeros
+          copy_row<T, WIDE>(slot(i) + (m * 2 + h) * 512, static_cast<const T*>(c.x) + (int64_t)f.row[there ? r : 0] * c.x_stride + (left > 0 ? k : 0),
+                            there ? left : 0);
+        }
+      if constexpr (S::kWeights) {
+#pragma unroll
+        for (int n = 0; n < R / 8; ++n) copy_ahead<16>(upper(i) + n * 512, down_at(i, n), true);
+      }
+    } else if (i < steps + runs) {
+      const unsigned at = (run + (i - steps) * kWarps) * S::kRun + quad * S::kEach;
+      const int left = (int)c.channels - (int)at;
+      if (c.base) {
+#pragma unroll
+        for (int m = 0; m < M; ++m) {
+          if (m >= tiles) break;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const unsigned r = m * 16 + h * 8 + g;
+            const bool there = r < f.count;
+            copy_row<T, WIDE>(slot(i) + (m * 2 + h) * 512,
+                              static_cast<const T*>(c.base) + (int64_t)f.row[there ? r : 0] * c.base_stride + (left > 0 ? at : 0), there ? left : 0);
+          }
+        }
+      }
+      if constexpr (S::kWeights) {
+#pragma unroll
+        for (int j = 0; j < S::kMatrices; ++j)
+#pragma unroll
+          for (int l = 0; l < S::kLoads; ++l) copy_ahead<S::kUpPiece>(up_piece(i, j * S::kLoads + l), up_at(i, j, l), true);
+      }
+    }
+    copies_end();
+  }
+};
 
 // ------------------------------------------------------------------- u = down x
 template <class T, int R, int M, bool WIDE>
-__device__ __forceinline__ void inner_product(const Call& c, const Found<M>& f, unsigned rank, unsigned blocks, float* sums) {
+__device__ __forceinline__ void inner_product(const Turns<T, R, M, WIDE>& t, float* sums) {
   using S = Shape<T, R, M>;
+  using P = Pack<T, S::kEach>;
   constexpr int kCols = R / 8;
-  const unsigned lane = threadIdx.x % 32, warp = threadIdx.x / 32, g = lane / 4, quad = lane % 4;
-  const unsigned across = warp % S::kAcross, along = warp / S::kAcross;
   float acc[S::kTiles][kCols][4] = {};
-  const unsigned tiles = (f.count + 15) / 16;
-  if (across * S::kTiles < tiles) {
-    const unsigned steps = c.padded / S::kStep, share = rank * S::kAlong + along, shares = blocks * S::kAlong;
-    const unsigned begin = (uint64_t)steps * share / shares, end = (uint64_t)steps * (share + 1) / shares;
-    // rows behind the unit's last stand for its first: what they give is not used
-    const T* x[S::kTiles][2];
+  for (unsigned i = 0; i < t.steps; ++i) {
+    P d[kCols], x[S::kTiles][2];
+    if constexpr (!S::kWeights) {
+#pragma unroll
+      for (int n = 0; n < kCols; ++n) d[n] = load_pack<T, S::kEach>(t.down_at(i, n));
+    }
+    copies_wait<S::kAhead - 1>();
 #pragma unroll
     for (int m = 0; m < S::kTiles; ++m)
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const unsigned r = (across * S::kTiles + m) * 16 + h * 8 + g;
-        x[m][h] = static_cast<const T*>(c.x) + (int64_t)f.row[r < f.count ? r : 0] * c.x_stride + quad * S::kEach;
-      }
-    const T* const down = static_cast<const T*>(c.down) + ((uint64_t)f.adapter * R + g) * c.padded + quad * S::kEach;
-    using P = Pack<T, S::kEach>;
-    P now[S::kTiles][2], next[S::kTiles][2];
-    auto load = [&](P(&to)[S::kTiles][2], unsigned step) {
-      const int left = (int)c.inner - (int)(step * S::kStep + quad * S::kEach);
+      for (int h = 0; h < 2; ++h) x[m][h] = own_shared<P>(t.slot(i) + (m * 2 + h) * 512);
+    if constexpr (S::kWeights) {
 #pragma unroll
-      for (int m = 0; m < S::kTiles; ++m)
+      for (int n = 0; n < kCols; ++n) d[n] = own_shared<P>(t.upper(i) + n * 512);
+    }
+    t.copy(i + S::kAhead);
+    if constexpr (S::kFloat) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) to[m][h] = load_part<T, S::kEach, WIDE>(x[m][h] + step * S::kStep, left, true);
-    };
-    if (begin < end) load(now, begin);
-    for (unsigned s = begin; s < end; ++s) {
-      P d[kCols];
+      for (int m = 0; m < S::kTiles; ++m) {
+        uint32_t a[3][4];
 #pragma unroll
-      for (int n = 0; n < kCols; ++n) d[n] = load_pack<T, S::kEach>(down + (size_t)n * 8 * c.padded + s * S::kStep);
-      if (s + 1 < end) load(next, s + 1);
-      if constexpr (S::kFloat) {
+        for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int m = 0; m < S::kTiles; ++m) {
-          uint32_t a[3][4];
+          for (int e = 0; e < 2; ++e) {
+            uint32_t p[3];
+            cut(x[m][h].v[2 * e], x[m][h].v[2 * e + 1], p);
 #pragma unroll
-          for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              uint32_t p[3];
-              cut(now[m][h].v[2 * i], now[m][h].v[2 * i + 1], p);
-#pragma unroll
-              for (int q = 0; q < 3; ++q) a[q][2 * i + h] = p[q];
-            }
-#pragma unroll
-          for (int n = 0; n < kCols; ++n) {
-            uint32_t b0[3], b1[3];
-            cut(d[n].v[0], d[n].v[1], b0);
-            cut(d[n].v[2], d[n].v[3], b1);
-            // summed apart and added in float: the matrix instruction's sums are cut off, not rounded
-            float part[4] = {};
-#pragma unroll
-            for (int q = 0; q < 6; ++q) multiply<bf16>(part, a[kTerms[q][0]], b0[kTerms[q][1]], b1[kTerms[q][1]]);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) acc[m][n][i] += part[i];
+            for (int q = 0; q < 3; ++q) a[q][2 * e + h] = p[q];
           }
-        }
-      } else {
 #pragma unroll
         for (int n = 0; n < kCols; ++n) {
-          const uint32_t* const b = reinterpret_cast<const uint32_t*>(&d[n]);
+          uint32_t b0[3], b1[3];
+          cut(d[n].v[0], d[n].v[1], b0);
+          cut(d[n].v[2], d[n].v[3], b1);
+          // summed apart and added in float: the matrix instruction's sums are cut off, not rounded
+          float part[4] = {};
 #pragma unroll
-          for (int m = 0; m < S::kTiles; ++m) {
-            const uint32_t* const lo = reinterpret_cast<const uint32_t*>(&now[m][0]);
-            const uint32_t* const hi = reinterpret_cast<const uint32_t*>(&now[m][1]);
+          for (int q = 0; q < 6; ++q) multiply<bf16>(part, a[kTerms[q][0]], b0[kTerms[q][1]], b1[kTerms[q][1]]);
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-              const uint32_t a[4] = {lo[2 * k], hi[2 * k], lo[2 * k + 1], hi[2 * k + 1]};
-              multiply<T>(acc[m][n], a, b[2 * k], b[2 * k + 1]);
-            }
+          for (int e = 0; e < 4; ++e) acc[m][n][e] += part[e];
+        }
+      }
+    } else {
+#pragma unroll
+      for (int n = 0; n < kCols; ++n) {
+        const uint32_t* const b = reinterpret_cast<const uint32_t*>(&d[n]);
+#pragma unroll
+        for (int m = 0; m < S::kTiles; ++m) {
+          const uint32_t* const lo = reinterpret_cast<const uint32_t*>(&x[m][0]);
+          const uint32_t* const hi = reinterpret_cast<const uint32_t*>(&x[m][1]);
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const uint32_t a[4] = {lo[2 * k], hi[2 * k], lo[2 * k + 1], hi[2 * k + 1]};
+            multiply<T>(acc[m][n], a, b[2 * k], b[2 * k + 1]);
           }
         }
       }
+    }
+  }
+  // the warps along the inner size write their sums, half of them at a time
+  const unsigned lane = threadIdx.x % 32, g = lane / 4, quad = lane % 4, along = threadIdx.x / 32 / S::kAcross;
+  constexpr unsigned kHalf = S::kAlong / S::kRounds;
+#pragma unroll
+  for (unsigned round = 0; round < S::kRounds; ++round) {
+    if (round) __syncthreads();
+    if (along / kHalf == round) {
 #pragma unroll
       for (int m = 0; m < S::kTiles; ++m)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) now[m][h] = next[m][h];
+        for (int h = 0; h < 2; ++h) {
+          float* const row = sums + ((along % kHalf * M + t.across * S::kTiles + m) * 16 + h * 8 + g) * R + 2 * quad;
+#pragma unroll
+          for (int n = 0; n < kCols; ++n) {
+            float2& to = *reinterpret_cast<float2*>(row + n * 8);
+            float2 v = make_float2(acc[m][n][2 * h], acc[m][n][2 * h + 1]);
+            if (round) v.x += to.x, v.y += to.y;
+            to = v;
+          }
+        }
     }
   }
-  float* const mine = sums + (size_t)along * M * 16 * R;
-#pragma unroll
-  for (int m = 0; m < S::kTiles; ++m)
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      float* const row = mine + ((across * S::kTiles + m) * 16 + h * 8 + g) * R + 2 * quad;
-#pragma unroll
-      for (int n = 0; n < kCols; ++n) *reinterpret_cast<float2*>(row + n * 8) = make_float2(acc[m][n][2 * h], acc[m][n][2 * h + 1]);
-    }
 }
 
 // --------------------------------------------------- u as the next product's fragments
@@ -335,7 +444,7 @@ __device__ __forceinline__ void lay_out(const Call& c, const Found<M>& f, unsign
       const unsigned r = 2 * (i * kLanes + q);
       u[i] = make_float2(0.f, 0.f);
       for (unsigned b = 0; b < blocks; ++b) {
-        const float2 v = cluster_load(part + row * R + r, b);
+        const float2 v = cluster_load(reinterpret_cast<const float2*>(part + row * R + r), b);
         u[i].x += v.x;
         u[i].y += v.y;
       }
@@ -389,51 +498,41 @@ __device__ __forceinline__ void lay_out(const Call& c, const Found<M>& f, unsign
 
 // ------------------------------------------------------- out = base + factor * up u
 template <class T, int R, int M, bool WIDE>
-__device__ __forceinline__ void outer_product(const Call& c, const Found<M>& f, unsigned rank, unsigned blocks, const uint32_t* fragments,
-                                              const float* factor) {
+__device__ __forceinline__ void outer_product(const Turns<T, R, M, WIDE>& t, const uint32_t* fragments, const float* factor) {
   using S = Shape<T, R, M>;
   using P = Pack<T, S::kRanks>;
-  using O = Pack<T, 8>;
-  const unsigned lane = threadIdx.x % 32, warp = threadIdx.x / 32, g = lane / 4, quad = lane % 4;
-  const unsigned tiles = (f.count + 15) / 16, runs = (c.channels + 31) / 32;
-  const unsigned begin = (uint64_t)runs * rank / blocks, end = (uint64_t)runs * (rank + 1) / blocks;
-  const T* const up = static_cast<const T*>(c.up) + (uint64_t)f.adapter * c.channels * R + quad * S::kRanks;
-  for (unsigned run = begin + warp; run < end; run += kWarps) {
-    const unsigned at = run * 32 + quad * 8;          // this lane's channels
+  using O = Pack<T, S::kEach>;
+  const Call& c = t.c;
+  const unsigned lane = threadIdx.x % 32, g = lane / 4, quad = lane % 4;
+  for (unsigned i = t.steps; i < t.steps + t.runs; ++i) {
+    const unsigned at = (t.run + (i - t.steps) * kWarps) * S::kRun + quad * S::kEach;          // this lane's channels
     const int left = (int)c.channels - (int)at;
+    P held[S::kKeep ? S::kMatrices : 1][S::kKeep ? S::kLoads : 1];
+    if constexpr (S::kKeep && !S::kWeights) {
+#pragma unroll
+      for (int j = 0; j < S::kMatrices; ++j)
+#pragma unroll
+        for (int l = 0; l < S::kLoads; ++l) held[j][l] = load_pack<T, S::kRanks>(t.up_at(i, j, l));
+    }
+    copies_wait<S::kAhead - 1>();
     O before[M][2];
-    auto load_base = [&](int m) {
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const unsigned r = m * 16 + h * 8 + g;
-        if (c.base && r < f.count)
-          before[m][h] = load_part<T, 8, WIDE>(static_cast<const T*>(c.base) + (int64_t)f.row[r] * c.base_stride + at, left, true);
-        else
+    for (int m = 0; m < M; ++m)
+      if (m < t.tiles && c.base) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) before[m][h].v[i] = from_float<T>(0.f);
+        for (int h = 0; h < 2; ++h) before[m][h] = own_shared<O>(t.slot(i) + (m * 2 + h) * 512);
       }
-    };
-    if constexpr (!S::kFloat) {
+    if constexpr (S::kWeights) {
 #pragma unroll
-      for (int m = 0; m < M; ++m)
-        if (m < tiles) load_base(m);
+      for (int j = 0; j < S::kMatrices; ++j)
+#pragma unroll
+        for (int l = 0; l < S::kLoads; ++l) held[j][l] = own_shared<P>(t.up_piece(i, j * S::kLoads + l));
     }
-    // column g of matrix j is channel 8 (g / 2) + 2 j + g % 2 of the run
-    const T* channel[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) channel[j] = up + (size_t)min(run * 32 + g / 2 * 8 + 2 * j + g % 2, c.channels - 1) * R;
-    P held[S::kKeep ? 4 : 1][S::kKeep ? S::kLoads : 1];
-    if constexpr (S::kKeep) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int l = 0; l < S::kLoads; ++l) held[j][l] = load_pack<T, S::kRanks>(channel[j] + l * 4 * S::kRanks);
-    }
+    t.copy(i + S::kAhead);
 #pragma unroll
     for (int m = 0; m < M; ++m) {
-      if (m >= tiles) break;
-      if constexpr (S::kFloat) load_base(m);
-      float acc[4][4] = {};
+      if (m >= t.tiles) break;
+      float acc[S::kMatrices][4] = {};
 #pragma unroll
       for (int l = 0; l < S::kLoads; ++l) {
 #pragma unroll
@@ -446,19 +545,19 @@ __device__ __forceinline__ void outer_product(const Call& c, const Found<M>& f, 
             a[p][0] = w.x, a[p][1] = w.y, a[p][2] = w.z, a[p][3] = w.w;
           }
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
+          for (int j = 0; j < S::kMatrices; ++j) {
             P d;
             if constexpr (S::kKeep) d = held[j][l];
-            else d = load_pack<T, S::kRanks>(channel[j] + l * 4 * S::kRanks);
+            else d = load_pack<T, S::kRanks>(t.up_at(i, j, l));
             if constexpr (S::kFloat) {
               uint32_t b0[3], b1[3] = {0, 0, 0};
               cut(d.v[0], d.v[1], b0);
               if constexpr (S::kRanks == 4) cut(d.v[2], d.v[3], b1);
               float part[4] = {};
 #pragma unroll
-              for (int t = 0; t < 6; ++t) multiply<bf16>(part, a[kTerms[t][0]], b0[kTerms[t][1]], b1[kTerms[t][1]]);
+              for (int n = 0; n < 6; ++n) multiply<bf16>(part, a[kTerms[n][0]], b0[kTerms[n][1]], b1[kTerms[n][1]]);
 #pragma unroll
-              for (int i = 0; i < 4; ++i) acc[j][i] += part[i];
+              for (int e = 0; e < 4; ++e) acc[j][e] += part[e];
             } else {
               const uint32_t* const b = reinterpret_cast<const uint32_t*>(&d);
               if constexpr (S::kPairsInOne) {
@@ -474,15 +573,20 @@ __device__ __forceinline__ void outer_product(const Call& c, const Found<M>& f, 
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const unsigned r = m * 16 + h * 8 + g;
-        if (r >= f.count) continue;
-        float v[8];
-        widen(before[m][h], v);
+        if (r >= t.f.count) continue;
+        float v[S::kEach];
+        if (c.base) {
+          widen(before[m][h], v);
+        } else {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
+          for (int e = 0; e < S::kEach; ++e) v[e] = 0.f;
+        }
+#pragma unroll
+        for (int j = 0; j < S::kMatrices; ++j) {
           v[2 * j] = fmaf(acc[j][2 * h], factor[r], v[2 * j]);
           v[2 * j + 1] = fmaf(acc[j][2 * h + 1], factor[r], v[2 * j + 1]);
         }
-        store_part<T, 8, WIDE>(static_cast<T*>(c.out) + (int64_t)f.row[r] * c.out_stride + at, left, narrow<T, 8>(v));
+        store_row<T, WIDE>(static_cast<T*>(c.out) + (int64_t)t.f.row[r] * c.out_stride + at, left, narrow<T, S::kEach>(v));
       }
     }
   }
@@ -492,18 +596,19 @@ __device__ __forceinline__ void outer_product(const Call& c, const Found<M>& f, 
 template <class T, int M, bool WIDE>
 __device__ __forceinline__ void copy_rows(const Call& c, const Found<M>& f, unsigned rank, unsigned blocks) {
   if (c.base == c.out) return;
-  const unsigned packs = (c.channels + 7) / 8;
-  const unsigned begin = (uint64_t)packs * rank / blocks, end = (uint64_t)packs * (rank + 1) / blocks;
+  constexpr unsigned V = WIDE ? 16 / sizeof(T) : 1;
+  const unsigned packs = (c.channels + V - 1) / V;
+  const unsigned begin = (unsigned)((uint64_t)packs * rank / blocks), end = (unsigned)((uint64_t)packs * (rank + 1) / blocks);
   for (unsigned r = threadIdx.x / 32; r < f.count; r += kWarps)
     for (unsigned p = begin + threadIdx.x % 32; p < end; p += 32) {
-      Pack<T, 8> v;
+      Pack<T, V> v;
       if (c.base) {
-        v = load_part<T, 8, WIDE>(static_cast<const T*>(c.base) + (int64_t)f.row[r] * c.base_stride + p * 8, (int)c.channels - (int)(p * 8), true);
+        v = load_once<T, V>(static_cast<const T*>(c.base) + (int64_t)f.row[r] * c.base_stride + p * V);
       } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v.v[i] = from_float<T>(0.f);
+        for (unsigned i = 0; i < V; ++i) v.v[i] = from_float<T>(0.f);
       }
-      store_part<T, 8, WIDE>(static_cast<T*>(c.out) + (int64_t)f.row[r] * c.out_stride + p * 8, (int)c.channels - (int)(p * 8), v);
+      store_pack<T, V>(static_cast<T*>(c.out) + (int64_t)f.row[r] * c.out_stride + p * V, v);
     }
 }
 
@@ -524,25 +629,29 @@ __global__ void __launch_bounds__(kThreads, 2) low_rank_rows(Call c) {
     copy_rows<T, M, WIDE>(c, found, rank, blocks);
     return;
   }
-  float* const sums = reinterpret_cast<float*>(shared);
-  float* const part = reinterpret_cast<float*>(shared + S::kBytes - S::kPart);
-  inner_product<T, R, M, WIDE>(c, found, rank, blocks, sums);
+  const Turns<T, R, M, WIDE> turns(c, found, rank, blocks, shared_at(shared));
+  for (unsigned i = 0; i < S::kAhead; ++i) turns.copy(i);
+  float* const part = reinterpret_cast<float*>(shared + S::kCopies);
+  uint32_t* const fragments = reinterpret_cast<uint32_t*>(shared + S::kCopies + S::kPart);
+  inner_product<T, R, M, WIDE>(turns, part);
   __syncthreads();
-  for (unsigned i = threadIdx.x; i < M * 16 * R / 4; i += kThreads) {
-    float4 s = reinterpret_cast<const float4*>(sums)[i];
+  constexpr int kWritten = S::kAlong / S::kRounds;
+  if constexpr (kWritten > 1) {
+    for (unsigned i = threadIdx.x; i < M * 16 * R / 4; i += kThreads) {
+      float4 s = reinterpret_cast<const float4*>(part)[i];
 #pragma unroll
-    for (int w = 1; w < S::kAlong; ++w) {
-      const float4 v = reinterpret_cast<const float4*>(sums)[w * (M * 16 * R / 4) + i];
-      s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
+      for (int w = 1; w < kWritten; ++w) {
+        const float4 v = reinterpret_cast<const float4*>(part)[w * (M * 16 * R / 4) + i];
+        s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
+      }
+      reinterpret_cast<float4*>(part)[i] = s;
     }
-    reinterpret_cast<float4*>(part)[i] = s;
   }
-  cluster_arrive();
-  cluster_wait();
-  lay_out<T, R, M>(c, found, blocks, part, reinterpret_cast<uint32_t*>(shared), factor);
+  cluster_sync();
+  lay_out<T, R, M>(c, found, blocks, part, fragments, factor);
   __syncthreads();
   cluster_arrive();                        // this block has read from the others
-  outer_product<T, R, M, WIDE>(c, found, rank, blocks, reinterpret_cast<const uint32_t*>(shared), factor);
+  outer_product<T, R, M, WIDE>(turns, fragments, factor);
   cluster_wait();                          // no block leaves while another reads from it
 }
 
@@ -562,11 +671,19 @@ __global__ void __launch_bounds__(kSortThreads) low_rank_sort(const int32_t* ids
   __syncthreads();
   const unsigned turns = (rows + kSortThreads - 1) / kSortThreads;
   auto each = [&](auto what) {              // whole warps; lanes of one adapter go together
-    for (unsigned i = 0; i < turns; ++i) {
-      const unsigned r = i * kSortThreads + t;
-      const uint32_t a = r < rows ? min((uint32_t)ids[r], adapters) : ~0u;
-      const unsigned peers = __match_any_sync(~0u, a);
-      if (r < rows) what(r, a, peers);
+    for (unsigned i = 0; i < turns; i += kSortBatch) {
+      uint32_t a[kSortBatch];
+#pragma unroll
+      for (unsigned j = 0; j < kSortBatch; ++j) {
+        const unsigned r = (i + j) * kSortThreads + t;
+        a[j] = r < rows ? min((uint32_t)ids[r], adapters) : ~0u;
+      }
+#pragma unroll
+      for (unsigned j = 0; j < kSortBatch; ++j) {
+        if (i + j >= turns) break;
+        const unsigned peers = __match_any_sync(~0u, a[j]);
+        if (a[j] != ~0u) what((i + j) * kSortThreads + t, a[j], peers);
+      }
     }
   };
   each([&](unsigned, uint32_t a, unsigned peers) {
@@ -756,7 +873,7 @@ int eps_b200_low_rank(const EpsB200LowRank* a, void* stream, EpsB200Status* stat
     c.channels = a->channels;
     OnDevice on(a->device);
     const bool wide = wide_rows(a->x, a->x_stride, size) && a->inner * size % 16 == 0 && wide_rows(a->out, a->out_stride, size) &&
-                      (!a->base || wide_rows(a->base, a->base_stride, size)) && a->channels % 8 == 0;
+                      (!a->base || wide_rows(a->base, a->base_stride, size)) && a->channels * size % 16 == 0;
     const auto s = static_cast<cudaStream_t>(stream);
     if (a->type == EPS_B200_F32) launch<float>(c, wide, a->workspace, a->device, s);
     else if (a->type == EPS_B200_BF16) launch<bf16>(c, wide, a->workspace, a->device, s);
