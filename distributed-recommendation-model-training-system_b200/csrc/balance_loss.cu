@@ -26,13 +26,13 @@ namespace eps_b200 {
 namespace dense {
 namespace {
 
-constexpr unsigned kThreads = 256, kWarps = kThreads / 32;
-// Blocks an SM, by the columns of a lane: what their registers leave room for.
-constexpr unsigned blocks_an_sm(int columns) { return columns <= 8 ? 4 : columns <= 16 ? 2 : 1; }
-constexpr unsigned kTogether = 4;         // blocks whose sums are added before they leave them
+// One block an SM, as many threads as the columns of a lane leave registers for.
+template <int COLUMNS> constexpr unsigned kThreadsFor = COLUMNS <= 8 ? 1024 : COLUMNS <= 16 ? 512 : 256;
 constexpr unsigned kMost = 1024;          // most blocks
-constexpr unsigned kFinish = 8, kFinishThreads = 512, kFinishWarps = kFinishThreads / 32;      // blocks that add up what is left
+constexpr unsigned kFinish = 8, kFinishThreads = 512, kFinishWarps = kFinishThreads / 32;      // blocks that add their sums up
 
+constexpr unsigned kAhead = 4;                                          // rows that a lane of the forward pass copies ahead
+template <class T> constexpr unsigned kAheadBack = sizeof(T) == 4 ? 3 : 4;      // of the backward pass, from two tensors
 struct Rows {
   const void* logits;
   int64_t stride;
@@ -49,7 +49,7 @@ struct Forward : Rows {
   int32_t* counts;
   float* mass;
   int32_t* counted;
-  uint32_t* sums;            // a cluster's mass, counts and counted tokens: 2 E + 1 words
+  uint32_t* sums;            // a block's mass, counts and counted tokens: 2 E + 1 words
 };
 
 struct Backward : Rows {
@@ -62,18 +62,30 @@ struct Backward : Rows {
   int64_t out_stride;
 };
 
-// e^x for x <= 88; 0 below -200, and NaN stays.  The power of two takes x log2 e rounded
-// to a float, off by |x| / 2 units; float logits add back what that lost (the product's
-// error by a fused multiply-add, and the rest of log2 e).
-template <bool FINE>
-__device__ __forceinline__ float power(float x) {
-  constexpr float kLog2e = 1.44269502f, kRest = 1.92596303e-8f, kLn2 = 0.693147182f;   // log2 e in two parts; ln 2
-  x = x < -200.f ? -200.f : x;
-  const float t = x * kLog2e;
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(t));
-  if constexpr (FINE) r = fmaf(r, fmaf(x, kRest, fmaf(x, kLog2e, -t)) * kLn2, r);
-  return r;
+// The larger and the smaller of two values; NaN if one is.
+__device__ __forceinline__ float most(float a, float b) { float r; asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b)); return r; }
+__device__ __forceinline__ float least(float a, float b) { float r; asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b)); return r; }
+
+// e^x of N values up to 88.5.  The power of two takes x log2 e rounded to a float, off by
+// |x| / 2 units; float logits add back what that lost, x less that power's logarithm.
+template <int N, bool FINE>
+__device__ __forceinline__ void powers(float (&x)[N]) {
+  constexpr float kLog2e = 1.44269504f, kLn2 = 0.693147181f;
+  if constexpr (FINE) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = most(x[i], -200.f);      // below it is 0 anyway, and an infinity has no rest
+  }
+  float t[N];
+  vmul<N>(t, x, kLog2e);
+  if constexpr (FINE) vfma<N>(x, t, -kLn2, x);
+#pragma unroll
+  for (int i = 0; i < N; ++i) asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(t[i]));
+  if constexpr (FINE) {
+    vfma<N>(x, t, x, t);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = t[i];
+  }
 }
 
 __device__ __forceinline__ float inverse(float x) {
@@ -89,52 +101,85 @@ __device__ __forceinline__ float row_add(float v, unsigned width) {
   for (unsigned o = width / 2; o; o /= 2) v += __shfl_xor_sync(~0u, v, o);
   return v;
 }
+__device__ __forceinline__ float row_most(float v, unsigned width) {
+  for (unsigned o = width / 2; o; o /= 2) v = fmaxf(v, __shfl_xor_sync(~0u, v, o));
+  return v;
+}
 
-// A lane's packs of a row: pack j covers the V columns from (j * width + lane) * V on.
-template <class T, int V, int J>
-struct Held {
-  Pack<T, V> p[J];
-  __device__ __forceinline__ void load(const T* row, unsigned first, unsigned width, unsigned columns, bool there) {
+// The sum of a lane's values, two halves at a time.
+template <int N>
+__device__ __forceinline__ float lane_sum(const float (&v)[N]) {
+  if constexpr (N == 1) {
+    return v[0];
+  } else {
+    float half[N / 2 + N % 2];
+    vadd<N / 2>(reinterpret_cast<float(&)[N / 2]>(half), reinterpret_cast<const float(&)[N / 2]>(v[0]), reinterpret_cast<const float(&)[N / 2]>(v[N / 2]));
+    if constexpr (N % 2) half[N / 2] = v[N - 1];
+    return lane_sum<N / 2 + N % 2>(half);
+  }
+}
+
+// A lane's packs of a row, pack j the V columns from (j * width + lane) * V on, copied ahead
+// to shared memory, AHEAD rows of them.
+template <class T, int V, int J, unsigned THREADS, unsigned AHEAD>
+struct Copies {
+  static constexpr unsigned kBytes = V * sizeof(T), kRow = J * THREADS * kBytes, kAll = AHEAD * kRow;
+  unsigned at, here;       // the packs of this lane in its row, a bit each
+  // What is behind the last column is `rest` once and for all: no copy reaches it.
+  __device__ __forceinline__ Copies(void* shared, unsigned first, unsigned width, unsigned columns, float rest)
+      : at(shared_at(shared) + threadIdx.x * kBytes), here(0) {
+    Pack<T, V> r;
+#pragma unroll
+    for (int i = 0; i < V; ++i) r.v[i] = from_float<T>(rest);
 #pragma unroll
     for (int j = 0; j < J; ++j) {
-      const unsigned c = first + j * width * V;
-      if (there && c < columns) p[j] = load_once<T, V>(row + c);
+      if (first + j * width * V < columns) {
+        here |= 1u << j;
+      } else {
+        for (unsigned k = 0; k < AHEAD; ++k) *reinterpret_cast<Pack<T, V>*>(static_cast<char*>(shared) + k * kRow + (j * THREADS + threadIdx.x) * kBytes) = r;
+      }
     }
+  }
+  __device__ __forceinline__ void copy(unsigned turn, const T* row, unsigned width, bool there) const {
+    const unsigned to = at + turn % AHEAD * kRow;
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      if (!there || !(here >> j & 1)) continue;
+      if constexpr (kBytes >= 4)
+        copy_ahead<(int)kBytes>(to + j * THREADS * kBytes, row + j * width * V, true);
+      else
+        asm volatile("st.shared.u16 [%0], %1;" ::"r"(to + j * THREADS * kBytes), "h"(reinterpret_cast<const unsigned short*>(row)[j * width * V]) : "memory");
+    }
+  }
+  __device__ __forceinline__ void read(unsigned turn, float (&v)[J * V]) const {
+    const unsigned from = at + turn % AHEAD * kRow;
+#pragma unroll
+    for (int j = 0; j < J; ++j) widen(own_shared<Pack<T, V>>(from + j * THREADS * kBytes), *reinterpret_cast<float(*)[V]>(v + j * V));
   }
 };
 
-// The scores of a row: its unnormalised p in v and, for sigmoids, 1 - s in rest.  What is
-// behind the last column, or in a row that is not there, is 0.
-template <class T, int V, int J, bool SIGMOID>
-__device__ __forceinline__ void scores(const Held<T, V, J>& h, unsigned first, unsigned width, unsigned columns, bool there, float (&v)[J * V],
-                                       float (&rest)[SIGMOID ? J * V : 1]) {
+// The scores of a row of logits, -inf behind its last column: its unnormalised p and, for
+// sigmoids, 1 - s in rest.
+template <class T, int N, bool SIGMOID>
+__device__ __forceinline__ void scores(float (&v)[N], float (&rest)[SIGMOID ? N : 1], unsigned width) {
   constexpr bool kFine = std::is_same_v<T, float>;
-#pragma unroll
-  for (int j = 0; j < J; ++j) {
-    if (there && first + j * width * V < columns) {
-      widen(h.p[j], *reinterpret_cast<float(*)[V]>(v + j * V));
-    } else {
-#pragma unroll
-      for (int i = 0; i < V; ++i) v[j * V + i] = -INFINITY;
-    }
-  }
   if constexpr (SIGMOID) {
+    // s = 1 / (1 + e), 1 - s = e s with e = e^-x; at 88.5 s is 0, as behind it
+    float e[N];
 #pragma unroll
-    for (int i = 0; i < J * V; ++i) {
-      const bool low = v[i] < -87.f;          // s would leave the normal floats: 0
-      const float e = low ? 1.f : power<kFine>(-v[i]);
-      const float s = inverse(1.f + e);
-      rest[i] = e * s;
-      v[i] = low ? 0.f : s;
-    }
+    for (int i = 0; i < N; ++i) e[i] = least(-v[i], 88.5f);
+    powers<N, kFine>(e);
+    vadd<N>(v, e, 1.f);
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = inverse(v[i]);
+    vmul<N>(rest, e, v);
   } else {
-    float top = -INFINITY;
+    float top = v[0];
 #pragma unroll
-    for (int i = 0; i < J * V; ++i) top = fmaxf(top, v[i]);
-    for (unsigned o = width / 2; o; o /= 2) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
-    const float less = top == -INFINITY ? 0.f : top;       // a row of -inf alone gives zeros, not NaN
-#pragma unroll
-    for (int i = 0; i < J * V; ++i) v[i] = power<kFine>(v[i] - less);
+    for (int i = 1; i < N; ++i) top = fmaxf(top, v[i]);
+    top = row_most(top, width);
+    vadd<N>(v, v, top == -INFINITY ? 0.f : -top);       // a row of -inf alone gives zeros, not NaN
+    powers<N, kFine>(v);
   }
 }
 
@@ -149,22 +194,34 @@ __device__ __forceinline__ double warp_sum(double v) {
   return v;
 }
 
-// Sums of a block's run of tokens, [tokens * b / blocks, tokens * (b + 1) / blocks), added
-// over a cluster; one block alone finishes by itself.
+// Sums of a block's run of tokens, [tokens * b / blocks, tokens * (b + 1) / blocks); one
+// block alone finishes by itself.
 template <class T, int V, int J, bool SIGMOID>
-__global__ void __launch_bounds__(kThreads, blocks_an_sm(J * V)) balance_forward(Forward f) {
-  extern __shared__ uint32_t shared[];
-  const unsigned E = f.experts, lane = threadIdx.x % 32, warp = threadIdx.x / 32, width = f.width;
-  float* const mass = reinterpret_cast<float*>(shared);       // [kWarps][E]
-  uint32_t* const counts = shared + kWarps * E;                 // [E], and the counted tokens behind them
+__global__ void __launch_bounds__(kThreadsFor<J * V>, 1) balance_forward(Forward f) {
+  constexpr unsigned kThreads = kThreadsFor<J * V>, kWarps = kThreads / 32;
+  extern __shared__ __align__(16) uint32_t shared[];
+  using C = Copies<T, V, J, kThreads, kAhead>;
+  const unsigned E = f.experts, lane = threadIdx.x % 32, warp = threadIdx.x / 32, width = f.width, first = lane % width * V;
+  const C copies(shared, first, width, E, -INFINITY);
+  float* const mass = reinterpret_cast<float*>(shared + C::kAll / 4);       // [kWarps][E]
+  uint32_t* const counts = shared + C::kAll / 4 + kWarps * E;                // [E], and the counted tokens behind them
   asm volatile("griddepcontrol.launch_dependents;");
   const unsigned begin = (uint64_t)f.tokens * blockIdx.x / gridDim.x, end = (uint64_t)f.tokens * (blockIdx.x + 1) / gridDim.x;
-  const unsigned step = kWarps * (32 / width), first = lane % width * V;
-  const T* const logits = static_cast<const T*>(f.logits);
-  Held<T, V, J> now, next;
-  unsigned row = begin + warp * (32 / width) + lane / width;
-  bool there = row < end && (!f.mask || f.mask[row]);
-  now.load(logits + (int64_t)row * f.stride, first, width, E, there);
+  // this lane's rows: `row` is the next to be copied, `there` has a bit for each that is under way
+  const unsigned step = kWarps * (32 / width);
+  unsigned row = begin + warp * (32 / width) + lane / width, there = 0;
+  const T* from = static_cast<const T*>(f.logits) + (int64_t)row * f.stride + first;
+  const int64_t jump = (int64_t)step * f.stride;
+  auto copy = [&](unsigned turn) {
+    const bool counts = row < end && (!f.mask || f.mask[row]);
+    copies.copy(turn, from, width, counts);
+    copies_end();
+    there = there >> 1 | (unsigned)counts << (kAhead - 1);
+    row += step;
+    from += jump;
+  };
+#pragma unroll
+  for (unsigned i = 0; i < kAhead; ++i) copy(i);
   for (unsigned i = threadIdx.x; i <= E; i += kThreads) counts[i] = 0;
   __syncthreads();
   // entries and counted tokens
@@ -182,24 +239,17 @@ __global__ void __launch_bounds__(kThreads, blocks_an_sm(J * V)) balance_forward
   }
   // mass
   float sum[J * V] = {};
-  while (__any_sync(~0u, row < end)) {
-    const unsigned after = row + step;
-    const bool more = after < end && (!f.mask || f.mask[after]);
-    next.load(logits + (int64_t)after * f.stride, first, width, E, more);
+  for (unsigned turn = 0; __any_sync(~0u, row < end + kAhead * step); ++turn) {
+    const bool now = there & 1;
     float v[J * V], rest[SIGMOID ? J * V : 1];
-    scores<T, V, J, SIGMOID>(now, first, width, E, there, v, rest);
+    copies_wait<kAhead - 1>();
+    copies.read(turn, v);
+    copy(turn + kAhead);
+    if (!__any_sync(~0u, now)) continue;
+    scores<T, J * V, SIGMOID>(v, rest, width);
     float by = 1.f;
-    if (!SIGMOID || f.normalise) {
-      float total = 0.f;
-#pragma unroll
-      for (int i = 0; i < J * V; ++i) total += v[i];
-      by = share(row_add(total, width));
-    }
-#pragma unroll
-    for (int i = 0; i < J * V; ++i) sum[i] = fmaf(v[i], by, sum[i]);
-    now = next;
-    there = more;
-    row = after;
+    if (!SIGMOID || f.normalise) by = share(row_add(lane_sum<J * V>(v), width));
+    if (now) vfma<J * V>(sum, v, by, sum);       // the others' packs hold what was there before
   }
 #pragma unroll
   for (int j = 0; j < J; ++j) {
@@ -213,32 +263,21 @@ __global__ void __launch_bounds__(kThreads, blocks_an_sm(J * V)) balance_forward
   }
   __syncthreads();
   if (gridDim.x > 1) {
+    uint32_t* const mine = f.sums + (size_t)blockIdx.x * (2 * E + 1);
     for (unsigned e = threadIdx.x; e < E; e += kThreads) {
       float s = 0.f;
-#pragma unroll
+#pragma unroll 8
       for (unsigned w = 0; w < kWarps; ++w) s += mass[w * E + e];
-      mass[e] = s;
+      mine[e] = __float_as_uint(s);
+      mine[E + e] = counts[e];
     }
-    cluster_sync();
-    uint32_t* const mine = f.sums + (size_t)(blockIdx.x / kTogether) * (2 * E + 1);
-    for (unsigned e = threadIdx.x * kTogether + cluster_rank(); e <= E; e += kThreads * kTogether) {
-      float s = 0.f;
-      uint32_t n = 0;
-#pragma unroll
-      for (unsigned r = 0; r < kTogether; ++r) {
-        if (e < E) s += cluster_load(mass + e, r);
-        n += cluster_load(counts + e, r);
-      }
-      if (e < E) mine[e] = __float_as_uint(s);
-      mine[E + e] = n;
-    }
-    cluster_sync();                      // no block leaves while another reads from it
+    if (threadIdx.x == 0) mine[2 * E] = counts[E];
     return;
   }
   double dot = 0;
   for (unsigned e = threadIdx.x; e < E; e += kThreads) {
     double s = 0;
-#pragma unroll
+#pragma unroll 8
     for (unsigned w = 0; w < kWarps; ++w) s += (double)mass[w * E + e];
     f.mass[e] = (float)s;
     f.counts[e] = (int32_t)counts[e];
@@ -256,7 +295,7 @@ __global__ void __launch_bounds__(kThreads, blocks_an_sm(J * V)) balance_forward
   }
 }
 
-// Adds the clusters' sums up, one cluster: each of its blocks takes some experts, 32 lanes
+// Adds the blocks' sums up, one cluster: each of its blocks takes some experts, 32 lanes
 // a run of them, its warps the sums in turn.
 __global__ void __cluster_dims__(kFinish) __launch_bounds__(kFinishThreads) balance_finish(Forward f, unsigned sums) {
   __shared__ double mass[kFinishWarps][32];
@@ -271,7 +310,7 @@ __global__ void __cluster_dims__(kFinish) __launch_bounds__(kFinishThreads) bala
     double m = 0;
     uint32_t n = 0;
     if (e < E)
-#pragma unroll 5
+#pragma unroll 10
       for (unsigned b = warp; b < sums; b += kFinishWarps) {
         m += (double)__uint_as_float(f.sums[(size_t)b * (2 * E + 1) + e]);
         n += f.sums[(size_t)b * (2 * E + 1) + E + e];
@@ -315,9 +354,34 @@ __global__ void __cluster_dims__(kFinish) __launch_bounds__(kFinishThreads) bala
 }
 
 template <class T, int V, int J, bool SIGMOID>
-__global__ void __launch_bounds__(kThreads, blocks_an_sm(J * V)) balance_backward(Backward b) {
+__global__ void __launch_bounds__(kThreadsFor<J * V>, 1) balance_backward(Backward b) {
+  constexpr unsigned kThreads = kThreadsFor<J * V>, kWarps = kThreads / 32;
+  extern __shared__ __align__(16) uint32_t shared[];
+  constexpr unsigned kAhead = kAheadBack<T>;
+  using C = Copies<T, V, J, kThreads, kAhead>;
   const unsigned E = b.experts, lane = threadIdx.x % 32, width = b.width, first = lane % width * V;
-  const bool shares = !SIGMOID || b.normalise;
+  const bool shares = !SIGMOID || b.normalise, plus = b.add != nullptr;
+  const C copies(shared, first, width, E, -INFINITY), extra(plus ? shared + C::kAll / 4 : shared, first, width, plus ? E : ~0u, 0.f);
+  // this lane's rows: `row` is the next to be copied, `there` has a bit for each that is under way
+  const uint64_t step = (uint64_t)gridDim.x * kWarps * (32 / width);
+  const uint64_t own = (threadIdx.x / 32 * gridDim.x + blockIdx.x) * (32 / width) + lane / width;
+  uint64_t row = own;
+  unsigned there = 0;
+  const T* from = static_cast<const T*>(b.logits) + (int64_t)own * b.stride + first;
+  const T* from_add = static_cast<const T*>(b.add) + (int64_t)own * b.add_stride + first;
+  T* out = static_cast<T*>(b.out) + (int64_t)own * b.out_stride + first;
+  auto copy = [&](unsigned turn) {
+    const bool counts = row < b.tokens && (!b.mask || b.mask[row]);
+    copies.copy(turn, from, width, counts);
+    if (plus) extra.copy(turn, from_add, width, row < b.tokens);
+    copies_end();
+    there = there >> 1 | (unsigned)counts << (kAhead - 1);
+    row += step;
+    from += (int64_t)step * b.stride;
+    from_add += (int64_t)step * b.add_stride;
+  };
+#pragma unroll
+  for (unsigned i = 0; i < kAhead; ++i) copy(i);
   // a column's d, less what the mean count gives
   float d[J * V];
   {
@@ -332,109 +396,96 @@ __global__ void __launch_bounds__(kThreads, blocks_an_sm(J * V)) balance_backwar
         d[j * V + i] = e < E ? (float)(c * (b.counts[e] - mean)) : 0.f;
       }
   }
-  const unsigned slots = gridDim.x * kWarps * (32 / width);
-  const T* const logits = static_cast<const T*>(b.logits);
-  const T* const add = static_cast<const T*>(b.add);
-  T* const out = static_cast<T*>(b.out);
-  Held<T, V, J> now, next, more, also;
-  uint64_t row = (uint64_t)(blockIdx.x * kWarps + threadIdx.x / 32) * (32 / width) + lane / width;
-  bool there = row < b.tokens && (!b.mask || b.mask[row]);
-  now.load(logits + (int64_t)row * b.stride, first, width, E, there);
-  if (add) more.load(add + (int64_t)row * b.add_stride, first, width, E, row < b.tokens);
-  while (__any_sync(~0u, row < b.tokens)) {
-    const uint64_t after = row + slots;
-    const bool then = after < b.tokens && (!b.mask || b.mask[after]);
-    next.load(logits + (int64_t)after * b.stride, first, width, E, then);
-    if (add) also.load(add + (int64_t)after * b.add_stride, first, width, E, after < b.tokens);
-    float v[J * V], rest[SIGMOID ? J * V : 1];
-    scores<T, V, J, SIGMOID>(now, first, width, E, there, v, rest);
-    float by = 1.f, dot = 0.f;
-    if (shares) {
-      float total = 0.f;
+  const uint64_t last = b.tokens + kAhead * step;      // what `row` is behind the last
+  for (unsigned turn = 0; __any_sync(~0u, row < last); ++turn) {
+    const bool now = there & 1, mine = row < last;
+    float v[J * V], g[J * V], rest[SIGMOID ? J * V : 1];
+    copies_wait<kAhead - 1>();
+    copies.read(turn, v);
+    if (plus) {
+      extra.read(turn, g);
+    } else {
 #pragma unroll
-      for (int i = 0; i < J * V; ++i) {
-        total += v[i];
-        dot = fmaf(v[i], d[i], dot);
-      }
-      by = share(row_add(total, width));
-      dot = row_add(dot, width) * by;
+      for (int i = 0; i < J * V; ++i) g[i] = 0.f;
     }
-    if (row < b.tokens) {
-#pragma unroll
-      for (int j = 0; j < J; ++j) {
-        const unsigned c = first + j * width * V;
-        if (c >= E) continue;
-        float g[V], plus[V];
-        if (add) {
-          widen(more.p[j], plus);
-        } else {
-#pragma unroll
-          for (int i = 0; i < V; ++i) plus[i] = 0.f;
-        }
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const int q = j * V + i;
-          float p = v[q] * by;
-          if constexpr (SIGMOID) p *= rest[q];
-          g[i] = there ? fmaf(p, d[q] - dot, plus[i]) : plus[i];
-        }
-        store_pack<T, V>(out + (int64_t)row * b.out_stride + c, narrow<T, V>(g));
+    copy(turn + kAhead);
+    if (__any_sync(~0u, now)) {
+      scores<T, J * V, SIGMOID>(v, rest, width);
+      float by = 1.f, dot = 0.f, slope[J * V];
+      if (shares) {
+        vmul<J * V>(slope, v, d);
+        by = share(row_add(lane_sum<J * V>(v), width));
+        dot = row_add(lane_sum<J * V>(slope), width) * by;
+      }
+      if (now) {
+        vadd<J * V>(slope, d, -dot);
+        vmul<J * V>(v, v, by);
+        if constexpr (SIGMOID) vmul<J * V>(v, v, rest);
+        vfma<J * V>(g, v, slope, g);
       }
     }
-    now = next;
-    more = also;
-    there = then;
-    row = after;
+    if (mine) {
+#pragma unroll
+      for (int j = 0; j < J; ++j)
+        if (copies.here >> j & 1) store_pack<T, V>(out + j * width * V, narrow<T, V>(*reinterpret_cast<const float(*)[V]>(g + j * V)));
+    }
+    out += (int64_t)step * b.out_stride;
   }
 }
 
 // The variants: whole packs of 16 bytes where every row begins on 16 bytes and ends with
-// a pack, single elements else; as many packs a lane as the row needs.
+// a pack, single elements else.  Of the packs a lane may have, those that cost a row the
+// fewest instructions: some 12 a column of a lane and 100 a turn, for 32 / width rows.
+// More columns than 16 a lane leave few warps and are taken only where a row needs them.
 template <class T, int V, class F>
 void by_packs(unsigned experts, unsigned* width, F launch) {
   const unsigned packs = (unsigned)ceil_div(experts, V);
-  *width = 1;
-  while (*width < 32 && *width < packs) *width *= 2;
-  const unsigned each = (unsigned)ceil_div(packs, *width);
-  if (each <= 1) launch(std::integral_constant<int, 1>{});
-  else if (each <= 2) launch(std::integral_constant<int, 2>{});
-  else if (each <= 4) launch(std::integral_constant<int, 4>{});
-  else if constexpr (V <= 4) {
-    if (each <= 8) launch(std::integral_constant<int, 8>{});
-    else if constexpr (V == 1) {
-      if (each <= 16) launch(std::integral_constant<int, 16>{});
-      else launch(std::integral_constant<int, 32>{});
-    }
+  unsigned best = 0, least = ~0u;
+  auto ask = [&](unsigned each) {
+    unsigned w = 1;
+    while (w * each < packs) w *= 2;
+    const unsigned cost = w * (12 * each * V + 100);
+    if (w <= 32 && (each * V <= 16 || !best) && cost < least) best = each, *width = w, least = cost;
+  };
+  auto go = [&](auto each) {
+    if constexpr (decltype(each)::value * V <= 32)
+      if (best == decltype(each)::value) launch(each);
+  };
+  if constexpr (V == 8) {
+    for (unsigned e : {1u, 2u, 4u}) ask(e);
+  } else if constexpr (V == 4) {
+    for (unsigned e : {1u, 2u, 3u, 4u, 8u}) ask(e);
+  } else {
+    for (unsigned e : {1u, 2u, 4u, 8u, 16u, 32u})
+      if (!best) ask(e);                     // single elements: as many lanes side by side as there are
   }
+  go(std::integral_constant<int, 1>{});
+  go(std::integral_constant<int, 2>{});
+  if constexpr (V == 4) go(std::integral_constant<int, 3>{});
+  go(std::integral_constant<int, 4>{});
+  if constexpr (V < 8) go(std::integral_constant<int, 8>{});
+  if constexpr (V == 1) go(std::integral_constant<int, 16>{});
+  if constexpr (V == 1) go(std::integral_constant<int, 32>{});
 }
 
 template <class T>
 void forward(Forward f, bool wide, bool sigmoid, unsigned grid, int device, cudaStream_t stream) {
-  const size_t bytes = (kWarps * (size_t)f.experts + f.experts + 1) * 4;
   auto run = [&](auto v) {
     constexpr int V = decltype(v)::value;
     by_packs<T, V>(f.experts, &f.width, [&](auto j) {
       constexpr int J = decltype(j)::value;
+      constexpr unsigned kThreads = kThreadsFor<J * V>;
+      const size_t bytes = Copies<T, V, J, kThreads, kAhead>::kAll + (kThreads / 32 * (size_t)f.experts + f.experts + 1) * 4;
       auto go = [&](auto s) {
         constexpr bool S = decltype(s)::value;
         room<balance_forward<T, V, J, S>>(device);
-        cudaLaunchAttribute together{};
-        together.id = cudaLaunchAttributeClusterDimension;
-        together.val.clusterDim.x = grid == 1 ? 1 : kTogether;
-        together.val.clusterDim.y = together.val.clusterDim.z = 1;
-        cudaLaunchConfig_t config{};
-        config.gridDim = grid;
-        config.blockDim = kThreads;
-        config.dynamicSmemBytes = bytes;
-        config.stream = stream;
-        config.attrs = &together;
-        config.numAttrs = 1;
-        check(cudaLaunchKernelEx(&config, balance_forward<T, V, J, S>, f), "balance_forward");
+        balance_forward<T, V, J, S><<<grid, kThreads, bytes, stream>>>(f);
       };
       sigmoid ? go(std::true_type{}) : go(std::false_type{});
     });
   };
   wide ? run(std::integral_constant<int, 16 / sizeof(T)>{}) : run(std::integral_constant<int, 1>{});
+  check(cudaGetLastError(), "balance_forward");
   if (grid == 1) return;
   cudaLaunchAttribute early{};
   early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -445,7 +496,7 @@ void forward(Forward f, bool wide, bool sigmoid, unsigned grid, int device, cuda
   config.stream = stream;
   config.attrs = &early;
   config.numAttrs = 1;
-  check(cudaLaunchKernelEx(&config, balance_finish, f, grid / kTogether), "balance_finish");
+  check(cudaLaunchKernelEx(&config, balance_finish, f, grid), "balance_finish");
 }
 
 template <class T>
@@ -454,21 +505,24 @@ void backward(Backward b, bool wide, bool sigmoid, int device, cudaStream_t stre
     constexpr int V = decltype(v)::value;
     by_packs<T, V>(b.experts, &b.width, [&](auto j) {
       constexpr int J = decltype(j)::value;
-      const unsigned rows = kWarps * (32 / b.width);
-      const unsigned grid = (unsigned)std::min<uint64_t>(ceil_div(b.tokens, rows), sm_count(device) * blocks_an_sm(J * V));
-      if (sigmoid) balance_backward<T, V, J, true><<<grid, kThreads, 0, stream>>>(b);
-      else balance_backward<T, V, J, false><<<grid, kThreads, 0, stream>>>(b);
+      constexpr unsigned kThreads = kThreadsFor<J * V>;
+      const size_t bytes = Copies<T, V, J, kThreads, kAheadBack<T>>::kAll * (b.add ? 2 : 1);
+      const unsigned grid = (unsigned)std::min<uint64_t>(ceil_div(b.tokens, 32 / b.width), sm_count(device));
+      auto go = [&](auto s) {
+        constexpr bool S = decltype(s)::value;
+        room<balance_backward<T, V, J, S>>(device);
+        balance_backward<T, V, J, S><<<grid, kThreads, bytes, stream>>>(b);
+      };
+      sigmoid ? go(std::true_type{}) : go(std::false_type{});
     });
   };
   wide ? run(std::integral_constant<int, 16 / sizeof(T)>{}) : run(std::integral_constant<int, 1>{});
   check(cudaGetLastError(), "balance_backward");
 }
 
-// Blocks of the forward pass: some 8192 values each, so that a small batch takes one;
-// more come in clusters.
+// Blocks of the forward pass: some 8192 values each, so that a small batch takes one.
 unsigned forward_blocks(uint64_t tokens, uint32_t experts, unsigned sms) {
-  const uint64_t n = ceil_div(tokens * experts, 8192);
-  return n <= 1 ? 1 : (unsigned)std::min<uint64_t>(round_up(n, kTogether), std::min(sms * 4, kMost) / kTogether * kTogether);
+  return (unsigned)std::max<uint64_t>(1, std::min<uint64_t>(ceil_div(tokens * experts, 8192), std::min(sms, kMost)));
 }
 
 bool wide_rows(const void* p, int64_t stride, size_t size) { return aligned(p, 16) && stride * (int64_t)size % 16 == 0; }
@@ -504,7 +558,7 @@ extern "C" {
 
 uint64_t eps_b200_balance_loss_workspace(uint64_t tokens, uint32_t experts) {
   const unsigned blocks = forward_blocks(tokens, experts, kMost);
-  return blocks == 1 ? 0 : (uint64_t)blocks / kTogether * (2 * (uint64_t)experts + 1) * 4;
+  return blocks == 1 ? 0 : (uint64_t)blocks * (2 * (uint64_t)experts + 1) * 4;
 }
 
 int eps_b200_balance_loss(const EpsB200BalanceLoss* a, const int32_t* chosen, float* loss, int32_t* counts, float* mass, int32_t* counted,

@@ -135,7 +135,7 @@ def test_low_rank_refuses(change):
 
 def test_low_rank_layout():
     assert [LIB.eps_b200_low_rank_rank(r) for r in (1, 8, 9, 16, 17, 33, 64, 65, 128, 129)] == [8, 8, 16, 16, 32, 64, 64, 128, 128, 0]
-    assert [LIB.eps_b200_low_rank_inner(k) for k in (1, 32, 33, 4096)] == [32, 32, 64, 4096]
+    assert [LIB.eps_b200_low_rank_inner(k) for k in (1, 32, 33, 4096)] == [64, 64, 64, 4096]
     assert LIB.eps_b200_low_rank_workspace(64, 100) == 0
     for rows, n in ((65, 1), (1000, 16384), (100000, 3)):      # the units of the worst split, the rows' order, and a count
         assert LIB.eps_b200_low_rank_workspace(rows, n) >= 16 + 16 * (rows // 64 + min(rows, n + 1)) + 4 * rows
