@@ -19,6 +19,7 @@
 // which a cluster adds up in block order: no float atomics, so results repeat exactly.
 #include <algorithm>
 #include <cmath>
+#include <initializer_list>
 
 #include "dense.cuh"
 
@@ -31,8 +32,11 @@ template <int COLUMNS> constexpr unsigned kThreadsFor = COLUMNS <= 8 ? 1024 : CO
 constexpr unsigned kMost = 1024;          // most blocks
 constexpr unsigned kFinish = 8, kFinishThreads = 512, kFinishWarps = kFinishThreads / 32;      // blocks that add their sums up
 
-constexpr unsigned kAhead = 4;                                          // rows that a lane of the forward pass copies ahead
-template <class T> constexpr unsigned kAheadBack = sizeof(T) == 4 ? 3 : 4;      // of the backward pass, from two tensors
+// Rows that a lane copies ahead, of the forward pass and, from two tensors, of the backward
+// pass.  Single 16-bit values cannot be copied to shared memory on their own: of those one
+// row waits in registers.
+template <int BYTES> constexpr unsigned kAheadOf = BYTES == 2 ? 1 : 4;
+template <class T, int BYTES> constexpr unsigned kAheadBack = BYTES == 2 ? 1 : sizeof(T) == 4 ? 3 : 4;
 struct Rows {
   const void* logits;
   int64_t stride;
@@ -123,7 +127,8 @@ __device__ __forceinline__ float lane_sum(const float (&v)[N]) {
 // to shared memory, AHEAD rows of them.
 template <class T, int V, int J, unsigned THREADS, unsigned AHEAD>
 struct Copies {
-  static constexpr unsigned kBytes = V * sizeof(T), kRow = J * THREADS * kBytes, kAll = AHEAD * kRow;
+  static constexpr unsigned kBytes = V * sizeof(T), kRow = J * THREADS * kBytes, kAll = kBytes == 2 ? 16 : AHEAD * kRow;
+  Pack<T, V> waiting[kBytes == 2 ? J : 1];
   unsigned at, here;       // the packs of this lane in its row, a bit each
   // What is behind the last column is `rest` once and for all: no copy reaches it.
   __device__ __forceinline__ Copies(void* shared, unsigned first, unsigned width, unsigned columns, float rest)
@@ -135,26 +140,30 @@ struct Copies {
     for (int j = 0; j < J; ++j) {
       if (first + j * width * V < columns) {
         here |= 1u << j;
+      } else if constexpr (kBytes == 2) {
+        waiting[j] = r;
       } else {
         for (unsigned k = 0; k < AHEAD; ++k) *reinterpret_cast<Pack<T, V>*>(static_cast<char*>(shared) + k * kRow + (j * THREADS + threadIdx.x) * kBytes) = r;
       }
     }
   }
-  __device__ __forceinline__ void copy(unsigned turn, const T* row, unsigned width, bool there) const {
+  __device__ __forceinline__ void copy(unsigned turn, const T* row, unsigned width, bool there) {
     const unsigned to = at + turn % AHEAD * kRow;
 #pragma unroll
     for (int j = 0; j < J; ++j) {
       if (!there || !(here >> j & 1)) continue;
-      if constexpr (kBytes >= 4)
-        copy_ahead<(int)kBytes>(to + j * THREADS * kBytes, row + j * width * V, true);
-      else
-        asm volatile("st.shared.u16 [%0], %1;" ::"r"(to + j * THREADS * kBytes), "h"(reinterpret_cast<const unsigned short*>(row)[j * width * V]) : "memory");
+      if constexpr (kBytes == 2) waiting[j] = load_pack<T, V>(row + j * width * V);
+      else copy_ahead<(int)kBytes>(to + j * THREADS * kBytes, row + j * width * V, true);
     }
   }
   __device__ __forceinline__ void read(unsigned turn, float (&v)[J * V]) const {
     const unsigned from = at + turn % AHEAD * kRow;
 #pragma unroll
-    for (int j = 0; j < J; ++j) widen(own_shared<Pack<T, V>>(from + j * THREADS * kBytes), *reinterpret_cast<float(*)[V]>(v + j * V));
+    for (int j = 0; j < J; ++j) {
+      float(&to)[V] = *reinterpret_cast<float(*)[V]>(v + j * V);
+      if constexpr (kBytes == 2) widen(waiting[j], to);
+      else widen(own_shared<Pack<T, V>>(from + j * THREADS * kBytes), to);
+    }
   }
 };
 
@@ -198,17 +207,19 @@ __device__ __forceinline__ double warp_sum(double v) {
 // block alone finishes by itself.
 template <class T, int V, int J, bool SIGMOID>
 __global__ void __launch_bounds__(kThreadsFor<J * V>, 1) balance_forward(Forward f) {
-  constexpr unsigned kThreads = kThreadsFor<J * V>, kWarps = kThreads / 32;
+  constexpr unsigned kThreads = kThreadsFor<J * V>;         // at most
+  const unsigned threads = blockDim.x, warps = threads / 32;
+  constexpr unsigned kAhead = kAheadOf<V * sizeof(T)>;
   extern __shared__ __align__(16) uint32_t shared[];
   using C = Copies<T, V, J, kThreads, kAhead>;
   const unsigned E = f.experts, lane = threadIdx.x % 32, warp = threadIdx.x / 32, width = f.width, first = lane % width * V;
-  const C copies(shared, first, width, E, -INFINITY);
-  float* const mass = reinterpret_cast<float*>(shared + C::kAll / 4);       // [kWarps][E]
-  uint32_t* const counts = shared + C::kAll / 4 + kWarps * E;                // [E], and the counted tokens behind them
+  C copies(shared, first, width, E, -INFINITY);
+  float* const mass = reinterpret_cast<float*>(shared + C::kAll / 4);       // [warps][E]
+  uint32_t* const counts = shared + C::kAll / 4 + warps * E;                // [E], and the counted tokens behind them
   asm volatile("griddepcontrol.launch_dependents;");
   const unsigned begin = (uint64_t)f.tokens * blockIdx.x / gridDim.x, end = (uint64_t)f.tokens * (blockIdx.x + 1) / gridDim.x;
   // this lane's rows: `row` is the next to be copied, `there` has a bit for each that is under way
-  const unsigned step = kWarps * (32 / width);
+  const unsigned step = warps * (32 / width);
   unsigned row = begin + warp * (32 / width) + lane / width, there = 0;
   const T* from = static_cast<const T*>(f.logits) + (int64_t)row * f.stride + first;
   const int64_t jump = (int64_t)step * f.stride;
@@ -222,16 +233,26 @@ __global__ void __launch_bounds__(kThreadsFor<J * V>, 1) balance_forward(Forward
   };
 #pragma unroll
   for (unsigned i = 0; i < kAhead; ++i) copy(i);
-  for (unsigned i = threadIdx.x; i <= E; i += kThreads) counts[i] = 0;
+  for (unsigned i = threadIdx.x; i <= E; i += threads) counts[i] = 0;
   __syncthreads();
-  // entries and counted tokens
-  for (unsigned i = begin * f.top_k + threadIdx.x; i < end * f.top_k; i += kThreads) {
-    const unsigned e = (unsigned)f.chosen[i];
-    if (e < E && (!f.mask || f.mask[i / f.top_k])) atomicAdd(&counts[e], 1u);
+  // entries and counted tokens; eight entries a thread are asked for at once
+  constexpr unsigned kMany = 8;
+  for (unsigned i = begin * f.top_k + threadIdx.x; i < end * f.top_k; i += threads * kMany) {
+    unsigned e[kMany];
+#pragma unroll
+    for (unsigned j = 0; j < kMany; ++j) {
+      const unsigned k = i + j * threads;
+      const bool entry = k < end * f.top_k;
+      e[j] = entry ? (unsigned)f.chosen[k] : ~0u;
+      if (f.mask && entry && !f.mask[k / f.top_k]) e[j] = ~0u;
+    }
+#pragma unroll
+    for (unsigned j = 0; j < kMany; ++j)
+      if (e[j] < E) atomicAdd(&counts[e[j]], 1u);
   }
   if (f.mask) {
     unsigned n = 0;
-    for (unsigned t = begin + threadIdx.x; t < end; t += kThreads) n += f.mask[t] != 0;
+    for (unsigned t = begin + threadIdx.x; t < end; t += threads) n += f.mask[t] != 0;
     n = __reduce_add_sync(~0u, n);
     if (lane == 0) atomicAdd(&counts[E], n);
   } else if (threadIdx.x == 0) {
@@ -264,10 +285,10 @@ __global__ void __launch_bounds__(kThreadsFor<J * V>, 1) balance_forward(Forward
   __syncthreads();
   if (gridDim.x > 1) {
     uint32_t* const mine = f.sums + (size_t)blockIdx.x * (2 * E + 1);
-    for (unsigned e = threadIdx.x; e < E; e += kThreads) {
+    for (unsigned e = threadIdx.x; e < E; e += threads) {
       float s = 0.f;
 #pragma unroll 8
-      for (unsigned w = 0; w < kWarps; ++w) s += mass[w * E + e];
+      for (unsigned w = 0; w < warps; ++w) s += mass[w * E + e];
       mine[e] = __float_as_uint(s);
       mine[E + e] = counts[e];
     }
@@ -275,21 +296,21 @@ __global__ void __launch_bounds__(kThreadsFor<J * V>, 1) balance_forward(Forward
     return;
   }
   double dot = 0;
-  for (unsigned e = threadIdx.x; e < E; e += kThreads) {
+  for (unsigned e = threadIdx.x; e < E; e += threads) {
     double s = 0;
 #pragma unroll 8
-    for (unsigned w = 0; w < kWarps; ++w) s += (double)mass[w * E + e];
+    for (unsigned w = 0; w < warps; ++w) s += (double)mass[w * E + e];
     f.mass[e] = (float)s;
     f.counts[e] = (int32_t)counts[e];
     dot += s * counts[e];
   }
-  __shared__ double each[kWarps];
+  __shared__ double each[32];
   dot = warp_sum(dot);
   if (lane == 0) each[warp] = dot;
   __syncthreads();
   if (threadIdx.x == 0) {
     dot = 0;
-    for (unsigned w = 0; w < kWarps; ++w) dot += each[w];
+    for (unsigned w = 0; w < warps; ++w) dot += each[w];
     *f.counted = (int32_t)counts[E];
     *f.loss = loss_of(dot, counts[E], f);
   }
@@ -355,15 +376,16 @@ __global__ void __cluster_dims__(kFinish) __launch_bounds__(kFinishThreads) bala
 
 template <class T, int V, int J, bool SIGMOID>
 __global__ void __launch_bounds__(kThreadsFor<J * V>, 1) balance_backward(Backward b) {
-  constexpr unsigned kThreads = kThreadsFor<J * V>, kWarps = kThreads / 32;
+  constexpr unsigned kThreads = kThreadsFor<J * V>;         // at most
+  const unsigned warps = blockDim.x / 32;
   extern __shared__ __align__(16) uint32_t shared[];
-  constexpr unsigned kAhead = kAheadBack<T>;
+  constexpr unsigned kAhead = kAheadBack<T, V * sizeof(T)>;
   using C = Copies<T, V, J, kThreads, kAhead>;
   const unsigned E = b.experts, lane = threadIdx.x % 32, width = b.width, first = lane % width * V;
   const bool shares = !SIGMOID || b.normalise, plus = b.add != nullptr;
-  const C copies(shared, first, width, E, -INFINITY), extra(plus ? shared + C::kAll / 4 : shared, first, width, plus ? E : ~0u, 0.f);
+  C copies(shared, first, width, E, -INFINITY), extra(plus ? shared + C::kAll / 4 : shared, first, width, plus ? E : ~0u, 0.f);
   // this lane's rows: `row` is the next to be copied, `there` has a bit for each that is under way
-  const uint64_t step = (uint64_t)gridDim.x * kWarps * (32 / width);
+  const uint64_t step = (uint64_t)gridDim.x * warps * (32 / width);
   const uint64_t own = (threadIdx.x / 32 * gridDim.x + blockIdx.x) * (32 / width) + lane / width;
   uint64_t row = own;
   unsigned there = 0;
@@ -433,9 +455,10 @@ __global__ void __launch_bounds__(kThreadsFor<J * V>, 1) balance_backward(Backwa
   }
 }
 
-// The variants: whole packs of 16 bytes where every row begins on 16 bytes and ends with
-// a pack, single elements else.  Of the packs a lane may have, those that cost a row the
-// fewest instructions: some 12 a column of a lane and 100 a turn, for 32 / width rows.
+// The variants: packs of 16 bytes where every row begins on 16 bytes and ends with a pack,
+// of 4 where that holds for 4, single elements else.  Of the packs a lane may have, those that cost a row the
+// fewest instructions: some 12 a column of a lane and 100 a turn, for 32 / width rows; but
+// four lanes side by side, for 64 bytes in a row (131072 x 16 floats: 12 us against 14).
 // More columns than 16 a lane leave few warps and are taken only where a row needs them.
 template <class T, int V, class F>
 void by_packs(unsigned experts, unsigned* width, F launch) {
@@ -445,7 +468,7 @@ void by_packs(unsigned experts, unsigned* width, F launch) {
     unsigned w = 1;
     while (w * each < packs) w *= 2;
     const unsigned cost = w * (12 * each * V + 100);
-    if (w <= 32 && (each * V <= 16 || !best) && cost < least) best = each, *width = w, least = cost;
+    if (w <= 32 && w >= std::min(packs, 4u) && (each * V <= 16 || !best) && cost < least) best = each, *width = w, least = cost;
   };
   auto go = [&](auto each) {
     if constexpr (decltype(each)::value * V <= 32)
@@ -457,34 +480,43 @@ void by_packs(unsigned experts, unsigned* width, F launch) {
     for (unsigned e : {1u, 2u, 3u, 4u, 8u}) ask(e);
   } else {
     for (unsigned e : {1u, 2u, 4u, 8u, 16u, 32u})
-      if (!best) ask(e);                     // single elements: as many lanes side by side as there are
+      if (!best) ask(e);                     // small packs: as many lanes side by side as there are
   }
   go(std::integral_constant<int, 1>{});
   go(std::integral_constant<int, 2>{});
   if constexpr (V == 4) go(std::integral_constant<int, 3>{});
   go(std::integral_constant<int, 4>{});
   if constexpr (V < 8) go(std::integral_constant<int, 8>{});
-  if constexpr (V == 1) go(std::integral_constant<int, 16>{});
+  if constexpr (V <= 2) go(std::integral_constant<int, 16>{});
   if constexpr (V == 1) go(std::integral_constant<int, 32>{});
 }
 
+template <class T, class F>
+void by_pack(size_t bytes, F run) {
+  if (bytes == 16) run(std::integral_constant<int, 16 / sizeof(T)>{});
+  else if (bytes == 4) run(std::integral_constant<int, 4 / sizeof(T)>{});
+  else if constexpr (sizeof(T) == 2) run(std::integral_constant<int, 1>{});
+}
+
 template <class T>
-void forward(Forward f, bool wide, bool sigmoid, unsigned grid, int device, cudaStream_t stream) {
+void forward(Forward f, size_t pack, bool sigmoid, unsigned grid, int device, cudaStream_t stream) {
   auto run = [&](auto v) {
     constexpr int V = decltype(v)::value;
     by_packs<T, V>(f.experts, &f.width, [&](auto j) {
       constexpr int J = decltype(j)::value;
       constexpr unsigned kThreads = kThreadsFor<J * V>;
-      const size_t bytes = Copies<T, V, J, kThreads, kAhead>::kAll + (kThreads / 32 * (size_t)f.experts + f.experts + 1) * 4;
+      // a block alone has as many warps as its tokens need
+      const unsigned threads = grid > 1 ? kThreads : std::min<unsigned>(kThreads, std::max<unsigned>(4, (unsigned)ceil_div(f.tokens, 32 / f.width)) * 32);
+      const size_t bytes = Copies<T, V, J, kThreads, kAheadOf<V * sizeof(T)>>::kAll + (threads / 32 * (size_t)f.experts + f.experts + 1) * 4;
       auto go = [&](auto s) {
         constexpr bool S = decltype(s)::value;
         room<balance_forward<T, V, J, S>>(device);
-        balance_forward<T, V, J, S><<<grid, kThreads, bytes, stream>>>(f);
+        balance_forward<T, V, J, S><<<grid, threads, bytes, stream>>>(f);
       };
       sigmoid ? go(std::true_type{}) : go(std::false_type{});
     });
   };
-  wide ? run(std::integral_constant<int, 16 / sizeof(T)>{}) : run(std::integral_constant<int, 1>{});
+  by_pack<T>(pack, run);
   check(cudaGetLastError(), "balance_forward");
   if (grid == 1) return;
   cudaLaunchAttribute early{};
@@ -500,23 +532,25 @@ void forward(Forward f, bool wide, bool sigmoid, unsigned grid, int device, cuda
 }
 
 template <class T>
-void backward(Backward b, bool wide, bool sigmoid, int device, cudaStream_t stream) {
+void backward(Backward b, size_t pack, bool sigmoid, int device, cudaStream_t stream) {
   auto run = [&](auto v) {
     constexpr int V = decltype(v)::value;
     by_packs<T, V>(b.experts, &b.width, [&](auto j) {
       constexpr int J = decltype(j)::value;
       constexpr unsigned kThreads = kThreadsFor<J * V>;
-      const size_t bytes = Copies<T, V, J, kThreads, kAheadBack<T>>::kAll * (b.add ? 2 : 1);
-      const unsigned grid = (unsigned)std::min<uint64_t>(ceil_div(b.tokens, 32 / b.width), sm_count(device));
+      const size_t bytes = Copies<T, V, J, kThreads, kAheadBack<T, V * sizeof(T)>>::kAll * (b.add ? 2 : 1);
+      const uint64_t turns = ceil_div(b.tokens, 32 / b.width);      // of a warp
+      const unsigned grid = (unsigned)std::min<uint64_t>(turns, sm_count(device));
+      const unsigned threads = (unsigned)std::min<uint64_t>(kThreads / 32, ceil_div(turns, grid)) * 32;
       auto go = [&](auto s) {
         constexpr bool S = decltype(s)::value;
         room<balance_backward<T, V, J, S>>(device);
-        balance_backward<T, V, J, S><<<grid, kThreads, bytes, stream>>>(b);
+        balance_backward<T, V, J, S><<<grid, threads, bytes, stream>>>(b);
       };
       sigmoid ? go(std::true_type{}) : go(std::false_type{});
     });
   };
-  wide ? run(std::integral_constant<int, 16 / sizeof(T)>{}) : run(std::integral_constant<int, 1>{});
+  by_pack<T>(pack, run);
   check(cudaGetLastError(), "balance_backward");
 }
 
@@ -525,7 +559,19 @@ unsigned forward_blocks(uint64_t tokens, uint32_t experts, unsigned sms) {
   return (unsigned)std::max<uint64_t>(1, std::min<uint64_t>(ceil_div(tokens * experts, 8192), std::min(sms, kMost)));
 }
 
-bool wide_rows(const void* p, int64_t stride, size_t size) { return aligned(p, 16) && stride * (int64_t)size % 16 == 0; }
+// The largest packs that every row of these tensors (not NULL) begins on and ends with.
+struct Place {
+  const void* p;
+  int64_t stride;
+};
+size_t pack_bytes(std::initializer_list<Place> places, uint64_t columns, size_t size) {
+  for (size_t n : {(size_t)16, (size_t)4}) {
+    bool all = columns * size % n == 0;
+    for (const Place& q : places) all = all && (!q.p || (aligned(q.p, n) && q.stride * (int64_t)size % (int64_t)n == 0));
+    if (all) return n;
+  }
+  return size;
+}
 
 Rows checked(const EpsB200BalanceLoss* a) {
   need(a, "null balance argument");
@@ -578,13 +624,13 @@ int eps_b200_balance_loss(const EpsB200BalanceLoss* a, const int32_t* chosen, fl
     f.sums = static_cast<uint32_t*>(workspace);
     OnDevice on(a->device);
     const size_t size = size_of(a->type);
-    const bool wide = wide_rows(a->logits, a->logits_stride, size) && a->experts * size % 16 == 0;
+    const size_t pack = pack_bytes({{a->logits, a->logits_stride}}, a->experts, size);
     const unsigned grid = forward_blocks(a->tokens, a->experts, sm_count(a->device));
     const auto s = static_cast<cudaStream_t>(stream);
     const bool sigmoid = a->score == EPS_B200_SCORE_SIGMOID;
-    if (a->type == EPS_B200_F32) forward<float>(f, wide, sigmoid, grid, a->device, s);
-    else if (a->type == EPS_B200_BF16) forward<bf16>(f, wide, sigmoid, grid, a->device, s);
-    else forward<f16>(f, wide, sigmoid, grid, a->device, s);
+    if (a->type == EPS_B200_F32) forward<float>(f, pack, sigmoid, grid, a->device, s);
+    else if (a->type == EPS_B200_BF16) forward<bf16>(f, pack, sigmoid, grid, a->device, s);
+    else forward<f16>(f, pack, sigmoid, grid, a->device, s);
   });
 }
 
@@ -606,13 +652,12 @@ int eps_b200_balance_loss_backward(const EpsB200BalanceLoss* a, const int32_t* c
     b.out_stride = dlogits_stride;
     OnDevice on(a->device);
     const size_t size = size_of(a->type);
-    const bool wide = wide_rows(a->logits, a->logits_stride, size) && wide_rows(dlogits, dlogits_stride, size) &&
-                      (!add || wide_rows(add, add_stride, size)) && a->experts * size % 16 == 0;
+    const size_t pack = pack_bytes({{a->logits, a->logits_stride}, {dlogits, dlogits_stride}, {add, add_stride}}, a->experts, size);
     const auto s = static_cast<cudaStream_t>(stream);
     const bool sigmoid = a->score == EPS_B200_SCORE_SIGMOID;
-    if (a->type == EPS_B200_F32) backward<float>(b, wide, sigmoid, a->device, s);
-    else if (a->type == EPS_B200_BF16) backward<bf16>(b, wide, sigmoid, a->device, s);
-    else backward<f16>(b, wide, sigmoid, a->device, s);
+    if (a->type == EPS_B200_F32) backward<float>(b, pack, sigmoid, a->device, s);
+    else if (a->type == EPS_B200_BF16) backward<bf16>(b, pack, sigmoid, a->device, s);
+    else backward<f16>(b, pack, sigmoid, a->device, s);
   });
 }
 

@@ -555,15 +555,16 @@ def balance_loss(logits, experts, *, score: str = "softmax", normalise: bool = T
     if experts.numel() != tokens * top_k:
         _refuse("experts and logits have different numbers of tokens")
     args = _balance_args(logits, stride, tokens, count, top_k, score, normalise, mask, weight)
-    loss = torch.empty((), dtype=torch.float32, device=device)
-    counted = torch.empty((), dtype=torch.int32, device=device)
-    counts = torch.empty(count, dtype=torch.int32, device=device)
-    mass = torch.empty(count, dtype=torch.float32, device=device)
+    # one allocation: counts, mass, loss and tokens, 4 bytes each
+    room = torch.empty(2 * count + 2, dtype=torch.int32, device=device)
+    at = room.data_ptr()
     space = _lib.eps_b200_balance_loss_workspace(tokens, count)
     workspace = torch.empty(space, dtype=torch.uint8, device=device) if space else None
-    _call(_lib.eps_b200_balance_loss, args, experts.data_ptr(), loss.data_ptr(), counts.data_ptr(), mass.data_ptr(),
-          counted.data_ptr(), _ptr(workspace), space, _stream(index))
-    return BalanceLoss(loss, counts, mass, counted)
+    _call(_lib.eps_b200_balance_loss, args, experts.data_ptr(), at + 8 * count, at, at + 4 * count, at + 8 * count + 4,
+          _ptr(workspace), space, _stream(index))
+    counts, mass, last = room.split_with_sizes((count, count, 2))
+    loss, counted = last.unbind()
+    return BalanceLoss(loss.view(torch.float32), counts, mass.view(torch.float32), counted)
 
 
 def balance_loss_backward(logits, counts, tokens, top_k: int, *, score: str = "softmax", normalise: bool = True,
