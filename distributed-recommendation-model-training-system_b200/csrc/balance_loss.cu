@@ -101,13 +101,18 @@ __device__ __forceinline__ float inverse(float x) {
 // 1 / total, 0 where that is 0.
 __device__ __forceinline__ float share(float total) { return total == 0.f ? 0.f : inverse(total); }
 
-__device__ __forceinline__ float row_add(float v, unsigned width) {
-  for (unsigned o = width / 2; o; o /= 2) v += __shfl_xor_sync(~0u, v, o);
-  return v;
+// Over the lanes of a row, U rows at once.
+template <int U>
+__device__ __forceinline__ void row_add(float (&v)[U], unsigned width) {
+  for (unsigned o = width / 2; o; o /= 2)
+#pragma unroll
+    for (int u = 0; u < U; ++u) v[u] += __shfl_xor_sync(~0u, v[u], o);
 }
-__device__ __forceinline__ float row_most(float v, unsigned width) {
-  for (unsigned o = width / 2; o; o /= 2) v = fmaxf(v, __shfl_xor_sync(~0u, v, o));
-  return v;
+template <int U>
+__device__ __forceinline__ void row_most(float (&v)[U], unsigned width) {
+  for (unsigned o = width / 2; o; o /= 2)
+#pragma unroll
+    for (int u = 0; u < U; ++u) v[u] = fmaxf(v[u], __shfl_xor_sync(~0u, v[u], o));
 }
 
 // The sum of a lane's values, two halves at a time.
@@ -167,28 +172,38 @@ struct Copies {
   }
 };
 
-// The scores of a row of logits, -inf behind its last column: its unnormalised p and, for
-// sigmoids, 1 - s in rest.
-template <class T, int N, bool SIGMOID>
-__device__ __forceinline__ void scores(float (&v)[N], float (&rest)[SIGMOID ? N : 1], unsigned width) {
+// The scores of U rows of logits, -inf behind their last columns: their unnormalised p and,
+// for sigmoids, 1 - s in rest.
+template <class T, int U, int N, bool SIGMOID>
+__device__ __forceinline__ void scores(float (&v)[U][N], float (&rest)[U][SIGMOID ? N : 1], unsigned width) {
   constexpr bool kFine = std::is_same_v<T, float>;
   if constexpr (SIGMOID) {
     // s = 1 / (1 + e), 1 - s = e s with e = e^-x; at 88.5 s is 0, as behind it
-    float e[N];
 #pragma unroll
-    for (int i = 0; i < N; ++i) e[i] = least(-v[i], 88.5f);
-    powers<N, kFine>(e);
-    vadd<N>(v, e, 1.f);
+    for (int u = 0; u < U; ++u) {
+      float e[N];
 #pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = inverse(v[i]);
-    vmul<N>(rest, e, v);
+      for (int i = 0; i < N; ++i) e[i] = least(-v[u][i], 88.5f);
+      powers<N, kFine>(e);
+      vadd<N>(v[u], e, 1.f);
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[u][i] = inverse(v[u][i]);
+      vmul<N>(rest[u], e, v[u]);
+    }
   } else {
-    float top = v[0];
+    float top[U];
 #pragma unroll
-    for (int i = 1; i < N; ++i) top = fmaxf(top, v[i]);
-    top = row_most(top, width);
-    vadd<N>(v, v, top == -INFINITY ? 0.f : -top);       // a row of -inf alone gives zeros, not NaN
-    powers<N, kFine>(v);
+    for (int u = 0; u < U; ++u) {
+      top[u] = v[u][0];
+#pragma unroll
+      for (int i = 1; i < N; ++i) top[u] = fmaxf(top[u], v[u][i]);
+    }
+    row_most<U>(top, width);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      vadd<N>(v[u], v[u], top[u] == -INFINITY ? 0.f : -top[u]);       // a row of -inf alone gives zeros, not NaN
+      powers<N, kFine>(v[u]);
+    }
   }
 }
 
@@ -223,8 +238,11 @@ __global__ void __launch_bounds__(kThreadsFor<J * V>, 1) balance_forward(Forward
   unsigned row = begin + warp * (32 / width) + lane / width, there = 0;
   const T* from = static_cast<const T*>(f.logits) + (int64_t)row * f.stride + first;
   const int64_t jump = (int64_t)step * f.stride;
+  auto mask_of = [&](unsigned r) { return f.mask && r < end ? f.mask[r] : (uint8_t)1; };
+  uint8_t mask = mask_of(row);             // asked for a turn before it decides on a copy
   auto copy = [&](unsigned turn) {
-    const bool counts = row < end && (!f.mask || f.mask[row]);
+    const bool counts = row < end && mask;
+    mask = mask_of(row + step);
     copies.copy(turn, from, width, counts);
     copies_end();
     there = there >> 1 | (unsigned)counts << (kAhead - 1);
@@ -260,17 +278,34 @@ __global__ void __launch_bounds__(kThreadsFor<J * V>, 1) balance_forward(Forward
   }
   // mass
   float sum[J * V] = {};
-  for (unsigned turn = 0; __any_sync(~0u, row < end + kAhead * step); ++turn) {
-    const bool now = there & 1;
-    float v[J * V], rest[SIGMOID ? J * V : 1];
-    copies_wait<kAhead - 1>();
-    copies.read(turn, v);
-    copy(turn + kAhead);
-    if (!__any_sync(~0u, now)) continue;
-    scores<T, J * V, SIGMOID>(v, rest, width);
-    float by = 1.f;
-    if (!SIGMOID || f.normalise) by = share(row_add(lane_sum<J * V>(v), width));
-    if (now) vfma<J * V>(sum, v, by, sum);       // the others' packs hold what was there before
+  // two rows a turn, whose chains of reductions run beside each other
+  constexpr int U = kAhead > 1 ? 2 : 1;
+  for (unsigned turn = 0; __any_sync(~0u, row < end + kAhead * step); turn += U) {
+    bool now[U];
+    float v[U][J * V], rest[U][SIGMOID ? J * V : 1], by[U];
+    copies_wait<kAhead - U>();
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      now[u] = there >> u & 1;
+      copies.read(turn + u, v[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) copy(turn + kAhead + u);
+    if (!__any_sync(~0u, now[0] || now[U - 1])) continue;
+    scores<T, U, J * V, SIGMOID>(v, rest, width);
+    if (!SIGMOID || f.normalise) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) by[u] = lane_sum<J * V>(v[u]);
+      row_add<U>(by, width);
+#pragma unroll
+      for (int u = 0; u < U; ++u) by[u] = share(by[u]);
+    } else {
+#pragma unroll
+      for (int u = 0; u < U; ++u) by[u] = 1.f;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (now[u]) vfma<J * V>(sum, v[u], by[u], sum);       // the others' packs hold what was there before
   }
 #pragma unroll
   for (int j = 0; j < J; ++j) {
@@ -392,8 +427,11 @@ __global__ void __launch_bounds__(kThreadsFor<J * V>, 1) balance_backward(Backwa
   const T* from = static_cast<const T*>(b.logits) + (int64_t)own * b.stride + first;
   const T* from_add = static_cast<const T*>(b.add) + (int64_t)own * b.add_stride + first;
   T* out = static_cast<T*>(b.out) + (int64_t)own * b.out_stride + first;
+  auto mask_of = [&](uint64_t r) { return b.mask && r < b.tokens ? b.mask[r] : (uint8_t)1; };
+  uint8_t mask = mask_of(row);             // asked for a turn before it decides on a copy
   auto copy = [&](unsigned turn) {
-    const bool counts = row < b.tokens && (!b.mask || b.mask[row]);
+    const bool counts = row < b.tokens && mask;
+    mask = mask_of(row + step);
     copies.copy(turn, from, width, counts);
     if (plus) extra.copy(turn, from_add, width, row < b.tokens);
     copies_end();
@@ -421,7 +459,8 @@ __global__ void __launch_bounds__(kThreadsFor<J * V>, 1) balance_backward(Backwa
   const uint64_t last = b.tokens + kAhead * step;      // what `row` is behind the last
   for (unsigned turn = 0; __any_sync(~0u, row < last); ++turn) {
     const bool now = there & 1, mine = row < last;
-    float v[J * V], g[J * V], rest[SIGMOID ? J * V : 1];
+    float score[1][J * V], g[J * V], rest[1][SIGMOID ? J * V : 1];
+    float(&v)[J * V] = score[0];
     copies_wait<kAhead - 1>();
     copies.read(turn, v);
     if (plus) {
@@ -432,17 +471,19 @@ __global__ void __launch_bounds__(kThreadsFor<J * V>, 1) balance_backward(Backwa
     }
     copy(turn + kAhead);
     if (__any_sync(~0u, now)) {
-      scores<T, J * V, SIGMOID>(v, rest, width);
+      scores<T, 1, J * V, SIGMOID>(score, rest, width);
       float by = 1.f, dot = 0.f, slope[J * V];
       if (shares) {
         vmul<J * V>(slope, v, d);
-        by = share(row_add(lane_sum<J * V>(v), width));
-        dot = row_add(lane_sum<J * V>(slope), width) * by;
+        float both[2] = {lane_sum<J * V>(v), lane_sum<J * V>(slope)};
+        row_add<2>(both, width);
+        by = share(both[0]);
+        dot = both[1] * by;
       }
       if (now) {
         vadd<J * V>(slope, d, -dot);
         vmul<J * V>(v, v, by);
-        if constexpr (SIGMOID) vmul<J * V>(v, v, rest);
+        if constexpr (SIGMOID) vmul<J * V>(v, v, rest[0]);
         vfma<J * V>(g, v, slope, g);
       }
     }
