@@ -595,9 +595,12 @@ void backward(Backward b, size_t pack, bool sigmoid, int device, cudaStream_t st
   check(cudaGetLastError(), "balance_backward");
 }
 
-// Blocks of the forward pass: some 8192 values each, so that a small batch takes one.
+// Blocks of the forward pass: one for a small batch, which then needs no second launch
+// (16384 values 6.4 us against 7.3; 32768 7.9 against 7.3), else some 8192 values each (131072
+// values 7.8 us; with 2048 each 8.4, with 32768 9.8).
 unsigned forward_blocks(uint64_t tokens, uint32_t experts, unsigned sms) {
-  return (unsigned)std::max<uint64_t>(1, std::min<uint64_t>(ceil_div(tokens * experts, 8192), std::min(sms, kMost)));
+  const uint64_t values = tokens * experts;
+  return values <= 16384 ? 1 : (unsigned)std::min<uint64_t>(ceil_div(values, 8192), std::min(sms, kMost));
 }
 
 // The largest packs that every row of these tensors (not NULL) begins on and ends with.

@@ -215,6 +215,32 @@ def test_beside_the_router_and_over_ranks():
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_logits_beyond_32_bits(dtype):
+    """Rows whose places pass 2^32 bytes; but a few are uniform, and add to each expert alike."""
+    T, E = 2_300_000, 1000
+    x = torch.zeros(T, E, dtype=dtype, device="cuda")
+    chosen = torch.zeros(T, 1, dtype=torch.int32, device="cuda")
+    odd = torch.tensor([5, T // 2, T - 2, T - 1], device="cuda")
+    x[odd] = (torch.randn(4, E, generator=torch.Generator(device="cuda").manual_seed(1), device="cuda") * 3).to(dtype)
+    r = dense.balance_loss(x, chosen)
+    p = torch.softmax(x[odd].double(), -1)
+    mass = p.sum(0) + (T - 4) / E
+    assert int(r.tokens) == T and int(r.counts[0]) == T and not r.counts[1:].any()
+    # a lane adds up to some 2000 rows' shares, each sum rounded to its half a unit
+    ref.close(r.mass, mass, mass, rel=2000 * 2.0 ** -24)
+    ref.close(r.loss, E / T * mass[0], mass[0], rel=2000 * 2.0 ** -24)
+    g = dense.balance_loss_backward(x, r.counts, r.tokens, 1, dloss=torch.tensor(float(T), device="cuda"))
+    d = torch.full((E,), -1.0, dtype=torch.float64, device="cuda")
+    d[0] = E - 1.0
+    want = p * (d - (p * d).sum(-1, keepdim=True))
+    ref.close(g[odd], want, E * p)
+    plain_row = (d - d.mean()) / E
+    for a in (0, T // 2 + 1, T - 3):
+        ref.close(g[a], plain_row, 1.0)
+
+
+@gpu
 def test_captured():
     x, chosen, mask = inputs(3000, 64, 4, BF16, 1, padded=True)
     want = dense.balance_loss(x, chosen, mask=mask)

@@ -13,7 +13,7 @@ from eps_b200 import EpsError, INVALID_ARGUMENT, dense  # noqa: E402
 
 gpu = pytest.mark.gpu
 F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
-SMALL = (1, 3, 0, 255, 4097, 8200, 31)                        # a single cluster's work
+SMALL = (1, 3, 0, 255, 4097, 8200, 31)                        # a single cluster's work (up to 16 spans of 16 KB)
 LARGE = (1, 700001, 5, 16384, 131073, 0, 1 << 20, 4095)        # more spans than that
 # the sum of squares in groups of eight floats: a few units of 2^-24, half of that in the root; the result rounded once more
 NORM = 8 * 2.0 ** -24
@@ -130,6 +130,17 @@ def test_neighbours_are_untouched_and_results_repeat():
     for i in (0, 5, 6, 900002, 3000000):
         assert room[i] == before[i]
     near(n.measure().norm, 1.0)
+
+
+@gpu
+def test_elements_beyond_32_bits():
+    g = torch.zeros((1 << 32) + 12345, dtype=BF16, device="cuda")
+    for at, v in ((0, 3.0), (1 << 31, 4.0), (1 << 32, 12.0), (len(g) - 1, 84.0)):
+        g[at] = v
+    r = dense.GradientNorm([g]).clip(8.5)
+    near(r.norm, math.sqrt(9 + 16 + 144 + 7056))
+    near(r.scale, 0.1)
+    assert [float(g[i]) for i in (0, 1 << 31, 1 << 32, -1)] == [float(torch.tensor(v * float(r.scale)).bfloat16()) for v in (3.0, 4.0, 12.0, 84.0)]
 
 
 @gpu

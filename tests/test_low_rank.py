@@ -15,7 +15,7 @@ gpu = pytest.mark.gpu
 F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
 # rows, adapters, rank, inner, channels
 SHAPES = [(1, 1, 1, 1, 1), (1, 3, 8, 64, 64), (5, 4, 16, 100, 72), (17, 2, 16, 33, 31), (64, 5, 12, 256, 264), (64, 1, 4, 40, 40),
-          (63, 2, 128, 96, 80), (65, 4, 16, 128, 64), (130, 3, 32, 512, 320), (300, 300, 7, 96, 50), (1000, 7, 64, 200, 136),
+          (63, 2, 128, 96, 80), (65, 4, 16, 128, 64), (130, 3, 32, 512, 320), (128, 90, 8, 64, 40), (127, 1, 16, 72, 64), (129, 5, 16, 72, 64), (300, 300, 7, 96, 50), (1000, 7, 64, 200, 136),
           (200, 3, 128, 160, 96), (401, 2, 100, 2050, 40), (2500, 1, 16, 64, 1000), (150, 9, 40, 7, 9), (9000, 40, 8, 72, 24), (70, 5, 3, 31, 33)]
 
 
@@ -80,7 +80,7 @@ def test_product(rows, n, rank, K, N, dtype):
 
 
 @gpu
-@pytest.mark.parametrize("rows", [40, 200])
+@pytest.mark.parametrize("rows", [40, 200, 700])
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_a_row_does_not_depend_on_the_others(rows, dtype):
     """Whatever the other rows hold and ask for, and wherever a row stands."""
@@ -98,7 +98,7 @@ def test_a_row_does_not_depend_on_the_others(rows, dtype):
 
 
 @gpu
-@pytest.mark.parametrize("rows", [9, 100])
+@pytest.mark.parametrize("rows", [9, 100, 400])
 @pytest.mark.parametrize("dtype", [BF16, F16, F32])
 def test_what_is_not_finite(rows, dtype):
     """An infinity of x in a row: as the formula has it in 16 bits, NaN at the latest in float; padded ranks and
@@ -124,7 +124,7 @@ def test_what_is_not_finite(rows, dtype):
 @pytest.mark.parametrize("size", [2.0 ** -20, 1.0, 2.0 ** 12])
 def test_float16_sums_beyond_its_range(size):
     """down x may leave float16's range on either side, as long as the result does not."""
-    x, base, down, up, scale, ids = make(90, 3, 16, 512, 64, F16)
+    x, base, down, up, scale, ids = make(300, 3, 16, 512, 64, F16)
     down = (down.float() * size * 8).half()
     x = (x.float() * 256 * min(1.0, size * 16)).half()
     up = (up.float() / 64).half()
@@ -133,7 +133,7 @@ def test_float16_sums_beyond_its_range(size):
     u = torch.einsum("tk,trk->tr", x.double(), down[ids.long()].double()).abs()
     assert size != 2.0 ** 12 or float(u.max()) > 65504
     a = dense.Adapters(down, up, scale)
-    for part in (slice(0, 90), slice(0, 30)):
+    for part in (slice(0, 300), slice(0, 90), slice(0, 30)):
         close(a.product(x[part], ids[part], base[part]), plain(x[part], ids[part], base[part], down, up, scale), 512, 16)
 
 
@@ -190,6 +190,31 @@ def test_no_rows():
     a = dense.Adapters(down, up, scale)
     out = a.product(torch.empty(0, 64, dtype=BF16, device="cuda"), torch.empty(0, dtype=torch.int32, device="cuda"))
     assert out.shape == (0, 48)
+
+
+@gpu
+def test_rows_beyond_32_bits():
+    """Rows whose places pass 2^32 bytes, in x, base and out."""
+    g = torch.Generator(device="cuda").manual_seed(1)
+    T, K, N = 540000, 4096, 4096
+    down, up = torch.randn(3, 8, K, generator=g, device="cuda").bfloat16() / 64, torch.randn(3, N, 8, generator=g, device="cuda").bfloat16()
+    x, base = torch.zeros(T, K, dtype=BF16, device="cuda"), torch.zeros(T, N, dtype=BF16, device="cuda")
+    rows = torch.cat([torch.arange(40, device="cuda"), torch.randint(0, T, (200,), generator=g, device="cuda"), torch.arange(T - 40, T, device="cuda")]).unique()
+    x[rows] = torch.randn(len(rows), K, generator=g, device="cuda").bfloat16()
+    base[rows] = torch.randn(len(rows), N, generator=g, device="cuda").bfloat16()
+    ids = (torch.arange(T, device="cuda") % 4).int() - 1
+    a = dense.Adapters(down, up)
+    assert a.product(x, ids, base, out=base) is base
+    small = torch.zeros(len(rows), N, dtype=BF16, device="cuda")
+    want = plain(x[rows], ids[rows], small, down, up, None)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    torch.randn(3, 8, K, generator=g, device="cuda"), torch.randn(3, N, 8, generator=g, device="cuda")
+    torch.randint(0, T, (200,), generator=g, device="cuda"), torch.randn(len(rows), K, generator=g, device="cuda")
+    start = torch.randn(len(rows), N, generator=g, device="cuda").bfloat16()
+    close(base[rows], (want[0] + start.double(), want[1] + start.double().abs(), want[2]), K, 8)
+    base[rows] = 0
+    for part in base.split(1 << 16):
+        assert not part.any()
 
 
 @gpu

@@ -126,8 +126,8 @@ def low_rank(**change):
                                     dict(inner=1 << 30), dict(rows=1 << 31), dict(down=None), dict(up=None), dict(down=A + 8), dict(up=A + 2),
                                     dict(ids=None), dict(x=None), dict(out=None), dict(x_stride=-1), dict(base_stride=-1), dict(out_stride=31),
                                     dict(out=A), dict(out=A + 2 * 63), dict(out=A + 64 * 2 * 3), dict(out=A * 2 + 16), dict(out=A * 2, out_stride=40),
-                                    dict(out=A * 2, base_stride=0), dict(rows=65), dict(rows=65, workspace=A + 8, workspace_bytes=1 << 20),
-                                    dict(rows=65, workspace=A, workspace_bytes=100)])
+                                    dict(out=A * 2, base_stride=0), dict(rows=129), dict(rows=129, workspace=A + 8, workspace_bytes=1 << 20),
+                                    dict(rows=129, workspace=A, workspace_bytes=100)])
 def test_low_rank_refuses(change):
     assert refused(LIB.eps_b200_low_rank, low_rank(**change), None) == eps.INVALID_ARGUMENT
     assert refused(LIB.eps_b200_low_rank, None, None) == eps.INVALID_ARGUMENT
@@ -136,8 +136,8 @@ def test_low_rank_refuses(change):
 def test_low_rank_layout():
     assert [LIB.eps_b200_low_rank_rank(r) for r in (1, 8, 9, 16, 17, 33, 64, 65, 128, 129)] == [8, 8, 16, 16, 32, 64, 64, 128, 128, 0]
     assert [LIB.eps_b200_low_rank_inner(k) for k in (1, 32, 33, 4096)] == [64, 64, 64, 4096]
-    assert LIB.eps_b200_low_rank_workspace(64, 100) == 0
-    for rows, n in ((65, 1), (1000, 16384), (100000, 3)):      # the units of the worst split, the rows' order, and a count
+    assert LIB.eps_b200_low_rank_workspace(128, 100) == 0
+    for rows, n in ((129, 1), (1000, 16384), (100000, 3)):      # the units of the worst split, the rows' order, and a count
         assert LIB.eps_b200_low_rank_workspace(rows, n) >= 16 + 16 * (rows // 64 + min(rows, n + 1)) + 4 * rows
 
 
