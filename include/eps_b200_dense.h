@@ -3,8 +3,9 @@
  *
  * The embedding store (eps_b200.h) pulls rows and applies their gradients; these
  * entry points are the dense block that stands beside it: the norms before and
- * after a block with its gate and residual scale, routing to experts, the
- * experts' products in 8-bit integers, and AdamW over many tensors.  None has a
+ * after a block with its gate and residual scale, routing to experts and the loss that
+ * balances them, the experts' products in 8-bit integers, low-rank adapters beside a
+ * shared layer, AdamW over many tensors and the norm that clips it.  None has a
  * counterpart in the reference, whose dense part is left to TensorFlow.
  *
  * Conventions:
@@ -343,12 +344,15 @@ EPS_B200_EXPORT int eps_b200_balance_loss_backward(const EpsB200BalanceLoss* arg
  *   a = ids[t];  out[t] = base[t] + scale[a] * up[a] (down[a] x[t])
  * An id outside [0, adapters) is no adapter: out[t] is base[t].  base NULL: 0; out may
  * be base itself.  out must not overlap x.  down [adapters, R, K'] and up [adapters,
- * channels, R] are contiguous and 16-byte aligned, with R = eps_b200_low_rank_rank(rank)
+ * channels, R] are contiguous and 16-byte aligned; inner, channels and strides are below
+ * 2^30.  R = eps_b200_low_rank_rank(rank)
  * and K' = eps_b200_low_rank_inner(inner), and zeros behind `rank` and `inner`.  All
- * have one type.  Products are exact and sums are held in 32 bits; down[a] x[t] is
+ * have one type.  `workspace` holds eps_b200_low_rank_workspace() bytes (0 for few rows).
+ * Products are exact and sums are held in 32 bits; down[a] x[t] is
  * kept to 16 bits of mantissa or more (24 with float, where infinity, NaN or a magnitude
  * from 3.38e38 on in x[t], down, up or a sum makes what it enters NaN).  A row's result
- * does not depend on the other rows' values. */
+ * does not depend on the other rows' values (on their number it does: sums are shared out
+ * by it). */
 #define EPS_B200_LOW_RANK 128u             /* most ranks */
 #define EPS_B200_LOW_RANK_ADAPTERS 16384u  /* most adapters */
 typedef struct {
