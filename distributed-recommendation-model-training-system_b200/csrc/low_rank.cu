@@ -7,19 +7,19 @@
 // for the rows that have it; 2 R operations a value of x and of out are far below what
 // the matrix instructions give, so what counts is that loads stay in flight.  Rows are
 // taken in units of one adapter and up to 32 rows (64 for larger ranks, whose adapters are
-// then read less often; 16 where the call has few).  A cluster works on a unit: its warps share out the inner size, each summing its share of
-// u for its rows, the parts are added over the warps and, through distributed shared
-// memory, over the blocks; then its warps share out the channels.  One launch, no u in
-// memory; a launch before it sorts more than 128 rows by adapter.
+// then read less often; 16 where the call has few).  A cluster works on a unit: its warps
+// share out the inner size, each summing its share of u for its rows, the parts are added
+// over the warps and, through distributed shared memory, over the blocks; then its warps
+// share out the channels.  One launch, no u in memory; a launch before it sorts more than
+// 128 rows by adapter.
 //
 // Fragments need no exchange between lanes: a sum over k may take its terms in any order,
 // so each lane of a matrix instruction's row takes 16 consecutive bytes and gives them to
 // the places that the instruction has for it, the same for both operands.  In the second
 // product the columns are dealt so that a lane ends up with 16 bytes of consecutive
-// channels.  Every warp copies what it needs itself, asynchronously and some turns ahead,
-// into shared memory of its own, whole lines of 128 bytes of a row at a time (what limits a
-// block is the number of requests under way: with 64 bytes each reading x took half as long
-// again); the copies of base go on while u is still being added up.
+// channels.  Every warp copies what it needs itself, asynchronously and a turn ahead, into
+// shared memory of its own, whole lines of 128 bytes of a row at a time; the copies of base
+// go on while u is still being added up.
 //
 //   8189 rows x 4096 x 4096 bf16, rank 16, 32 adapters: 51.4 us, 210 MB at 4.1 TB/s.  7 us of
 // it are the sort, finding the units and joining u; x takes 15 and base and out 25, one
@@ -30,7 +30,7 @@
 // Precision: 16-bit products are exact and summed in float.  u is not rounded to 16
 // bits: it goes on as the sum of two 16-bit values (float16: under a power of two of the
 // row, so that its range does not matter).  Floats are cut into three bfloat16 values,
-// which is exact, and the six largest of the nine products are summed; the others are
+// which is exact but next to the smallest floats, and the six largest of the nine products are summed; the others are
 // below 2^-25 of the first.
 #include <algorithm>
 #include <cmath>
@@ -159,7 +159,9 @@ struct Shape {
   static constexpr int kMatrices = kEach / 2;                    // of 8 channels
   static constexpr bool kHold = M * kMultiplies * kParts <= 8;    // u's stay in registers for all runs
   // a warp's copies under way: lines of 128 bytes of x and down, or of base and up
-  static constexpr bool kWeights = R * sizeof(T) <= 64;          // down and up are copied ahead too
+  // down and up are copied ahead too, where shared memory has room: rank 16 of 8192 rows x 4096
+  // x 4096 takes 52 us so and 108 without; rank 64 of 4096 rows 52 both ways
+  static constexpr bool kWeights = R * sizeof(T) <= 64;
   static constexpr int kRows = M * 16 * 128;
   static constexpr int kDown = kWeights ? R * 128 : 0;
   static constexpr int kUp = kWeights ? kRun * R * (int)sizeof(T) : 0;

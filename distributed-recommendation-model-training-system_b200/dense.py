@@ -807,8 +807,8 @@ class GradientNorm:
     `gradients` are contiguous float32, bfloat16 or float16 tensors of one device, each of
     its own type, no two of which overlap (the buffers of one AdamW or of several): their
     addresses go to the GPU now, their values are read by each call.  Sums are held in 64
-    bits and taken in a fixed order.  A captured call keeps the buffers it reads alive; the
-    object has to outlive the graph."""
+    bits and taken in a fixed order.  A captured call keeps its max_norm and the buffers it
+    reads alive; the object has to outlive the graph."""
 
     def __init__(self, gradients: Sequence[torch.Tensor], *, kind: str = "l2"):
         self._kind, self._kept = _choice(_NORMS, kind, "kind"), []
