@@ -697,7 +697,8 @@ class Adapters:
     """Low-rank adapters beside a linear layer that many requests share, each row with its
     own: out[t] = base[t] + scale[a] * up[a] (down[a] x[t]) for a = ids[t].
 
-    Laid out once; load() puts another adapter in the place of one."""
+    Laid out once; load() puts another adapter in the place of one.  A captured product reads
+    what is held here, so the object has to outlive the graph."""
 
     def __init__(self, down, up, scale=None):
         """down [adapters, rank, inner] and up [adapters, channels, rank] of one type
