@@ -677,18 +677,15 @@ __device__ __forceinline__ void copy_rows(const Call& c, const Found<M>& f, unsi
   if (c.base == c.out) return;
   constexpr unsigned V = ALIGN / sizeof(T) > 0 ? ALIGN / sizeof(T) : 1, kMany = 8;
   const unsigned packs = (c.channels + V - 1) / V;
-  const unsigned begin = (unsigned)((uint64_t)packs * rank / blocks), width = (unsigned)((uint64_t)packs * (rank + 1) / blocks) - begin;
-  const unsigned many = width * f.count;      // of this block, row by row
-  for (unsigned i = threadIdx.x; i < many; i += kThreads * kMany) {
+  const unsigned begin = (unsigned)((uint64_t)packs * rank / blocks), end = (unsigned)((uint64_t)packs * (rank + 1) / blocks);
+  each_pack<kMany>(begin, end, f.count, threadIdx.x, kThreads, [&](const unsigned (&row)[kMany], const unsigned (&pack)[kMany], unsigned n) {
     Pack<T, V> v[kMany];
-    uint32_t row[kMany], at[kMany];
+    uint32_t to[kMany];
 #pragma unroll
     for (unsigned j = 0; j < kMany; ++j) {
-      const unsigned k = min(i + j * kThreads, many - 1), r = k / width;
-      row[j] = (uint32_t)f.row[r];
-      at[j] = (begin + k - r * width) * V;
+      to[j] = (uint32_t)f.row[row[j]];
       if (c.base) {
-        v[j] = load_pack<T, V>(reinterpret_cast<const T*>(static_cast<const char*>(c.base) + (uint64_t)row[j] * c.base_stride) + at[j]);
+        v[j] = load_pack<T, V>(reinterpret_cast<const T*>(static_cast<const char*>(c.base) + (uint64_t)to[j] * c.base_stride) + pack[j] * V);
       } else {
 #pragma unroll
         for (unsigned e = 0; e < V; ++e) v[j].v[e] = from_float<T>(0.f);
@@ -696,9 +693,8 @@ __device__ __forceinline__ void copy_rows(const Call& c, const Found<M>& f, unsi
     }
 #pragma unroll
     for (unsigned j = 0; j < kMany; ++j)
-      if (i + j * kThreads < many)
-        store_pack<T, V>(reinterpret_cast<T*>(static_cast<char*>(c.out) + (uint64_t)row[j] * c.out_stride) + at[j], v[j]);
-  }
+      if (j < n) store_pack<T, V>(reinterpret_cast<T*>(static_cast<char*>(c.out) + (uint64_t)to[j] * c.out_stride) + pack[j] * V, v[j]);
+  });
 }
 
 template <class T, int R, int M, int ALIGN>
