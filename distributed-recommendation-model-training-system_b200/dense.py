@@ -273,8 +273,11 @@ class _Streams:
     freed memory out again in the order of the stream that it was made on; it has to hear of
     the others, or what is dropped here could be overwritten under a running kernel."""
 
-    def __init__(self, device, *tensors):
-        self.seen, self.tensors = {_stream(device)}, [t for t in tensors if t is not None]
+    def __init__(self, device, *own, given=()):
+        """own: made now, on the current stream; given: made by the caller, on streams that
+        are not known here."""
+        self.seen = set() if given else {_stream(device)}
+        self.tensors = [t for t in (*own, *given) if t is not None]
 
     def use(self, stream, device):
         if stream not in self.seen:
@@ -646,7 +649,7 @@ class QuantizedExperts:
         self.scale = scale.reshape(self.experts, self.channels)
         self.bias = None if bias is None else bias.reshape(self.experts, self.channels)
         self._index, self._fixed = self.device.index, (self.weight.data_ptr(), self.scale.data_ptr(), _ptr(self.bias))
-        self._streams = _Streams(self._index, self.weight, self.scale, self.bias)
+        self._streams = _Streams(self._index, self.weight, given=(self.scale, self.bias))
 
     @classmethod
     def from_weights(cls, weight, bias=None):
@@ -837,7 +840,7 @@ class GradientNorm:
         plan = host.to(device)
         self.device, self.gradients = device, gradients
         self._bound = (gradients, plan, blocks.value, _lib.eps_b200_gradient_norm_workspace(blocks.value),
-                       _Streams(index, plan, *gradients))
+                       _Streams(index, plan, given=gradients))
 
     def _run(self, clip, max_norm, gradient_scale):
         _, plan, blocks, space, streams = self._bound
@@ -933,7 +936,8 @@ class AdamW:
         # an AdamWClock: no step taken, no rate of its own; used from the first captured step on
         self._clock = torch.tensor(list(struct.unpack("@4q", bytes(AdamWClock(0, -1.0)))), device=self.device)
         self._counted, self._kept = False, []
-        self._streams = _Streams(index, self.first, self.second, self.first_scale, self.second_scale, self.master, self._clock)
+        self._streams = _Streams(index, self.first, self.second, self.first_scale, self.second_scale, self.master, self._clock,
+                                given=self.parameters)
         self._bound = None
         if gradients is not None:
             self.bind(gradients)
@@ -984,7 +988,7 @@ class AdamW:
         blocks = C.c_uint64(0)
         _call(_lib.eps_b200_adamw_plan, tensors, len(gradients), host.data_ptr(), size, C.byref(blocks))
         plan = host.to(self.device)
-        self._bound = (gradients, plan, blocks.value, _TYPES[dtype], _Streams(self.device.index, plan, *gradients))
+        self._bound = (gradients, plan, blocks.value, _TYPES[dtype], _Streams(self.device.index, plan, given=gradients))
 
     def step(self, gradients: Sequence[torch.Tensor] | None = None, *, gradient_scale=None, skip=None):
         """One step.  gradient_scale: a float32 scalar on the GPU that multiplies
