@@ -311,6 +311,13 @@ int eps_b200_gradient_norm(const EpsB200GradientNorm* a, void* stream, EpsB200St
     need(!a->blocks || (a->plan && aligned(a->plan, 16)), "a plan is 16-byte aligned");
     const uint64_t space = eps_b200_gradient_norm_workspace(a->blocks);
     need(!space || (a->workspace && aligned(a->workspace, 8) && a->workspace_bytes >= space), "the norm's workspace is too small");
+    // every block reads the factor, after the first launch left its sums and while one block writes the result
+    auto apart = [](const void* p, uint64_t n, const void* q, uint64_t m) {
+      const auto a = reinterpret_cast<uintptr_t>(p), b = reinterpret_cast<uintptr_t>(q);
+      return !p || !q || a + n <= b || b + m <= a;
+    };
+    need(apart(a->gradient_scale, sizeof(float), a->result, sizeof(EpsB200GradientResult)), "gradient_scale is a part of result");
+    need(apart(a->gradient_scale, sizeof(float), a->workspace, space), "gradient_scale is a part of the workspace");
     OnDevice on(a->device);
     Call c{static_cast<const Span*>(a->plan), (unsigned)a->blocks, a->gradient_scale, a->max_norm, a->result, static_cast<double*>(a->workspace)};
     const auto s = static_cast<cudaStream_t>(stream);

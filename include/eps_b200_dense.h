@@ -293,9 +293,10 @@ typedef struct {
   int32_t reserved;
   const void* plan;
   uint64_t blocks;
-  const float* gradient_scale;   /* device scalar or NULL */
+  const float* gradient_scale;   /* device scalar or NULL; no part of result, such as the
+                                    scale of the call before, nor of a gradient */
   double max_norm;               /* >= 0; infinity: nothing is clipped */
-  EpsB200GradientResult* result; /* device */
+  EpsB200GradientResult* result; /* device; with gradient_scale, outside the workspace */
   void* workspace;
   uint64_t workspace_bytes;
 } EpsB200GradientNorm;
