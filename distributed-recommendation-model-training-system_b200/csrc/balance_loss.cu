@@ -700,8 +700,17 @@ int eps_b200_balance_loss_backward(const EpsB200BalanceLoss* a, const int32_t* c
     b.add_stride = add_stride;
     b.out = dlogits;
     b.out_stride = dlogits_stride;
-    OnDevice on(a->device);
+    // A lane reads its packs of a row before it writes them: what lies at the same place may be the same
+    // tensor.  Elsewhere a row would be written before another lane has read it.
     const size_t size = size_of(a->type);
+    const Matrix to{dlogits, dlogits_stride, a->experts};
+    need(a->tokens == 1 || dlogits_stride >= (int64_t)a->experts || dlogits_stride <= -(int64_t)a->experts, "rows of dlogits overlap");
+    auto apart = [&](const void* p, int64_t stride) {
+      return !p || (p == dlogits && (a->tokens == 1 || stride == dlogits_stride)) || !overlap(to, {p, stride, a->experts}, a->tokens, size);
+    };
+    need(apart(a->logits, a->logits_stride), "dlogits overlaps logits without being it");
+    need(apart(add, add_stride), "dlogits overlaps add without being it");
+    OnDevice on(a->device);
     const size_t pack = pack_bytes({{a->logits, a->logits_stride}, {dlogits, dlogits_stride}, {add, add_stride}}, a->experts, size);
     const auto s = static_cast<cudaStream_t>(stream);
     const bool sigmoid = a->score == EPS_B200_SCORE_SIGMOID;

@@ -924,17 +924,6 @@ void launch(Call c, int align, void* workspace, int device, cudaStream_t stream)
   run(std::false_type{}, most, cluster);
 }
 
-// Whether two tensors of rows share memory; columns of one wider tensor do not.
-bool overlap(const void* a, int64_t a_stride, uint64_t a_columns, const void* b, int64_t b_stride, uint64_t b_columns, uint64_t rows, uint64_t size) {
-  const auto at = reinterpret_cast<uintptr_t>(a), bt = reinterpret_cast<uintptr_t>(b);
-  const uint64_t a_end = at + ((rows - 1) * (uint64_t)a_stride + a_columns) * size, b_end = bt + ((rows - 1) * (uint64_t)b_stride + b_columns) * size;
-  if (a_end <= bt || b_end <= at) return false;
-  if (a_stride != b_stride || a_stride <= 0) return true;
-  const uint64_t pitch = (uint64_t)a_stride * size;
-  const uint64_t ahead = bt >= at ? (bt - at) % pitch : (pitch - (at - bt) % pitch) % pitch;     // of b's columns before a's next
-  return ahead < a_columns * size || ahead + b_columns * size > pitch;
-}
-
 // Whether every row begins and ends on n bytes.
 bool rows_on(size_t n, const void* p, int64_t stride, uint64_t columns, size_t size) {
   return aligned(p, n) && stride * (int64_t)size % (int64_t)n == 0 && columns * size % n == 0;
@@ -970,9 +959,9 @@ int eps_b200_low_rank(const EpsB200LowRank* a, void* stream, EpsB200Status* stat
     need(a->rows == 1 || (a->x_stride < (1 << 30) && a->base_stride < (1 << 30) && a->out_stride < (1 << 30)), "row strides are below 2^30");
     need(a->rows == 1 || a->out_stride >= (int64_t)a->channels, "rows of out overlap");
     const size_t size = size_of(a->type);
-    need(!overlap(a->out, a->out_stride, a->channels, a->x, a->x_stride, a->inner, a->rows, size), "out overlaps x");
+    need(!overlap({a->out, a->out_stride, a->channels}, {a->x, a->x_stride, a->inner}, a->rows, size), "out overlaps x");
     if (a->base && !(a->base == a->out && (a->rows == 1 || a->base_stride == a->out_stride)))
-      need(!overlap(a->out, a->out_stride, a->channels, a->base, a->base_stride, a->channels, a->rows, size), "out overlaps base without being it");
+      need(!overlap({a->out, a->out_stride, a->channels}, {a->base, a->base_stride, a->channels}, a->rows, size), "out overlaps base without being it");
     const Space space(a->rows, a->adapters);
     need(!space.bytes || (a->workspace && aligned(a->workspace, 16) && a->workspace_bytes >= space.bytes), "the adapters' workspace is too small");
     Call c{};

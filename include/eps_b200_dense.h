@@ -333,8 +333,8 @@ EPS_B200_EXPORT int eps_b200_balance_loss(const EpsB200BalanceLoss* args, const 
                                           void* workspace, uint64_t workspace_bytes,
                                           void* stream, EpsB200Status* status);
 /* dlogits = *dloss * (the loss's gradient) + add, rounded once; masked tokens get `add`
- * alone.  dloss NULL: 1; add NULL: 0; dlogits may be `add` itself.  The counts take no
- * gradient. */
+ * alone.  dloss NULL: 1; add NULL: 0; dlogits may be `add` or the logits themselves, and
+ * must not overlap them otherwise.  The counts take no gradient. */
 EPS_B200_EXPORT int eps_b200_balance_loss_backward(const EpsB200BalanceLoss* args, const int32_t* counts,
                                                    const int32_t* counted, const float* dloss,
                                                    const void* add, int64_t add_stride,
