@@ -76,7 +76,7 @@ struct Backward : Rows {
 __device__ __forceinline__ float most(float a, float b) { float r; asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b)); return r; }
 __device__ __forceinline__ float least(float a, float b) { float r; asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b)); return r; }
 
-// e^x of N values up to 88.5.  The power of two takes x log2 e rounded to a float, off by
+// e^x of N values up to 88.72.  The power of two takes x log2 e rounded to a float, off by
 // |x| / 2 units; float logits add back what that lost, x less that power's logarithm.
 template <int N, bool FINE>
 __device__ __forceinline__ void powers(float (&x)[N]) {
@@ -178,39 +178,25 @@ struct Copies {
   }
 };
 
-// A row of sigmoids whose largest logit is below kLow: its scores are e^x to all bits, and
-// may be below the normal floats, down to what a float can tell from 0 (there e^-x passes
-// the largest float, and the router's scores end as well).  They go on as e^(x - top).
-constexpr float kLow = -40.f, kLeast = -88.7228394f;
+// What the scores of sigmoids are divided by, so that the reciprocal keeps them normal floats
+// as far down as a float can tell them from 0: e^-x passes 2^127.99 at -88.716, behind which
+// they are 0 (the router's are behind 2^128).  It costs no instruction.
+constexpr float kUnit = 0.2518f, kLeast = 88.72f;      // kUnit e^kLeast is above 2^126, e^kLeast below 2^128
 
 // The scores of U rows of logits, -inf behind their last columns: their unnormalised p and,
-// for sigmoids, 1 - s in rest.  now: rows that count.  unit: what a score of 1 stands for.
+// for sigmoids, 1 - s in rest, both over kUnit.
 template <class T, int U, int N, bool SIGMOID>
-__device__ __forceinline__ void scores(float (&v)[U][N], float (&rest)[U][SIGMOID ? N : 1], const bool (&now)[U], float (&unit)[U], unsigned width) {
+__device__ __forceinline__ void scores(float (&v)[U][N], float (&rest)[U][SIGMOID ? N : 1], unsigned width) {
   constexpr bool kFine = std::is_same_v<T, float>;
-#pragma unroll
-  for (int u = 0; u < U; ++u) unit[u] = 1.f;
   if constexpr (SIGMOID) {
-    // s = 1 / (1 + e), 1 - s = e s with e = e^-x; at 88.5 s is 0, as behind it
-    const unsigned lane = threadIdx.x % 32, row = (width == 32 ? ~0u : (1u << width) - 1) << (lane & ~(width - 1));
+    // s = 1 / (1 + e), 1 - s = e s with e = e^-x; s is 0 from -kLeast down
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      float one = 1.f, top = v[u][0];
-#pragma unroll
-      for (int i = 1; i < N; ++i) top = fmaxf(top, v[u][i]);
-      if (!(__ballot_sync(~0u, top >= kLow) & row) && now[u]) {
-        for (unsigned o = width / 2; o; o /= 2) top = fmaxf(top, __shfl_xor_sync(row, top, o));
-        if (top >= kLeast && top < kLow) {
-          one = 0.f;                       // 1 beside e^-top is nothing
-          unit[u] = expf(top);
-          vadd<N>(v[u], v[u], -top);
-        }
-      }
       float e[N];
 #pragma unroll
-      for (int i = 0; i < N; ++i) e[i] = least(-v[u][i], 88.5f);
+      for (int i = 0; i < N; ++i) e[i] = least(-v[u][i], kLeast);
       powers<N, kFine>(e);
-      vadd<N>(v[u], e, one);
+      vfma<N>(v[u], e, +kUnit, +kUnit);
 #pragma unroll
       for (int i = 0; i < N; ++i) v[u][i] = inverse(v[u][i]);
       vmul<N>(rest[u], e, v[u]);
@@ -307,7 +293,7 @@ __global__ void __launch_bounds__(kThreadsFor<J * V>, 1) balance_forward(Forward
   constexpr int U = kAhead > 1 ? 2 : 1;
   for (unsigned turn = 0; __any_sync(~0u, row < end + kAhead * step); turn += U) {
     bool now[U];
-    float v[U][J * V], rest[U][SIGMOID ? J * V : 1], by[U], unit[U];
+    float v[U][J * V], rest[U][SIGMOID ? J * V : 1], by[U];
     copies_wait<kAhead - U>();
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -317,7 +303,7 @@ __global__ void __launch_bounds__(kThreadsFor<J * V>, 1) balance_forward(Forward
 #pragma unroll
     for (int u = 0; u < U; ++u) copy(turn + kAhead + u);
     if (!__any_sync(~0u, now[0] || now[U - 1])) continue;
-    scores<T, U, J * V, SIGMOID>(v, rest, now, unit, width);
+    scores<T, U, J * V, SIGMOID>(v, rest, width);
     if (!SIGMOID || f.normalise) {
 #pragma unroll
       for (int u = 0; u < U; ++u) by[u] = lane_sum<J * V>(v[u]);
@@ -326,7 +312,7 @@ __global__ void __launch_bounds__(kThreadsFor<J * V>, 1) balance_forward(Forward
       for (int u = 0; u < U; ++u) by[u] = share(by[u]);
     } else {
 #pragma unroll
-      for (int u = 0; u < U; ++u) by[u] = unit[u];
+      for (int u = 0; u < U; ++u) by[u] = kUnit;
     }
 #pragma unroll
     for (int u = 0; u < U; ++u)
@@ -483,7 +469,7 @@ __global__ void __launch_bounds__(kThreadsFor<J * V>, 1) balance_backward(Backwa
   }
   const uint64_t last = b.tokens + kAhead * step;      // what `row` is behind the last
   for (unsigned turn = 0; __any_sync(~0u, row < last); ++turn) {
-    const bool now[1] = {(there & 1) != 0}, mine = row < last;
+    const bool now = there & 1, mine = row < last;
     float score[1][J * V], g[J * V], rest[1][SIGMOID ? J * V : 1];
     float(&v)[J * V] = score[0];
     copies_wait<kAhead - 1>();
@@ -495,10 +481,9 @@ __global__ void __launch_bounds__(kThreadsFor<J * V>, 1) balance_backward(Backwa
       for (int i = 0; i < J * V; ++i) g[i] = 0.f;
     }
     copy(turn + kAhead);
-    if (__any_sync(~0u, now[0])) {
-      float unit[1];
-      scores<T, 1, J * V, SIGMOID>(score, rest, now, unit, width);
-      float by = unit[0], dot = 0.f, slope[J * V];
+    if (__any_sync(~0u, now)) {
+      scores<T, 1, J * V, SIGMOID>(score, rest, width);
+      float by = kUnit, dot = 0.f, slope[J * V];
       if (shares) {
         vmul<J * V>(slope, v, d);
         float both[2] = {lane_sum<J * V>(v), lane_sum<J * V>(slope)};
@@ -506,7 +491,8 @@ __global__ void __launch_bounds__(kThreadsFor<J * V>, 1) balance_backward(Backwa
         by = share(both[0]);
         dot = both[1] * by;
       }
-      if (now[0]) {
+      if (now) {
+        if constexpr (SIGMOID) by *= kUnit;      // of rest
         vadd<J * V>(slope, d, -dot);
         vmul<J * V>(v, v, by);
         if constexpr (SIGMOID) vmul<J * V>(v, v, rest[0]);

@@ -307,9 +307,8 @@ EPS_B200_EXPORT int eps_b200_gradient_norm(const EpsB200GradientNorm* args, void
  *   s = softmax(logits) or sigmoid(logits)       a row of -inf alone has s = 0
  *   p = s / sum_e s                              s itself if not `normalise` (0 if the
  *                                                sum is 0; a softmax is normalised as it is)
- * A sigmoid's sum is 0 where a float tells none of its scores from 0: no logit is above
- * -88.72 (the router's weights end there too).  A score below 2^-126 beside one above 2^-57
- * counts as 0.
+ * A sigmoid counts as 0 where a float hardly tells it from 0, at logits of -88.71 and below
+ * (the router's weights end at -88.72).
  * over the tokens whose mask is not 0 (all without a mask), n of them:
  *   counts[e] = entries of chosen[t, :] that are e; entries outside [0, experts) count for none
  *   mass[e] = sum_t p[t, e]
