@@ -241,7 +241,8 @@ __global__ void __launch_bounds__(kThreadsFor<J * V>, 1) balance_forward(Forward
   const unsigned E = f.experts, lane = threadIdx.x % 32, warp = threadIdx.x / 32, width = f.width, first = lane % width * V;
   C copies(shared, first, width, E, -INFINITY);
   float* const mass = reinterpret_cast<float*>(shared + C::kAll / 4);       // [warps][E]
-  uint32_t* const counts = shared + C::kAll / 4 + warps * E;                // [E], and the counted tokens behind them
+  double* const total = reinterpret_cast<double*>(shared + C::kAll / 4 + (warps * E + 1) / 2 * 2);      // [E]
+  uint32_t* const counts = reinterpret_cast<uint32_t*>(total + E);          // [E], and the counted tokens behind them
   asm volatile("griddepcontrol.launch_dependents;");
   const unsigned begin = (uint64_t)f.tokens * blockIdx.x / gridDim.x, end = (uint64_t)f.tokens * (blockIdx.x + 1) / gridDim.x;
   // this lane's rows: `row` is the next to be copied, `there` has a bit for each that is under way
@@ -287,54 +288,71 @@ __global__ void __launch_bounds__(kThreadsFor<J * V>, 1) balance_forward(Forward
   } else if (threadIdx.x == 0) {
     counts[E] = end - begin;
   }
-  // mass
-  float sum[J * V] = {};
-  // two rows a turn, whose chains of reductions run beside each other
+  // mass, two rows a turn, whose chains of reductions run beside each other.  Up to kRun rows of
+  // a lane are added in float, over the block too; where it has more, such sums go on in double,
+  // so that they are as exact for many tokens as for few
   constexpr int U = kAhead > 1 ? 2 : 1;
-  for (unsigned turn = 0; __any_sync(~0u, row < end + kAhead * step); turn += U) {
-    bool now[U];
-    float v[U][J * V], rest[U][SIGMOID ? J * V : 1], by[U];
-    copies_wait<kAhead - U>();
+  constexpr unsigned kRun = 32;
+  float sum[J * V] = {};
+  bool before = false;                     // a run is in total already
+  for (unsigned turn = 0, left = end - begin;; left -= kRun * step) {
+    const unsigned until = end + kAhead * step - (left > kRun * step ? left - kRun * step : 0);      // what `row` is behind the run
+    for (; __any_sync(~0u, row < until); turn += U) {
+      bool now[U];
+      float v[U][J * V], rest[U][SIGMOID ? J * V : 1], by[U];
+      copies_wait<kAhead - U>();
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      now[u] = there >> u & 1;
-      copies.read(turn + u, v[u]);
+      for (int u = 0; u < U; ++u) {
+        now[u] = there >> u & 1;
+        copies.read(turn + u, v[u]);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) copy(turn + kAhead + u);
+      if (!__any_sync(~0u, now[0] || now[U - 1])) continue;
+      scores<T, U, J * V, SIGMOID>(v, rest, width);
+      if (!SIGMOID || f.normalise) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) by[u] = lane_sum<J * V>(v[u]);
+        row_add<U>(by, width);
+#pragma unroll
+        for (int u = 0; u < U; ++u) by[u] = share(by[u]);
+      } else {
+#pragma unroll
+        for (int u = 0; u < U; ++u) by[u] = kUnit;
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (now[u]) vfma<J * V>(sum, v[u], by[u], sum);       // the others' packs hold what was there before
     }
 #pragma unroll
-    for (int u = 0; u < U; ++u) copy(turn + kAhead + u);
-    if (!__any_sync(~0u, now[0] || now[U - 1])) continue;
-    scores<T, U, J * V, SIGMOID>(v, rest, width);
-    if (!SIGMOID || f.normalise) {
+    for (int j = 0; j < J; ++j) {
+      const unsigned c = first + j * width * V;
 #pragma unroll
-      for (int u = 0; u < U; ++u) by[u] = lane_sum<J * V>(v[u]);
-      row_add<U>(by, width);
-#pragma unroll
-      for (int u = 0; u < U; ++u) by[u] = share(by[u]);
-    } else {
-#pragma unroll
-      for (int u = 0; u < U; ++u) by[u] = kUnit;
+      for (int i = 0; i < V; ++i) {
+        float s = sum[j * V + i];
+        for (unsigned o = width; o < 32; o *= 2) s += __shfl_xor_sync(~0u, s, o);
+        if (lane < width && c + i < E) mass[warp * E + c + i] = s;
+      }
     }
+    __syncthreads();
+    if (left <= kRun * step) break;
+    for (unsigned e = threadIdx.x; e < E; e += threads) {
+      double all = before ? total[e] : 0;
+      for (unsigned w = 0; w < warps; ++w) all += (double)mass[w * E + e];
+      total[e] = all;
+    }
+    before = true;
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (now[u]) vfma<J * V>(sum, v[u], by[u], sum);       // the others' packs hold what was there before
+    for (int i = 0; i < J * V; ++i) sum[i] = 0.f;
+    __syncthreads();                       // the next run writes over mass
   }
-#pragma unroll
-  for (int j = 0; j < J; ++j) {
-    const unsigned c = first + j * width * V;
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      float s = sum[j * V + i];
-      for (unsigned o = width; o < 32; o *= 2) s += __shfl_xor_sync(~0u, s, o);
-      if (lane < width && c + i < E) mass[warp * E + c + i] = s;
-    }
-  }
-  __syncthreads();
   if (gridDim.x > 1) {
     uint32_t* const mine = f.sums + (size_t)blockIdx.x * (2 * E + 1);
     for (unsigned e = threadIdx.x; e < E; e += threads) {
       float s = 0.f;
 #pragma unroll 8
       for (unsigned w = 0; w < warps; ++w) s += mass[w * E + e];
+      if (before) s = (float)(total[e] + s);
       mine[e] = __float_as_uint(s);
       mine[E + e] = counts[e];
     }
@@ -343,7 +361,7 @@ __global__ void __launch_bounds__(kThreadsFor<J * V>, 1) balance_forward(Forward
   }
   double dot = 0;
   for (unsigned e = threadIdx.x; e < E; e += threads) {
-    double s = 0;
+    double s = before ? total[e] : 0;
 #pragma unroll 8
     for (unsigned w = 0; w < warps; ++w) s += (double)mass[w * E + e];
     f.mass[e] = (float)s;
@@ -560,7 +578,7 @@ void forward(Forward f, size_t pack, bool sigmoid, unsigned grid, int device, cu
       constexpr unsigned kThreads = kThreadsFor<J * V>;
       // a block alone has as many warps as its tokens need
       const unsigned threads = grid > 1 ? kThreads : std::min<unsigned>(kThreads, std::max<unsigned>(4, (unsigned)ceil_div(f.tokens, 32 / f.width)) * 32);
-      const size_t bytes = Copies<T, V, J, kThreads, kAheadOf<V * sizeof(T)>>::kAll + (threads / 32 * (size_t)f.experts + f.experts + 1) * 4;
+      const size_t bytes = Copies<T, V, J, kThreads, kAheadOf<V * sizeof(T)>>::kAll + (round_up(threads / 32 * f.experts, 2) + 3 * (size_t)f.experts + 1) * 4;
       auto go = [&](auto s) {
         constexpr bool S = decltype(s)::value;
         room<balance_forward<T, V, J, S>>(device);
