@@ -17,8 +17,9 @@ F32, BF16 = torch.float32, torch.bfloat16
                                        (2_000_000, 33, F32), (6_000_000, 8, BF16), (9_000_000, 1, F32)])
 @pytest.mark.parametrize("score,normalise", [("softmax", True), ("sigmoid", True), ("sigmoid", False)])
 def test_equal_rows(T, E, dtype, score, normalise):
-    """A share is within some ten units of 2^-24; a lane adds 32 rows, a warp's lanes five times, and the rest in double: 48
-    roundings of half a unit or less, and one to each block's sum.  That is below CHAIN, whatever T."""
+    """A share is within some ten units of 2^-24; equal shares, added 64 times, are off by 32 of them (each sum by one of its
+    own size), by 3 over a warp's lanes and by 16 over a block's warps, the rest is added in double, and a block's sum is
+    rounded once.  That is below CHAIN, whatever T."""
     row = torch.linspace(-2, 2, E).to(dtype)
     x = row.cuda().expand(T, E).contiguous()
     chosen = torch.zeros(T, 1, dtype=torch.int32, device="cuda")
