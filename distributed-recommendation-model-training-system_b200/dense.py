@@ -27,6 +27,7 @@ import ctypes as C
 import math
 import struct
 import threading
+from array import array
 from typing import NamedTuple, Sequence
 
 import torch
@@ -94,7 +95,7 @@ class Int8Product(C.Structure):
                 ("workspace", C.c_void_p), ("workspace_bytes", C.c_uint64)]
 
 
-class AdamWTensor(C.Structure):
+class AdamWTensor(C.Structure):      # four words
     _fields_ = [("parameter", C.c_void_p), ("gradient", C.c_void_p), ("elements", C.c_uint64),
                 ("state_begin", C.c_uint64)]
 
@@ -113,7 +114,7 @@ class AdamWClock(C.Structure):
                 ("inverse_root", C.c_float), ("key", C.c_uint32)]
 
 
-class Gradient(C.Structure):
+class Gradient(C.Structure):      # three words, of which the last is the type
     _fields_ = [("gradient", C.c_void_p), ("elements", C.c_uint64), ("type", C.c_int32), ("reserved", C.c_int32)]
 
 
@@ -826,12 +827,13 @@ class GradientNorm:
         index = _tensor(gradients[0], "a gradient")
         if _capturing(index):
             _refuse("gradients are bound before a capture")
-        tensors = (Gradient * len(gradients))()
-        for i, g in enumerate(gradients):
+        words = array("Q")
+        for g in gradients:
             _tensor(g, "a gradient", index)
             if g.dtype not in _TYPES or not g.is_contiguous():
                 _refuse("gradients are contiguous, of float32, bfloat16 or float16")
-            tensors[i] = Gradient(g.data_ptr(), g.numel(), _TYPES[g.dtype], 0)
+            words.extend((g.data_ptr(), g.numel(), _TYPES[g.dtype]))
+        tensors = (Gradient * len(gradients)).from_buffer(words)
         size = _lib.eps_b200_gradient_norm_plan_bytes(tensors, len(gradients))
         host = torch.empty(size, dtype=torch.uint8)
         blocks = C.c_uint64(0)
@@ -977,12 +979,13 @@ class AdamW:
         dtype = gradients[0].dtype if isinstance(gradients[0], torch.Tensor) else None
         if dtype not in (self.parameters[0].dtype, torch.float32):
             _refuse("gradients have the parameters' type or float32")
-        tensors = (AdamWTensor * len(gradients))()
-        for i, (p, g, a) in enumerate(zip(self.parameters, gradients, self.starts)):
-            _tensor(g, "a gradient", self.device.index)
+        index, words = self.device.index, array("Q")
+        for p, g, a in zip(self.parameters, gradients, self.starts):
+            _tensor(g, "a gradient", index)
             if g.dtype != dtype or g.shape != p.shape or not g.is_contiguous():
                 _refuse("gradients are contiguous, of one type and of the parameters' shapes")
-            tensors[i] = AdamWTensor(p.data_ptr(), g.data_ptr(), p.numel(), a)
+            words.extend((p.data_ptr(), g.data_ptr(), p.numel(), a))
+        tensors = (AdamWTensor * len(gradients)).from_buffer(words)
         size = _lib.eps_b200_adamw_plan_bytes(tensors, len(gradients))
         host = torch.empty(size, dtype=torch.uint8)
         blocks = C.c_uint64(0)
