@@ -193,7 +193,9 @@ __global__ void __launch_bounds__(kThreads, kBlocksEach) gradient_finish(Call c,
 
 // Few spans: one cluster, whose blocks read each other's values, in one launch.  That takes
 // the GPU 4.2 us for 8 spans and 4.5 for 16, against 3.2 and 3.4 in two launches, and the
-// host 11 us a call against 16; from 32 on (5.9 against 3.4) two launches are faster on both.
+// host 11 us a call against 16, however many they are.  A call takes as long as the host
+// there; at 32 spans (5.9 us of the GPU against 3.4) the GPU's loss is half of the host's
+// gain, and it grows with the spans.
 constexpr unsigned kCluster = 8, kClusterThreads = 1024, kClusterSpans = 16;
 template <int KIND, bool CLIP>
 __global__ void __cluster_dims__(kCluster) __launch_bounds__(kClusterThreads) gradient_few(Call c) {

@@ -76,8 +76,8 @@ EPS_B200_EXPORT int eps_b200_block_norm(const EpsB200BlockNorm* args, const void
  * statistics recomputed from h and y.  dx is the gradient of x and, where a user
  * differentiates h alone, of h.  Outputs may be NULL if unwanted; dy and dgate are
  * NULL without y.  The parameters' gradients are float32, written, not added.
- * Row sums over the batch are taken in an order that only the sizes and the GPU
- * decide, so results repeat exactly.  `workspace` holds
+ * Row sums over the batch are taken in an order that only the sizes, alignment, strides
+ * and the GPU decide, so results repeat exactly.  `workspace` holds
  * eps_b200_block_norm_workspace() bytes. */
 typedef struct {
   const void *dh, *dz, *h;
@@ -262,9 +262,10 @@ EPS_B200_EXPORT int eps_b200_adamw_counted(const EpsB200AdamW* args, const void*
  *   scale = u * min(1, max_norm / norm)          u where norm is 0
  * Where norm is not finite (as a float) skip is 1 and scale 0; else skip is 0.  scale
  * and skip are what eps_b200_adamw takes.  With `clip` every gradient becomes
- * gradient * scale, rounded once, and stays as it is where skip is 1.  Sums are taken
- * in 64 bits, in an order that only the sizes and the GPU decide, so results repeat
- * exactly. */
+ * gradient * scale, a product in float that is then rounded to the gradient's type, and
+ * stays as it is where skip is 1.  Sums are taken in 64 bits (the squares of 16 bytes
+ * first in float, where it holds them), in an order that only the sizes, the gradients'
+ * alignment and the GPU decide, so results repeat exactly. */
 enum { EPS_B200_GRADIENT_L2 = 0, EPS_B200_GRADIENT_MAX = 1 };
 
 typedef struct {
@@ -314,7 +315,9 @@ EPS_B200_EXPORT int eps_b200_gradient_norm(const EpsB200GradientNorm* args, void
  *   mass[e] = sum_t p[t, e]
  *   loss = weight * experts / (top_k * n^2) * sum_e counts[e] * mass[e]     0 if n is 0
  * What masked tokens hold is read by no sum.  Sums over tokens are taken in an order
- * that only the sizes and the GPU decide.  Of several ranks with a batch each, counts,
+ * that only the sizes, the logits' alignment and stride and the GPU decide, in float over
+ * 64 rows a lane at most and in 64 bits beyond, so their error does not grow with the
+ * tokens.  Of several ranks with a batch each, counts,
  * mass and counted add up to those of the joint batch; backward takes the sums. */
 typedef struct {
   int32_t device;
@@ -346,7 +349,7 @@ EPS_B200_EXPORT int eps_b200_balance_loss_backward(const EpsB200BalanceLoss* arg
 /* ---- Low-rank adapters of many requests at once, beside a layer that they share.
  *   a = ids[t];  out[t] = base[t] + scale[a] * up[a] (down[a] x[t])
  * An id outside [0, adapters) is no adapter: out[t] is base[t].  base NULL: 0; out may
- * be base itself.  out must not overlap x.  down [adapters, R, K'] and up [adapters,
+ * be base itself.  out must not overlap x, nor what else is read.  down [adapters, R, K'] and up [adapters,
  * channels, R] are contiguous and 16-byte aligned; inner, channels and strides are below
  * 2^30.  R = eps_b200_low_rank_rank(rank)
  * and K' = eps_b200_low_rank_inner(inner), and zeros behind `rank` and `inner`.  All
@@ -354,8 +357,8 @@ EPS_B200_EXPORT int eps_b200_balance_loss_backward(const EpsB200BalanceLoss* arg
  * Products are exact and sums are held in 32 bits; down[a] x[t] is
  * kept to 16 bits of mantissa or more (24 with float, where infinity, NaN or a magnitude
  * from 3.38e38 on in x[t], down, up or a sum makes what it enters NaN).  A row's result
- * does not depend on the other rows' values (on their number it does: sums are shared out
- * by it). */
+ * does not depend on the other rows' values (on the numbers of rows and of adapters it does,
+ * by a rounding: sums are shared out by them). */
 #define EPS_B200_LOW_RANK 128u             /* most ranks */
 #define EPS_B200_LOW_RANK_ADAPTERS 16384u  /* most adapters */
 typedef struct {
