@@ -660,6 +660,7 @@ Rows checked(const EpsB200BalanceLoss* a) {
   need(a->tokens < (1ull << 31) && a->tokens * a->top_k < (1ull << 31), "tokens * top_k must be below 2^31");
   need(std::isfinite(a->weight), "the weight must be finite");
   need(a->logits || !a->tokens, "null logits");
+  need(aligned(a->logits, size_of(a->type)), "logits are not aligned to their type");
   Rows r{};
   r.logits = a->logits;
   r.stride = a->logits_stride;
@@ -692,6 +693,7 @@ int eps_b200_balance_loss(const EpsB200BalanceLoss* a, const int32_t* chosen, fl
     static_cast<Rows&>(f) = checked(a);
     need(loss && counts && mass && counted, "null balance output");
     need(chosen || !a->tokens, "null chosen experts");
+    need(words(chosen, loss, counts, mass, counted), "experts and outputs are 4-byte aligned");
     const uint64_t space = eps_b200_balance_loss_workspace(a->tokens, a->experts);
     need(!space || (workspace && aligned(workspace, 4) && workspace_bytes >= space), "the balance loss's workspace is too small");
     f.chosen = chosen;
@@ -720,6 +722,8 @@ int eps_b200_balance_loss_backward(const EpsB200BalanceLoss* a, const int32_t* c
     static_cast<Rows&>(b) = checked(a);
     need(counts && counted, "null counts");
     need(dlogits || !a->tokens, "null dlogits");
+    need(words(counts, counted, dloss), "counts and dloss are 4-byte aligned");
+    need(aligned(add, size_of(a->type)) && aligned(dlogits, size_of(a->type)), "a gradient is not aligned to its type");
     if (!a->tokens) return;
     b.counts = counts;
     b.counted = counted;

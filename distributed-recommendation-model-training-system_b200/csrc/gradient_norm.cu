@@ -311,6 +311,7 @@ int eps_b200_gradient_norm(const EpsB200GradientNorm* a, void* stream, EpsB200St
     need(a->max_norm >= 0, "max_norm is 0 or more");            // and no NaN
     need(a->blocks < (1ull << 31), "too many elements for one norm");
     need(!a->blocks || (a->plan && aligned(a->plan, 16)), "a plan is 16-byte aligned");
+    need(words(a->gradient_scale, a->result), "gradient_scale and result are 4-byte aligned");
     const uint64_t space = eps_b200_gradient_norm_workspace(a->blocks);
     need(!space || (a->workspace && aligned(a->workspace, 8) && a->workspace_bytes >= space), "the norm's workspace is too small");
     // every block reads the factor, after the first launch left its sums and while one block writes the result

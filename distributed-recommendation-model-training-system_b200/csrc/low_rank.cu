@@ -959,6 +959,8 @@ int eps_b200_low_rank(const EpsB200LowRank* a, void* stream, EpsB200Status* stat
     need(a->rows == 1 || (a->x_stride < (1 << 30) && a->base_stride < (1 << 30) && a->out_stride < (1 << 30)), "row strides are below 2^30");
     need(a->rows == 1 || a->out_stride >= (int64_t)a->channels, "rows of out overlap");
     const size_t size = size_of(a->type);
+    need(aligned(a->x, size) && aligned(a->base, size) && aligned(a->out, size), "rows are not aligned to their type");
+    need(words(a->scale, a->ids), "scale and ids are 4-byte aligned");
     need(!overlap({a->out, a->out_stride, a->channels}, {a->x, a->x_stride, a->inner}, a->rows, size), "out overlaps x");
     if (a->base && !(a->base == a->out && (a->rows == 1 || a->base_stride == a->out_stride)))
       need(!overlap({a->out, a->out_stride, a->channels}, {a->base, a->base_stride, a->channels}, a->rows, size), "out overlaps base without being it");
