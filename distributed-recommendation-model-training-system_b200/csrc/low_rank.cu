@@ -678,7 +678,7 @@ __device__ __forceinline__ void copy_rows(const Call& c, const Found<M>& f, unsi
   constexpr unsigned V = ALIGN / sizeof(T) > 0 ? ALIGN / sizeof(T) : 1, kMany = 8;
   const unsigned packs = (c.channels + V - 1) / V;
   const unsigned begin = (unsigned)((uint64_t)packs * rank / blocks), end = (unsigned)((uint64_t)packs * (rank + 1) / blocks);
-  each_pack<kMany>(begin, end, f.count, threadIdx.x, kThreads, [&](const unsigned (&row)[kMany], const unsigned (&pack)[kMany], unsigned n) {
+  each_pack<kMany>(begin, end, f.count, threadIdx.x, kThreads, [&](const unsigned (&row)[kMany], const unsigned (&pack)[kMany], const bool (&there)[kMany]) {
     Pack<T, V> v[kMany];
     uint32_t to[kMany];
 #pragma unroll
@@ -693,7 +693,7 @@ __device__ __forceinline__ void copy_rows(const Call& c, const Found<M>& f, unsi
     }
 #pragma unroll
     for (unsigned j = 0; j < kMany; ++j)
-      if (j < n) store_pack<T, V>(reinterpret_cast<T*>(static_cast<char*>(c.out) + (uint64_t)to[j] * c.out_stride) + pack[j] * V, v[j]);
+      if (there[j]) store_pack<T, V>(reinterpret_cast<T*>(static_cast<char*>(c.out) + (uint64_t)to[j] * c.out_stride) + pack[j] * V, v[j]);
   });
 }
 

@@ -10,11 +10,11 @@ int main(int, char** argument) {
   const unsigned rows = std::strtoul(argument[3], nullptr, 0), thread = std::strtoul(argument[4], nullptr, 0);
   const unsigned long long most = std::strtoull(argument[5], nullptr, 0);      // places, and no end beyond them
   unsigned long long places = 0, sum = 0;
-  eps_b200::dense::each_pack<8>(begin, end, rows, thread, 256, [&](const unsigned (&row)[8], const unsigned (&pack)[8], unsigned n) {
+  eps_b200::dense::each_pack<8>(begin, end, rows, thread, 256, [&](const unsigned (&row)[8], const unsigned (&pack)[8], const bool (&there)[8]) {
     if (places > most) std::exit(1);
     for (unsigned j = 0; j < 8; ++j) {
       if (row[j] >= rows || pack[j] < begin || pack[j] >= end) std::exit(2);
-      if (j < n) ++places, sum += row[j] * 3ull + pack[j];
+      if (there[j]) ++places, sum += row[j] * 3ull + pack[j];
     }
   });
   std::printf("%llu %llu\n", places, sum);
