@@ -21,8 +21,8 @@
 // of two waits for some 20 dependent steps), the block's sums, and the second launch (4 us).
 // 32771 x 256 floats, sigmoid: 16.5 us; 131071 x 96 bf16, half of it padding: 19.7; backward
 // of 65521 x 256 bf16 with `add`, half of it padding: 21.9, 59 % of the copy rate for the 84
-// MB that it moves (a plain sum of two tensors of that size takes 16.7).  Before rows were copied ahead, with twice the instructions a
-// column: 30.3, 37.5 and 25.9.
+// MB that it moves (a plain sum of two tensors of that size takes 16.7).  Before rows were
+// copied ahead, with twice the instructions a column: 30.3, 37.5 and 25.9.
 #include <algorithm>
 #include <cmath>
 #include <initializer_list>

@@ -549,7 +549,8 @@ def balance_loss(logits, experts, *, score: str = "softmax", normalise: bool = T
     logits [tokens, E]; experts [tokens, top_k] int32, as route gives them (entries outside
     [0, E) count for none).  mask [tokens] bool: only these n tokens count, the others'
     logits are not read.  A row of masked logits (-inf) alone has p = 0, and so has one of
-    sigmoids of -88.71 and less, where float scores end; without a token the loss is 0.  At most 1024 experts and top_k 32."""
+    sigmoids of -88.71 and less, where float scores end; without a token the loss is 0.  At
+    most 1024 experts and top_k 32."""
     logits, stride, tokens, count = _matrix(logits, "logits")
     index, device = logits.get_device(), logits.device
     _tensor(experts, "experts", index)
@@ -812,8 +813,8 @@ class GradientNorm:
     `gradients` are contiguous float32, bfloat16 or float16 tensors of one device, each of
     its own type, no two of which overlap (the buffers of one AdamW or of several): their
     addresses go to the GPU now, their values are read by each call.  Sums are held in 64
-    bits and taken in an order that sizes and alignment fix.  A captured call keeps its max_norm and the buffers it
-    reads alive; the object has to outlive the graph."""
+    bits and taken in an order that sizes and alignment fix.  A captured call keeps its
+    max_norm and the buffers it reads alive; the object has to outlive the graph."""
 
     def __init__(self, gradients: Sequence[torch.Tensor], *, kind: str = "l2"):
         self._kind, self._kept = _choice(_NORMS, kind, "kind"), []

@@ -349,8 +349,8 @@ EPS_B200_EXPORT int eps_b200_balance_loss_backward(const EpsB200BalanceLoss* arg
 /* ---- Low-rank adapters of many requests at once, beside a layer that they share.
  *   a = ids[t];  out[t] = base[t] + scale[a] * up[a] (down[a] x[t])
  * An id outside [0, adapters) is no adapter: out[t] is base[t].  base NULL: 0; out may
- * be base itself.  out must not overlap x, nor what else is read.  down [adapters, R, K'] and up [adapters,
- * channels, R] are contiguous and 16-byte aligned; inner, channels and strides are below
+ * be base itself, and must overlap nothing else that is read.  down [adapters, R, K'] and
+ * up [adapters, channels, R] are contiguous and 16-byte aligned; inner, channels and strides are below
  * 2^30.  R = eps_b200_low_rank_rank(rank)
  * and K' = eps_b200_low_rank_inner(inner), and zeros behind `rank` and `inner`.  All
  * have one type.  `workspace` holds eps_b200_low_rank_workspace() bytes (0 for few rows).
